@@ -91,6 +91,25 @@ class CallPlanInfo(ctypes.Structure):
         "chunk_rows")] + [("scratch", ctypes.c_size_t)]
 
 
+class _KvCacheDesc(ctypes.Structure):
+    """atn_kv_cache."""
+    _fields_ = [("K", ctypes.c_void_p), ("V", ctypes.c_void_p),
+                ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+                ("len", ctypes.c_void_p), ("seen", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+                ("dtype", ctypes.c_int), ("batch", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("capacity", ctypes.c_int), ("head_d", ctypes.c_int)]
+
+
+class _DraftsDesc(ctypes.Structure):
+    """atn_drafts."""
+    _fields_ = [("Q", ctypes.c_void_p), ("K", ctypes.c_void_p), ("V", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3),
+                ("v_stride", ctypes.c_int64 * 3),
+                ("count", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+                ("heads", ctypes.c_int), ("tokens", ctypes.c_int)]
+
+
 class AtnError(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -131,6 +150,13 @@ _SIGS = {
                           _i),
     "atn_call_plan_ex": ([_i] * 6 + [ctypes.POINTER(PeDesc), ctypes.c_size_t,
                                      ctypes.POINTER(CallPlanInfo)], _i),
+    "atn_tree_attention_ex": ([_vp, _vp, _vp, _vp, _vp, _f, _i, _vp, ctypes.c_size_t, _vp], _i),
+    "atn_tree_attention_workspace_bytes": ([_vp, _vp, _i], ctypes.c_size_t),
+    "atn_cache_commit_ex": ([_vp, _vp, _vp, _vp, _i, _vp], _i),
+    "atn_cache_weigh_ex": ([_vp, _vp, _vp, _vp, _vp, _i, _vp, _f, _i, _vp], _i),
+    "atn_cache_evict_ex": ([_vp, _i, _i, _vp, ctypes.c_size_t, _vp], _i),
+    "atn_cache_evict_workspace_bytes": ([_vp, _i], ctypes.c_size_t),
+    "atn_cache_advance_ex": ([_vp, _vp, _vp, _vp, _i, _i, _vp], _i),
     "atn_rerun_count": ([_i], ctypes.c_long),
     "atn_retained_bytes_ex": ([], ctypes.c_size_t),
     "atn_release_ex": ([], _i),
@@ -279,13 +305,17 @@ def release() -> None:
 # ---------------------------------------------------------------- array helpers
 # Arguments are hip_rt.DeviceArray objects ([B,H,L,D], 'f32' or 'bf16').
 def _ptr(t):
+    if t is not None and t.strides is not None:
+        raise ValueError("a strided array where a contiguous one is needed")
     return None if t is None else t.ptr
 
 
-def _check(t, dtype, shape, name):
+def _check(t, dtype, shape, name, strided=False):
     from hip_rt import DeviceArray
     if not isinstance(t, DeviceArray):
         raise ValueError(f"{name} must be a hip_rt.DeviceArray")
+    if not strided and t.strides is not None:
+        raise ValueError(f"{name} must be contiguous")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if tuple(t.shape) != tuple(shape):
@@ -301,7 +331,8 @@ def _dtype_code(t) -> int:
 
 
 def _stream_handle(stream) -> int | None:
-    return None if stream is None else stream.handle
+    """A hip_rt.Stream, a hipStream_t as an int, or None (the null stream)."""
+    return stream if stream is None or isinstance(stream, int) else stream.handle
 
 
 def make_pe(kind: str = "none", pairing: str = "interleaved", rotary_dim: int = 0,
@@ -455,14 +486,15 @@ def attention_forward_separate_rope(Q, K, V, Q_rope, K_rope, out, cos_cache, sin
 def rope_forward(x, out, cos_cache, sin_cache, rotary_dim: int, seq_len: int):
     D = x.shape[-1]
     _rot_check(rotary_dim, D)
-    lib().rope_forward(x.ptr, out.ptr, cos_cache.ptr, sin_cache.ptr, x.size // D, D, rotary_dim,
-                       seq_len)
+    lib().rope_forward(_ptr(x), _ptr(out), _ptr(cos_cache), _ptr(sin_cache), x.size // D, D,
+                       rotary_dim, seq_len)
     return out
 
 
 def apply_sinusoidal_embeddings(x, sin_table, cos_table, out, seqlen: int):
     D = x.shape[-1]
-    lib().apply_sinusoidal_embeddings(x.ptr, sin_table.ptr, cos_table.ptr, out.ptr, x.size // D,
+    lib().apply_sinusoidal_embeddings(_ptr(x), _ptr(sin_table), _ptr(cos_table), _ptr(out),
+                                      x.size // D,
                                       D, seqlen)
     return out
 
@@ -516,6 +548,217 @@ def attention_forward_sinusoidal_bf16(Q, K, V, out):
     B, H, Lq, Lk, D = _dropin_check("bf16", Q, K, V, out)
     lib().attention_forward_sinusoidal_bf16(Q.ptr, K.ptr, V.ptr, out.ptr, B, H, Lq, Lk, D)
     return out
+
+
+# ---------------------------------------------------------------- decoding over a cache
+ATN_TREE_MAX_TOKENS = 256
+ATN_CACHE_MAX_HEAD_D = 8192
+
+
+def _strides(t, name):
+    """Batch, head and row strides of a [B][heads][rows][D] array (0, 0, 0: contiguous)."""
+    if t is None or t.strides is None:
+        return (ctypes.c_int64 * 3)(0, 0, 0)
+    if t.strides[3] != 1 and t.shape[3] != 1:
+        raise ValueError(f"{name}: the elements of a row must be adjacent")
+    if not any(t.strides[:3]):
+        raise ValueError(f"{name}: strides 0, 0, 0 mean a contiguous array to the library")
+    return (ctypes.c_int64 * 3)(*t.strides[:3])
+
+
+class KvCache:
+    """A key/value cache (atn_kv_cache): K and V [B][kv heads][capacity][D], `length` [B] rows in
+    use, and where the calls need them `seen` [B], `weight` and `pos` [B][kv heads][capacity].
+    Holds the arrays it is made of."""
+
+    def __init__(self, K, V, length, seen=None, weight=None, pos=None):
+        _check(K, K.dtype, K.shape, "K", strided=True)
+        if len(K.shape) != 4:
+            raise ValueError("K must be [batch][kv heads][capacity][head_d]")
+        _check(V, K.dtype, K.shape, "V", strided=True)
+        B, G, cap, D = K.shape
+        _check(length, "i32", (B,), "length")
+        for t, dt, shape, name in ((seen, "i32", (B,), "seen"), (weight, "f32", (B, G, cap), "weight"),
+                                   (pos, "i32", (B, G, cap), "pos")):
+            if t is not None:
+                _check(t, dt, shape, name)
+        self.K, self.V, self.length, self.seen, self.weight, self.pos = K, V, length, seen, weight, pos
+        self.dtype, self.shape = K.dtype, (B, G, cap, D)
+        self.desc = _KvCacheDesc(K.ptr, V.ptr, _strides(K, "K"), _strides(V, "V"), _ptr(length),
+                                 _ptr(seen), _ptr(weight), _ptr(pos), _dtype_code(K), B, G, cap, D)
+
+
+class Drafts:
+    """Drafted tokens (atn_drafts): Q [B][heads][T][D], K and V [B][kv heads][T][D], `count` [B]
+    tokens of each sequence, `mask` [B][T][ceil(T / 32)] words (tree_mask)."""
+
+    def __init__(self, Q, K=None, V=None, count=None, mask=None):
+        if len(Q.shape) != 4:
+            raise ValueError("Q must be [batch][heads][tokens][head_d]")
+        B, H, T, D = Q.shape
+        _check(Q, Q.dtype, Q.shape, "Q", strided=True)
+        if (K is None) != (V is None):
+            raise ValueError("K and V go together")
+        if K is not None:
+            _check(K, Q.dtype, (B, K.shape[1], T, D), "K", strided=True)
+            _check(V, Q.dtype, K.shape, "V", strided=True)
+        if count is not None:
+            _check(count, "i32", (B,), "count")
+        if mask is not None:
+            _check(mask, "i32", (B, T, (T + 31) // 32), "mask")
+        self.Q, self.K, self.V, self.count, self.mask = Q, K, V, count, mask
+        self.dtype, self.shape = Q.dtype, (B, H, T, D)
+        self.desc = _DraftsDesc(Q.ptr, None if K is None else K.ptr, None if V is None else V.ptr,
+                                _strides(Q, "Q"), _strides(K, "K"), _strides(V, "V"), _ptr(count),
+                                _ptr(mask), H, T)
+
+    def check(self, cache: KvCache) -> None:
+        B, G, _, D = cache.shape
+        if self.dtype != cache.dtype or self.shape[0] != B or self.shape[3] != D:
+            raise ValueError(f"drafts {self.dtype} {self.shape} do not fit a cache "
+                             f"{cache.dtype} {cache.shape}")
+        if self.shape[1] % G:
+            raise ValueError("heads must be a multiple of the cache's kv heads")
+        if self.K is not None and self.K.shape[1] != G:
+            raise ValueError(f"K must have the cache's {G} kv heads")
+
+
+def tree_mask(parents):
+    """Mask words (int32 numpy [B][T][ceil(T / 32)]) of trees given by parents [B][T]: draft t
+    attends itself, its parent parents[b][t] < t and that one's ancestors; -1: none."""
+    import numpy as np
+    parents = np.asarray(parents)
+    B, T = parents.shape
+    see = np.zeros((B, T, (T + 31) // 32 * 32), dtype=bool)
+    for b in range(B):
+        for t in range(T):
+            p = int(parents[b, t])
+            if not -1 <= p < t:
+                raise ValueError(f"parent {p} of draft {t} must be an earlier draft or -1")
+            if p >= 0:
+                see[b, t] = see[b, p]
+            see[b, t, t] = True
+    return np.packbits(see, axis=-1, bitorder="little").view("<i4")
+
+
+class Call:
+    """An entry point bound to its arguments: call it with a stream (hip_rt.Stream, hipStream_t as
+    an int, or None) as often as its buffers hold new values.  Raises AtnError."""
+
+    def __init__(self, name, args, result, keep):
+        self.name, self.fn, self.args, self.result, self._keep = (name, getattr(lib(), name), args,
+                                                                  result, keep)
+
+    def __call__(self, stream=None):
+        st = self.fn(*self.args, _stream_handle(stream))
+        if st != ATN_OK:
+            raise AtnError(st, self.name)
+        return self.result
+
+
+def _ref(desc):
+    return ctypes.cast(ctypes.pointer(desc), _vp)
+
+
+def _path_args(cache, path, accepted, tokens):
+    B = cache.shape[0]
+    n = tokens
+    if path is not None:
+        n = path.shape[-1]
+        _check(path, "i32", (B, n), "path")
+    if accepted is not None:
+        _check(accepted, "i32", (B,), "accepted")
+    return _ptr(path), _ptr(accepted), n
+
+
+def tree_attention_workspace_bytes(cache: KvCache, drafts: Drafts, max_len: int = 0) -> int:
+    return lib().atn_tree_attention_workspace_bytes(_ref(cache.desc), _ref(drafts.desc), max_len)
+
+
+def tree_attention_call(cache: KvCache, drafts: Drafts, out=None, lse=None, scale: float = 0.0,
+                        max_len: int = 0, workspace=None) -> Call:
+    """atn_tree_attention_ex bound to its arguments; calling it returns out [B][heads][T][D]."""
+    from hip_rt import DeviceArray
+    drafts.check(cache)
+    if out is None:
+        out = DeviceArray(drafts.shape, drafts.dtype)
+    _check(out, drafts.dtype, drafts.shape, "out", strided=True)
+    if lse is not None:
+        _check(lse, "f32", drafts.shape[:3], "lse")
+    strides = _strides(out, "out")
+    args = (_ref(cache.desc), _ref(drafts.desc), out.ptr, ctypes.cast(strides, _vp), _ptr(lse),
+            scale, max_len, _ptr(workspace), workspace.nbytes if workspace is not None else 0)
+    return Call("atn_tree_attention_ex", args, out, (cache, drafts, lse, strides, workspace))
+
+
+def tree_attention_ex(cache, drafts, out=None, lse=None, scale=0.0, max_len=0, workspace=None,
+                      stream=None):
+    """atn_tree_attention_ex; asynchronous on `stream`.  Raises AtnError."""
+    return tree_attention_call(cache, drafts, out, lse, scale, max_len, workspace)(stream)
+
+
+def cache_commit_call(cache: KvCache, drafts: Drafts, path=None, accepted=None) -> Call:
+    drafts.check(cache)
+    p, a, n = _path_args(cache, path, accepted, drafts.shape[2])
+    return Call("atn_cache_commit_ex", (_ref(cache.desc), _ref(drafts.desc), p, a, n), cache,
+                (cache, drafts, path, accepted))
+
+
+def cache_commit_ex(cache, drafts, path=None, accepted=None, stream=None):
+    """atn_cache_commit_ex: accepted drafts become rows of the cache (lengths stay)."""
+    return cache_commit_call(cache, drafts, path, accepted)(stream)
+
+
+def cache_weigh_call(cache: KvCache, drafts: Drafts, lse, path=None, accepted=None, weight_in="own",
+                     scale: float = 0.0, max_len: int = 0) -> Call:
+    """weight_in: an array, None for zeros, or "own": cache.weight, in place."""
+    drafts.check(cache)
+    if weight_in == "own":
+        weight_in = cache.weight
+    _check(lse, "f32", drafts.shape[:3], "lse")
+    if weight_in is not None:
+        _check(weight_in, "f32", cache.shape[:3], "weight_in")
+    p, a, n = _path_args(cache, path, accepted, drafts.shape[2])
+    args = (_ref(cache.desc), _ref(drafts.desc), _ptr(lse), p, a, n, _ptr(weight_in), scale, max_len)
+    return Call("atn_cache_weigh_ex", args, cache.weight,
+                (cache, drafts, lse, path, accepted, weight_in))
+
+
+def cache_weigh_ex(cache, drafts, lse, path=None, accepted=None, weight_in="own", scale=0.0,
+                   max_len=0, stream=None):
+    """atn_cache_weigh_ex: the rows gather the accepted drafts' attention weight."""
+    return cache_weigh_call(cache, drafts, lse, path, accepted, weight_in, scale, max_len)(stream)
+
+
+def cache_evict_workspace_bytes(cache: KvCache, budget: int) -> int:
+    return lib().atn_cache_evict_workspace_bytes(_ref(cache.desc), budget)
+
+
+def cache_evict_call(cache: KvCache, budget: int, recent: int = 0, workspace=None) -> Call:
+    args = (_ref(cache.desc), budget, recent, _ptr(workspace),
+            workspace.nbytes if workspace is not None else 0)
+    return Call("atn_cache_evict_ex", args, cache, (cache, workspace))
+
+
+def cache_evict_ex(cache, budget, recent=0, workspace=None, stream=None):
+    """atn_cache_evict_ex: keeps the recent and heaviest `budget` rows of each head (lengths stay)."""
+    return cache_evict_call(cache, budget, recent, workspace)(stream)
+
+
+def cache_advance_call(cache: KvCache, drafts: Drafts | None = None, path=None, accepted=None,
+                       limit: int = 0) -> Call:
+    p, a, n = None, None, 1
+    if drafts is not None:
+        drafts.check(cache)
+        p, a, n = _path_args(cache, path, accepted, drafts.shape[2])
+    return Call("atn_cache_advance_ex",
+                (_ref(cache.desc), None if drafts is None else _ref(drafts.desc), p, a, n, limit),
+                cache, (cache, drafts, path, accepted))
+
+
+def cache_advance_ex(cache, drafts=None, path=None, accepted=None, limit=0, stream=None):
+    """atn_cache_advance_ex: the lengths take in the committed rows, then come down to `limit`."""
+    return cache_advance_call(cache, drafts, path, accepted, limit)(stream)
 
 
 def precompute_rope_cache(max_seq_len: int, rotary_dim: int, base: float = 10000.0):

@@ -23,6 +23,7 @@
 
 #include "../kernels/launch.hpp"
 #include "attn_mi355x.h"
+#include "host.hpp"
 
 namespace {
 
@@ -1718,6 +1719,17 @@ atn_pe_desc sin_desc(bool q, bool k, const float* sin_t, const float* cos_t) {
 }
 
 }  // namespace
+
+// ---------------------------------------------------------------- for the other host files
+namespace atn_host {
+static_assert(kSyncBytes == kSyncRegion, "sync region");
+int fail(hipError_t e) { return hip_fail(e); }
+int device(int* dev) { return current_device(dev); }
+int workspace(size_t bytes, hipStream_t stream, void** ws) {
+    return ensure_workspace(bytes, stream, ws);
+}
+size_t workspace_cap() { return library_cap(); }
+}  // namespace atn_host
 
 // ====================================================================== C ABI
 extern "C" {

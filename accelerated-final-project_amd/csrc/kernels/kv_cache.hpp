@@ -1,0 +1,94 @@
+// Argument views and launchers of the decoding operators: attention of
+// drafted tokens over a key/value cache (tree_attn.hip), and the cache's
+// commit, weights, eviction and lengths (kv_cache.hip).  The launchers
+// validate nothing (the C-ABI layer does) and are asynchronous on `st`.
+//
+// Lengths live on the device, so that a captured graph replays with whatever
+// they hold; the kernels clamp them to what the tensors hold, and no index
+// read from device memory reaches an address unchecked.
+#pragma once
+
+#include "launch.hpp"
+
+namespace atn {
+
+constexpr int kTreeMaxTokens = 256;  // drafted tokens of a call, entries of a path
+
+// K and V of [batch][kv head][row][head_d], strides in elements.
+struct CacheView {
+    void* K;
+    void* V;
+    int64_t ks[3], vs[3];  // batch, head, row
+    const int* len;        // [B] rows in use
+    float* weight;         // [B][G][cap]
+    int* pos;              // [B][G][cap]
+    int* seen;             // [B]
+    int B, G, cap, D;
+};
+
+// Drafted tokens: Q [batch][head][token][head_d], K and V [batch][kv head][token][head_d].
+struct DraftView {
+    const void* Q;
+    const void* K;
+    const void* V;
+    int64_t qs[3], ks[3], vs[3];  // batch, head, token
+    const int* count;             // [B] tokens of each sequence, or null: T
+    const uint32_t* mask;         // [B][T][W], or null: a chain
+    int H, T, W;                  // W = ceil(T / 32)
+};
+
+// The drafts of each sequence that became part of it.
+struct PathView {
+    const int* path;      // [B][n] drafts, or null: 0, 1, ...
+    const int* accepted;  // [B] entries of it that count, or null: all
+    int n;
+};
+
+struct TreePlan {
+    int nsplit;      // key splits
+    int row_tiles;   // tiles of query rows of one kv head
+    int rows;        // query rows of a tile
+    size_t scratch;  // bytes
+    int64_t workgroups;
+};
+
+struct TreeArgs {
+    CacheView c;
+    DraftView d;
+    void* out;
+    int64_t os[3];  // batch, head, token
+    float* lse;     // [B][H][T] or null
+    float scale;    // times log2(e)
+    TreePlan plan;
+    float* part;    // scratch
+};
+
+// rows in use of sequence b, and its drafts
+__device__ __forceinline__ int rows_in_use(const CacheView& c, int b) {
+    return min(max(c.len[b], 0), c.cap);
+}
+__device__ __forceinline__ int drafts_of(const DraftView& d, int b) {
+    return d.count ? min(max(d.count[b], 0), d.T) : d.T;
+}
+// Whether draft t of sequence b (of n drafts) attends draft j.
+__device__ __forceinline__ bool sees(const DraftView& d, int b, int t, int j) {
+    if (!d.mask) return j <= t;
+    return (d.mask[((size_t)b * d.T + t) * d.W + (j >> 5)] >> (j & 31)) & 1u;
+}
+
+// The plan depends on no device, so that workspace queries hold for any.
+TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, size_t scratch_cap);
+hipError_t launch_tree_attention(int dtype, const TreeArgs& a, hipStream_t st);
+
+hipError_t launch_cache_commit(int dtype, const CacheView& c, const DraftView& d,
+                               const PathView& p, hipStream_t st);
+hipError_t launch_cache_weigh(int dtype, const CacheView& c, const DraftView& d,
+                              const PathView& p, const float* lse, const float* weight_in,
+                              float scale, int max_len, hipStream_t st);
+hipError_t launch_cache_advance(const CacheView& c, int* len, const DraftView* d,
+                                const PathView& p, int limit, hipStream_t st);
+size_t evict_scratch(int B, int G, int cap, int budget);
+hipError_t launch_cache_evict(int dtype, const CacheView& c, int budget, int recent,
+                              int* scratch, hipStream_t st);
+
+}  // namespace atn

@@ -116,13 +116,29 @@ def bf16_bits_to_f32(b: np.ndarray) -> np.ndarray:
 
 
 # ---------------------------------------------------------------- buffers
+_ITEMSIZE = {"f32": 4, "bf16": 2, "i32": 4}
+_HOST_TYPE = {"f32": np.float32, "bf16": np.uint16, "i32": np.int32}
+
+
+def contiguous_strides(shape) -> tuple:
+    out, n = [], 1
+    for s in reversed(tuple(shape)):
+        out.append(n)
+        n *= int(s)
+    return tuple(reversed(out))
+
+
 class DeviceArray:
-    """A device allocation with a shape and an element type ('f32' | 'bf16')."""
+    """A device allocation with a shape and an element type ('f32' | 'bf16';
+    'i32' for lengths, positions and masks).  `strides` are in elements, None for
+    a contiguous array; only wrap() and strided() make others."""
+
+    strides = None
 
     def __init__(self, shape, dtype: str = "f32", fill=None):
         self.shape = tuple(int(s) for s in shape)
         self.dtype = dtype
-        self.itemsize = 4 if dtype == "f32" else 2
+        self.itemsize = _ITEMSIZE[dtype]
         self.size = int(np.prod(self.shape)) if self.shape else 1
         self.nbytes = self.size * self.itemsize
         p = _vp()
@@ -139,7 +155,7 @@ class DeviceArray:
         obj = cls.__new__(cls)
         obj.shape = tuple(shape)
         obj.dtype = dtype or base.dtype
-        obj.itemsize = 4 if obj.dtype == "f32" else 2
+        obj.itemsize = _ITEMSIZE[obj.dtype]
         obj.size = int(np.prod(obj.shape))
         obj.nbytes = obj.size * obj.itemsize
         obj.base = base.base
@@ -149,11 +165,37 @@ class DeviceArray:
         return obj
 
     @classmethod
+    def wrap(cls, ptr: int, shape, dtype: str, strides=None, keep=None) -> "DeviceArray":
+        """Non-owning array over device memory of another owner (a tensor of a
+        library on the same HIP runtime); `keep` is held as long as the array."""
+        obj = cls.__new__(cls)
+        obj.shape = tuple(int(s) for s in shape)
+        obj.dtype = dtype
+        obj.itemsize = _ITEMSIZE[dtype]
+        obj.size = int(np.prod(obj.shape)) if obj.shape else 1
+        obj.nbytes = obj.size * obj.itemsize
+        obj.base = obj.ptr = ptr
+        obj._owner = False
+        obj._keep = keep
+        if strides is not None and tuple(strides) != contiguous_strides(obj.shape):
+            obj.strides = tuple(int(s) for s in strides)
+        return obj
+
+    @classmethod
+    def strided(cls, base: "DeviceArray", shape, strides, offset_elems: int = 0) -> "DeviceArray":
+        """Non-owning strided view of an array (kernel arguments only: it has no
+        host copy)."""
+        obj = cls.wrap(base.ptr + offset_elems * base.itemsize, shape, base.dtype, strides, base)
+        return obj
+
+    @classmethod
     def from_numpy(cls, a: np.ndarray, dtype: str = "f32") -> "DeviceArray":
         """Upload float32 data; dtype 'bf16' rounds (RNE) on the host first.
         A uint16 array with dtype 'bf16' is taken as raw bf16 bits."""
         if dtype == "bf16":
             host = a if a.dtype == np.uint16 else f32_to_bf16_bits(a)
+        elif dtype == "i32":
+            host = np.ascontiguousarray(a).astype(np.int32)
         else:
             host = np.ascontiguousarray(a, dtype=np.float32)
         host = np.ascontiguousarray(host)
@@ -163,20 +205,21 @@ class DeviceArray:
 
     def upload(self, a: np.ndarray) -> None:
         host = f32_to_bf16_bits(a) if (self.dtype == "bf16" and a.dtype != np.uint16) else a
-        host = np.ascontiguousarray(host, dtype=np.uint16 if self.dtype == "bf16" else np.float32)
+        host = np.ascontiguousarray(host, dtype=_HOST_TYPE[self.dtype])
         assert host.nbytes == self.nbytes
         check(hip().hipMemcpy(_vp(self.ptr), host.ctypes.data_as(_vp), self.nbytes, H2D), "H2D")
 
     def bits(self) -> np.ndarray:
-        """Raw contents: float32 array, or uint16 bf16 bits."""
-        out = np.empty(self.shape, dtype=np.float32 if self.dtype == "f32" else np.uint16)
+        """Raw contents: float32 or int32 array, or uint16 bf16 bits."""
+        assert self.strides is None, "a strided view has no host copy"
+        out = np.empty(self.shape, dtype=_HOST_TYPE[self.dtype])
         check(hip().hipMemcpy(out.ctypes.data_as(_vp), _vp(self.ptr), self.nbytes, D2H), "D2H")
         return out
 
     def numpy(self) -> np.ndarray:
-        """Contents widened to float32."""
+        """Contents, bf16 widened to float32."""
         b = self.bits()
-        return b if self.dtype == "f32" else bf16_bits_to_f32(b)
+        return bf16_bits_to_f32(b) if self.dtype == "bf16" else b
 
     def fill_nan(self) -> None:
         check(hip().hipMemset(_vp(self.ptr), 0xFF, self.nbytes), "hipMemset")

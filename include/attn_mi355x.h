@@ -313,6 +313,123 @@ int atn_attention_path_ex(int dtype, int batch, int heads, int len_q, int len_k,
 /* Number of visible HIP devices (0 when none); never aborts. */
 int atn_device_count(void);
 
+/* ==================== decoding over a key/value cache ====================
+ * No counterpart in the reference, whose launchers take whole sequences.  A
+ * decoding program keeps the keys and values of each sequence in a cache and
+ * attends a few new tokens at a time: one token, or a tree of drafted tokens of
+ * which the model then accepts a path.  A step is
+ *     atn_tree_attention_ex     the drafts over the cache (every layer's cache)
+ *     atn_cache_commit_ex       accepted drafts become rows of each cache
+ *     atn_cache_weigh_ex        rows gather the accepted drafts' attention weight
+ *     atn_cache_advance_ex      the lengths move on, once
+ * and, where a cache has grown past a bound,
+ *     atn_cache_evict_ex        each cache keeps its recent and heaviest rows
+ *     atn_cache_advance_ex      the lengths come down to the bound, once.
+ * Only advance changes lengths, so that the caches of all layers can share them.
+ *
+ * Lengths, counts, masks and paths are device memory, read when the kernels
+ * run: a captured graph replays with what they then hold.  Values out of range
+ * are clamped to what the tensors hold (len to [0, capacity], count to
+ * [0, tokens]; a path ends before its first entry that names no draft); they
+ * never lead to an access outside a tensor.
+ *
+ * All calls validate their arguments before any HIP call, return an ATN_*
+ * status and enqueue on `stream`; calls on one cache belong on one stream (or in
+ * an order of the caller's).  Results do not depend on timing: no atomics on
+ * floating-point values, every sum in one order.  Elements are
+ * head_d-contiguous; head_d <= 8192; any alignment to the element size (16-byte
+ * aligned rows are read as vectors). */
+#define ATN_TREE_MAX_TOKENS 256
+#define ATN_CACHE_MAX_HEAD_D 8192
+
+/* A cache.  Strides in elements for batch, kv head and row; all three 0: contiguous
+ * [batch][kv_heads][capacity][head_d].  Rows at or past len hold anything. */
+typedef struct atn_kv_cache {
+    void *K, *V;
+    int64_t k_stride[3], v_stride[3];
+    int32_t *len;  /* [batch] rows in use of each head */
+    int32_t *seen; /* [batch] tokens the sequence has had (commit, advance and evict) */
+    float *weight; /* [batch][kv_heads][capacity] attention weight of the rows (weigh, evict;
+                      commit sets new rows to 0), or NULL */
+    int32_t *pos;  /* [batch][kv_heads][capacity] position of the rows' tokens (evict; commit
+                      sets seen, seen + 1, ...), or NULL */
+    int dtype;     /* ATN_DTYPE_* of the cache, the drafts and the output */
+    int batch, kv_heads, capacity, head_d;
+} atn_kv_cache;
+
+/* Drafted tokens.  heads is a multiple of the cache's kv_heads; head h reads kv
+ * head h / (heads / kv_heads).  Strides in elements for batch, head and token
+ * (0 repeats); all three 0: contiguous [batch][heads][tokens][head_d].  Positional
+ * encodings are applied by the caller beforehand. */
+typedef struct atn_drafts {
+    const void *Q;             /* queries of every head */
+    const void *K, *V;         /* keys and values of every kv head; both NULL: the tokens
+                                  attend the cache alone (padded encoder states, say) */
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const int32_t *count;      /* [batch] tokens of each sequence; NULL: tokens */
+    const uint32_t *mask;      /* [batch][tokens][(tokens + 31) / 32]: bit j % 32 of word j / 32
+                                  of token t is set where t attends draft j; NULL: j <= t */
+    int heads, tokens;         /* tokens <= ATN_TREE_MAX_TOKENS */
+} atn_drafts;
+
+/* out[b][h][t] = softmax over cache rows r < len[b] and the drafts j < count[b] of
+ * token t's mask of (scale q . k) times v, for t < count[b]; the rows behind are
+ * left as they were.  scale 0: 1 / sqrtf(head_d).  A token that attends nothing
+ * (or only scores of -infinity) gets zeros.  lse (may be NULL): [batch][heads]
+ * [tokens] fp32, the natural log of the softmax's denominator (-infinity for such a
+ * token).  Keys and values that a token does not attend do not reach its output,
+ * whatever they hold.  out_stride: as atn_drafts.q_stride, of distinct elements;
+ * NULL: contiguous.  max_len: an upper bound of len known on the host (0: the
+ * capacity), for the choice of key splits alone: a smaller one is slower, not
+ * wrong.  workspace as for atn_attention_fwd_ex (NULL: the stream's library
+ * workspace; else zero-filled once, at least
+ * atn_tree_attention_workspace_bytes()). */
+int atn_tree_attention_ex(const atn_kv_cache *cache, const atn_drafts *drafts, void *out,
+                          const int64_t *out_stride, float *lse, float scale, int max_len,
+                          void *workspace, size_t workspace_bytes, void *stream);
+/* 0 on bad input.  Needs no device. */
+size_t atn_tree_attention_workspace_bytes(const atn_kv_cache *cache, const atn_drafts *drafts,
+                                          int max_len);
+
+/* Writes the accepted drafts behind the rows in use: cache row len[b] + i takes
+ * K and V of draft path[b][i], i < accepted[b], weight 0 and position seen[b] + i.
+ * path: [batch][path_len] draft numbers, NULL: 0, 1, ...; accepted: [batch], NULL:
+ * path_len (or count[b] where that is less).  Rows that the capacity does not hold
+ * are dropped. */
+int atn_cache_commit_ex(const atn_kv_cache *cache, const atn_drafts *drafts, const int32_t *path,
+                        const int32_t *accepted, int path_len, void *stream);
+
+/* The attention weight that the accepted drafts gave the rows, after commit and
+ * before advance: for every row r < len[b] + (rows committed),
+ *   weight[b][g][r] = weight_in[b][g][r]
+ *                     + sum over the group's heads h and path entries i with r <= len[b] + i
+ *                       of exp(scale q . k_r - lse[b][h][path[b][i]]);
+ * other rows stay.  lse: atn_tree_attention_ex's (entries of -infinity add
+ * nothing).  weight_in: NULL for zeros; may be cache->weight. */
+int atn_cache_weigh_ex(const atn_kv_cache *cache, const atn_drafts *drafts, const float *lse,
+                       const int32_t *path, const int32_t *accepted, int path_len,
+                       const float *weight_in, float scale, int max_len, void *stream);
+
+/* Cuts every head of more than `budget` rows to `budget`: it keeps the rows of
+ * positions from seen[b] - recent on (the lower rows where these alone exceed the
+ * budget), then the heaviest of the others (equal weights: the lower row; NaN: below
+ * all).  Kept rows below `budget` stay where they are; the
+ * i-th kept row from `budget` on moves (K, V, weight, pos) into the i-th slot below
+ * that a dropped row leaves.  Rows lie in no order of age afterwards: attention
+ * does not depend on it, and pos holds it.  0 <= recent <= budget, 1 <= budget.
+ * Then atn_cache_advance_ex with limit = budget. */
+int atn_cache_evict_ex(const atn_kv_cache *cache, int budget, int recent, void *workspace,
+                       size_t workspace_bytes, void *stream);
+/* 0 on bad input. */
+size_t atn_cache_evict_workspace_bytes(const atn_kv_cache *cache, int budget);
+
+/* len[b] += rows that atn_cache_commit_ex writes for the same arguments, seen[b] (if
+ * not NULL) likewise, then len[b] = min(len[b], limit) where limit > 0.  drafts NULL:
+ * the limit alone (path, accepted and path_len are not used). */
+int atn_cache_advance_ex(const atn_kv_cache *cache, const atn_drafts *drafts,
+                         const int32_t *path, const int32_t *accepted, int path_len, int limit,
+                         void *stream);
+
 /* ==================== tuning, test controls and introspection ====================
  * None of these has a counterpart in the reference (whose launchers take no
  * options).  They exist for measurement and tests; a program that never
