@@ -295,8 +295,10 @@ def test_captured_calls_follow_the_lengths(am, dev, dtype, Hq, G, T, D):
 def test_capture_refuses_to_allocate(am, dev):
     import hip_rt
     s = hip_rt.Stream()
-    p = Problem(am, "bf16", 1, 8, 8, 1, 128, 8192, [8000])
-    needs = am.tree_attention_workspace_bytes(p.cache, p.drafts) > 40960
+    # (more scratch than the workspace of any stream of the other tests, whose handle this one
+    # may have)
+    p = Problem(am, "bf16", 1, 32, 8, 64, 128, 4096, [4000])
+    assert am.tree_attention_workspace_bytes(p.cache, p.drafts) > 8 << 20
     status = []
 
     def call():
@@ -306,7 +308,7 @@ def test_capture_refuses_to_allocate(am, dev):
             status.append(e.status)
 
     hip_rt.Graph(s, call).destroy()
-    assert status == ([am.ATN_ERR_CAPTURE] if needs else [])
+    assert status == [am.ATN_ERR_CAPTURE]
     p.run(stream=s)
     p.check()
     s.destroy()
