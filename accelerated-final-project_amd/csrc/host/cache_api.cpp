@@ -97,6 +97,7 @@ int check_cache(const atn_kv_cache* c, atn::CacheView* v, Ranges* r) {
     v->G = c->kv_heads;
     v->cap = c->capacity;
     v->D = c->head_d;
+    v->rows = c->capacity;
     return ATN_OK;
 }
 
@@ -150,10 +151,10 @@ int check_scale(float scale, int D, float* out) {
     return std::isfinite(*out) ? ATN_OK : ATN_ERR_BAD_ARGUMENT;
 }
 
-// rows that the host expects at most
-int rows_bound(int max_len, int cap, int* out) {
+// lengths count up to max_len (0: the capacity)
+int bound_rows(int max_len, atn::CacheView* c) {
     if (max_len < 0) return ATN_ERR_BAD_DIMENSION;
-    *out = max_len == 0 ? cap : std::min(max_len, cap);
+    if (max_len > 0) c->rows = std::min(max_len, c->cap);
     return ATN_OK;
 }
 
@@ -184,9 +185,8 @@ bool any_meet(std::initializer_list<Range> writes, std::initializer_list<Range> 
     return false;
 }
 
-atn::TreePlan plan_tree(const atn::CacheView& c, const atn::DraftView& d, int dtype, int rows,
-                        size_t cap) {
-    return atn::tree_plan(dtype, c.B, c.G, d.H, d.T, c.D, rows, cap);
+atn::TreePlan plan_tree(const atn::CacheView& c, const atn::DraftView& d, int dtype, size_t cap) {
+    return atn::tree_plan(dtype, c.B, c.G, d.H, d.T, c.D, c.rows, d.K != nullptr, cap);
 }
 
 }  // namespace
@@ -198,12 +198,11 @@ size_t atn_tree_attention_workspace_bytes(const atn_kv_cache* cache, const atn_d
     atn::CacheView c;
     atn::DraftView d;
     Ranges r;
-    int rows;
     if (check_cache(cache, &c, &r) != ATN_OK ||
         check_drafts(cache, drafts, true, false, &d, &r) != ATN_OK ||
-        rows_bound(max_len, c.cap, &rows) != ATN_OK)
+        bound_rows(max_len, &c) != ATN_OK)
         return 0;
-    return kSyncRegion + plan_tree(c, d, cache->dtype, rows, atn_host::workspace_cap()).scratch;
+    return kSyncRegion + plan_tree(c, d, cache->dtype, atn_host::workspace_cap()).scratch;
 }
 
 int atn_tree_attention_ex(const atn_kv_cache* cache, const atn_drafts* drafts, void* out,
@@ -224,8 +223,7 @@ int atn_tree_attention_ex(const atn_kv_cache* cache, const atn_drafts* drafts, v
     if (lse) rl = range(lse, (int64_t)a.c.B * a.d.H * a.d.T * 4);
     if (any_meet({ro, rl}, {r.k, r.v, r.qd, r.kd, r.vd})) return ATN_ERR_ALIASING;
     st = check_scale(scale, a.c.D, &a.scale);
-    int rows = 0;
-    if (st == ATN_OK) st = rows_bound(max_len, a.c.cap, &rows);
+    if (st == ATN_OK) st = bound_rows(max_len, &a.c);
     if (st != ATN_OK) return st;
     a.out = out;
     a.lse = lse;
@@ -234,16 +232,17 @@ int atn_tree_attention_ex(const atn_kv_cache* cache, const atn_drafts* drafts, v
         if (workspace_bytes < kSyncRegion) return ATN_ERR_WORKSPACE;
         room = workspace_bytes - kSyncRegion;
     }
-    a.plan = plan_tree(a.c, a.d, cache->dtype, rows, room);
+    a.plan = plan_tree(a.c, a.d, cache->dtype, room);
     if (a.plan.workgroups > INT32_MAX) return ATN_ERR_SIZE_OVERFLOW;
     if (workspace != nullptr && a.plan.scratch > room) return ATN_ERR_WORKSPACE;
     int dev;
     st = atn_host::device(&dev);
     if (st != ATN_OK) return st;
-    void* part;
-    st = scratch(a.plan.scratch, workspace, workspace_bytes, (hipStream_t)stream, &part);
+    void* ws;
+    st = scratch(a.plan.scratch, workspace, workspace_bytes, (hipStream_t)stream, &ws);
     if (st != ATN_OK) return st;
-    a.part = static_cast<float*>(part);
+    a.scores = static_cast<float*>(ws);
+    a.part = a.scores + a.plan.scores;
     return launched(atn::launch_tree_attention(cache->dtype, a, (hipStream_t)stream));
 }
 
@@ -291,14 +290,13 @@ int atn_cache_weigh_ex(const atn_kv_cache* cache, const atn_drafts* drafts, cons
     if (weight_in && weight_in != c.weight && meet(rw, range(weight_in, wb)))
         return ATN_ERR_ALIASING;
     float s = 0.f;
-    int rows = 0;
     st = check_scale(scale, c.D, &s);
-    if (st == ATN_OK) st = rows_bound(max_len, c.cap, &rows);
+    if (st == ATN_OK) st = bound_rows(max_len, &c);
     if (st != ATN_OK) return st;
     int dev;
     st = atn_host::device(&dev);
     if (st != ATN_OK) return st;
-    return launched(atn::launch_cache_weigh(cache->dtype, c, d, p, lse, weight_in, s, rows,
+    return launched(atn::launch_cache_weigh(cache->dtype, c, d, p, lse, weight_in, s,
                                             (hipStream_t)stream));
 }
 

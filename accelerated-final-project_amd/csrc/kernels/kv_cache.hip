@@ -281,7 +281,7 @@ hipError_t launch_cache_advance(const CacheView& c, int* len, const DraftView* d
 
 hipError_t launch_cache_weigh(int dtype, const CacheView& c, const DraftView& d,
                               const PathView& p, const float* lse, const float* weight_in,
-                              float scale, int, hipStream_t st) {
+                              float scale, hipStream_t st) {
     const dim3 grid((unsigned)((c.cap + 3) / 4), (unsigned)(c.B * c.G));
     if (dtype == kDtypeF32)
         hipLaunchKernelGGL(k_weigh<float>, grid, dim3(256), 0, st, c, d, p, lse, weight_in, scale);

@@ -24,6 +24,7 @@ struct CacheView {
     int* pos;              // [B][G][cap]
     int* seen;             // [B]
     int B, G, cap, D;
+    int rows;              // bound of len (the capacity, or less where the call says so)
 };
 
 // Drafted tokens: Q [batch][head][token][head_d], K and V [batch][kv head][token][head_d].
@@ -44,12 +45,17 @@ struct PathView {
     int n;
 };
 
+// How a call runs (tree_plan).  heads: (sequence, kv head) pairs of one pass; a call whose
+// scratch would pass its limit runs in several.
 struct TreePlan {
-    int nsplit;      // key splits
-    int row_tiles;   // tiles of query rows of one kv head
     int rows;        // query rows of a tile
+    int row_tiles;   // tiles of the query rows of one kv head
+    int nsplit;      // key splits, whose results k_tree_merge adds up
+    int heads;
+    int ld_scores;   // head_d > 256: row of the scores, floats
+    size_t scores;   // floats of the scores of a pass
     size_t scratch;  // bytes
-    int64_t workgroups;
+    int64_t workgroups;  // of a pass, at most
 };
 
 struct TreeArgs {
@@ -60,12 +66,14 @@ struct TreeArgs {
     float* lse;     // [B][H][T] or null
     float scale;    // times log2(e)
     TreePlan plan;
-    float* part;    // scratch
+    float* scores;  // scratch: [heads][row tiles of rows][ld_scores]
+    float* part;    // scratch: [heads][H / G * T][nsplit] statistics, then as many rows of D
+    int bg0, bgs;   // first pair of this pass, and pairs
 };
 
 // rows in use of sequence b, and its drafts
 __device__ __forceinline__ int rows_in_use(const CacheView& c, int b) {
-    return min(max(c.len[b], 0), c.cap);
+    return min(max(c.len[b], 0), c.rows);
 }
 __device__ __forceinline__ int drafts_of(const DraftView& d, int b) {
     return d.count ? min(max(d.count[b], 0), d.T) : d.T;
@@ -77,14 +85,15 @@ __device__ __forceinline__ bool sees(const DraftView& d, int b, int t, int j) {
 }
 
 // The plan depends on no device, so that workspace queries hold for any.
-TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, size_t scratch_cap);
-hipError_t launch_tree_attention(int dtype, const TreeArgs& a, hipStream_t st);
+TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bool draft_keys,
+                   size_t scratch_cap);
+hipError_t launch_tree_attention(int dtype, TreeArgs a, hipStream_t st);
 
 hipError_t launch_cache_commit(int dtype, const CacheView& c, const DraftView& d,
                                const PathView& p, hipStream_t st);
 hipError_t launch_cache_weigh(int dtype, const CacheView& c, const DraftView& d,
                               const PathView& p, const float* lse, const float* weight_in,
-                              float scale, int max_len, hipStream_t st);
+                              float scale, hipStream_t st);
 hipError_t launch_cache_advance(const CacheView& c, int* len, const DraftView* d,
                                 const PathView& p, int limit, hipStream_t st);
 size_t evict_scratch(int B, int G, int cap, int budget);

@@ -19,7 +19,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;
-constexpr int kStat = 3;  // floats of a row's statistics in a split
+constexpr int kTreeNarrow = 256;  // head_d up to which a wave holds a row tile's output
 constexpr float kLn2 = 0.69314718055994531f;
 
 // A row's scores lie in 4 lanes (L, L ^ 16, L ^ 32, L ^ 48): their maximum and sum.
@@ -44,7 +44,13 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // the reference point of exponentials for a maximum m: nothing seen yet counts from 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-// N = 16 / sizeof(T) elements of a row whose `left` elements are valid
+// two values as bf16, rounded to nearest even
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f32x2 x = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+}
+
+// BYTES / sizeof(T) elements of a row whose `left` elements are valid
 // (EXACT: all of them), zeros past those.  Rows need only element alignment.
 template <typename T, int BYTES>
 struct Words {
@@ -175,38 +181,63 @@ struct Narrow {
         }
     }
 
+    // bf16: O^T += V^T P^T with the weights' operands in registers
+    static __device__ __forceinline__ void products(v4f (&o)[MT][VS][VL], const Vals& v,
+                                                    const KPiece (&f)[MT]) {
+#pragma unroll
+        for (int i = 0; i < VS; ++i)
+#pragma unroll
+            for (int c = 0; c < VL; ++c) {
+                KPiece a;
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    a.w[h] = __builtin_amdgcn_perm(v.p[2 * h + 1][i].w[c / 2],
+                                                   v.p[2 * h][i].w[c / 2],
+                                                   (c & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    o[t][i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, f[t]), o[t][i][c],
+                        0, 0, 0);
+            }
+    }
+
+    // O^T += V^T P^T with the weights in LDS, rows of ld elements: operands of the keys of load_v
+    static __device__ __forceinline__ void accumulate_lds(v4f (&o)[MT][VS][VL], const Vals& v,
+                                                          const T* p, int ld, int lane) {
+        float w[MT][SUB][4];
+        KPiece f[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const T* at = p + (16 * t + (lane & 15)) * ld + 4 * (lane >> 4);
+            if constexpr (kBf) {
+                const uint2 lo = *reinterpret_cast<const uint2*>(at);
+                const uint2 hi = *reinterpret_cast<const uint2*>(at + 16);
+                f[t].w[0] = lo.x, f[t].w[1] = lo.y, f[t].w[2] = hi.x, f[t].w[3] = hi.y;
+            } else {
+                const float4 x = *reinterpret_cast<const float4*>(at);
+                w[t][0][0] = x.x, w[t][0][1] = x.y, w[t][0][2] = x.z, w[t][0][3] = x.w;
+            }
+        }
+        if constexpr (kBf)
+            products(o, v, f);
+        else
+            accumulate(o, v, w);
+    }
+
     // O^T += V^T P^T for all tiles
     static __device__ __forceinline__ void accumulate(v4f (&o)[MT][VS][VL], const Vals& v,
                                                       const float (&p)[MT][SUB][4]) {
         if constexpr (kBf) {
-            bf16x8 pf[MT];
+            // the weights as bf16, half a step (2^-8 of their size) off at most: V's own
+            // precision, and what lets one MFMA take both
+            KPiece f[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                Words<T, 16> w;
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    // the weights as bf16, half a step (2^-9 of their size) off: V's own
-                    // precision, and what lets one MFMA take both
-                    const f32x2 x = {p[t][h >> 1][2 * (h & 1)], p[t][h >> 1][2 * (h & 1) + 1]};
-                    w.w[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
-                }
-                pf[t] = __builtin_bit_cast(bf16x8, w);
-            }
-#pragma unroll
-            for (int i = 0; i < VS; ++i)
-#pragma unroll
-                for (int c = 0; c < VL; ++c) {
-                    Words<T, 16> a;
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
-                        a.w[h] = __builtin_amdgcn_perm(v.p[2 * h + 1][i].w[c / 2],
-                                                       v.p[2 * h][i].w[c / 2],
-                                                       (c & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t)
-                        o[t][i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(bf16x8, a), pf[t], o[t][i][c], 0, 0, 0);
-                }
+                for (int h = 0; h < 4; ++h)
+                    f[t].w[h] = pack2(p[t][h >> 1][2 * (h & 1)], p[t][h >> 1][2 * (h & 1) + 1]);
+            products(o, v, f);
         } else {
 #pragma unroll
             for (int i = 0; i < VS; ++i)
@@ -257,7 +288,41 @@ __device__ __forceinline__ float not_finite_sum(const TreeArgs& a, int b, int g,
     return sum;
 }
 
-// Keys [0, 32 n) of the cache, then the drafts in blocks of their own: where
+// A row's results in a split: maximum and sum, then, behind all of these, the dims.
+__device__ __forceinline__ float2* stats_of(const TreeArgs& a) {
+    return reinterpret_cast<float2*>(a.part);
+}
+__device__ __forceinline__ float* parts_of(const TreeArgs& a) {
+    return a.part + 2 * (size_t)a.plan.heads * (a.d.H / a.c.G) * a.d.T * a.plan.nsplit;
+}
+
+// not_finite_sum() added to dims [d0, d1) of a row where its result lies (a wave's work, after
+// the wave has written it): the output, or the split's part.
+template <typename T>
+__device__ void add_not_finite(const TreeArgs& a, int bg, int row, int split, int n, int d0, int d1,
+                               int lane) {
+    const int g = bg % a.c.G, b = bg / a.c.G, rep = a.d.H / a.c.G;
+    const int tok = row % a.d.T;
+    if (row >= rep * a.d.T || tok >= n) return;
+    T* out = (T*)a.out + b * a.os[0] + (g * rep + row / a.d.T) * a.os[1] + tok * a.os[2];
+    float* part =
+        parts_of(a) + (((size_t)(bg - a.bg0) * rep * a.d.T + row) * a.plan.nsplit + split) * a.c.D;
+    for (int d = d0 + lane; d < d1; d += 64) {
+        const float x = not_finite_sum<T>(a, b, g, n, tok, d);
+        if (x == 0.f) continue;
+        if (a.plan.nsplit > 1)
+            part[d] += x;
+        else
+            Elem<T>::st(out, d, Elem<T>::ld(out, d) + x);
+    }
+}
+
+// Blocks of a split: whole turns of a workgroup's waves, so that every split but the last is full.
+__device__ __forceinline__ int split_blocks(int all, int nsplit) {
+    return ((all + nsplit - 1) / nsplit + kWaves - 1) / kWaves * kWaves;
+}
+
+// The cache's keys in blocks, then the drafts in blocks of their own: where
 // a split's blocks lie.
 struct Blocks {
     int cache, all;    // blocks of the cache, and with the drafts'
@@ -268,11 +333,19 @@ __device__ __forceinline__ Blocks blocks_of(const TreeArgs& a, int L, int n, int
     Blocks x;
     x.cache = (L + KB - 1) / KB;
     x.all = x.cache + (a.d.K ? (n + KB - 1) / KB : 0);
-    // whole turns of the workgroup's waves, so that every split but the last is full
-    const int per = ((x.all + a.plan.nsplit - 1) / a.plan.nsplit + kWaves - 1) / kWaves * kWaves;
+    const int per = split_blocks(x.all, a.plan.nsplit);
     x.first = min(split * per, x.all);
     x.last = min(x.first + per, x.all);
     return x;
+}
+
+// Workgroup -> (unit of keys, tile of it): workgroups go to the 8 XCDs in turn, so the tiles
+// that read the same keys are 8 apart and share an L2.
+__device__ __forceinline__ void tile_of(int id, int units, int tiles, int* unit, int* tile) {
+    const int full = units / 8 * 8 * tiles, whole = id < full;
+    const int x = whole ? id % 8 : 0, y = whole ? id / 8 : id - full;
+    *tile = y % tiles;
+    *unit = whole ? y / tiles * 8 + x : units / 8 * 8 + y / tiles;
 }
 
 template <typename T, int DP, int MT, bool EXACT>
@@ -283,20 +356,10 @@ k_tree_narrow(TreeArgs a) {
     __shared__ __align__(16) char lds[N::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
-    // workgroups go to the 8 XCDs in turn: the row tiles that read the same keys are 8 apart
     const int tiles = a.plan.row_tiles, nsplit = a.plan.nsplit;
-    const int units = a.c.B * a.c.G * nsplit, full = units / 8 * 8 * tiles;
     int unit, tile;
-    if ((int)blockIdx.x < full) {
-        const int x = blockIdx.x % 8, y = blockIdx.x / 8;
-        tile = y % tiles;
-        unit = y / tiles * 8 + x;
-    } else {
-        const int y = blockIdx.x - full;
-        tile = y % tiles;
-        unit = units / 8 * 8 + y / tiles;
-    }
-    const int split = unit % nsplit, bg = unit / nsplit, g = bg % a.c.G, b = bg / a.c.G;
+    tile_of(blockIdx.x, a.bgs * nsplit, tiles, &unit, &tile);
+    const int split = unit % nsplit, bg = a.bg0 + unit / nsplit, g = bg % a.c.G, b = bg / a.c.G;
     const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), D = a.c.D;
     const int rep = a.d.H / a.c.G, R = rep * a.d.T;
     const Blocks blk = blocks_of<KB>(a, L, n, split);
@@ -494,17 +557,10 @@ k_tree_narrow(TreeArgs a) {
         const int row = tile * N::ROWS + 16 * t + col;
         const int h = g * rep + row / a.d.T, tok = row % a.d.T;
         if (row >= R || tok >= n) continue;
-        const size_t at = ((size_t)b * a.d.H + h) * a.d.T + tok;
+        const size_t at = (size_t)(bg - a.bg0) * R + row;
         if (nsplit > 1) {
-            float* to = a.part + (at * nsplit + split) * D;
-            // behind the parts: maximum, sum and whether infinities or NaNs were left out
-            float* st = a.part + (size_t)a.c.B * a.d.H * a.d.T * nsplit * D +
-                        (at * nsplit + split) * kStat;
-            if (q == 0) {
-                st[0] = m[t];
-                st[1] = l[t];
-                st[2] = odd ? 1.f : 0.f;
-            }
+            float* to = parts_of(a) + (at * nsplit + split) * D;
+            if (q == 0) stats_of(a)[at * nsplit + split] = make_float2(m[t], l[t]);
 #pragma unroll
             for (int x = 0; x < VS; ++x)
 #pragma unroll
@@ -519,7 +575,7 @@ k_tree_narrow(TreeArgs a) {
             // (l == 0: nothing visible, or no score above -infinity)
             const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
             if (q == 0 && a.lse)
-                a.lse[at] = l[t] == 0.f ? -INFINITY : (m[t] + log2f(l[t])) * kLn2;
+                a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] = l[t] == 0.f ? -INFINITY : (m[t] + log2f(l[t])) * kLn2;
 #pragma unroll
             for (int x = 0; x < VS; ++x)
 #pragma unroll
@@ -531,17 +587,263 @@ k_tree_narrow(TreeArgs a) {
                     }
         }
     }
-    if (nsplit == 1 && __builtin_amdgcn_ballot_w64(odd)) {
+    if (__builtin_amdgcn_ballot_w64(odd)) {
         __threadfence_block();  // (this wave's own stores, from other lanes)
-        for (int r = 0; r < N::ROWS; ++r) {
-            const int row = tile * N::ROWS + r, tok = row % a.d.T;
-            if (row >= R || tok >= n) continue;
-            T* to = (T*)a.out + b * a.os[0] + (g * rep + row / a.d.T) * a.os[1] + tok * a.os[2];
-            for (int d = lane; d < D; d += 64) {
-                const float x = not_finite_sum<T>(a, b, g, n, tok, d);
-                if (x != 0.f) Elem<T>::st(to, d, Elem<T>::ld(to, d) + x);
+        for (int r = 0; r < N::ROWS; ++r)
+            add_not_finite<T>(a, bg, tile * N::ROWS + r, split, n, 0, D, lane);
+    }
+}
+
+// ---------------------------------------------------------------- head_d > 256
+// No output tile fits a wave's registers, so two kernels with the scores between them:
+// k_tree_scores writes x (rows of R floats, small beside K and V's rows of head_d), each
+// workgroup's 8 waves sharing a tile's dims and adding up through LDS; k_tree_values is the
+// softmax over them and the product with V, each wave 16 VL dims of the output.
+// Keys lie in blocks of 32: the cache's, then the drafts'.
+constexpr int kBlock = 32;
+constexpr int kScoreWaves = 8;
+constexpr int kValueKeys = 128;  // keys between barriers of k_tree_values
+
+template <typename T, int MT, bool EXACT>
+__global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
+    using N = Narrow<T, 64, MT, EXACT>;
+    constexpr int EL = N::EL, STEP = 4 * EL, U = 4, SUB = kBlock / 16;
+    __shared__ v4f red[kScoreWaves][MT * SUB * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q = lane >> 4, col = lane & 15;
+    const int tiles = a.plan.row_tiles, most = a.plan.ld_scores / kBlock;
+    int unit, tile;
+    tile_of(blockIdx.x, a.bgs * most, tiles, &unit, &tile);
+    const int i = unit % most, bgl = unit / most, bg = a.bg0 + bgl, g = bg % a.c.G, b = bg / a.c.G;
+    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), D = a.c.D;
+    const int cache = (L + kBlock - 1) / kBlock;
+    const int all = cache + (a.d.K ? (n + kBlock - 1) / kBlock : 0);
+    if (i >= all) return;
+    const bool in = i < cache;
+    const int j0 = (in ? i : i - cache) * kBlock, rows = min(kBlock, (in ? L : n) - j0);
+    const int rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const T* kp[SUB];
+    const T* qp[MT];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+        const int64_t r = j0 + min(16 * u + col, rows - 1);
+        kp[u] = (in ? (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1] + r * a.c.ks[2]
+                    : (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1] + r * a.d.ks[2]) +
+                EL * q;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {  // (rows past R: the last one's scores, which nobody reads)
+        const int row = min((tile * MT + t) * 16 + col, R - 1);
+        qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + (g * rep + row / a.d.T) * a.d.qs[1] +
+                (row % a.d.T) * a.d.qs[2] + EL * q;
+    }
+    v4f s[MT][SUB];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
+    // each wave a run of whole U-step pieces
+    const int per = ((D + STEP * U - 1) / (STEP * U) + kScoreWaves - 1) / kScoreWaves * STEP * U;
+    const int d1 = min(D, (wave + 1) * per);
+    for (int d = wave * per; d < d1; d += STEP * U) {
+        typename N::KPiece k[U][SUB], f[U][MT];
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+            const int at = d + STEP * e, left = D - at - EL * q;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) k[e][u] = ld_words<EXACT, 16>(kp[u] + at, left);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) f[e][t] = ld_words<EXACT, 16>(qp[t] + at, left);
+        }
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) s[t][u] = N::dot(k[e][u], f[e][t], s[t][u]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) red[wave][(t * SUB + u) * 64 + lane] = s[t][u];
+    __syncthreads();
+    // one thread per row and 4 keys
+    if (threadIdx.x >= MT * SUB * 64) return;
+    const int u = (threadIdx.x >> 6) % SUB, t = (threadIdx.x >> 6) / SUB;
+    v4f x = red[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < kScoreWaves; ++w) x += red[w][threadIdx.x];
+    const int row = (tile * MT + t) * 16 + col, tok = row % a.d.T, k0 = 16 * u + 4 * q;
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const bool on = k0 + e < rows && row < R && (in || sees(a.d, b, tok, j0 + k0 + e));
+        y[e] = on ? x[e] * a.scale : -INFINITY;
+    }
+    float* to = a.scores + ((size_t)bgl * tiles * N::ROWS + row) * a.plan.ld_scores + i * kBlock + k0;
+    *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+}
+
+template <typename T, int MT, bool EXACT>
+__global__ __launch_bounds__(64 * kWaves) void k_tree_values(TreeArgs a) {
+    constexpr bool kBf = sizeof(T) == 2;
+    // (a wave's dims: one V step of 128 in bf16, 64 in fp32)
+    using N = Narrow<T, kBf ? 128 : 64, MT, EXACT>;
+    constexpr int VL = N::VL, WD = N::VD, ROWS = N::ROWS, PK = N::KB;
+    constexpr int LDP = kValueKeys + 16 / (int)sizeof(T);
+    __shared__ __align__(16) T pl[2][ROWS * LDP];
+    __shared__ float alpha[2][ROWS];
+    __shared__ float2 fin[ROWS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q = lane >> 4, col = lane & 15;
+    const int D = a.c.D, groups = (D + WD * kWaves - 1) / (WD * kWaves);
+    const int tiles = a.plan.row_tiles, nsplit = a.plan.nsplit;
+    int unit, tile;
+    tile_of(blockIdx.x, a.bgs * nsplit * groups, tiles, &unit, &tile);
+    const int split = unit / groups % nsplit, bgl = unit / groups / nsplit, bg = a.bg0 + bgl;
+    const int d0 = (unit % groups * kWaves + wave) * WD;
+    const int g = bg % a.c.G, b = bg / a.c.G;
+    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
+    const int rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const int cache = (L + kBlock - 1) / kBlock;
+    const int all = cache + (a.d.K ? (n + kBlock - 1) / kBlock : 0);
+    const int per = split_blocks(all, nsplit);
+    const int first = min(split * per, all), last = min(first + per, all);
+    if (first >= last && split > 0) return;
+    const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1] + d0;
+    const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d0;
+    const float* sc = a.scores + ((size_t)bgl * tiles + tile) * ROWS * a.plan.ld_scores;
+
+    // softmax: 16 threads a row, 8 keys each, one pass per 16 rows
+    const int sr = threadIdx.x >> 4, sk = (threadIdx.x & 15) * 8;
+    float m[MT], l[MT];
+    v4f o[MT][1][VL];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int c = 0; c < VL; ++c) o[t][0][c] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    bool odd = false;
+    int buf = 0;
+    for (int i0 = first; i0 < last; i0 += kValueKeys / kBlock, buf ^= 1) {
+        const int k1 = (last - i0) * kBlock;  // scores of this step
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            float x[8];
+            const float* from = sc + (size_t)(16 * t + sr) * a.plan.ld_scores + i0 * kBlock + sk;
+            if (sk < k1) {
+                const float4 u = *reinterpret_cast<const float4*>(from);
+                const float4 w = *reinterpret_cast<const float4*>(from + 4);
+                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+                x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = -INFINITY;
+            }
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
+            top = fmaxf(top, dpp<kDppQuadXor1>(top));
+            top = fmaxf(top, dpp<kDppQuadXor2>(top));
+            top = fmaxf(top, dpp<kDppRowHalfMirror>(top));
+            top = fmaxf(top, dpp<kDppRowMirror>(top));
+            const float m_new = fmaxf(m[t], top), base = base_of(m_new);
+            const float f = exp2_(m[t] - base);
+            m[t] = m_new;
+            l[t] *= f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = exp2_(x[e] - base);
+                l[t] += x[e];
+            }
+            if ((threadIdx.x & 15) == 0) alpha[buf][16 * t + sr] = f;
+            T* to = pl[buf] + (16 * t + sr) * LDP + sk;
+            if constexpr (kBf) {
+                // (weights as bf16: see Narrow::accumulate)
+                uint4 w;
+                w.x = pack2(x[0], x[1]), w.y = pack2(x[2], x[3]);
+                w.z = pack2(x[4], x[5]), w.w = pack2(x[6], x[7]);
+                *reinterpret_cast<uint4*>(to) = w;
+            } else {
+                *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
             }
         }
+        // (two buffers: a wave past this barrier writes the other one, and comes to write this
+        // one only after the next barrier, when every wave has read it)
+        __syncthreads();
+        if (d0 >= D) continue;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float f = alpha[buf][16 * t + col];
+            if (__builtin_amdgcn_ballot_w64(f != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < VL; ++c) o[t][0][c] *= f;
+            }
+        }
+        for (int k = 0; k < kValueKeys && k < k1; k += PK) {
+            const int i = i0 + k / kBlock, sub = k % kBlock;
+            const bool in = i < cache;
+            const int j0 = (in ? i : i - cache) * kBlock + sub;
+            const int rows = min(PK, (in ? L : n) - j0);
+            if (rows <= 0) continue;  // (fp32: the second half of a last block)
+            typename N::Vals v;
+            const int64_t s = in ? a.c.vs[2] : a.d.vs[2];
+            N::load_v(v, (in ? vc : vd) + j0 * s, s, rows, D - d0, lane);
+            if (!in) odd |= clear_not_finite<T>(v);
+            N::accumulate_lds(o, v, pl[buf] + k, LDP, lane);
+        }
+    }
+    // sums of the rows, for the waves that hold their outputs
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        float x = l[t];
+        x += dpp<kDppQuadXor1>(x);
+        x += dpp<kDppQuadXor2>(x);
+        x += dpp<kDppRowHalfMirror>(x);
+        x += dpp<kDppRowMirror>(x);
+        if ((threadIdx.x & 15) == 0) fin[16 * t + sr] = make_float2(m[t], x);
+    }
+    __syncthreads();
+    if (d0 >= D) return;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int row = tile * ROWS + 16 * t + col, tok = row % a.d.T, h = g * rep + row / a.d.T;
+        if (row >= R || tok >= n) continue;
+        const float2 z = fin[16 * t + col];
+        const size_t at = (size_t)bgl * R + row;
+        const bool teller = q == 0 && d0 == 0;
+        if (nsplit > 1) {
+            float* to = parts_of(a) + (at * nsplit + split) * D + d0;
+            if (teller) stats_of(a)[at * nsplit + split] = z;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < VL; ++c) {
+                    const int d = N::RUN * q + VL * e + c;
+                    if (EXACT || d0 + d < D) to[d] = o[t][0][c][e];
+                }
+        } else {
+            T* to = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2] + d0;
+            const float inv = z.y == 0.f ? 0.f : 1.f / z.y;
+            if (teller && a.lse)
+                a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
+                    z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < VL; ++c) {
+                    const int d = N::RUN * q + VL * e + c;
+                    if (EXACT || d0 + d < D) Elem<T>::st(to, d, o[t][0][c][e] * inv);
+                }
+        }
+    }
+    if (odd) {
+        __threadfence_block();
+        for (int r = 0; r < ROWS; ++r)
+            add_not_finite<T>(a, bg, tile * ROWS + r, split, n, d0, min(D, d0 + WD), lane);
     }
 }
 
@@ -549,124 +851,40 @@ k_tree_narrow(TreeArgs a) {
 // The splits of a row added up: one workgroup per (row, 256 dims).
 template <typename T>
 __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb) {
-    const int D = a.c.D, chunks = (D + 255) / 256;
+    const int D = a.c.D, chunks = (D + 255) / 256, rep = a.d.H / a.c.G, R = rep * a.d.T;
     const size_t at = blockIdx.x / chunks;
     const int d = (blockIdx.x % chunks) * 256 + threadIdx.x;
-    const int tok = at % a.d.T, h = (at / a.d.T) % a.d.H, b = at / a.d.T / a.d.H;
+    const int row = at % R, bg = a.bg0 + (int)(at / R), g = bg % a.c.G, b = bg / a.c.G;
+    const int tok = row % a.d.T, h = g * rep + row / a.d.T;
     const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), nsplit = a.plan.nsplit;
     if (tok >= n) return;
-    int used = 1;
-    {
-        const int all = (L + kb - 1) / kb + (a.d.K ? (n + kb - 1) / kb : 0);
-        const int per = ((all + nsplit - 1) / nsplit + kWaves - 1) / kWaves * kWaves;
-        if (all > 0) used = (all + per - 1) / per;
-    }
-    const float* st = a.part + (size_t)a.c.B * a.d.H * a.d.T * nsplit * D + at * nsplit * kStat;
-    const float* part = a.part + at * nsplit * D;
+    const int all = (L + kb - 1) / kb + (a.d.K ? (n + kb - 1) / kb : 0);
+    const int per = split_blocks(all, nsplit), used = all > 0 ? (all + per - 1) / per : 1;
+    const float2* st = stats_of(a) + at * nsplit;
+    const float* part = parts_of(a) + at * nsplit * D;
     float M = -INFINITY, l = 0.f, acc = 0.f;
-    bool odd = false;
-    for (int s = 0; s < used; ++s) M = fmaxf(M, st[s * kStat]);
+    for (int s = 0; s < used; ++s) M = fmaxf(M, st[s].x);
     const float base = base_of(M);
 #pragma unroll 4
     for (int s = 0; s < used; ++s) {
-        const float f = exp2_(st[s * kStat] - base);
-        l += f * st[s * kStat + 1];
-        odd |= st[s * kStat + 2] != 0.f;
-        if (d < D) acc += f * part[(size_t)s * D + d];
+        const float f = exp2_(st[s].x - base);
+        l += f * st[s].y;
+        if (d < D) {
+            const float x = part[(size_t)s * D + d];
+            // (infinity times a weight too small for fp32 stays infinity)
+            acc += f == 0.f && !(fabsf(x) < INFINITY) ? x : f * x;
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (d < D) {
-        float x = acc * inv;
-        if (odd) x += not_finite_sum<T>(a, b, h / (a.d.H / a.c.G), n, tok, d);
-        Elem<T>::st((T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2], d, x);
-    }
-    if (d == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (M + log2f(l)) * kLn2;
-}
-
-// ---------------------------------------------------------------- head_d > 256
-// One workgroup per row: keys in blocks of 256 (a wave per key, lanes over
-// the dims), the running maximum and sum in fp32, the output's dims in
-// registers (32 per thread at head_d 8192).
-constexpr int kDimsPerThread = 32;
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_tree_rows(TreeArgs a) {
-    __shared__ float p[256];
-    __shared__ float red[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t = blockIdx.x % a.d.T, h = (blockIdx.x / a.d.T) % a.d.H;
-    const int b = blockIdx.x / (a.d.T * a.d.H), g = h / (a.d.H / a.c.G);
-    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), D = a.c.D;
-    if (t >= n) return;
-    const T* q = (const T*)a.d.Q + b * a.d.qs[0] + h * a.d.qs[1] + t * a.d.qs[2];
-    const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
-    const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1];
-    const T* kd = (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
-    const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
-    const int keys = L + (a.d.K ? n : 0);
-    float m = -INFINITY, l = 0.f, acc[kDimsPerThread];
-#pragma unroll
-    for (int i = 0; i < kDimsPerThread; ++i) acc[i] = 0.f;
-    for (int k0 = 0; k0 < keys; k0 += 256) {
-        const int nk = min(256, keys - k0);
-        for (int i = wave; i < nk; i += 4) {
-            const int j = k0 + i;
-            float s = -INFINITY;
-            if (j < L || sees(a.d, b, t, j - L)) {
-                const T* k = j < L ? kc + j * a.c.ks[2] : kd + (j - L) * a.d.ks[2];
-                float x = 0.f;
-                for (int d = lane; d < D; d += 64) x = fmaf(Elem<T>::ld(q, d), Elem<T>::ld(k, d), x);
-                s = wave_sum(x) * a.scale;
-            }
-            if (lane == 0) p[i] = s;
-        }
-        __syncthreads();
-        const float s = threadIdx.x < nk ? p[threadIdx.x] : -INFINITY;
-        const float wm = wave_max(s);
-        if (lane == 0) red[wave] = wm;
-        __syncthreads();
-        const float m_new = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        // no key seen so far: nothing to scale, and no key of this block counts
-        const float base = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = m == -INFINITY ? 0.f : exp2f(m - base);
-        const float e = exp2f(s - base);
-        const float ws = wave_sum(e);
-        __syncthreads();
-        if (lane == 0) red[wave] = ws;
-        if (threadIdx.x < nk) p[threadIdx.x] = e;
-        __syncthreads();
-        l = l * alpha + (red[0] + red[1]) + (red[2] + red[3]);
-        m = m_new;
-#pragma unroll
-        for (int i = 0; i < kDimsPerThread; ++i) acc[i] *= alpha;
-        for (int i = 0; i < nk; ++i) {
-            const int j = k0 + i;
-            if (j >= L && !sees(a.d, b, t, j - L)) continue;  // its V may be anything
-            const T* v = j < L ? vc + j * a.c.vs[2] : vd + (j - L) * a.d.vs[2];
-#pragma unroll
-            for (int c = 0; c < kDimsPerThread; ++c) {
-                const int d = threadIdx.x + 256 * c;
-                if (d < D) acc[c] = fmaf(p[i], Elem<T>::ld(v, d), acc[c]);
-            }
-        }
-        __syncthreads();
-    }
-    T* o = (T*)a.out + b * a.os[0] + h * a.os[1] + t * a.os[2];
-    // (l == 0: nothing visible, or no score above -infinity)
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int c = 0; c < kDimsPerThread; ++c) {
-        const int d = threadIdx.x + 256 * c;
-        if (d < D) Elem<T>::st(o, d, l == 0.f ? 0.f : acc[c] * inv);
-    }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[((size_t)b * a.d.H + h) * a.d.T + t] =
-            l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (d < D) Elem<T>::st((T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2], d, acc * inv);
+    if (d == 0 && a.lse)
+        a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
+            l == 0.f ? -INFINITY : (M + log2f(l)) * kLn2;
 }
 
 template <typename T, int DP, int MT>
 void go_narrow(const TreeArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)a.plan.workgroups);
+    const dim3 grid((unsigned)(a.bgs * a.plan.row_tiles * a.plan.nsplit));
     if (a.c.D == DP)
         hipLaunchKernelGGL((k_tree_narrow<T, DP, MT, true>), grid, dim3(64 * kWaves), 0, st, a);
     else
@@ -676,55 +894,107 @@ void go_narrow(const TreeArgs& a, hipStream_t st) {
 template <typename T, int DP>
 void go_rows(const TreeArgs& a, hipStream_t st) {
     if (a.plan.rows == 16) return go_narrow<T, DP, 1>(a, st);
-    if (a.plan.rows == 32 || DP > 128 || sizeof(T) == 4) return go_narrow<T, DP, 2>(a, st);
+    if (a.plan.rows == 32) return go_narrow<T, DP, 2>(a, st);
     if constexpr (DP <= 128 && sizeof(T) == 2) go_narrow<T, DP, 4>(a, st);
+}
+
+template <typename T>
+constexpr int kWideDims = (sizeof(T) == 2 ? 128 : 64) * kWaves;  // dims of a value workgroup
+
+template <typename T, int MT, bool EXACT>
+void go_wide(const TreeArgs& a, hipStream_t st) {
+    const int tiles = a.bgs * a.plan.row_tiles;
+    hipLaunchKernelGGL((k_tree_scores<T, MT, EXACT>),
+                       dim3((unsigned)(tiles * (a.plan.ld_scores / kBlock))),
+                       dim3(64 * kScoreWaves), 0, st, a);
+    const int groups = (a.c.D + kWideDims<T> - 1) / kWideDims<T>;
+    hipLaunchKernelGGL((k_tree_values<T, MT, EXACT>), dim3((unsigned)(tiles * a.plan.nsplit * groups)),
+                       dim3(64 * kWaves), 0, st, a);
+}
+
+template <typename T, int MT>
+void go_wide(const TreeArgs& a, hipStream_t st) {
+    // (exact: a wave's steps over the dims all lie inside the row)
+    if (a.c.D % 128 == 0) return go_wide<T, MT, true>(a, st);
+    go_wide<T, MT, false>(a, st);
 }
 
 template <typename T>
 void go(const TreeArgs& a, hipStream_t st) {
     const int D = a.c.D;
-    if (D > 256) {
-        hipLaunchKernelGGL(k_tree_rows<T>, dim3((unsigned)a.plan.workgroups), dim3(256), 0, st, a);
-        return;
+    if (D > kTreeNarrow) {
+        if (a.plan.rows == 16) go_wide<T, 1>(a, st);
+        else if (a.plan.rows == 32) go_wide<T, 2>(a, st);
+        else go_wide<T, 4>(a, st);
+    } else if (D <= 64) {
+        go_rows<T, 64>(a, st);
+    } else if (D <= 128) {
+        go_rows<T, 128>(a, st);
+    } else if (D <= 192) {
+        go_rows<T, 192>(a, st);
+    } else {
+        go_rows<T, 256>(a, st);
     }
-    if (D <= 64) go_rows<T, 64>(a, st);
-    else if (D <= 128) go_rows<T, 128>(a, st);
-    else if (D <= 192) go_rows<T, 192>(a, st);
-    else go_rows<T, 256>(a, st);
-    if (a.plan.nsplit > 1)
-        hipLaunchKernelGGL(k_tree_merge<T>,
-                           dim3((unsigned)((size_t)a.c.B * a.d.H * a.d.T * ((D + 255) / 256))),
-                           dim3(256), 0, st, a, sizeof(T) == 2 ? 32 : 16);
+    if (a.plan.nsplit > 1) {
+        const int kb = D > kTreeNarrow || sizeof(T) == 2 ? 32 : 16;
+        hipLaunchKernelGGL(
+            k_tree_merge<T>,
+            dim3((unsigned)((size_t)a.bgs * (a.d.H / a.c.G) * a.d.T * ((D + 255) / 256))), dim3(256),
+            0, st, a, kb);
+    }
 }
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 }  // namespace
 
-TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, size_t scratch_cap) {
+TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bool draft_keys,
+                   size_t scratch_cap) {
     TreePlan p{};
-    if (D > 256) return TreePlan{1, 1, 1, 0, (int64_t)B * H * T};
+    const bool bf = dtype == kDtypeBF16, wide = D > kTreeNarrow;
     const int R = H / G * T;
-    const int most = dtype == kDtypeBF16 && D <= 128 ? 64 : 32;
+    const int most = wide || (bf && D <= 128) ? 64 : 32;
     p.rows = R <= 16 ? 16 : R <= 32 ? 32 : most;
-    p.row_tiles = (R + p.rows - 1) / p.rows;
-    const int kb = dtype == kDtypeBF16 ? 32 : 16;
-    const int64_t units = (int64_t)B * G * p.row_tiles;
-    // splits of at least two blocks a wave, and about three workgroups per CU
-    const int64_t blocks = (max_len + kb - 1) / kb + (T + kb - 1) / kb;
-    int64_t ns = std::min<int64_t>((768 + units - 1) / units, blocks / (2 * kWaves));
-    const size_t per = (size_t)B * H * T * (D + kStat) * sizeof(float);
-    if (ns > (int64_t)(scratch_cap / per)) ns = (int64_t)(scratch_cap / per);
-    p.nsplit = (int)std::max<int64_t>(1, ns);
-    p.scratch = p.nsplit > 1 ? per * p.nsplit : 0;
-    p.workgroups = units * p.nsplit;
+    p.row_tiles = ceil_div(R, p.rows);
+    const int kb = wide || bf ? 32 : 16;
+    const int64_t blocks = ceil_div(max_len, kb) + (draft_keys ? ceil_div(T, kb) : 0);
+    // workgroups of a pair without splits
+    const int groups = wide ? ceil_div(D, (bf ? 128 : 64) * kWaves) : 1;
+    const int64_t units = (int64_t)B * G * p.row_tiles * groups;
+    // splits of at least two blocks a wave (wide: two steps), and about three workgroups per CU
+    int64_t ns = std::max<int64_t>(1, std::min<int64_t>((768 + units - 1) / units,
+                                                        blocks / (2 * kWaves)));
+    p.ld_scores = wide ? (int)std::max<int64_t>(blocks, 1) * kBlock : 0;
+    const size_t sc = wide ? (size_t)p.row_tiles * p.rows * p.ld_scores : 0;  // floats of a pair
+    const size_t part = (size_t)R * (D + 2);                                   // ... and split
+    const size_t room = scratch_cap / sizeof(float);
+    // fewer splits where the scratch does not hold them, then fewer pairs at a time
+    auto need = [&](int64_t heads, int64_t n) { return heads * (sc + (n > 1 ? n * part : 0)); };
+    const int64_t pairs = (int64_t)B * G;
+    while (ns > 1 && need(pairs, ns) > room) --ns;
+    p.nsplit = (int)ns;
+    p.heads = (int)pairs;
+    if (need(pairs, ns) > room) p.heads = (int)std::max<size_t>(1, room / std::max<size_t>(sc, 1));
+    p.scores = sc * p.heads;
+    p.scratch = need(p.heads, ns) * sizeof(float);
+    const int64_t most_groups = wide ? std::max<int64_t>(groups * ns, p.ld_scores / kBlock) : ns;
+    p.workgroups = std::max((int64_t)p.heads * p.row_tiles * most_groups,
+                            (int64_t)p.heads * R * ceil_div(D, 256));
     return p;
 }
 
-hipError_t launch_tree_attention(int dtype, const TreeArgs& a, hipStream_t st) {
-    if (dtype == kDtypeF32)
-        go<float>(a, st);
-    else
-        go<uint16_t>(a, st);
-    return hipGetLastError();
+hipError_t launch_tree_attention(int dtype, TreeArgs a, hipStream_t st) {
+    const int pairs = a.c.B * a.c.G;
+    for (a.bg0 = 0; a.bg0 < pairs; a.bg0 += a.plan.heads) {
+        a.bgs = std::min(a.plan.heads, pairs - a.bg0);
+        if (dtype == kDtypeF32)
+            go<float>(a, st);
+        else
+            go<uint16_t>(a, st);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace atn

@@ -379,9 +379,9 @@ typedef struct atn_drafts {
  * [tokens] fp32, the natural log of the softmax's denominator (-infinity for such a
  * token).  Keys and values that a token does not attend do not reach its output,
  * whatever they hold.  out_stride: as atn_drafts.q_stride, of distinct elements;
- * NULL: contiguous.  max_len: an upper bound of len known on the host (0: the
- * capacity), for the choice of key splits alone: a smaller one is slower, not
- * wrong.  workspace as for atn_attention_fwd_ex (NULL: the stream's library
+ * NULL: contiguous.  max_len: an upper bound of len that the host knows (0: the
+ * capacity); the call is laid out for it, and rows from there on are not attended.
+ * workspace as for atn_attention_fwd_ex (NULL: the stream's library
  * workspace; else zero-filled once, at least
  * atn_tree_attention_workspace_bytes()). */
 int atn_tree_attention_ex(const atn_kv_cache *cache, const atn_drafts *drafts, void *out,
@@ -405,7 +405,8 @@ int atn_cache_commit_ex(const atn_kv_cache *cache, const atn_drafts *drafts, con
  *                     + sum over the group's heads h and path entries i with r <= len[b] + i
  *                       of exp(scale q . k_r - lse[b][h][path[b][i]]);
  * other rows stay.  lse: atn_tree_attention_ex's (entries of -infinity add
- * nothing).  weight_in: NULL for zeros; may be cache->weight. */
+ * nothing).  weight_in: NULL for zeros; may be cache->weight.  max_len: as for
+ * atn_tree_attention_ex. */
 int atn_cache_weigh_ex(const atn_kv_cache *cache, const atn_drafts *drafts, const float *lse,
                        const int32_t *path, const int32_t *accepted, int path_len,
                        const float *weight_in, float scale, int max_len, void *stream);

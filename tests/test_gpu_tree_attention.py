@@ -236,11 +236,11 @@ def test_lengths_out_of_range_are_clamped(am, dev):
 
 
 @pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f32", 128), ("bf16", 640)])
-def test_max_len_is_a_hint(am, dev, dtype, D):
+def test_max_len_bounds_the_lengths(am, dev, dtype, D):
     p = Problem(am, dtype, 2, 4, 2, 5, D, 1500, [1500, 700], mask="tree")
-    for max_len in (1, 100, 1500, 1 << 30):
+    for max_len in (1, 100, 701, 1499, 1500, 1 << 30):
         p.run(max_len=max_len)
-        p.check()
+        p.check(lens=[min(l, max_len) for l in p.lens])
 
 
 @pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f32", 96), ("bf16", 520)])
