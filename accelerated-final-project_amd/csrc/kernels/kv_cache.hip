@@ -1,6 +1,5 @@
 // The key/value cache of a decoding program: accepted drafts written into it,
-// the attention weight of its rows, eviction of the lightest ones, and its
-// lengths.
+// eviction of the lightest rows, and its lengths.
 #include <algorithm>
 
 #include "kv_cache.hpp"
@@ -8,32 +7,6 @@
 namespace atn {
 
 namespace {
-
-// Drafts of sequence b that become rows of its cache: the path's entries up
-// to the first that names no draft, as many as the cache still holds.  Every
-// lane of a full wave calls it and gets the count.
-__device__ __forceinline__ int rows_accepted(const CacheView& c, const DraftView& d,
-                                             const PathView& p, int b) {
-    const int n = drafts_of(d, b);
-    int a = p.accepted ? min(max(p.accepted[b], 0), p.n) : p.n;
-    if (!p.path) {
-        a = min(a, n);
-    } else {
-        for (int i0 = 0; i0 < a; i0 += 64) {
-            const int i = i0 + (int)(threadIdx.x & 63);
-            const int t = i < a ? p.path[(size_t)b * p.n + i] : 0;
-            const uint64_t bad = __builtin_amdgcn_ballot_w64(i < a && (t < 0 || t >= n));
-            if (bad) {
-                a = i0 + __builtin_ctzll(bad);
-                break;
-            }
-        }
-    }
-    return min(a, c.cap - rows_in_use(c, b));
-}
-__device__ __forceinline__ int path_at(const PathView& p, int b, int i) {
-    return p.path ? p.path[(size_t)b * p.n + i] : i;
-}
 
 // One row of D elements by one wave, `vec` elements (16 bytes) at a time
 // where both rows allow it.
@@ -79,34 +52,6 @@ __global__ __launch_bounds__(64) void k_advance(CacheView c, int* len, DraftView
         len[b] = limit > 0 ? min(L, limit) : L;
         if (c.seen && add) c.seen[b] += A;
     }
-}
-
-// weight[r] = weight_in[r] + sum over the accepted drafts i and the group's
-// heads of exp2(scale q . k_r - log2(e) lse), draft i seeing the rows in use
-// and the path up to itself (the row it was written to).  One wave per row.
-template <typename T>
-__global__ __launch_bounds__(256) void k_weigh(CacheView c, DraftView d, PathView p,
-                                               const float* __restrict__ lse,
-                                               const float* weight_in, float scale) {
-    const int lane = threadIdx.x & 63;
-    const int bg = blockIdx.y, g = bg % c.G, b = bg / c.G;
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int L = rows_in_use(c, b), A = rows_accepted(c, d, p, b), rep = d.H / c.G;
-    if (r >= L + A) return;
-    const T* k = (const T*)c.K + b * c.ks[0] + g * c.ks[1] + r * c.ks[2];
-    float w = 0.f;
-    for (int i = max(0, r - L); i < A; ++i) {
-        const int t = path_at(p, b, i);
-        for (int h = g * rep; h < (g + 1) * rep; ++h) {
-            const T* q = (const T*)d.Q + b * d.qs[0] + h * d.qs[1] + t * d.qs[2];
-            float x = 0.f;
-            for (int e = lane; e < c.D; e += 64) x = fmaf(Elem<T>::ld(q, e), Elem<T>::ld(k, e), x);
-            const float z = lse[((size_t)b * d.H + h) * d.T + t];
-            if (z != -INFINITY) w += exp2f(wave_sum(x) * scale - z * 1.4426950408889634f);
-        }
-    }
-    const size_t m = (size_t)bg * c.cap + r;
-    if (lane == 0) c.weight[m] = (weight_in ? weight_in[m] : 0.f) + w;
 }
 
 // ---------------------------------------------------------------- eviction
@@ -276,18 +221,6 @@ hipError_t launch_cache_advance(const CacheView& c, int* len, const DraftView* d
                                 const PathView& p, int limit, hipStream_t st) {
     hipLaunchKernelGGL(k_advance, dim3(c.B), dim3(64), 0, st, c, len, d ? *d : DraftView{}, p,
                        d != nullptr, limit);
-    return hipGetLastError();
-}
-
-hipError_t launch_cache_weigh(int dtype, const CacheView& c, const DraftView& d,
-                              const PathView& p, const float* lse, const float* weight_in,
-                              float scale, hipStream_t st) {
-    const dim3 grid((unsigned)((c.cap + 3) / 4), (unsigned)(c.B * c.G));
-    if (dtype == kDtypeF32)
-        hipLaunchKernelGGL(k_weigh<float>, grid, dim3(256), 0, st, c, d, p, lse, weight_in, scale);
-    else
-        hipLaunchKernelGGL(k_weigh<uint16_t>, grid, dim3(256), 0, st, c, d, p, lse, weight_in,
-                           scale);
     return hipGetLastError();
 }
 

@@ -45,6 +45,39 @@ struct PathView {
     int n;
 };
 
+// rows in use of sequence b, and its drafts
+__device__ __forceinline__ int rows_in_use(const CacheView& c, int b) {
+    return min(max(c.len[b], 0), c.rows);
+}
+__device__ __forceinline__ int drafts_of(const DraftView& d, int b) {
+    return d.count ? min(max(d.count[b], 0), d.T) : d.T;
+}
+// Drafts of sequence b that become rows of its cache: the path's entries up
+// to the first that names no draft, as many as the cache still holds.  Every
+// lane of a full wave calls it and gets the count.
+__device__ __forceinline__ int rows_accepted(const CacheView& c, const DraftView& d,
+                                             const PathView& p, int b) {
+    const int n = drafts_of(d, b);
+    int a = p.accepted ? min(max(p.accepted[b], 0), p.n) : p.n;
+    if (!p.path) {
+        a = min(a, n);
+    } else {
+        for (int i0 = 0; i0 < a; i0 += 64) {
+            const int i = i0 + (int)(threadIdx.x & 63);
+            const int t = i < a ? p.path[(size_t)b * p.n + i] : 0;
+            const uint64_t bad = __builtin_amdgcn_ballot_w64(i < a && (t < 0 || t >= n));
+            if (bad) {
+                a = i0 + __builtin_ctzll(bad);
+                break;
+            }
+        }
+    }
+    return min(a, c.cap - min(max(c.len[b], 0), c.cap));
+}
+__device__ __forceinline__ int path_at(const PathView& p, int b, int i) {
+    return p.path ? p.path[(size_t)b * p.n + i] : i;
+}
+
 // How a call runs (tree_plan).  heads: (sequence, kv head) pairs of one pass; a call whose
 // scratch would pass its limit runs in several.
 struct TreePlan {
@@ -71,13 +104,6 @@ struct TreeArgs {
     int bg0, bgs;   // first pair of this pass, and pairs
 };
 
-// rows in use of sequence b, and its drafts
-__device__ __forceinline__ int rows_in_use(const CacheView& c, int b) {
-    return min(max(c.len[b], 0), c.rows);
-}
-__device__ __forceinline__ int drafts_of(const DraftView& d, int b) {
-    return d.count ? min(max(d.count[b], 0), d.T) : d.T;
-}
 // Whether draft t of sequence b (of n drafts) attends draft j.
 __device__ __forceinline__ bool sees(const DraftView& d, int b, int t, int j) {
     if (!d.mask) return j <= t;
