@@ -148,7 +148,7 @@ int check_scale(float scale, int D, float* out) {
     if (!std::isfinite(scale)) return ATN_ERR_BAD_ARGUMENT;
     if (scale == 0.f) scale = 1.f / std::sqrt((float)D);
     *out = scale * 1.4426950408889634f;
-    return std::isfinite(*out) ? ATN_OK : ATN_ERR_BAD_ARGUMENT;
+    return std::isnormal(*out) ? ATN_OK : ATN_ERR_BAD_ARGUMENT;
 }
 
 // lengths count up to max_len (0: the capacity)

@@ -29,6 +29,14 @@ __device__ __forceinline__ float row_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// the sum over a row of 16 lanes
+__device__ __forceinline__ float row16_sum(float x) {
+    x += dpp<kDppQuadXor1>(x);
+    x += dpp<kDppQuadXor2>(x);
+    x += dpp<kDppRowHalfMirror>(x);
+    return x + dpp<kDppRowMirror>(x);
+}
+
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // the reference point of exponentials for a maximum m: nothing seen yet counts from 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
@@ -39,35 +47,71 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
 }
 
-// BYTES / sizeof(T) elements of a row whose `left` elements are valid
-// (EXACT: all of them), zeros past those.  Rows need only element alignment.
+// sum + both halves of a pair of bf16
+__device__ __forceinline__ float add2(uint32_t w, float sum) {
+    const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), one, sum, false);
+}
+
+// BYTES of a row.  Rows need only element alignment (the hardware loads 16 bytes from any).
 template <typename T, int BYTES>
 struct Words {
     uint32_t w[BYTES / 4];
 };
-template <bool EXACT, int BYTES, typename T>
-__device__ __forceinline__ Words<T, BYTES> ld_words(const T* p, int left) {
+template <int BYTES, typename T>
+__device__ __forceinline__ Words<T, BYTES> ld_words(const T* p) {
+    Words<T, BYTES> v;
+    __builtin_memcpy(&v, p, BYTES);
+    return v;
+}
+// The first `left` elements, then zeros.
+template <int BYTES, typename T>
+__device__ __forceinline__ Words<T, BYTES> ld_some(const T* p, int left) {
     constexpr int N = BYTES / (int)sizeof(T);
     Words<T, BYTES> v;
-    if (EXACT || left >= N) {
-        __builtin_memcpy(&v, p, BYTES);
-        return v;
-    }
 #pragma unroll
     for (int i = 0; i < BYTES / 4; ++i) v.w[i] = 0;
-    if (left > 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i < left) {
-                if constexpr (sizeof(T) == 4)
-                    v.w[i] = __float_as_uint(p[i]);
-                else
-                    v.w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
-            }
+    for (int i = 0; i < N; ++i) {
+        if (i < left) {
+            if constexpr (sizeof(T) == 4)
+                v.w[i] = __float_as_uint(p[i]);
+            else
+                v.w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
         }
     }
     return v;
 }
+// Zeros in the first z elements (any z).
+template <int BYTES, typename T>
+__device__ __forceinline__ void clear_first(Words<T, BYTES>& v, int z) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) {
+        if constexpr (sizeof(T) == 4)
+            v.w[i] = i < z ? 0u : v.w[i];
+        else
+            v.w[i] &= 2 * i >= z ? ~0u : 2 * i + 1 >= z ? 0xffff0000u : 0u;
+    }
+}
+
+// x, as a value that the compiler knows nothing about from here on: what follows is computed
+// where it stands, not kept in registers across a loop.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+template <typename T>
+__device__ __forceinline__ const T* opaque(const T* p) {
+    uint64_t x = (uint64_t)p;
+    asm volatile("" : "+v"(x));
+    return (const T*)(const __attribute__((address_space(1))) T*)x;  // (global loads, not flat)
+}
+
+// How the pieces of a row of D elements are read.  kExact: every piece lies in the row.
+// kClamp (D holds a piece at least): a piece that would pass the row's end is read where the row
+// ends.  In a score the elements that other pieces hold already are then cleared, in K and Q
+// alike; as dims of an output they are computed twice, alike.  kElem: element by element.
+constexpr int kExact = 0, kClamp = 1, kElem = 2;
 
 // Tiles of keys against tiles of queries, MFMA 16 x 16 with keys as rows and queries as columns:
 // S^T = K Q^T leaves a lane the scores of query L % 16 for 4 consecutive keys, which are the
@@ -79,8 +123,8 @@ __device__ __forceinline__ Words<T, BYTES> ld_words(const T* p, int left) {
 //     output tile c holds dims VL m + c, so a lane ends with whole runs of dims.
 //   fp32: 16 keys a block, 16x16x4 in fp32 (exact products); V's operands are
 //     the loaded words themselves.
-// DP dims (head_d rounded up; EXACT: head_d itself), MT tiles of 16 query rows.
-template <typename T, int DP, int MT, bool EXACT>
+// DP dims (more than head_d by less than 64), read as MODE says; MT tiles of 16 query rows.
+template <typename T, int DP, int MT, int MODE>
 struct CacheTiles {
     static constexpr bool kBf = sizeof(T) == 2;
     static constexpr int KB = kBf ? 32 : 16;       // keys of a block
@@ -94,17 +138,6 @@ struct CacheTiles {
     static constexpr int KEYS = KB / 4;            // keys of a lane
     static constexpr int RUN = 4 * VL;             // consecutive dims of a lane per V step
     static constexpr int ROWS = 16 * MT;
-    // registers: the output tile, K and V of a block, the scores and weights, addresses; with the
-    // next block's K loaded ahead except where only that would not leave two waves a SIMD
-    static constexpr int kRegs = DP / 4 * (MT + 1) + 20 * MT + 44;
-    static constexpr int kWith = kRegs + DP / 4;
-    static constexpr bool kAhead = kWith <= 250 || kRegs > 220;
-    static constexpr int kOccupancy = kWith <= 124 ? 4 : kWith <= 164 ? 3 : kRegs <= 220 ? 2 : 1;
-    static constexpr int LDO = DP + 4;             // row of the exchange, floats
-    static constexpr int kQBytes = ROWS * DP * (int)sizeof(T);
-    static constexpr int kXBytes = 2 * ROWS * LDO * 4;
-    static constexpr int kLds = (kQBytes > kXBytes ? kQBytes : kXBytes) + 2 * ROWS * 16;
-
     using KPiece = Words<T, 16>;
     using VPiece = Words<T, VB>;
 
@@ -115,16 +148,34 @@ struct CacheTiles {
         VPiece p[KEYS][VS];
     };
 
+    // Piece i of a row of K or Q for the lanes of group q (`row`: piece 0's place in the row)
+    static __device__ __forceinline__ KPiece piece(const T* row, int i, int q, int D) {
+        const int d = 4 * EL * i + EL * q;
+        if constexpr (MODE == kElem) {
+            return ld_some<16>(row + 4 * EL * i, D - d);
+        } else if (MODE == kExact || 4 * EL * (i + 1) <= DP - 64) {
+            return ld_words<16>(row + 4 * EL * i);
+        } else {
+            const int past = max(0, opaque(d) - (D - EL));
+            KPiece v = ld_words<16>(row + 4 * EL * i - past);
+            clear_first(v, past);
+            return v;
+        }
+    }
+
+    // K of a block whose first row is `base`.  FULL: of KB rows, else `rows` (the last one again
+    // in the places behind)
+    template <bool FULL>
     static __device__ __forceinline__ void load_k(Keys& k, const T* base, int64_t stride, int rows,
                                                   int D, int lane) {
-        const int q = lane >> 4;
+        if (!FULL) lane = opaque(lane);
+        const T* p0 = opaque(base + (lane & 15) * stride + EL * (lane >> 4));
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const int r = min(16 * s + (lane & 15), rows - 1);
-            const T* p = base + r * stride + EL * q;
+            const T* p = p0 + 16 * s * stride;
+            if (!FULL) p = base + min(16 * s + (lane & 15), rows - 1) * stride + EL * (lane >> 4);
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
-                k.p[s][i] = ld_words<EXACT, 16>(p + 4 * EL * i, D - 4 * EL * i - EL * q);
+            for (int i = 0; i < KS; ++i) k.p[s][i] = piece(p, i, lane >> 4, D);
         }
     }
 
@@ -132,19 +183,29 @@ struct CacheTiles {
     static __device__ __forceinline__ int key_of(int lane, int j) {
         return 16 * (j >> 2) + 4 * (lane >> 4) + (j & 3);
     }
+    // first dim of V's piece m (of 16) in step i, where the row ends at D
+    static __device__ __forceinline__ int dim_of(int i, int m, int D) {
+        const int d = VD * i + VL * m;
+        return MODE == kClamp ? min(d, D - VL) : d;
+    }
 
-    // (rows past the block's are zeros: a weight of 0 times whatever they hold must be 0)
+    // V of a block; rows past it are zeros: a weight of 0 times whatever they hold must be 0
+    template <bool FULL>
     static __device__ __forceinline__ void load_v(Vals& v, const T* base, int64_t stride, int rows,
                                                   int D, int lane) {
+        if (!FULL) lane = opaque(lane);
+        const T* p0 = opaque(base + key_of(lane, 0) * stride);
 #pragma unroll
         for (int j = 0; j < KEYS; ++j) {
-            const int r = key_of(lane, j);
-            const T* p = base + min(r, rows - 1) * stride + VL * (lane & 15);
+            const T* p = p0 + key_of(0, j) * stride;
+            if (!FULL) p = base + min(key_of(lane, j), rows - 1) * stride;
 #pragma unroll
-            for (int i = 0; i < VS; ++i)
-                v.p[j][i] = ld_words<EXACT, VB>(p + VD * i, D - VD * i - VL * (lane & 15));
+            for (int i = 0; i < VS; ++i) {
+                const int d = dim_of(i, lane & 15, D);
+                v.p[j][i] = MODE == kElem ? ld_some<VB>(p + d, D - d) : ld_words<VB>(p + d);
+            }
         }
-        if (rows < KB) {
+        if (!FULL && rows < KB) {
 #pragma unroll
             for (int j = 0; j < KEYS; ++j)
                 if (key_of(lane, j) >= rows)
@@ -206,24 +267,29 @@ struct CacheTiles {
                 w[t][0][0] = x.x, w[t][0][1] = x.y, w[t][0][2] = x.z, w[t][0][3] = x.w;
             }
         }
-        if constexpr (kBf)
+        if constexpr (kBf) {
             products(o, v, f);
-        else
-            accumulate(o, v, w);
+        } else {
+            float none[MT];
+            accumulate(o, v, w, none);
+        }
     }
 
-    // O^T += V^T P^T for all tiles
+    // O^T += V^T P^T for all tiles.  bf16: the weights enter as bf16 (V's own precision, and what
+    // lets one MFMA take both), half a step (2^-8 of their size) off at most; `used` gathers
+    // them as rounded, so that the output is their exact mean of V
     static __device__ __forceinline__ void accumulate(v4f (&o)[MT][VS][VL], const Vals& v,
-                                                      const float (&p)[MT][SUB][4]) {
+                                                      const float (&p)[MT][SUB][4],
+                                                      float (&used)[MT]) {
         if constexpr (kBf) {
-            // the weights as bf16, half a step (2^-8 of their size) off at most: V's own
-            // precision, and what lets one MFMA take both
             KPiece f[MT];
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int h = 0; h < 4; ++h)
+                for (int h = 0; h < 4; ++h) {
                     f[t].w[h] = pack2(p[t][h >> 1][2 * (h & 1)], p[t][h >> 1][2 * (h & 1) + 1]);
+                    used[t] = add2(f[t].w[h], used[t]);
+                }
             products(o, v, f);
         } else {
 #pragma unroll
@@ -241,12 +307,12 @@ struct CacheTiles {
 };
 
 // Scores of 32 keys against 16 MT query rows over this wave's share of the dims (`waves` share
-// them), from row pointers of each lane (at its piece of the rows).  EXACT: every step of 4
-// pieces lies inside the rows.
-template <typename T, int MT, bool EXACT, int WAVES>
+// them), from each lane's row pointers.  All loads of a step go out before its products: left
+// to itself the compiler keeps six in flight, and the memory idles.
+template <typename T, int MT, int WAVES>
 __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp)[2],
                                             const T* const (&qp)[MT], int D, int wave, int q) {
-    using N = CacheTiles<T, 64, MT, EXACT>;
+    using N = CacheTiles<T, 64, MT, kExact>;
     constexpr int EL = N::EL, STEP = 4 * EL, U = 4;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -254,22 +320,44 @@ __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp
         for (int u = 0; u < 2; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
     const int per = ((D + STEP * U - 1) / (STEP * U) + WAVES - 1) / WAVES * STEP * U;
     const int d1 = min(D, (wave + 1) * per);
-    for (int d = wave * per; d < d1; d += STEP * U) {
-        typename N::KPiece k[U][2], f[U][MT];
-#pragma unroll
-        for (int e = 0; e < U; ++e) {
-            const int at = d + STEP * e, left = D - at - EL * q;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) k[e][u] = ld_words<EXACT, 16>(kp[u] + at, left);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) f[e][t] = ld_words<EXACT, 16>(qp[t] + at, left);
-        }
+    typename N::KPiece k[U][2], f[U][MT];
+    auto products = [&] {
 #pragma unroll
         for (int e = 0; e < U; ++e)
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) s[t][u] = N::dot(k[e][u], f[e][t], s[t][u]);
+    };
+    int d = wave * per;
+    for (; d + STEP * U <= d1; d += STEP * U) {
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+            const int at = d + STEP * e + EL * q;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) k[e][u] = ld_words<16>(kp[u] + at);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) f[e][t] = ld_words<16>(qp[t] + at);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        products();
+    }
+    if (d < d1) {  // the row's end (kClamp's pieces)
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+            const int want = d + STEP * e + EL * q, at = min(want, D - EL);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                k[e][u] = ld_words<16>(kp[u] + at);
+                clear_first(k[e][u], want - at);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                f[e][t] = ld_words<16>(qp[t] + at);
+                clear_first(f[e][t], want - at);
+            }
+        }
+        products();
     }
 }
 

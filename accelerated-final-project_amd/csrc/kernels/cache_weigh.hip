@@ -47,13 +47,6 @@ __device__ __forceinline__ float2 reach_of(const WeighArgs& a, int b, int g, int
     return make_float2(__int_as_float(z == -INFINITY ? -1 : L + x.entry), z * kLog2e);
 }
 
-__device__ __forceinline__ float row16_sum(float x) {
-    x += dpp<kDppQuadXor1>(x);
-    x += dpp<kDppQuadXor2>(x);
-    x += dpp<kDppRowHalfMirror>(x);
-    return x + dpp<kDppRowMirror>(x);
-}
-
 // Lane (col, q) of a 16-lane row holds its row's sums for keys k0 + 4 q + e: lanes col 0..3 write
 // one each.
 __device__ __forceinline__ void put_weights(const WeighArgs& a, size_t at, bool first, float4 sum,
@@ -68,9 +61,9 @@ __device__ __forceinline__ void put_weights(const WeighArgs& a, size_t at, bool 
 
 // head_d <= 256: a wave holds a block of keys in registers and runs the pass's query rows over
 // it from LDS, the next block's keys on their way.
-template <typename T, int DP, bool EXACT>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
-    using N = CacheTiles<T, DP, 1, EXACT>;
+    using N = CacheTiles<T, DP, 1, MODE>;
     constexpr int KB = N::KB, SUB = N::SUB, KS = N::KS;
     __shared__ typename N::KPiece qs[kRows / 16 * KS * 64];
     __shared__ float2 reach[kRows];
@@ -85,19 +78,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
     for (int row0 = 0; row0 == 0 || row0 < R; row0 += kRows) {
         typename N::Keys k;
         if (i0 < blocks)
-            N::load_k(k, kc + (int64_t)i0 * KB * a.c.ks[2], a.c.ks[2], min(KB, end - i0 * KB), D,
-                      lane);
+            N::template load_k<false>(k, kc + (int64_t)i0 * KB * a.c.ks[2], a.c.ks[2],
+                                      min(KB, end - i0 * KB), D, lane);
         const int tiles = (min(kRows, R - row0) + 15) / 16;
         __syncthreads();
         for (int e = threadIdx.x; e < tiles * KS * 64; e += 64 * kWaves) {
             const int el = e & 63, i = (e >> 6) % KS, t = (e >> 6) / KS;
-            const int row = row0 + 16 * t + (el & 15), d0 = 4 * N::EL * i + N::EL * (el >> 4);
+            const int row = row0 + 16 * t + (el & 15);
             typename N::KPiece z{};
             if (row < R) {
                 const QueryRow x = query_row(a, b, g, A, row);
-                z = ld_words<EXACT, 16>((const T*)a.d.Q + b * a.d.qs[0] + x.head * a.d.qs[1] +
-                                            x.tok * a.d.qs[2] + d0,
-                                        D - d0);
+                z = N::piece((const T*)a.d.Q + b * a.d.qs[0] + x.head * a.d.qs[1] +
+                                 x.tok * a.d.qs[2] + N::EL * (el >> 4),
+                             i, el >> 4, D);
             }
             qs[e] = z;
         }
@@ -131,8 +124,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
             }
             const int nx = i + step;
             if (nx < blocks)
-                N::load_k(k, kc + (int64_t)nx * KB * a.c.ks[2], a.c.ks[2], min(KB, end - nx * KB),
-                          D, lane);
+                N::template load_k<false>(k, kc + (int64_t)nx * KB * a.c.ks[2], a.c.ks[2],
+                                          min(KB, end - nx * KB), D, lane);
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const float4 w = make_float4(row16_sum(sum[u][0]), row16_sum(sum[u][1]),
@@ -146,9 +139,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
 // head_d > 256: 8 waves share the dims of a block of 32 keys and add up through LDS.
 constexpr int kBlock = 32, kScoreWaves = 8;
 
-template <typename T, int MT, bool EXACT>
+template <typename T, int MT>
 __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
-    using N = CacheTiles<T, 64, MT, EXACT>;
     constexpr int SUB = kBlock / 16;
     __shared__ v4f red[kScoreWaves][MT * SUB * 64];
     __shared__ float part[MT][kBlock];
@@ -163,7 +155,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
         kp[u] = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1] +
-                (int64_t)(j0 + min(16 * u + col, rows - 1)) * a.c.ks[2] + N::EL * q;
+                (int64_t)(j0 + min(16 * u + col, rows - 1)) * a.c.ks[2];
     for (int row0 = 0; row0 == 0 || row0 < R; row0 += 16 * MT) {
         v4f s[MT][SUB] = {};
         if (R > 0) {
@@ -171,10 +163,9 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const QueryRow x = query_row(a, b, g, A, min(row0 + 16 * t + col, R - 1));
-                qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + x.head * a.d.qs[1] + x.tok * a.d.qs[2] +
-                        N::EL * q;
+                qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + x.head * a.d.qs[1] + x.tok * a.d.qs[2];
             }
-            wide_scores<T, MT, EXACT, kScoreWaves>(s, kp, qp, D, wave, q);
+            wide_scores<T, MT, kScoreWaves>(s, kp, qp, D, wave, q);
         }
 #pragma unroll
         for (int t = 0; t < MT; ++t)
@@ -213,17 +204,16 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
 template <typename T, int DP>
 void go_narrow(const WeighArgs& a, dim3 grid, hipStream_t st) {
     if (a.c.D == DP)
-        hipLaunchKernelGGL((k_weigh_narrow<T, DP, true>), grid, dim3(64 * kWaves), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_weigh_narrow<T, DP, false>), grid, dim3(64 * kWaves), 0, st, a);
+        hipLaunchKernelGGL((k_weigh_narrow<T, DP, kExact>), grid, dim3(64 * kWaves), 0, st, a);
+    else if (DP > 64 || a.c.D >= 16 / (int)sizeof(T))
+        hipLaunchKernelGGL((k_weigh_narrow<T, DP, kClamp>), grid, dim3(64 * kWaves), 0, st, a);
+    else if constexpr (DP == 64)
+        hipLaunchKernelGGL((k_weigh_narrow<T, DP, kElem>), grid, dim3(64 * kWaves), 0, st, a);
 }
 
 template <typename T, int MT>
 void go_wide(const WeighArgs& a, dim3 grid, hipStream_t st) {
-    if (a.c.D % 128 == 0)
-        hipLaunchKernelGGL((k_weigh_wide<T, MT, true>), grid, dim3(64 * kScoreWaves), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_weigh_wide<T, MT, false>), grid, dim3(64 * kScoreWaves), 0, st, a);
+    hipLaunchKernelGGL((k_weigh_wide<T, MT>), grid, dim3(64 * kScoreWaves), 0, st, a);
 }
 
 template <typename T>

@@ -78,13 +78,16 @@ __device__ __forceinline__ int path_at(const PathView& p, int b, int i) {
     return p.path ? p.path[(size_t)b * p.n + i] : i;
 }
 
-// How a call runs (tree_plan).  heads: (sequence, kv head) pairs of one pass; a call whose
-// scratch would pass its limit runs in several.
+// How a call runs (tree_plan): in passes over `seqs` sequences by `kv` kv heads (all of both
+// unless the scratch would pass its limit), the blocks of keys of a pass dealt to `ranges`
+// equal ranges, or a range per (sequence, kv head) where split is 0.
 struct TreePlan {
     int rows;        // query rows of a tile
     int row_tiles;   // tiles of the query rows of one kv head
-    int nsplit;      // key splits, whose results k_tree_merge adds up
-    int heads;
+    int waves;       // of a workgroup (head_d <= 256)
+    int split;
+    int ranges;
+    int seqs, kv;
     int ld_scores;   // head_d > 256: row of the scores, floats
     size_t scores;   // floats of the scores of a pass
     size_t scratch;  // bytes
@@ -99,9 +102,9 @@ struct TreeArgs {
     float* lse;     // [B][H][T] or null
     float scale;    // times log2(e)
     TreePlan plan;
-    float* scores;  // scratch: [heads][row tiles of rows][ld_scores]
-    float* part;    // scratch: [heads][H / G * T][nsplit] statistics, then as many rows of D
-    int bg0, bgs;   // first pair of this pass, and pairs
+    float* scores;  // scratch: [pairs of a pass][row tiles of rows][ld_scores]
+    float* part;    // scratch: parts of rows (2 of each range and tile): statistics, dims
+    int b0, bs, g0, gs;  // this pass
 };
 
 // Whether draft t of sequence b (of n drafts) attends draft j.

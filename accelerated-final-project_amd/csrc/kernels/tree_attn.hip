@@ -5,7 +5,14 @@
 //
 // The query rows of one kv head (its heads times the tokens) share the reads
 // of K and V: tiles of 16 MT rows.  Scores are in units of log2 throughout.
+//
+// The lengths are on the device, so the host only fixes how many workgroups there
+// are.  The blocks of keys of all (sequence, kv head) pairs lie in one line; each
+// workgroup takes an equal range of it, which may end one pair and begin the next.
+// A pair inside one range is written at once; the parts of one that ranges cut
+// lie in the scratch until k_tree_merge has added them up.
 #include <algorithm>
+#include <cfloat>
 
 #include "cache_tiles.hpp"
 
@@ -13,14 +20,119 @@ namespace atn {
 
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kTreeNarrow = 256;  // head_d up to which a wave holds a row tile's output
 constexpr float kLn2 = 0.69314718055994531f;
 
-// ---------------------------------------------------------------- head_d <= 256
-// Every wave walks its own blocks of keys, alone: scores, running maximum and
-// sum, and its own output tile in registers (cache_tiles.hpp); nothing passes through LDS
-// but Q and, at the end, the four waves' results.
+// ---------------------------------------------------------------- the line of blocks
+// Blocks of sequence b for each of its kv heads: the cache's, then the drafts'.  At least
+// one, so that some workgroup writes the outputs of tokens that attend nothing.
+__device__ __forceinline__ int blocks_of(const TreeArgs& a, int b, int kb) {
+    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
+    return max(1, (L + kb - 1) / kb + (a.d.K ? (n + kb - 1) / kb : 0));
+}
+
+__device__ __forceinline__ int wave_scan(int x, int lane) {  // sums of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+// The line: its length, and the blocks of a range (whole turns of `turn`).  A wave's work, as
+// are the others here; results are uniform.
+struct Line {
+    int total, per;
+};
+__device__ __forceinline__ Line line_from(const TreeArgs& a, int total, int turn) {
+    const int per = (total + a.plan.ranges - 1) / a.plan.ranges;
+    return Line{total, max((per + turn - 1) / turn * turn, 2 * turn)};
+}
+__device__ __forceinline__ Line line_of(const TreeArgs& a, int kb, int turn, int lane) {
+    int sum = 0;
+    for (int i = lane; i < a.bs; i += 64) sum += blocks_of(a, a.b0 + i, kb);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    return line_from(a, __builtin_amdgcn_readfirstlane(sum) * a.gs, turn);
+}
+
+// The sequence at position `at` of the line, and its place there.
+struct Place {
+    int b, blocks, start;  // sequence, blocks of each kv head, position of the first
+};
+__device__ __forceinline__ Place place_at(const TreeArgs& a, int at, int kb, int lane) {
+    int before = 0;
+    for (int i0 = 0;; i0 += 64) {
+        const int n = i0 + lane < a.bs ? blocks_of(a, a.b0 + i0 + lane, kb) : 0;
+        const int upto = before + wave_scan(n * a.gs, lane);
+        const uint64_t done = __builtin_amdgcn_ballot_w64(upto <= at);
+        if (done != ~0ull || i0 + 64 >= a.bs) {
+            const int l = min(__builtin_popcountll(done), min(63, a.bs - 1 - i0));
+            Place p;
+            p.b = a.b0 + i0 + l;
+            p.blocks = __builtin_amdgcn_readlane(n, l);
+            p.start = __builtin_amdgcn_readlane(upto, l) - p.blocks * a.gs;
+            return p;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+
+// One pair's blocks [first, last) of a range, and where they go: `part` < 0: the output,
+// else the range's part of that number.
+struct Span {
+    int b, g, first, last, part;
+};
+// The span of range r that begins at `at` (*next: the position after it).
+__device__ __forceinline__ Span span_at(const TreeArgs& a, int r, int at, int end, int kb, int lane,
+                                        int* next) {
+    const Place p = place_at(a, at, kb, lane);
+    Span s;
+    const int off = at - p.start;
+    s.b = p.b;
+    s.g = a.g0 + off / p.blocks;
+    s.first = off % p.blocks;
+    s.last = min(p.blocks, s.first + end - at);
+    s.part = s.first == 0 && s.last == p.blocks ? -1 : 2 * r + (s.first == 0 ? 1 : 0);
+    *next = at + s.last - s.first;
+    return s;
+}
+// The whole of pair r, where ranges are pairs.
+__device__ __forceinline__ Span span_whole(const TreeArgs& a, int r, int kb) {
+    Span s;
+    s.b = a.b0 + r / a.gs;
+    s.g = a.g0 + r % a.gs;
+    s.first = 0;
+    s.last = blocks_of(a, s.b, kb);
+    s.part = -1;
+    return s;
+}
+
+// Parts: statistics of the rows (maximum, sum of the weights, their sum as they entered the
+// product with V), then, behind all of them, the rows' dims.
+__device__ __forceinline__ size_t part_row(const TreeArgs& a, int part, int row) {
+    return (size_t)part * a.plan.row_tiles * a.plan.rows + row;
+}
+__device__ __forceinline__ float4* part_stats(const TreeArgs& a) {
+    return reinterpret_cast<float4*>(a.part);
+}
+__device__ __forceinline__ float* part_dims(const TreeArgs& a) {
+    return a.part + 4 * part_row(a, 2 * a.plan.ranges, 0);
+}
+
+// Workgroup -> (range, tile): workgroups go to the 8 XCDs in turn, so the tiles that read the
+// same keys are 8 apart and share an L2.
+__device__ __forceinline__ void tile_of(int id, int ranges, int tiles, int* range, int* tile) {
+    const int full = ranges / 8 * 8 * tiles, whole = id < full;
+    const int x = whole ? id % 8 : 0, y = whole ? id / 8 : id - full;
+    *tile = y % tiles;
+    *range = whole ? y / tiles * 8 + x : ranges / 8 * 8 + y / tiles;
+}
+
+// ---------------------------------------------------------------- infinities and NaNs
+// A draft that some rows attend and others do not: an infinity or NaN in its V belongs to the
+// first alone.  The product runs without it; it is added where the results are written.
 // Whether any lane's V holds an infinity or NaN, which are cleared.
 template <typename T, typename V>
 __device__ __forceinline__ bool clear_not_finite(V& v) {
@@ -56,143 +168,112 @@ __device__ __forceinline__ float not_finite_sum(const TreeArgs& a, int b, int g,
     return sum;
 }
 
-// A row's results in a split: maximum and sum, then, behind all of these, the dims.
-__device__ __forceinline__ float2* stats_of(const TreeArgs& a) {
-    return reinterpret_cast<float2*>(a.part);
-}
-__device__ __forceinline__ float* parts_of(const TreeArgs& a) {
-    return a.part + 2 * (size_t)a.plan.heads * (a.d.H / a.c.G) * a.d.T * a.plan.nsplit;
-}
-
 // not_finite_sum() added to dims [d0, d1) of a row where its result lies (a wave's work, after
-// the wave has written it): the output, or the split's part.
+// the wave has written it): the output, or a part.
 template <typename T>
-__device__ void add_not_finite(const TreeArgs& a, int bg, int row, int split, int n, int d0, int d1,
+__device__ void add_not_finite(const TreeArgs& a, const Span& s, int row, int n, int d0, int d1,
                                int lane) {
-    const int g = bg % a.c.G, b = bg / a.c.G, rep = a.d.H / a.c.G;
-    const int tok = row % a.d.T;
+    const int rep = a.d.H / a.c.G, tok = row % a.d.T;
     if (row >= rep * a.d.T || tok >= n) return;
-    T* out = (T*)a.out + b * a.os[0] + (g * rep + row / a.d.T) * a.os[1] + tok * a.os[2];
-    float* part =
-        parts_of(a) + (((size_t)(bg - a.bg0) * rep * a.d.T + row) * a.plan.nsplit + split) * a.c.D;
+    T* out = (T*)a.out + s.b * a.os[0] + (s.g * rep + row / a.d.T) * a.os[1] + tok * a.os[2];
     for (int d = d0 + lane; d < d1; d += 64) {
-        const float x = not_finite_sum<T>(a, b, g, n, tok, d);
+        const float x = not_finite_sum<T>(a, s.b, s.g, n, tok, d);
         if (x == 0.f) continue;
-        if (a.plan.nsplit > 1)
-            part[d] += x;
+        if (s.part >= 0)
+            part_dims(a)[part_row(a, s.part, row) * a.c.D + d] += x;
         else
             Elem<T>::st(out, d, Elem<T>::ld(out, d) + x);
     }
 }
 
-// Blocks of a split: whole turns of a workgroup's waves, so that every split but the last is full.
-__device__ __forceinline__ int split_blocks(int all, int nsplit) {
-    return ((all + nsplit - 1) / nsplit + kWaves - 1) / kWaves * kWaves;
-}
-
-// The cache's keys in blocks, then the drafts in blocks of their own: where
-// a split's blocks lie.
-struct Blocks {
-    int cache, all;    // blocks of the cache, and with the drafts'
-    int first, last;   // this split's
+// ---------------------------------------------------------------- head_d <= 256
+// Every wave walks its own blocks of keys, alone: scores, running maximum and
+// sum, and its own output tile in registers (cache_tiles.hpp); nothing passes through LDS
+// but Q and, at the end, the waves' results.
+template <typename T, int DP, int MT, int MODE, int WAVES>
+struct Narrow : CacheTiles<T, DP, MT, MODE> {
+    using N = CacheTiles<T, DP, MT, MODE>;
+    // registers: the output tile, K and V of a block, the scores and weights, addresses; with the
+    // next block's K loaded ahead except where only that would not leave two waves a SIMD
+    static constexpr int kRegs = DP / 4 * (MT + 1) + 20 * MT + 44;
+    static constexpr int kWith = kRegs + DP / 4;
+    static constexpr bool kAhead = kWith <= 250 || kRegs > 220;
+    static constexpr int kPerSimd = kWith <= 124 ? 4 : kWith <= 164 ? 3 : kRegs <= 220 ? 2 : 1;
+    static constexpr int kMinWaves = WAVES == 8 ? 2 : kPerSimd;
+    static constexpr int LDO = DP + 4;  // row of the exchange, floats
+    static constexpr int kQBytes = N::ROWS * DP * (int)sizeof(T);
+    static constexpr int kXBytes = WAVES / 2 * N::ROWS * LDO * 4;
+    static constexpr int kOBytes = kQBytes > kXBytes ? kQBytes : kXBytes;
+    static constexpr int kLds = kOBytes + WAVES / 2 * N::ROWS * 16;
 };
-template <int KB>
-__device__ __forceinline__ Blocks blocks_of(const TreeArgs& a, int L, int n, int split) {
-    Blocks x;
-    x.cache = (L + KB - 1) / KB;
-    x.all = x.cache + (a.d.K ? (n + KB - 1) / KB : 0);
-    const int per = split_blocks(x.all, a.plan.nsplit);
-    x.first = min(split * per, x.all);
-    x.last = min(x.first + per, x.all);
-    return x;
-}
 
-// Workgroup -> (unit of keys, tile of it): workgroups go to the 8 XCDs in turn, so the tiles
-// that read the same keys are 8 apart and share an L2.
-__device__ __forceinline__ void tile_of(int id, int units, int tiles, int* unit, int* tile) {
-    const int full = units / 8 * 8 * tiles, whole = id < full;
-    const int x = whole ? id % 8 : 0, y = whole ? id / 8 : id - full;
-    *tile = y % tiles;
-    *unit = whole ? y / tiles * 8 + x : units / 8 * 8 + y / tiles;
-}
-
-template <typename T, int DP, int MT, bool EXACT>
-__global__ __launch_bounds__(64 * kWaves, (CacheTiles<T, DP, MT, EXACT>::kOccupancy)) void
+template <typename T, int DP, int MT, int MODE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (Narrow<T, DP, MT, MODE, WAVES>::kMinWaves)) void
 k_tree_narrow(TreeArgs a) {
-    using N = CacheTiles<T, DP, MT, EXACT>;
-    constexpr int KB = N::KB, SUB = N::SUB, KS = N::KS, VS = N::VS, VL = N::VL, RUN = N::RUN;
+    using N = Narrow<T, DP, MT, MODE, WAVES>;
+    constexpr int KB = N::KB, SUB = N::SUB, KS = N::KS, VS = N::VS, VL = N::VL;
     __shared__ __align__(16) char lds[N::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
-    const int tiles = a.plan.row_tiles, nsplit = a.plan.nsplit;
-    int unit, tile;
-    tile_of(blockIdx.x, a.bgs * nsplit, tiles, &unit, &tile);
-    const int split = unit % nsplit, bg = a.bg0 + unit / nsplit, g = bg % a.c.G, b = bg / a.c.G;
-    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), D = a.c.D;
-    const int rep = a.d.H / a.c.G, R = rep * a.d.T;
-    const Blocks blk = blocks_of<KB>(a, L, n, split);
-    // (nothing for this split: the merge knows; a call of one split writes zeros)
-    if (blk.first >= blk.last && nsplit > 1 && split > 0) return;
+    int range, tile;
+    tile_of(blockIdx.x, a.plan.ranges, a.plan.row_tiles, &range, &tile);
+    const int D = a.c.D, rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const float scale = fabsf(a.scale);
+    const uint32_t flip = a.scale < 0.f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
 
-    // Q in the order of the fragments: piece (t, i) of lane L is piece i of row 16 t + L % 16
-    auto* qs = reinterpret_cast<typename N::KPiece*>(lds);
-    for (int e = threadIdx.x; e < MT * KS * 64; e += 64 * kWaves) {
-        const int el = e & 63, i = (e >> 6) % KS, t = (e >> 6) / KS;
-        const int row = tile * N::ROWS + 16 * t + (el & 15);
-        typename N::KPiece z{};
-        if (row < R && row % a.d.T < n) {
-            const int d0 = 4 * N::EL * i + N::EL * (el >> 4);
-            z = ld_words<EXACT, 16>((const T*)a.d.Q + b * a.d.qs[0] +
-                                        (g * rep + row / a.d.T) * a.d.qs[1] +
-                                        (row % a.d.T) * a.d.qs[2] + d0,
-                                    D - d0);
+    int at = 0, end = 1;
+    if (a.plan.split) {
+        const Line line = line_of(a, KB, WAVES, lane);
+        at = range * line.per;
+        end = min(line.total, at + line.per);
+    }
+    while (at < end) {
+        Span sp;
+        if (a.plan.split) {
+            sp = span_at(a, range, at, end, KB, lane, &at);
+        } else {
+            sp = span_whole(a, range, KB);
+            at = end;
         }
-        qs[e] = z;
-    }
-    __syncthreads();
+        const int b = sp.b, g = sp.g, L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
+        const int cache = (L + KB - 1) / KB;  // its blocks; the drafts' follow
 
-    const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
-    const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1];
-    const T* kd = (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
-    const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
-
-    v4f o[MT][VS][VL];
-    float m[MT], l[MT];
+        // Q in the order of the fragments: piece (t, i) of lane L is piece i of row 16 t + L % 16
+        auto* qs = reinterpret_cast<typename N::KPiece*>(lds);
+        __syncthreads();  // (the last span's exchange)
+        for (int e = threadIdx.x; e < MT * KS * 64; e += 64 * WAVES) {
+            const int el = e & 63, i = (e >> 6) % KS, t = (e >> 6) / KS;
+            const int row = tile * N::ROWS + 16 * t + (el & 15);
+            typename N::KPiece z{};
+            if (row < R && row % a.d.T < n) {
+                z = N::piece((const T*)a.d.Q + b * a.d.qs[0] + (g * rep + row / a.d.T) * a.d.qs[1] +
+                                 (row % a.d.T) * a.d.qs[2] + N::EL * (el >> 4),
+                             i, el >> 4, D);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.f;
-#pragma unroll
-        for (int i = 0; i < VS; ++i)
-#pragma unroll
-            for (int c = 0; c < VL; ++c) o[t][i][c] = v4f{0.f, 0.f, 0.f, 0.f};
-    }
+                for (int w = 0; w < 4; ++w) z.w[w] ^= flip;
+            }
+            qs[e] = z;
+        }
+        __syncthreads();
 
-    auto rows_of = [&](int i) {
-        return i < blk.cache ? min(KB, L - i * KB) : min(KB, n - (i - blk.cache) * KB);
-    };
-    auto load_k = [&](typename N::Keys& k, int i) {
-        const bool in = i < blk.cache;
-        const int64_t s = in ? a.c.ks[2] : a.d.ks[2];
-        N::load_k(k, (in ? kc : kd) + (int64_t)(in ? i : i - blk.cache) * KB * s, s, rows_of(i), D,
-                  lane);
-    };
-
-    bool odd = false;
-    typename N::Keys k;
-    int i = blk.first + wave;
-    if (N::kAhead && i < blk.last) load_k(k, i);
-    for (; i < blk.last; i += kWaves) {
-        const bool in = i < blk.cache;
-        const int j0 = in ? i * KB : (i - blk.cache) * KB, rows = rows_of(i);
-        if (!N::kAhead) load_k(k, i);
+        const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
+        const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1];
+        v4f o[MT][VS][VL];
+        float m[MT], l[MT], used[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = used[t] = 0.f;
+#pragma unroll
+            for (int i = 0; i < VS; ++i)
+#pragma unroll
+                for (int c = 0; c < VL; ++c) o[t][i][c] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        bool odd = false;
+        typename N::Keys k;
         typename N::Vals v;
-        {
-            const int64_t s = in ? a.c.vs[2] : a.d.vs[2];
-            N::load_v(v, (in ? vc : vd) + (int64_t)j0 * s, s, rows, D, lane);
-        }
         float p[MT][SUB][4];
-        {
+        auto scores = [&] {
             v4f s[MT][SUB];
 #pragma unroll
             for (int t = 0; t < MT; ++t)
@@ -211,154 +292,188 @@ k_tree_narrow(TreeArgs a) {
 #pragma unroll
                 for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[t][u][e] = s[t][u][e] * a.scale;
-        }
-        if (N::kAhead && i + kWaves < blk.last) load_k(k, i + kWaves);
-        uint32_t see[MT];  // bit 16 u + 4 q + e: the row attends key 16 u + 4 q + e of the block
-        const uint32_t valid = rows >= 32 ? ~0u : (1u << rows) - 1;
-        if (!in || rows < KB) {
+                    for (int e = 0; e < 4; ++e) p[t][u][e] = s[t][u][e];
+        };
+        // The running maximum moves only when a score passes it by more than 8 (weights up to
+        // 2^8 lose nothing in fp32 or bf16), so the tile is rarely rescaled.
+        auto weights = [&] {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                see[t] = valid;
+                float top = p[t][0][0];
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, p[t][u][e]);
+                if (__builtin_amdgcn_ballot_w64(top * scale > m[t] + 8.f)) {
+                    const float m_new = fmaxf(m[t], row_max(top) * scale);
+                    const float f = exp2_(m[t] - base_of(m_new));
+                    m[t] = m_new;
+                    l[t] *= f;
+                    used[t] *= f;
+#pragma unroll
+                    for (int x = 0; x < VS; ++x)
+#pragma unroll
+                        for (int c = 0; c < VL; ++c) o[t][x][c] *= f;
+                }
+                const float base = base_of(m[t]);
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[t][u][e] = exp2_(fmaf(p[t][u][e], scale, -base));
+                        l[t] += p[t][u][e];
+                    }
+            }
+        };
+
+        // whole blocks of the cache: nothing masked, the next block's loads on their way
+        const int whole = min(sp.last, L / KB);
+        int i = sp.first + wave;
+        auto k_at = [&](int x) {
+            N::template load_k<true>(k, kc + (int64_t)x * KB * a.c.ks[2], a.c.ks[2], KB, D, lane);
+        };
+        if (N::kAhead && i < whole) k_at(i);
+        for (; i < whole; i += WAVES) {
+            if (!N::kAhead) k_at(i);
+            N::template load_v<true>(v, vc + (int64_t)i * KB * a.c.vs[2], a.c.vs[2], KB, D, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            scores();
+            if (N::kAhead && i + WAVES < whole) k_at(i + WAVES);
+            __builtin_amdgcn_sched_barrier(0);
+            weights();
+            N::accumulate(o, v, p, used);
+        }
+        // the cache's last block and the drafts
+        for (; i < sp.last; i += WAVES) {
+            const bool in = i < cache;
+            const int j0 = (in ? i : i - cache) * KB;
+            const int rows = min(KB, (in ? L : a.d.K ? n : 0) - j0);
+            if (rows <= 0) break;  // (the one block of a pair without any)
+            const int64_t ks = in ? a.c.ks[2] : a.d.ks[2], vs = in ? a.c.vs[2] : a.d.vs[2];
+            const T* kb = in ? kc : (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
+            const T* vb = in ? vc : (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
+            N::template load_k<false>(k, kb + j0 * ks, ks, rows, D, lane);
+            N::template load_v<false>(v, vb + j0 * vs, vs, rows, D, lane);
+            scores();
+            const uint32_t valid = rows >= 32 ? ~0u : (1u << rows) - 1;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                uint32_t see = valid;  // bit j: the row attends key j of the block
                 if (!in) {
                     const int row = tile * N::ROWS + 16 * t + col, tok = row % a.d.T;
                     if (a.d.mask) {
                         const uint32_t w =
                             row < R ? a.d.mask[((size_t)b * a.d.T + tok) * a.d.W + (j0 >> 5)] : 0u;
-                        see[t] &= w >> (j0 & 31);
+                        see &= w >> (j0 & 31);
                     } else {
                         const int upto = tok - j0;  // keys 0 .. upto
-                        see[t] &= upto < 0 ? 0u : upto >= 31 ? ~0u : (2u << upto) - 1;
+                        see &= upto < 0 ? 0u : upto >= 31 ? ~0u : (2u << upto) - 1;
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < SUB; ++u)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!((see[t] >> (16 * u + 4 * q + e)) & 1u)) p[t][u][e] = -INFINITY;
+                        if (!((see >> (16 * u + 4 * q + e)) & 1u)) p[t][u][e] = -INFINITY;
             }
+            if (!in) odd |= clear_not_finite<T>(v);
+            weights();
+            N::accumulate(o, v, p, used);
         }
-        // The running maximum moves only when a score passes it by more than 8 (weights up to
-        // 2^8 lose nothing in fp32 or bf16), so the tile is rarely rescaled.
+
+        // the waves' tiles into wave 0: the upper half hands theirs to the lower, again and again
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            float top = p[t][0][0];
+            l[t] = row_sum(l[t]);
+            used[t] = sizeof(T) == 2 ? row_sum(used[t]) : l[t];
+        }
+        float* xo = reinterpret_cast<float*>(lds);
+        float4* xs = reinterpret_cast<float4*>(lds + N::kOBytes);
+        for (int half = WAVES / 2; half > 0; half /= 2) {
+            __syncthreads();
+            if (wave >= half && wave < 2 * half) {
+                float* to = xo + (wave - half) * N::ROWS * N::LDO;
 #pragma unroll
-            for (int u = 0; u < SUB; ++u)
+                for (int t = 0; t < MT; ++t) {
+                    if (q == 0)
+                        xs[(wave - half) * N::ROWS + 16 * t + col] =
+                            make_float4(m[t], l[t], used[t], odd ? 1.f : 0.f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top = fmaxf(top, p[t][u][e]);
-            if (__builtin_amdgcn_ballot_w64(top > m[t] + 8.f)) {
-                const float m_new = fmaxf(m[t], row_max(top));
-                const float alpha = exp2_(m[t] - base_of(m_new));
-                m[t] = m_new;
-                l[t] *= alpha;
+                    for (int x = 0; x < VS; ++x)
 #pragma unroll
-                for (int x = 0; x < VS; ++x)
+                        for (int c = 0; c < VL; ++c)
 #pragma unroll
-                    for (int c = 0; c < VL; ++c) o[t][x][c] *= alpha;
-            }
-            const float base = base_of(m[t]);
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[t][u][e] = exp2_(p[t][u][e] - base);
-                    l[t] += p[t][u][e];
+                            for (int e = 0; e < 4; ++e)
+                                to[(16 * t + col) * N::LDO + N::VD * x + N::RUN * q + VL * e + c] =
+                                    o[t][x][c][e];
                 }
+            }
+            __syncthreads();
+            if (wave < half) {
+                const float* from = xo + wave * N::ROWS * N::LDO;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const float4 y = xs[wave * N::ROWS + 16 * t + col];
+                    const float m_new = fmaxf(m[t], y.x), base = base_of(m_new);
+                    const float fa = exp2_(m[t] - base), fb = exp2_(y.x - base);
+                    m[t] = m_new;
+                    l[t] = l[t] * fa + y.y * fb;
+                    used[t] = used[t] * fa + y.z * fb;
+                    odd |= y.w != 0.f;
+#pragma unroll
+                    for (int x = 0; x < VS; ++x)
+#pragma unroll
+                        for (int c = 0; c < VL; ++c)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                o[t][x][c][e] = o[t][x][c][e] * fa +
+                                                fb * from[(16 * t + col) * N::LDO + N::VD * x +
+                                                          N::RUN * q + VL * e + c];
+                }
+            }
         }
-        // A draft that some rows attend and others do not: an infinity or NaN in its V belongs
-        // to the first alone.  The product runs without it; not_finite_sum() adds it at the end.
-        if (!in) odd |= clear_not_finite<T>(v);
-        N::accumulate(o, v, p);
-    }
-
-    // the waves' tiles into wave 0: 2 and 3 hand theirs to 0 and 1, then 1 to 0
+        if (wave != 0) continue;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) l[t] = row_sum(l[t]);
-    float* xo = reinterpret_cast<float*>(lds);
-    float4* xs = reinterpret_cast<float4*>(lds + N::kLds - 2 * N::ROWS * 16);
-    for (int half = kWaves / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-            float* to = xo + (wave - half) * N::ROWS * N::LDO;
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                if (q == 0)
-                    xs[(wave - half) * N::ROWS + 16 * t + col] =
-                        make_float4(m[t], l[t], odd ? 1.f : 0.f, 0.f);
+        for (int t = 0; t < MT; ++t) {
+            const int row = tile * N::ROWS + 16 * t + col;
+            const int h = g * rep + row / a.d.T, tok = row % a.d.T;
+            if (row >= R || tok >= n) continue;
+            if (sp.part >= 0) {
+                const size_t to = part_row(a, sp.part, row);
+                float* dims = part_dims(a) + to * D;
+                if (q == 0) part_stats(a)[to] = make_float4(m[t], l[t], used[t], 0.f);
 #pragma unroll
                 for (int x = 0; x < VS; ++x)
 #pragma unroll
-                    for (int c = 0; c < VL; ++c)
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = N::dim_of(x, 4 * q + e, D);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            to[(16 * t + col) * N::LDO + N::VD * x + RUN * q + VL * e + c] =
-                                o[t][x][c][e];
-            }
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float* from = xo + wave * N::ROWS * N::LDO;
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const float4 y = xs[wave * N::ROWS + 16 * t + col];
-                const float m_new = fmaxf(m[t], y.x), base = base_of(m_new);
-                const float fa = exp2_(m[t] - base), fb = exp2_(y.x - base);
-                m[t] = m_new;
-                l[t] = l[t] * fa + y.y * fb;
-                odd |= y.z != 0.f;
+                        for (int c = 0; c < VL; ++c)
+                            if (MODE != kElem || d + c < D) dims[d + c] = o[t][x][c][e];
+                    }
+            } else {
+                T* to = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2];
+                // (0: nothing visible, or no score above -infinity)
+                const float inv = used[t] == 0.f ? 0.f : 1.f / used[t];
+                if (q == 0 && a.lse)
+                    a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
+                        l[t] == 0.f ? -INFINITY : (m[t] + log2f(l[t])) * kLn2;
 #pragma unroll
                 for (int x = 0; x < VS; ++x)
 #pragma unroll
-                    for (int c = 0; c < VL; ++c)
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = N::dim_of(x, 4 * q + e, D);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            o[t][x][c][e] = o[t][x][c][e] * fa +
-                                            fb * from[(16 * t + col) * N::LDO + N::VD * x +
-                                                      RUN * q + VL * e + c];
+                        for (int c = 0; c < VL; ++c)
+                            if (MODE != kElem || d + c < D) Elem<T>::st(to, d + c, o[t][x][c][e] * inv);
+                    }
             }
         }
-    }
-    if (wave != 0) return;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int row = tile * N::ROWS + 16 * t + col;
-        const int h = g * rep + row / a.d.T, tok = row % a.d.T;
-        if (row >= R || tok >= n) continue;
-        const size_t at = (size_t)(bg - a.bg0) * R + row;
-        if (nsplit > 1) {
-            float* to = parts_of(a) + (at * nsplit + split) * D;
-            if (q == 0) stats_of(a)[at * nsplit + split] = make_float2(m[t], l[t]);
-#pragma unroll
-            for (int x = 0; x < VS; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int c = 0; c < VL; ++c) {
-                        const int d = N::VD * x + RUN * q + VL * e + c;
-                        if (EXACT || d < D) to[d] = o[t][x][c][e];
-                    }
-        } else {
-            T* to = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2];
-            // (l == 0: nothing visible, or no score above -infinity)
-            const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
-            if (q == 0 && a.lse)
-                a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] = l[t] == 0.f ? -INFINITY : (m[t] + log2f(l[t])) * kLn2;
-#pragma unroll
-            for (int x = 0; x < VS; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int c = 0; c < VL; ++c) {
-                        const int d = N::VD * x + RUN * q + VL * e + c;
-                        if (EXACT || d < D) Elem<T>::st(to, d, o[t][x][c][e] * inv);
-                    }
+        if (__builtin_amdgcn_ballot_w64(odd)) {
+            __threadfence_block();  // (this wave's own stores, from other lanes)
+            for (int r = 0; r < N::ROWS; ++r)
+                add_not_finite<T>(a, sp, tile * N::ROWS + r, n, 0, D, lane);
         }
-    }
-    if (__builtin_amdgcn_ballot_w64(odd)) {
-        __threadfence_block();  // (this wave's own stores, from other lanes)
-        for (int r = 0; r < N::ROWS; ++r)
-            add_not_finite<T>(a, bg, tile * N::ROWS + r, split, n, 0, D, lane);
     }
 }
 
@@ -370,19 +485,20 @@ k_tree_narrow(TreeArgs a) {
 // Keys lie in blocks of 32: the cache's, then the drafts'.
 constexpr int kBlock = 32;
 constexpr int kScoreWaves = 8;
+constexpr int kWaves = 4;        // of a value workgroup
 constexpr int kValueKeys = 128;  // keys between barriers of k_tree_values
 
-template <typename T, int MT, bool EXACT>
+template <typename T, int MT>
 __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
-    using N = CacheTiles<T, 64, MT, EXACT>;
-    constexpr int EL = N::EL, SUB = kBlock / 16;
+    using N = CacheTiles<T, 64, MT, kExact>;
+    constexpr int SUB = kBlock / 16;
     __shared__ v4f red[kScoreWaves][MT * SUB * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
     const int tiles = a.plan.row_tiles, most = a.plan.ld_scores / kBlock;
     int unit, tile;
-    tile_of(blockIdx.x, a.bgs * most, tiles, &unit, &tile);
-    const int i = unit % most, bgl = unit / most, bg = a.bg0 + bgl, g = bg % a.c.G, b = bg / a.c.G;
+    tile_of(blockIdx.x, a.bs * a.gs * most, tiles, &unit, &tile);
+    const int i = unit % most, pair = unit / most, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
     const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), D = a.c.D;
     const int cache = (L + kBlock - 1) / kBlock;
     const int all = cache + (a.d.K ? (n + kBlock - 1) / kBlock : 0);
@@ -395,18 +511,17 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
         const int64_t r = j0 + min(16 * u + col, rows - 1);
-        kp[u] = (in ? (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1] + r * a.c.ks[2]
-                    : (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1] + r * a.d.ks[2]) +
-                EL * q;
+        kp[u] = in ? (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1] + r * a.c.ks[2]
+                   : (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1] + r * a.d.ks[2];
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {  // (rows past R: the last one's scores, which nobody reads)
         const int row = min((tile * MT + t) * 16 + col, R - 1);
         qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + (g * rep + row / a.d.T) * a.d.qs[1] +
-                (row % a.d.T) * a.d.qs[2] + EL * q;
+                (row % a.d.T) * a.d.qs[2];
     }
     v4f s[MT][SUB];
-    wide_scores<T, MT, EXACT, kScoreWaves>(s, kp, qp, D, wave, q);
+    wide_scores<T, MT, kScoreWaves>(s, kp, qp, D, wave, q);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -425,243 +540,339 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
         const bool on = k0 + e < rows && row < R && (in || sees(a.d, b, tok, j0 + k0 + e));
         y[e] = on ? x[e] * a.scale : -INFINITY;
     }
-    float* to = a.scores + ((size_t)bgl * tiles * N::ROWS + row) * a.plan.ld_scores + i * kBlock + k0;
+    float* to =
+        a.scores + ((size_t)pair * tiles * N::ROWS + row) * a.plan.ld_scores + i * kBlock + k0;
     *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
 }
 
-template <typename T, int MT, bool EXACT>
-__global__ __launch_bounds__(64 * kWaves) void k_tree_values(TreeArgs a) {
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : MT == 2 ? 2 : 1) void k_tree_values(TreeArgs a) {
     constexpr bool kBf = sizeof(T) == 2;
-    // (a wave's dims: one V step of 128 in bf16, 64 in fp32)
-    using N = CacheTiles<T, kBf ? 128 : 64, MT, EXACT>;
-    constexpr int VL = N::VL, WD = N::VD, ROWS = N::ROWS, PK = N::KB;
+    // (a wave's dims: one V step of 128 in bf16, 64 in fp32; where the row ends before, its last
+    // ones; those before d0 are the wave's before)
+    using N = CacheTiles<T, kBf ? 128 : 64, MT, kClamp>;
+    constexpr int VL = N::VL, WD = N::VD, ROWS = N::ROWS, PK = N::KB, NB = kValueKeys / PK;
     constexpr int LDP = kValueKeys + 16 / (int)sizeof(T);
     __shared__ __align__(16) T pl[2][ROWS * LDP];
     __shared__ float alpha[2][ROWS];
-    __shared__ float2 fin[ROWS];
+    __shared__ float4 fin[ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
     const int D = a.c.D, groups = (D + WD * kWaves - 1) / (WD * kWaves);
-    const int tiles = a.plan.row_tiles, nsplit = a.plan.nsplit;
+    const int tiles = a.plan.row_tiles;
     int unit, tile;
-    tile_of(blockIdx.x, a.bgs * nsplit * groups, tiles, &unit, &tile);
-    const int split = unit / groups % nsplit, bgl = unit / groups / nsplit, bg = a.bg0 + bgl;
-    const int d0 = (unit % groups * kWaves + wave) * WD;
-    const int g = bg % a.c.G, b = bg / a.c.G;
-    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
+    tile_of(blockIdx.x, a.plan.ranges * groups, tiles, &unit, &tile);
+    const int range = unit / groups, d0 = (unit % groups * kWaves + wave) * WD;
     const int rep = a.d.H / a.c.G, R = rep * a.d.T;
-    const int cache = (L + kBlock - 1) / kBlock;
-    const int all = cache + (a.d.K ? (n + kBlock - 1) / kBlock : 0);
-    const int per = split_blocks(all, nsplit);
-    const int first = min(split * per, all), last = min(first + per, all);
-    if (first >= last && split > 0) return;
-    const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1] + d0;
-    const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d0;
-    const float* sc = a.scores + ((size_t)bgl * tiles + tile) * ROWS * a.plan.ld_scores;
-
+    const bool busy = d0 < D;
     // softmax: 16 threads a row, 8 keys each, one pass per 16 rows
     const int sr = threadIdx.x >> 4, sk = (threadIdx.x & 15) * 8;
-    float m[MT], l[MT];
-    v4f o[MT][1][VL];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.f;
-#pragma unroll
-        for (int c = 0; c < VL; ++c) o[t][0][c] = v4f{0.f, 0.f, 0.f, 0.f};
+
+    int at = 0, end = 1;
+    if (a.plan.split) {
+        const Line line = line_of(a, kBlock, kValueKeys / kBlock, lane);
+        at = range * line.per;
+        end = min(line.total, at + line.per);
     }
-    bool odd = false;
-    int buf = 0;
-    for (int i0 = first; i0 < last; i0 += kValueKeys / kBlock, buf ^= 1) {
-        const int k1 = (last - i0) * kBlock;  // scores of this step
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            float x[8];
-            const float* from = sc + (size_t)(16 * t + sr) * a.plan.ld_scores + i0 * kBlock + sk;
-            if (sk < k1) {
-                const float4 u = *reinterpret_cast<const float4*>(from);
-                const float4 w = *reinterpret_cast<const float4*>(from + 4);
-                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-                x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = -INFINITY;
-            }
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
-            top = fmaxf(top, dpp<kDppQuadXor1>(top));
-            top = fmaxf(top, dpp<kDppQuadXor2>(top));
-            top = fmaxf(top, dpp<kDppRowHalfMirror>(top));
-            top = fmaxf(top, dpp<kDppRowMirror>(top));
-            const float m_new = fmaxf(m[t], top), base = base_of(m_new);
-            const float f = exp2_(m[t] - base);
-            m[t] = m_new;
-            l[t] *= f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = exp2_(x[e] - base);
-                l[t] += x[e];
-            }
-            if ((threadIdx.x & 15) == 0) alpha[buf][16 * t + sr] = f;
-            T* to = pl[buf] + (16 * t + sr) * LDP + sk;
-            if constexpr (kBf) {
-                // (weights as bf16: see CacheTiles::accumulate)
-                uint4 w;
-                w.x = pack2(x[0], x[1]), w.y = pack2(x[2], x[3]);
-                w.z = pack2(x[4], x[5]), w.w = pack2(x[6], x[7]);
-                *reinterpret_cast<uint4*>(to) = w;
-            } else {
-                *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            }
-        }
-        // (two buffers: a wave past this barrier writes the other one, and comes to write this
-        // one only after the next barrier, when every wave has read it)
-        __syncthreads();
-        if (d0 >= D) continue;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const float f = alpha[buf][16 * t + col];
-            if (__builtin_amdgcn_ballot_w64(f != 1.f)) {
-#pragma unroll
-                for (int c = 0; c < VL; ++c) o[t][0][c] *= f;
-            }
-        }
-        for (int k = 0; k < kValueKeys && k < k1; k += PK) {
-            const int i = i0 + k / kBlock, sub = k % kBlock;
-            const bool in = i < cache;
-            const int j0 = (in ? i : i - cache) * kBlock + sub;
-            const int rows = min(PK, (in ? L : n) - j0);
-            if (rows <= 0) continue;  // (fp32: the second half of a last block)
-            typename N::Vals v;
-            const int64_t s = in ? a.c.vs[2] : a.d.vs[2];
-            N::load_v(v, (in ? vc : vd) + j0 * s, s, rows, D - d0, lane);
-            if (!in) odd |= clear_not_finite<T>(v);
-            N::accumulate_lds(o, v, pl[buf] + k, LDP, lane);
-        }
-    }
-    // sums of the rows, for the waves that hold their outputs
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        float x = l[t];
-        x += dpp<kDppQuadXor1>(x);
-        x += dpp<kDppQuadXor2>(x);
-        x += dpp<kDppRowHalfMirror>(x);
-        x += dpp<kDppRowMirror>(x);
-        if ((threadIdx.x & 15) == 0) fin[16 * t + sr] = make_float2(m[t], x);
-    }
-    __syncthreads();
-    if (d0 >= D) return;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int row = tile * ROWS + 16 * t + col, tok = row % a.d.T, h = g * rep + row / a.d.T;
-        if (row >= R || tok >= n) continue;
-        const float2 z = fin[16 * t + col];
-        const size_t at = (size_t)bgl * R + row;
-        const bool teller = q == 0 && d0 == 0;
-        if (nsplit > 1) {
-            float* to = parts_of(a) + (at * nsplit + split) * D + d0;
-            if (teller) stats_of(a)[at * nsplit + split] = z;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int c = 0; c < VL; ++c) {
-                    const int d = N::RUN * q + VL * e + c;
-                    if (EXACT || d0 + d < D) to[d] = o[t][0][c][e];
-                }
+    while (at < end) {
+        Span sp;
+        if (a.plan.split) {
+            sp = span_at(a, range, at, end, kBlock, lane, &at);
         } else {
-            T* to = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2] + d0;
-            const float inv = z.y == 0.f ? 0.f : 1.f / z.y;
-            if (teller && a.lse)
-                a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
-                    z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int c = 0; c < VL; ++c) {
-                    const int d = N::RUN * q + VL * e + c;
-                    if (EXACT || d0 + d < D) Elem<T>::st(to, d, o[t][0][c][e] * inv);
-                }
+            sp = span_whole(a, range, kBlock);
+            at = end;
         }
-    }
-    if (odd) {
-        __threadfence_block();
-        for (int r = 0; r < ROWS; ++r)
-            add_not_finite<T>(a, bg, tile * ROWS + r, split, n, d0, min(D, d0 + WD), lane);
+        const int b = sp.b, g = sp.g, L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
+        const int cache = (L + kBlock - 1) / kBlock;
+        const bool none = L == 0 && (!a.d.K || n == 0);  // a pair without keys has no scores either
+        const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1] + d0;
+        const float* sc = a.scores +
+                          ((size_t)((b - a.b0) * a.gs + g - a.g0) * tiles + tile) * ROWS *
+                              a.plan.ld_scores;
+        float m[MT], l[MT], used[MT], x[MT][8];
+        v4f o[MT][1][VL];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = used[t] = 0.f;
+#pragma unroll
+            for (int c = 0; c < VL; ++c) o[t][0][c] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        bool odd = false;
+        // scores of the step at block i
+        auto load_x = [&](int i) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float* from = sc + (size_t)(16 * t + sr) * a.plan.ld_scores + i * kBlock + sk;
+                float4 u, w;
+                u.x = u.y = u.z = u.w = -INFINITY;
+                w = u;
+                if (sk < (sp.last - i) * kBlock) {
+                    u = *reinterpret_cast<const float4*>(from);
+                    w = *reinterpret_cast<const float4*>(from + 4);
+                }
+                x[t][0] = u.x, x[t][1] = u.y, x[t][2] = u.z, x[t][3] = u.w;
+                x[t][4] = w.x, x[t][5] = w.y, x[t][6] = w.z, x[t][7] = w.w;
+            }
+        };
+        // ... into weights in LDS
+        auto weights = [&](int buf) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                float top = x[t][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) top = fmaxf(top, x[t][e]);
+                top = fmaxf(top, dpp<kDppQuadXor1>(top));
+                top = fmaxf(top, dpp<kDppQuadXor2>(top));
+                top = fmaxf(top, dpp<kDppRowHalfMirror>(top));
+                top = fmaxf(top, dpp<kDppRowMirror>(top));
+                const float m_new = fmaxf(m[t], top), base = base_of(m_new);
+                const float f = exp2_(m[t] - base);
+                m[t] = m_new;
+                l[t] *= f;
+                used[t] *= f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[t][e] = exp2_(x[t][e] - base);
+                    l[t] += x[t][e];
+                }
+                if ((threadIdx.x & 15) == 0) alpha[buf][16 * t + sr] = f;
+                T* to = pl[buf] + (16 * t + sr) * LDP + sk;
+                if constexpr (kBf) {  // (rounded: see CacheTiles::accumulate)
+                    uint32_t w[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        w[h] = pack2(x[t][2 * h], x[t][2 * h + 1]);
+                        used[t] = add2(w[h], used[t]);
+                    }
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    *reinterpret_cast<float4*>(to) =
+                        make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
+                    *reinterpret_cast<float4*>(to + 4) =
+                        make_float4(x[t][4], x[t][5], x[t][6], x[t][7]);
+                }
+            }
+        };
+        auto rescale = [&](int buf) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float f = alpha[buf][16 * t + col];
+                if (__builtin_amdgcn_ballot_w64(f != 1.f)) {
+#pragma unroll
+                    for (int c = 0; c < VL; ++c) o[t][0][c] *= f;
+                }
+            }
+        };
+        auto load_whole = [&](typename N::Vals& v, int j) {  // rows j .. of the cache
+            N::template load_v<true>(v, vc + (int64_t)j * a.c.vs[2], a.c.vs[2], PK, D - d0, lane);
+        };
+        // Two buffers of weights: a wave past a barrier writes the other one, and comes to write
+        // this one only after the next barrier, when every wave has read it.
+        int i = sp.first, buf = 0;
+        const int whole = min(sp.last, L / kBlock);
+        constexpr int STEP = kValueKeys / kBlock;
+        __syncthreads();  // (the last span's)
+        if (!none && i < sp.last) load_x(i);
+        // steps of whole cache blocks: the next rows of V and the next scores on their way
+        if (i + STEP <= whole) {
+            typename N::Vals v[2];
+            if (busy) load_whole(v[0], i * kBlock);
+            for (; i + STEP <= whole; i += STEP, buf ^= 1) {
+                weights(buf);
+                if (i + STEP < sp.last) load_x(i + STEP);
+                __syncthreads();
+                if (!busy) continue;
+                rescale(buf);
+#pragma unroll
+                for (int k = 0; k < NB; ++k) {
+                    if (k + 1 < NB || i + 2 * STEP <= whole)
+                        load_whole(v[(k + 1) & 1], i * kBlock + (k + 1) * PK);
+                    __builtin_amdgcn_sched_barrier(0);
+                    N::accumulate_lds(o, v[k & 1], pl[buf] + k * PK, LDP, lane);
+                }
+            }
+        }
+        for (; !none && i < sp.last; i += STEP, buf ^= 1) {
+            weights(buf);
+            if (i + STEP < sp.last) load_x(i + STEP);
+            __syncthreads();
+            if (!busy) continue;
+            rescale(buf);
+            for (int k = 0; k < kValueKeys && k < (sp.last - i) * kBlock; k += PK) {
+                const int x = i + k / kBlock;
+                const bool in = x < cache;
+                const int j0 = (in ? x : x - cache) * kBlock + k % kBlock;
+                const int rows = min(PK, (in ? L : n) - j0);
+                if (rows <= 0) continue;  // (fp32: the second half of a last block)
+                const T* vb = in ? vc : (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d0;
+                const int64_t s = in ? a.c.vs[2] : a.d.vs[2];
+                typename N::Vals v;
+                N::template load_v<false>(v, vb + j0 * s, s, rows, D - d0, lane);
+                if (!in) odd |= clear_not_finite<T>(v);
+                N::accumulate_lds(o, v, pl[buf] + k, LDP, lane);
+            }
+        }
+        // sums of the rows, for the waves that hold their outputs
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float y = row16_sum(l[t]), z = kBf ? row16_sum(used[t]) : y;
+            if ((threadIdx.x & 15) == 0) fin[16 * t + sr] = make_float4(m[t], y, z, 0.f);
+        }
+        __syncthreads();
+        if (!busy) continue;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int row = tile * ROWS + 16 * t + col, tok = row % a.d.T, h = g * rep + row / a.d.T;
+            if (row >= R || tok >= n) continue;
+            const float4 z = fin[16 * t + col];
+            const bool teller = q == 0 && d0 == 0;
+            if (sp.part >= 0) {
+                const size_t to = part_row(a, sp.part, row);
+                float* dims = part_dims(a) + to * D + d0;
+                if (teller) part_stats(a)[to] = z;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = N::dim_of(0, 4 * q + e, D - d0);
+#pragma unroll
+                    for (int c = 0; c < VL; ++c)
+                        if (d + c >= 0) dims[d + c] = o[t][0][c][e];
+                }
+            } else {
+                T* to = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2] + d0;
+                const float inv = z.z == 0.f ? 0.f : 1.f / z.z;
+                if (teller && a.lse)
+                    a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
+                        z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = N::dim_of(0, 4 * q + e, D - d0);
+#pragma unroll
+                    for (int c = 0; c < VL; ++c)
+                        if (d + c >= 0) Elem<T>::st(to, d + c, o[t][0][c][e] * inv);
+                }
+            }
+        }
+        if (odd) {
+            __threadfence_block();
+            for (int r = 0; r < ROWS; ++r)
+                add_not_finite<T>(a, sp, tile * ROWS + r, n, d0, min(D, d0 + WD), lane);
+        }
     }
 }
 
-// ---------------------------------------------------------------- splits
-// The splits of a row added up: one workgroup per (row, 256 dims).
+// ---------------------------------------------------------------- parts
+// The parts of a row added up, in their order: a workgroup per (row, 256 dims), its 4 waves
+// every fourth part.  Rows of one range alone are written already.
 template <typename T>
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb) {
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn) {
+    __shared__ float acc[4][256];
+    __shared__ float2 sums[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int D = a.c.D, chunks = (D + 255) / 256, rep = a.d.H / a.c.G, R = rep * a.d.T;
-    const size_t at = blockIdx.x / chunks;
-    const int d = (blockIdx.x % chunks) * 256 + threadIdx.x;
-    const int row = at % R, bg = a.bg0 + (int)(at / R), g = bg % a.c.G, b = bg / a.c.G;
+    const int d0 = (blockIdx.x % chunks) * 256, row = blockIdx.x / chunks % R;
+    const int pair = blockIdx.x / chunks / R, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
     const int tok = row % a.d.T, h = g * rep + row / a.d.T;
-    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), nsplit = a.plan.nsplit;
-    if (tok >= n) return;
-    const int all = (L + kb - 1) / kb + (a.d.K ? (n + kb - 1) / kb : 0);
-    const int per = split_blocks(all, nsplit), used = all > 0 ? (all + per - 1) / per : 1;
-    const float2* st = stats_of(a) + at * nsplit;
-    const float* part = parts_of(a) + at * nsplit * D;
-    float M = -INFINITY, l = 0.f, acc = 0.f;
-    for (int s = 0; s < used; ++s) M = fmaxf(M, st[s].x);
+    if (tok >= drafts_of(a.d, b)) return;
+    int before = 0, total = 0;  // blocks of a kv head of the sequences before, and of all
+    for (int i = lane; i < a.bs; i += 64) {
+        const int n = blocks_of(a, a.b0 + i, kb);
+        total += n;
+        if (a.b0 + i < b) before += n;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        total += __shfl_xor(total, o);
+        before += __shfl_xor(before, o);
+    }
+    const int blocks = blocks_of(a, b, kb);
+    const Line line = line_from(a, total * a.gs, turn);
+    const int first = before * a.gs + (g - a.g0) * blocks;
+    const int r0 = first / line.per, r1 = (first + blocks - 1) / line.per;
+    if (r0 == r1) return;
+    const float4* st = part_stats(a);
+    // part i is range r0 + i's: its second where the pair begins, its first after that
+    auto row_of = [&](int i) { return part_row(a, 2 * (r0 + i) + (i == 0 ? 1 : 0), row); };
+    const int parts = r1 - r0 + 1;
+    float M = -INFINITY;
+    for (int i = lane; i < parts; i += 64) M = fmaxf(M, st[row_of(i)].x);
+    M = wave_max(M);
     const float base = base_of(M);
+    float l = 0.f, used = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = 0; s < used; ++s) {
-        const float f = exp2_(st[s].x - base);
-        l += f * st[s].y;
-        if (d < D) {
-            const float x = part[(size_t)s * D + d];
+    for (int i = wave; i < parts; i += 4) {
+        const size_t at = row_of(i);
+        const float4 z = st[at];
+        const float f = exp2_(z.x - base);
+        l += f * z.y;
+        used += f * z.z;
+        const float* from = part_dims(a) + at * D + d0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int d = lane + 64 * c;
+            const float y = d0 + d < D ? from[d] : 0.f;
             // (infinity times a weight too small for fp32 stays infinity)
-            acc += f == 0.f && !(fabsf(x) < INFINITY) ? x : f * x;
+            x[c] += f == 0.f && !(fabsf(y) < INFINITY) ? y : f * y;
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (d < D) Elem<T>::st((T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2], d, acc * inv);
-    if (d == 0 && a.lse)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[wave][lane + 64 * c] = x[c];
+    if (lane == 0) sums[wave] = make_float2(l, used);
+    __syncthreads();
+    l = (sums[0].x + sums[1].x) + (sums[2].x + sums[3].x);
+    used = (sums[0].y + sums[1].y) + (sums[2].y + sums[3].y);
+    const float inv = used == 0.f ? 0.f : 1.f / used;
+    const int d = threadIdx.x;
+    if (d0 + d < D)
+        Elem<T>::st((T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2], d0 + d,
+                    ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv);
+    if (d0 + d == 0 && a.lse)
         a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
             l == 0.f ? -INFINITY : (M + log2f(l)) * kLn2;
 }
 
-template <typename T, int DP, int MT>
+// ---------------------------------------------------------------- launches
+template <typename T, int DP, int MT, int MODE>
 void go_narrow(const TreeArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)(a.bgs * a.plan.row_tiles * a.plan.nsplit));
-    if (a.c.D == DP)
-        hipLaunchKernelGGL((k_tree_narrow<T, DP, MT, true>), grid, dim3(64 * kWaves), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_tree_narrow<T, DP, MT, false>), grid, dim3(64 * kWaves), 0, st, a);
+    const dim3 grid((unsigned)(a.plan.ranges * a.plan.row_tiles));
+    if constexpr (MT <= 2 && DP <= 128) {
+        if (a.plan.waves == 8) {
+            hipLaunchKernelGGL((k_tree_narrow<T, DP, MT, MODE, 8>), grid, dim3(512), 0, st, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_tree_narrow<T, DP, MT, MODE, 4>), grid, dim3(256), 0, st, a);
+}
+
+template <typename T, int DP, int MODE>
+void go_rows(const TreeArgs& a, hipStream_t st) {
+    if (a.plan.rows == 16) return go_narrow<T, DP, 1, MODE>(a, st);
+    if (a.plan.rows == 32) return go_narrow<T, DP, 2, MODE>(a, st);
+    if constexpr (DP <= 128 && sizeof(T) == 2) go_narrow<T, DP, 4, MODE>(a, st);
 }
 
 template <typename T, int DP>
-void go_rows(const TreeArgs& a, hipStream_t st) {
-    if (a.plan.rows == 16) return go_narrow<T, DP, 1>(a, st);
-    if (a.plan.rows == 32) return go_narrow<T, DP, 2>(a, st);
-    if constexpr (DP <= 128 && sizeof(T) == 2) go_narrow<T, DP, 4>(a, st);
+void go_dims(const TreeArgs& a, hipStream_t st) {
+    if (a.c.D == DP) return go_rows<T, DP, kExact>(a, st);
+    if constexpr (DP == 64) {
+        if (a.c.D < 16 / (int)sizeof(T)) return go_rows<T, DP, kElem>(a, st);
+    }
+    go_rows<T, DP, kClamp>(a, st);
 }
 
-template <typename T>
-constexpr int kWideDims = (sizeof(T) == 2 ? 128 : 64) * kWaves;  // dims of a value workgroup
-
-template <typename T, int MT, bool EXACT>
-void go_wide(const TreeArgs& a, hipStream_t st) {
-    const int tiles = a.bgs * a.plan.row_tiles;
-    hipLaunchKernelGGL((k_tree_scores<T, MT, EXACT>),
-                       dim3((unsigned)(tiles * (a.plan.ld_scores / kBlock))),
-                       dim3(64 * kScoreWaves), 0, st, a);
-    const int groups = (a.c.D + kWideDims<T> - 1) / kWideDims<T>;
-    hipLaunchKernelGGL((k_tree_values<T, MT, EXACT>), dim3((unsigned)(tiles * a.plan.nsplit * groups)),
-                       dim3(64 * kWaves), 0, st, a);
-}
+// dims of a value workgroup
+constexpr int wide_dims(bool bf) { return (bf ? 128 : 64) * kWaves; }
 
 template <typename T, int MT>
 void go_wide(const TreeArgs& a, hipStream_t st) {
-    // (exact: a wave's steps over the dims all lie inside the row)
-    if (a.c.D % 128 == 0) return go_wide<T, MT, true>(a, st);
-    go_wide<T, MT, false>(a, st);
+    hipLaunchKernelGGL(
+        (k_tree_scores<T, MT>),
+        dim3((unsigned)(a.bs * a.gs * a.plan.row_tiles * (a.plan.ld_scores / kBlock))),
+        dim3(64 * kScoreWaves), 0, st, a);
+    const int wd = wide_dims(sizeof(T) == 2), groups = (a.c.D + wd - 1) / wd;
+    hipLaunchKernelGGL((k_tree_values<T, MT>),
+                       dim3((unsigned)(a.plan.ranges * groups * a.plan.row_tiles)),
+                       dim3(64 * kWaves), 0, st, a);
 }
 
 template <typename T>
@@ -672,24 +883,24 @@ void go(const TreeArgs& a, hipStream_t st) {
         else if (a.plan.rows == 32) go_wide<T, 2>(a, st);
         else go_wide<T, 4>(a, st);
     } else if (D <= 64) {
-        go_rows<T, 64>(a, st);
+        go_dims<T, 64>(a, st);
     } else if (D <= 128) {
-        go_rows<T, 128>(a, st);
+        go_dims<T, 128>(a, st);
     } else if (D <= 192) {
-        go_rows<T, 192>(a, st);
+        go_dims<T, 192>(a, st);
     } else {
-        go_rows<T, 256>(a, st);
+        go_dims<T, 256>(a, st);
     }
-    if (a.plan.nsplit > 1) {
-        const int kb = D > kTreeNarrow || sizeof(T) == 2 ? 32 : 16;
-        hipLaunchKernelGGL(
-            k_tree_merge<T>,
-            dim3((unsigned)((size_t)a.bgs * (a.d.H / a.c.G) * a.d.T * ((D + 255) / 256))), dim3(256),
-            0, st, a, kb);
+    if (a.plan.split) {
+        const bool wide = D > kTreeNarrow;
+        const size_t rows = (size_t)a.bs * a.gs * (a.d.H / a.c.G) * a.d.T;
+        hipLaunchKernelGGL(k_tree_merge<T>, dim3((unsigned)(rows * ((D + 255) / 256))), dim3(256),
+                           0, st, a, wide || sizeof(T) == 2 ? 32 : 16,
+                           wide ? kValueKeys / kBlock : a.plan.waves);
     }
 }
 
-int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
@@ -700,45 +911,64 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     const int R = H / G * T;
     const int most = wide || (bf && D <= 128) ? 64 : 32;
     p.rows = R <= 16 ? 16 : R <= 32 ? 32 : most;
-    p.row_tiles = ceil_div(R, p.rows);
-    const int kb = wide || bf ? 32 : 16;
-    const int64_t blocks = ceil_div(max_len, kb) + (draft_keys ? ceil_div(T, kb) : 0);
-    // workgroups of a pair without splits
-    const int groups = wide ? ceil_div(D, (bf ? 128 : 64) * kWaves) : 1;
-    const int64_t units = (int64_t)B * G * p.row_tiles * groups;
-    // splits of at least two blocks a wave (wide: two steps), and about three workgroups per CU
-    int64_t ns = std::max<int64_t>(1, std::min<int64_t>((768 + units - 1) / units,
-                                                        blocks / (2 * kWaves)));
-    p.ld_scores = wide ? (int)std::max<int64_t>(blocks, 1) * kBlock : 0;
-    const size_t sc = wide ? (size_t)p.row_tiles * p.rows * p.ld_scores : 0;  // floats of a pair
-    const size_t part = (size_t)R * (D + 2);                                   // ... and split
+    p.row_tiles = (int)ceil_div(R, p.rows);
+    p.waves = 4;
+    const int kb = wide || bf ? 32 : 16, mt = p.rows / 16;
+    const int64_t blocks =  // of a pair, at most
+        std::max<int64_t>(1, ceil_div(max_len, kb) + (draft_keys ? ceil_div(T, kb) : 0));
+    const int64_t pairs = (int64_t)B * G, rows = (int64_t)p.row_tiles * p.rows;
+    const int groups = wide ? (int)ceil_div(D, wide_dims(bf)) : 1;
+    p.ld_scores = wide ? (int)blocks * kBlock : 0;
+    // workgroups that the card holds at once (256 CUs; the kernels' registers)
+    const int per_cu = wide ? (mt == 1 ? 3 : mt == 2 ? 2 : 1)
+                            : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
+    const int64_t slots = std::max<int64_t>(1, 256 * per_cu / (p.row_tiles * groups));
+    const int64_t turn = wide ? kValueKeys / kBlock : p.waves;
+    int64_t ranges = std::min(slots, ceil_div(pairs * blocks, 2 * turn));
+    // one workgroup of 8 waves a pair where that leaves a wave few blocks: no second launch
+    const bool small = !wide && mt <= 2 && D <= 128 && blocks <= 32 && pairs * p.row_tiles <= 512;
+    p.split = !small && ranges > 1 && pairs < 4 * slots && blocks > turn;
+    if (small) p.waves = 8;
     const size_t room = scratch_cap / sizeof(float);
-    // fewer splits where the scratch does not hold them, then fewer pairs at a time
-    auto need = [&](int64_t heads, int64_t n) { return heads * (sc + (n > 1 ? n * part : 0)); };
-    const int64_t pairs = (int64_t)B * G;
-    while (ns > 1 && need(pairs, ns) > room) --ns;
-    p.nsplit = (int)ns;
-    p.heads = (int)pairs;
-    if (need(pairs, ns) > room) p.heads = (int)std::max<size_t>(1, room / std::max<size_t>(sc, 1));
-    p.scores = sc * p.heads;
-    p.scratch = need(p.heads, ns) * sizeof(float);
-    const int64_t most_groups = wide ? std::max<int64_t>(groups * ns, p.ld_scores / kBlock) : ns;
-    p.workgroups = std::max((int64_t)p.heads * p.row_tiles * most_groups,
-                            (int64_t)p.heads * R * ceil_div(D, 256));
+    const size_t sc = wide ? (size_t)rows * p.ld_scores : 0;  // floats of a pair
+    const size_t part = 2 * (size_t)rows * (D + 4);           // ... of a range
+    int64_t in_pass = pairs;
+    if (sc * pairs + (p.split ? part * ranges : 0) > room) {
+        // fewer pairs a pass where the scratch does not hold their scores, fewer ranges where it
+        // does not hold their parts
+        const size_t for_parts = p.split ? std::min(room / 2, (size_t)ranges * part) : 0;
+        if (sc > 0)
+            in_pass = std::max<int64_t>(1, std::min<int64_t>(pairs, (room - for_parts) / sc));
+        const size_t left = room > sc * in_pass ? room - sc * in_pass : 0;
+        ranges = std::min<int64_t>(ranges, left / part);
+        if (ranges < 2) p.split = 0;
+    }
+    p.seqs = in_pass >= G ? (int)(in_pass / G) : 1;
+    p.kv = in_pass >= G ? G : (int)in_pass;
+    in_pass = (int64_t)p.seqs * p.kv;
+    p.ranges = (int)(p.split ? ranges : in_pass);
+    p.scores = sc * in_pass;
+    p.scratch = (p.scores + (p.split ? part * ranges : 0)) * sizeof(float);
+    p.workgroups = std::max({(int64_t)p.ranges * p.row_tiles * groups,
+                             in_pass * p.row_tiles * (p.ld_scores / kBlock),
+                             in_pass * R * ceil_div(D, 256)});
     return p;
 }
 
 hipError_t launch_tree_attention(int dtype, TreeArgs a, hipStream_t st) {
-    const int pairs = a.c.B * a.c.G;
-    for (a.bg0 = 0; a.bg0 < pairs; a.bg0 += a.plan.heads) {
-        a.bgs = std::min(a.plan.heads, pairs - a.bg0);
-        if (dtype == kDtypeF32)
-            go<float>(a, st);
-        else
-            go<uint16_t>(a, st);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
+    for (a.b0 = 0; a.b0 < a.c.B; a.b0 += a.plan.seqs)
+        for (a.g0 = 0; a.g0 < a.c.G; a.g0 += a.plan.kv) {
+            a.bs = std::min(a.plan.seqs, a.c.B - a.b0);
+            a.gs = std::min(a.plan.kv, a.c.G - a.g0);
+            TreeArgs pass = a;
+            if (!a.plan.split) pass.plan.ranges = a.bs * a.gs;
+            if (dtype == kDtypeF32)
+                go<float>(pass, st);
+            else
+                go<uint16_t>(pass, st);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
     return hipSuccess;
 }
 
