@@ -132,6 +132,9 @@ int check_drafts(const atn_kv_cache* c, const atn_drafts* d, bool need_q, bool n
     v->H = d->heads;
     v->T = d->tokens;
     v->W = (d->tokens + 31) / 32;
+    v->by_t = d->tokens > 1 ? (uint32_t)(((1ull << 32) + d->tokens - 1) / d->tokens) : 0;
+    // (rows of a kv head times tokens below 2^32: the division by multiplication is exact)
+    if ((int64_t)(d->heads / c->kv_heads) * d->tokens >= (1 << 24)) return ATN_ERR_SIZE_OVERFLOW;
     return ATN_OK;
 }
 

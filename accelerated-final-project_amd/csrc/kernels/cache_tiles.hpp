@@ -94,19 +94,12 @@ __device__ __forceinline__ void clear_first(Words<T, BYTES>& v, int z) {
     }
 }
 
-// x, as a value that the compiler knows nothing about from here on: what follows is computed
-// where it stands, not kept in registers across a loop.
+// x, as a value that the compiler knows nothing about: what follows is computed where it stands,
+// not before a loop and kept in registers across it.
 __device__ __forceinline__ int opaque(int x) {
     asm volatile("" : "+v"(x));
     return x;
 }
-template <typename T>
-__device__ __forceinline__ const T* opaque(const T* p) {
-    uint64_t x = (uint64_t)p;
-    asm volatile("" : "+v"(x));
-    return (const T*)(const __attribute__((address_space(1))) T*)x;  // (global loads, not flat)
-}
-
 // How the pieces of a row of D elements are read.  kExact: every piece lies in the row.
 // kClamp (D holds a piece at least): a piece that would pass the row's end is read where the row
 // ends.  In a score the elements that other pieces hold already are then cleared, in K and Q
@@ -163,17 +156,13 @@ struct CacheTiles {
         }
     }
 
-    // K of a block whose first row is `base`.  FULL: of KB rows, else `rows` (the last one again
-    // in the places behind)
-    template <bool FULL>
-    static __device__ __forceinline__ void load_k(Keys& k, const T* base, int64_t stride, int rows,
-                                                  int D, int lane) {
-        if (!FULL) lane = opaque(lane);
-        const T* p0 = opaque(base + (lane & 15) * stride + EL * (lane >> 4));
+    // K of the block at row j0 of `rows` rows from `base` on (the last one again in the places
+    // behind it)
+    static __device__ __forceinline__ void load_k(Keys& k, const T* base, int64_t stride, int j0,
+                                                  int rows, int D, int lane) {
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const T* p = p0 + 16 * s * stride;
-            if (!FULL) p = base + min(16 * s + (lane & 15), rows - 1) * stride + EL * (lane >> 4);
+            const T* p = base + min(j0 + 16 * s + (lane & 15), rows - 1) * stride + EL * (lane >> 4);
 #pragma unroll
             for (int i = 0; i < KS; ++i) k.p[s][i] = piece(p, i, lane >> 4, D);
         }
@@ -189,30 +178,18 @@ struct CacheTiles {
         return MODE == kClamp ? min(d, D - VL) : d;
     }
 
-    // V of a block; rows past it are zeros: a weight of 0 times whatever they hold must be 0
-    template <bool FULL>
-    static __device__ __forceinline__ void load_v(Vals& v, const T* base, int64_t stride, int rows,
-                                                  int D, int lane) {
-        if (!FULL) lane = opaque(lane);
-        const T* p0 = opaque(base + key_of(lane, 0) * stride);
+    // V of the block, likewise (the rows behind enter with a weight of 0: whoever calls takes out
+    // what times 0 is not 0)
+    static __device__ __forceinline__ void load_v(Vals& v, const T* base, int64_t stride, int j0,
+                                                  int rows, int D, int lane) {
 #pragma unroll
         for (int j = 0; j < KEYS; ++j) {
-            const T* p = p0 + key_of(0, j) * stride;
-            if (!FULL) p = base + min(key_of(lane, j), rows - 1) * stride;
+            const T* p = base + min(j0 + key_of(lane, j), rows - 1) * stride;
 #pragma unroll
             for (int i = 0; i < VS; ++i) {
                 const int d = dim_of(i, lane & 15, D);
                 v.p[j][i] = MODE == kElem ? ld_some<VB>(p + d, D - d) : ld_words<VB>(p + d);
             }
-        }
-        if (!FULL && rows < KB) {
-#pragma unroll
-            for (int j = 0; j < KEYS; ++j)
-                if (key_of(lane, j) >= rows)
-#pragma unroll
-                    for (int i = 0; i < VS; ++i)
-#pragma unroll
-                        for (int w = 0; w < VB / 4; ++w) v.p[j][i].w[w] = 0;
         }
     }
 
@@ -247,6 +224,8 @@ struct CacheTiles {
                     o[t][i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                         __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, f[t]), o[t][i][c],
                         0, 0, 0);
+                // (the permutes of all tiles ahead of the products would take 32 registers)
+                if (c & 1) __builtin_amdgcn_sched_barrier(0);
             }
     }
 
@@ -306,19 +285,20 @@ struct CacheTiles {
     }
 };
 
-// Scores of 32 keys against 16 MT query rows over this wave's share of the dims (`waves` share
-// them), from each lane's row pointers.  All loads of a step go out before its products: left
+// Scores of 32 keys against 16 MT query rows over wave `wave`'s share of the dims (of `waves`),
+// from each lane's row pointers.  All loads of a step go out before its products: left
 // to itself the compiler keeps six in flight, and the memory idles.
-template <typename T, int MT, int WAVES>
+template <typename T, int MT>
 __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp)[2],
-                                            const T* const (&qp)[MT], int D, int wave, int q) {
+                                            const T* const (&qp)[MT], int D, int wave, int waves,
+                                            int q) {
     using N = CacheTiles<T, 64, MT, kExact>;
     constexpr int EL = N::EL, STEP = 4 * EL, U = 4;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int u = 0; u < 2; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
-    const int per = ((D + STEP * U - 1) / (STEP * U) + WAVES - 1) / WAVES * STEP * U;
+    const int per = ((D + STEP * U - 1) / (STEP * U) + waves - 1) / waves * STEP * U;
     const int d1 = min(D, (wave + 1) * per);
     typename N::KPiece k[U][2], f[U][MT];
     auto products = [&] {

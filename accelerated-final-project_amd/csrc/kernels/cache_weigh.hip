@@ -78,8 +78,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
     for (int row0 = 0; row0 == 0 || row0 < R; row0 += kRows) {
         typename N::Keys k;
         if (i0 < blocks)
-            N::template load_k<false>(k, kc + (int64_t)i0 * KB * a.c.ks[2], a.c.ks[2],
-                                      min(KB, end - i0 * KB), D, lane);
+            N::load_k(k, kc, a.c.ks[2], i0 * KB, end, D, lane);
         const int tiles = (min(kRows, R - row0) + 15) / 16;
         __syncthreads();
         for (int e = threadIdx.x; e < tiles * KS * 64; e += 64 * kWaves) {
@@ -124,8 +123,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
             }
             const int nx = i + step;
             if (nx < blocks)
-                N::template load_k<false>(k, kc + (int64_t)nx * KB * a.c.ks[2], a.c.ks[2],
-                                          min(KB, end - nx * KB), D, lane);
+                N::load_k(k, kc, a.c.ks[2], nx * KB, end, D, lane);
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const float4 w = make_float4(row16_sum(sum[u][0]), row16_sum(sum[u][1]),
@@ -165,7 +163,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
                 const QueryRow x = query_row(a, b, g, A, min(row0 + 16 * t + col, R - 1));
                 qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + x.head * a.d.qs[1] + x.tok * a.d.qs[2];
             }
-            wide_scores<T, MT, kScoreWaves>(s, kp, qp, D, wave, q);
+            wide_scores<T, MT>(s, kp, qp, D, wave, kScoreWaves, q);
         }
 #pragma unroll
         for (int t = 0; t < MT; ++t)

@@ -36,7 +36,13 @@ struct DraftView {
     const int* count;             // [B] tokens of each sequence, or null: T
     const uint32_t* mask;         // [B][T][W], or null: a chain
     int H, T, W;                  // W = ceil(T / 32)
+    uint32_t by_t;                // 2^32 / T rounded up (T > 1)
 };
+
+// A query row of a kv head (its heads, each with T tokens): head and token of `row`.
+__device__ __forceinline__ int head_of(const DraftView& d, int row) {
+    return d.T == 1 ? row : (int)__umulhi((uint32_t)row, d.by_t);
+}
 
 // The drafts of each sequence that became part of it.
 struct PathView {
@@ -89,6 +95,7 @@ struct TreePlan {
     int ranges;
     int seqs, kv;
     int ld_scores;   // head_d > 256: row of the scores, floats
+    int shares;      // ... workgroups that share the dims of a tile of scores
     size_t scores;   // floats of the scores of a pass
     size_t scratch;  // bytes
     int64_t workgroups;  // of a pass, at most
@@ -102,7 +109,7 @@ struct TreeArgs {
     float* lse;     // [B][H][T] or null
     float scale;    // times log2(e)
     TreePlan plan;
-    float* scores;  // scratch: [pairs of a pass][row tiles of rows][ld_scores]
+    float* scores;  // scratch: [shares][pairs of a pass][rows of the tiles][ld_scores]
     float* part;    // scratch: parts of rows (2 of each range and tile): statistics, dims
     int b0, bs, g0, gs;  // this pass
 };

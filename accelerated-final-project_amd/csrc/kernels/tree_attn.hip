@@ -124,15 +124,43 @@ __device__ __forceinline__ float* part_dims(const TreeArgs& a) {
 // Workgroup -> (range, tile): workgroups go to the 8 XCDs in turn, so the tiles that read the
 // same keys are 8 apart and share an L2.
 __device__ __forceinline__ void tile_of(int id, int ranges, int tiles, int* range, int* tile) {
+    if (tiles == 1) {
+        *tile = 0;
+        *range = id;
+        return;
+    }
     const int full = ranges / 8 * 8 * tiles, whole = id < full;
     const int x = whole ? id % 8 : 0, y = whole ? id / 8 : id - full;
     *tile = y % tiles;
     *range = whole ? y / tiles * 8 + x : ranges / 8 * 8 + y / tiles;
 }
 
+// The first `left` of 4 consecutive elements stored, any alignment.
+__device__ __forceinline__ void store4(float* to, const float (&x)[4], int left) {
+    if (left >= 4) {
+        __builtin_memcpy(to, x, 16);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+            if (c < left) to[c] = x[c];
+    }
+}
+__device__ __forceinline__ void store4(uint16_t* to, const float (&x)[4], int left) {
+    const uint32_t w[2] = {pack2(x[0], x[1]), pack2(x[2], x[3])};
+    if (left >= 4) {
+        __builtin_memcpy(to, w, 8);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+            if (c < left) to[c] = (uint16_t)(w[c / 2] >> (16 * (c & 1)));
+    }
+}
+
 // ---------------------------------------------------------------- infinities and NaNs
-// A draft that some rows attend and others do not: an infinity or NaN in its V belongs to the
-// first alone.  The product runs without it; it is added where the results are written.
+// A block that is not whole cache rows alone -- the cache's last rows, the drafts -- meets
+// weights of 0: places behind its rows, drafts that a row does not attend.  An infinity or NaN in
+// its V belongs only to the rows that attend it.  The product runs without it; it is added
+// where the results are written.
 // Whether any lane's V holds an infinity or NaN, which are cleared.
 template <typename T, typename V>
 __device__ __forceinline__ bool clear_not_finite(V& v) {
@@ -154,13 +182,20 @@ __device__ __forceinline__ bool clear_not_finite(V& v) {
     return __builtin_amdgcn_ballot_w64(any) != 0;
 }
 
-// What the infinities and NaNs that clear_not_finite() took out of the drafts' V add to dim d of
-// token tok: every weight is above 0, so whatever it is, theirs is the value itself.
+// What the infinities and NaNs that clear_not_finite() took out (of the cache's rows from
+// `from` to L, and of n drafts) add to dim d of token tok: every weight is above 0, so whatever
+// it is, theirs is the value itself.
 template <typename T>
-__device__ __forceinline__ float not_finite_sum(const TreeArgs& a, int b, int g, int n, int tok,
-                                                int d) {
-    const T* v = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d;
+__device__ __forceinline__ float not_finite_sum(const TreeArgs& a, int b, int g, int from, int L,
+                                                int n, int tok, int d) {
     float sum = 0.f;
+    const T* v = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1] + d;
+    for (int r = from; r < L; ++r) {
+        const float x = Elem<T>::ld(v + r * a.c.vs[2], 0);
+        if (!(fabsf(x) < INFINITY)) sum += x;
+    }
+    if (!a.d.K) return sum;
+    v = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d;
     for (int j = 0; j < n; ++j) {
         const float x = Elem<T>::ld(v + j * a.d.vs[2], 0);
         if (!(fabsf(x) < INFINITY) && sees(a.d, b, tok, j)) sum += x;
@@ -171,13 +206,13 @@ __device__ __forceinline__ float not_finite_sum(const TreeArgs& a, int b, int g,
 // not_finite_sum() added to dims [d0, d1) of a row where its result lies (a wave's work, after
 // the wave has written it): the output, or a part.
 template <typename T>
-__device__ void add_not_finite(const TreeArgs& a, const Span& s, int row, int n, int d0, int d1,
-                               int lane) {
-    const int rep = a.d.H / a.c.G, tok = row % a.d.T;
+__device__ void add_not_finite(const TreeArgs& a, const Span& s, int row, int from, int L, int n,
+                               int d0, int d1, int lane) {
+    const int rep = a.d.H / a.c.G, h = head_of(a.d, row), tok = row - h * a.d.T;
     if (row >= rep * a.d.T || tok >= n) return;
-    T* out = (T*)a.out + s.b * a.os[0] + (s.g * rep + row / a.d.T) * a.os[1] + tok * a.os[2];
+    T* out = (T*)a.out + s.b * a.os[0] + (s.g * rep + h) * a.os[1] + tok * a.os[2];
     for (int d = d0 + lane; d < d1; d += 64) {
-        const float x = not_finite_sum<T>(a, s.b, s.g, n, tok, d);
+        const float x = not_finite_sum<T>(a, s.b, s.g, from, L, n, tok, d);
         if (x == 0.f) continue;
         if (s.part >= 0)
             part_dims(a)[part_row(a, s.part, row) * a.c.D + d] += x;
@@ -189,7 +224,9 @@ __device__ void add_not_finite(const TreeArgs& a, const Span& s, int row, int n,
 // ---------------------------------------------------------------- head_d <= 256
 // Every wave walks its own blocks of keys, alone: scores, running maximum and
 // sum, and its own output tile in registers (cache_tiles.hpp); nothing passes through LDS
-// but Q and, at the end, the waves' results.
+// but Q and, at the end, the waves' results.  A launch starts with a cold instruction
+// cache, about 60 ns a 64-byte line, so what runs once is kept short: one loop for whole
+// and other blocks, results added up in a loop.
 template <typename T, int DP, int MT, int MODE, int WAVES>
 struct Narrow : CacheTiles<T, DP, MT, MODE> {
     using N = CacheTiles<T, DP, MT, MODE>;
@@ -200,11 +237,12 @@ struct Narrow : CacheTiles<T, DP, MT, MODE> {
     static constexpr bool kAhead = kWith <= 250 || kRegs > 220;
     static constexpr int kPerSimd = kWith <= 124 ? 4 : kWith <= 164 ? 3 : kRegs <= 220 ? 2 : 1;
     static constexpr int kMinWaves = WAVES == 8 ? 2 : kPerSimd;
-    static constexpr int LDO = DP + 4;  // row of the exchange, floats
+    static constexpr int LDO = DP + 4;  // row of the waves' results, floats
     static constexpr int kQBytes = N::ROWS * DP * (int)sizeof(T);
-    static constexpr int kXBytes = WAVES / 2 * N::ROWS * LDO * 4;
-    static constexpr int kOBytes = kQBytes > kXBytes ? kQBytes : kXBytes;
-    static constexpr int kLds = kOBytes + WAVES / 2 * N::ROWS * 16;
+    static constexpr int kXBytes = WAVES * N::ROWS * LDO * 4;
+    static constexpr int kLds = (kQBytes > kXBytes ? kQBytes : kXBytes) + WAVES * N::ROWS * 16;
+    static constexpr int kQ = (MT * N::KS * 64 + 64 * WAVES - 1) / (64 * WAVES);  // pieces a thread
+    static_assert(kLds <= 160 * 1024, "LDS");
 };
 
 template <typename T, int DP, int MT, int MODE, int WAVES>
@@ -219,7 +257,6 @@ k_tree_narrow(TreeArgs a) {
     tile_of(blockIdx.x, a.plan.ranges, a.plan.row_tiles, &range, &tile);
     const int D = a.c.D, rep = a.d.H / a.c.G, R = rep * a.d.T;
     const float scale = fabsf(a.scale);
-    const uint32_t flip = a.scale < 0.f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
 
     int at = 0, end = 1;
     if (a.plan.split) {
@@ -235,29 +272,43 @@ k_tree_narrow(TreeArgs a) {
             sp = span_whole(a, range, KB);
             at = end;
         }
-        const int b = sp.b, g = sp.g, L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
-        const int cache = (L + KB - 1) / KB;  // its blocks; the drafts' follow
+        const int b = sp.b, g = sp.g;
 
-        // Q in the order of the fragments: piece (t, i) of lane L is piece i of row 16 t + L % 16
+        // Q in the order of the fragments: piece (t, i) of lane L is piece i of row 16 t + L % 16.
+        // (Rows of no token hold the last token's: nobody reads their results.)
         auto* qs = reinterpret_cast<typename N::KPiece*>(lds);
-        __syncthreads();  // (the last span's exchange)
-        for (int e = threadIdx.x; e < MT * KS * 64; e += 64 * WAVES) {
-            const int el = e & 63, i = (e >> 6) % KS, t = (e >> 6) / KS;
-            const int row = tile * N::ROWS + 16 * t + (el & 15);
-            typename N::KPiece z{};
-            if (row < R && row % a.d.T < n) {
-                z = N::piece((const T*)a.d.Q + b * a.d.qs[0] + (g * rep + row / a.d.T) * a.d.qs[1] +
-                                 (row % a.d.T) * a.d.qs[2] + N::EL * (el >> 4),
-                             i, el >> 4, D);
+        {
+            typename N::KPiece z[N::kQ];
+            const T* qb = (const T*)a.d.Q + b * a.d.qs[0] + g * rep * a.d.qs[1] + N::EL * q;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) z.w[w] ^= flip;
+            for (int x = 0; x < N::kQ; ++x) {
+                const int e = x * WAVES + wave, i = e % KS, t = min(e / KS, MT - 1);
+                const int row = min(tile * N::ROWS + 16 * t + col, R - 1), h = head_of(a.d, row);
+                z[x] = N::piece(qb + h * a.d.qs[1] + (row - h * a.d.T) * a.d.qs[2], i, q, D);
             }
-            qs[e] = z;
+            if (a.scale < 0.f) {
+#pragma unroll
+                for (int x = 0; x < N::kQ; ++x)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        z[x].w[w] ^= sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+            }
+            __syncthreads();  // (the last span's results are out of LDS)
+#pragma unroll
+            for (int x = 0; x < N::kQ; ++x)
+                if (x * WAVES + wave < MT * KS) qs[(x * WAVES + wave) * 64 + lane] = z[x];
         }
         __syncthreads();
 
+        const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
+        const int cache = (L + KB - 1) / KB;  // its blocks; the drafts' follow
+        const int whole = L / KB;
         const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
         const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1];
+        const T* kd = (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
+        const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
+        // (a pair without keys has one block of none)
+        const int last = L > 0 || (a.d.K && n > 0) ? sp.last : 0;
         v4f o[MT][VS][VL];
         float m[MT], l[MT], used[MT];
 #pragma unroll
@@ -271,32 +322,71 @@ k_tree_narrow(TreeArgs a) {
         }
         bool odd = false;
         typename N::Keys k;
-        typename N::Vals v;
-        float p[MT][SUB][4];
-        auto scores = [&] {
-            v4f s[MT][SUB];
+        auto load_k = [&](int i) {
+            const bool in = i < cache;
+            N::load_k(k, in ? kc : kd, in ? a.c.ks[2] : a.d.ks[2], (in ? i : i - cache) * KB,
+                      in ? L : n, D, lane);
+        };
+        int i = sp.first + wave;
+        if (N::kAhead && i < last) load_k(i);
+        for (; i < last; i += WAVES) {
+            if (!N::kAhead) load_k(i);
+            const bool in = i < cache;
+            const int j0 = (in ? i : i - cache) * KB;
+            typename N::Vals v;
+            N::load_v(v, in ? vc : vd, in ? a.c.vs[2] : a.d.vs[2], j0, in ? L : n, D, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            float p[MT][SUB][4];
+            {
+                v4f s[MT][SUB];
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+                for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int u = 0; u < SUB; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
+                    for (int u = 0; u < SUB; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < KS; ++e)
+                for (int e = 0; e < KS; ++e)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        const typename N::KPiece f = qs[(t * KS + e) * 64 + lane];
+#pragma unroll
+                        for (int u = 0; u < SUB; ++u) s[t][u] = N::dot(k.p[u][e], f, s[t][u]);
+                    }
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[t][u][e] = s[t][u][e];
+            }
+            if (N::kAhead && i + WAVES < last) load_k(i + WAVES);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i >= whole) {
+                odd |= clear_not_finite<T>(v);
+                const int rows = (in ? L : n) - j0;
+                const uint32_t valid = rows >= 32 ? ~0u : (1u << rows) - 1;
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
-                    const typename N::KPiece f = qs[(t * KS + e) * 64 + lane];
+                    uint32_t see = valid;  // bit j: the row attends key j of the block
+                    if (!in) {
+                        const int row = tile * N::ROWS + 16 * t + col;
+                        const int tok = row - head_of(a.d, row) * a.d.T;
+                        if (a.d.mask) {
+                            see &= a.d.mask[((size_t)b * a.d.T + tok) * a.d.W + (j0 >> 5)] >>
+                                   (j0 & 31);
+                        } else {
+                            const int upto = tok - j0;  // keys 0 .. upto
+                            see &= upto < 0 ? 0u : upto >= 31 ? ~0u : (2u << upto) - 1;
+                        }
+                    }
 #pragma unroll
-                    for (int u = 0; u < SUB; ++u) s[t][u] = N::dot(k.p[u][e], f, s[t][u]);
+                    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!((see >> (16 * u + 4 * q + e)) & 1u)) p[t][u][e] = -INFINITY;
                 }
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[t][u][e] = s[t][u][e];
-        };
-        // The running maximum moves only when a score passes it by more than 8 (weights up to
-        // 2^8 lose nothing in fp32 or bf16), so the tile is rarely rescaled.
-        auto weights = [&] {
+            }
+            // The running maximum moves only when a score passes it by more than 8 (weights up
+            // to 2^8 lose nothing in fp32 or bf16), so the tile is rarely rescaled.
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 float top = p[t][0][0];
@@ -324,155 +414,92 @@ k_tree_narrow(TreeArgs a) {
                         l[t] += p[t][u][e];
                     }
             }
-        };
-
-        // whole blocks of the cache: nothing masked, the next block's loads on their way
-        const int whole = min(sp.last, L / KB);
-        int i = sp.first + wave;
-        auto k_at = [&](int x) {
-            N::template load_k<true>(k, kc + (int64_t)x * KB * a.c.ks[2], a.c.ks[2], KB, D, lane);
-        };
-        if (N::kAhead && i < whole) k_at(i);
-        for (; i < whole; i += WAVES) {
-            if (!N::kAhead) k_at(i);
-            N::template load_v<true>(v, vc + (int64_t)i * KB * a.c.vs[2], a.c.vs[2], KB, D, lane);
-            __builtin_amdgcn_sched_barrier(0);
-            scores();
-            if (N::kAhead && i + WAVES < whole) k_at(i + WAVES);
-            __builtin_amdgcn_sched_barrier(0);
-            weights();
-            N::accumulate(o, v, p, used);
-        }
-        // the cache's last block and the drafts
-        for (; i < sp.last; i += WAVES) {
-            const bool in = i < cache;
-            const int j0 = (in ? i : i - cache) * KB;
-            const int rows = min(KB, (in ? L : a.d.K ? n : 0) - j0);
-            if (rows <= 0) break;  // (the one block of a pair without any)
-            const int64_t ks = in ? a.c.ks[2] : a.d.ks[2], vs = in ? a.c.vs[2] : a.d.vs[2];
-            const T* kb = in ? kc : (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
-            const T* vb = in ? vc : (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
-            N::template load_k<false>(k, kb + j0 * ks, ks, rows, D, lane);
-            N::template load_v<false>(v, vb + j0 * vs, vs, rows, D, lane);
-            scores();
-            const uint32_t valid = rows >= 32 ? ~0u : (1u << rows) - 1;
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                uint32_t see = valid;  // bit j: the row attends key j of the block
-                if (!in) {
-                    const int row = tile * N::ROWS + 16 * t + col, tok = row % a.d.T;
-                    if (a.d.mask) {
-                        const uint32_t w =
-                            row < R ? a.d.mask[((size_t)b * a.d.T + tok) * a.d.W + (j0 >> 5)] : 0u;
-                        see &= w >> (j0 & 31);
-                    } else {
-                        const int upto = tok - j0;  // keys 0 .. upto
-                        see &= upto < 0 ? 0u : upto >= 31 ? ~0u : (2u << upto) - 1;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!((see >> (16 * u + 4 * q + e)) & 1u)) p[t][u][e] = -INFINITY;
-            }
-            if (!in) odd |= clear_not_finite<T>(v);
-            weights();
             N::accumulate(o, v, p, used);
         }
 
-        // the waves' tiles into wave 0: the upper half hands theirs to the lower, again and again
+        // The waves' results added up: each scales its own to the maximum of all and leaves it in
+        // LDS, where every thread sums a few dims over the waves and writes them.
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             l[t] = row_sum(l[t]);
             used[t] = sizeof(T) == 2 ? row_sum(used[t]) : l[t];
         }
         float* xo = reinterpret_cast<float*>(lds);
-        float4* xs = reinterpret_cast<float4*>(lds + N::kOBytes);
-        for (int half = WAVES / 2; half > 0; half /= 2) {
-            __syncthreads();
-            if (wave >= half && wave < 2 * half) {
-                float* to = xo + (wave - half) * N::ROWS * N::LDO;
+        float4* xs = reinterpret_cast<float4*>(lds + N::kLds - WAVES * N::ROWS * 16);
+        if (q == 0) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    if (q == 0)
-                        xs[(wave - half) * N::ROWS + 16 * t + col] =
-                            make_float4(m[t], l[t], used[t], odd ? 1.f : 0.f);
-#pragma unroll
-                    for (int x = 0; x < VS; ++x)
-#pragma unroll
-                        for (int c = 0; c < VL; ++c)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                to[(16 * t + col) * N::LDO + N::VD * x + N::RUN * q + VL * e + c] =
-                                    o[t][x][c][e];
-                }
-            }
-            __syncthreads();
-            if (wave < half) {
-                const float* from = xo + wave * N::ROWS * N::LDO;
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const float4 y = xs[wave * N::ROWS + 16 * t + col];
-                    const float m_new = fmaxf(m[t], y.x), base = base_of(m_new);
-                    const float fa = exp2_(m[t] - base), fb = exp2_(y.x - base);
-                    m[t] = m_new;
-                    l[t] = l[t] * fa + y.y * fb;
-                    used[t] = used[t] * fa + y.z * fb;
-                    odd |= y.w != 0.f;
-#pragma unroll
-                    for (int x = 0; x < VS; ++x)
-#pragma unroll
-                        for (int c = 0; c < VL; ++c)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                o[t][x][c][e] = o[t][x][c][e] * fa +
-                                                fb * from[(16 * t + col) * N::LDO + N::VD * x +
-                                                          N::RUN * q + VL * e + c];
-                }
-            }
+            for (int t = 0; t < MT; ++t)
+                xs[wave * N::ROWS + 16 * t + col] = make_float4(m[t], l[t], used[t], odd ? 1.f : 0.f);
         }
-        if (wave != 0) continue;
+        __syncthreads();  // (and Q is no longer read)
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int row = tile * N::ROWS + 16 * t + col;
-            const int h = g * rep + row / a.d.T, tok = row % a.d.T;
-            if (row >= R || tok >= n) continue;
+            float top = m[t];
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) top = fmaxf(top, xs[w * N::ROWS + 16 * t + col].x);
+            const float f = exp2_(m[t] - base_of(top));
+            float* to = xo + (wave * N::ROWS + 16 * t + col) * N::LDO + N::RUN * q;
+#pragma unroll
+            for (int x = 0; x < VS; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int c = 0; c < VL; c += 4)
+                        *reinterpret_cast<float4*>(to + N::VD * x + VL * e + c) =
+                            make_float4(o[t][x][c][e] * f, o[t][x][c + 1][e] * f,
+                                        o[t][x][c + 2][e] * f, o[t][x][c + 3][e] * f);
+        }
+        __syncthreads();
+        odd = false;
+        // (opaque: or what this computes is hoisted out of the loop over spans, into registers)
+        for (int e = opaque(threadIdx.x); e < N::ROWS * (DP / 4); e += 64 * WAVES) {
+            const int r = e / (DP / 4), d = e % (DP / 4) * 4, row = tile * N::ROWS + r;
+            const int h = head_of(a.d, row), tok = row - h * a.d.T;
+            if (row >= R || tok >= n || d >= D) continue;
+            float M = -INFINITY, sum = 0.f, su = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) M = fmaxf(M, xs[w * N::ROWS + r].x);
+            const float base = base_of(M);
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float4 z = xs[w * N::ROWS + r];
+                const float f = exp2_(z.x - base);
+                sum += z.y * f;
+                su += z.z * f;
+                odd |= z.w != 0.f;
+                const float* from = xo + (w * N::ROWS + r) * N::LDO;
+                if constexpr (MODE == kClamp) {
+                    // (a piece that the row's end cut holds the row's last dims)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int piece = (d + c) / VL * VL;
+                        x[c] += from[min(d + c + max(0, piece - (D - VL)), DP - 1)];
+                    }
+                } else {
+                    const float4 y = *reinterpret_cast<const float4*>(from + d);
+                    x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+                }
+            }
             if (sp.part >= 0) {
                 const size_t to = part_row(a, sp.part, row);
-                float* dims = part_dims(a) + to * D;
-                if (q == 0) part_stats(a)[to] = make_float4(m[t], l[t], used[t], 0.f);
-#pragma unroll
-                for (int x = 0; x < VS; ++x)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = N::dim_of(x, 4 * q + e, D);
-#pragma unroll
-                        for (int c = 0; c < VL; ++c)
-                            if (MODE != kElem || d + c < D) dims[d + c] = o[t][x][c][e];
-                    }
+                if (d == 0) part_stats(a)[to] = make_float4(M, sum, su, 0.f);
+                store4(part_dims(a) + to * D + d, x, D - d);
             } else {
-                T* to = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2];
                 // (0: nothing visible, or no score above -infinity)
-                const float inv = used[t] == 0.f ? 0.f : 1.f / used[t];
-                if (q == 0 && a.lse)
-                    a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
-                        l[t] == 0.f ? -INFINITY : (m[t] + log2f(l[t])) * kLn2;
+                const float inv = su == 0.f ? 0.f : 1.f / su;
+                if (d == 0 && a.lse)
+                    a.lse[((size_t)b * a.d.H + g * rep + h) * a.d.T + tok] =
+                        sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
 #pragma unroll
-                for (int x = 0; x < VS; ++x)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = N::dim_of(x, 4 * q + e, D);
-#pragma unroll
-                        for (int c = 0; c < VL; ++c)
-                            if (MODE != kElem || d + c < D) Elem<T>::st(to, d + c, o[t][x][c][e] * inv);
-                    }
+                for (int c = 0; c < 4; ++c) x[c] *= inv;
+                store4((T*)a.out + b * a.os[0] + (g * rep + h) * a.os[1] + tok * a.os[2] + d, x, D - d);
             }
         }
-        if (__builtin_amdgcn_ballot_w64(odd)) {
-            __threadfence_block();  // (this wave's own stores, from other lanes)
-            for (int r = 0; r < N::ROWS; ++r)
-                add_not_finite<T>(a, sp, tile * N::ROWS + r, n, 0, D, lane);
+        if (__syncthreads_or(odd)) {
+            // (behind the barrier, which waits for the workgroup's stores)
+            for (int r = wave; r < N::ROWS; r += WAVES)
+                add_not_finite<T>(a, sp, tile * N::ROWS + r, whole * KB, L, n, 0, D, lane);
         }
     }
 }
@@ -480,7 +507,7 @@ k_tree_narrow(TreeArgs a) {
 // ---------------------------------------------------------------- head_d > 256
 // No output tile fits a wave's registers, so two kernels with the scores between them:
 // k_tree_scores writes x (rows of R floats, small beside K and V's rows of head_d), each
-// workgroup's 8 waves sharing a tile's dims and adding up through LDS; k_tree_values is the
+// workgroup's 8 waves sharing a tile's dims, or its share of them, and adding up through LDS; k_tree_values is the
 // softmax over them and the product with V, each wave 16 VL dims of the output.
 // Keys lie in blocks of 32: the cache's, then the drafts'.
 constexpr int kBlock = 32;
@@ -488,17 +515,24 @@ constexpr int kScoreWaves = 8;
 constexpr int kWaves = 4;        // of a value workgroup
 constexpr int kValueKeys = 128;  // keys between barriers of k_tree_values
 
+// Scores of a row: [shares][pairs of the pass][rows of the tiles][ld_scores], to be added over
+// the shares of the dims.
+__device__ __forceinline__ size_t score_row(const TreeArgs& a, int share, int pair, int row) {
+    return ((size_t)(share * a.bs * a.gs + pair) * a.plan.row_tiles * a.plan.rows + row) *
+           a.plan.ld_scores;
+}
+
 template <typename T, int MT>
 __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
-    using N = CacheTiles<T, 64, MT, kExact>;
     constexpr int SUB = kBlock / 16;
     __shared__ v4f red[kScoreWaves][MT * SUB * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
     const int tiles = a.plan.row_tiles, most = a.plan.ld_scores / kBlock;
     int unit, tile;
-    tile_of(blockIdx.x, a.bs * a.gs * most, tiles, &unit, &tile);
-    const int i = unit % most, pair = unit / most, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
+    tile_of(blockIdx.x, a.bs * a.gs * a.plan.shares * most, tiles, &unit, &tile);
+    const int share = unit % a.plan.shares, i = unit / a.plan.shares % most;
+    const int pair = unit / a.plan.shares / most, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
     const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), D = a.c.D;
     const int cache = (L + kBlock - 1) / kBlock;
     const int all = cache + (a.d.K ? (n + kBlock - 1) / kBlock : 0);
@@ -516,12 +550,12 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {  // (rows past R: the last one's scores, which nobody reads)
-        const int row = min((tile * MT + t) * 16 + col, R - 1);
-        qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + (g * rep + row / a.d.T) * a.d.qs[1] +
-                (row % a.d.T) * a.d.qs[2];
+        const int row = min((tile * MT + t) * 16 + col, R - 1), h = head_of(a.d, row);
+        qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + (g * rep + h) * a.d.qs[1] +
+                (row - h * a.d.T) * a.d.qs[2];
     }
     v4f s[MT][SUB];
-    wide_scores<T, MT, kScoreWaves>(s, kp, qp, D, wave, q);
+    wide_scores<T, MT>(s, kp, qp, D, share * kScoreWaves + wave, a.plan.shares * kScoreWaves, q);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -533,20 +567,20 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
     v4f x = red[0][threadIdx.x];
 #pragma unroll
     for (int w = 1; w < kScoreWaves; ++w) x += red[w][threadIdx.x];
-    const int row = (tile * MT + t) * 16 + col, tok = row % a.d.T, k0 = 16 * u + 4 * q;
+    const int row = (tile * MT + t) * 16 + col, tok = row - head_of(a.d, row) * a.d.T;
+    const int k0 = 16 * u + 4 * q;
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const bool on = k0 + e < rows && row < R && (in || sees(a.d, b, tok, j0 + k0 + e));
         y[e] = on ? x[e] * a.scale : -INFINITY;
     }
-    float* to =
-        a.scores + ((size_t)pair * tiles * N::ROWS + row) * a.plan.ld_scores + i * kBlock + k0;
+    float* to = a.scores + score_row(a, share, pair, row) + i * kBlock + k0;
     *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
 }
 
 template <typename T, int MT>
-__global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : MT == 2 ? 2 : 1) void k_tree_values(TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(TreeArgs a) {
     constexpr bool kBf = sizeof(T) == 2;
     // (a wave's dims: one V step of 128 in bf16, 64 in fp32; where the row ends before, its last
     // ones; those before d0 are the wave's before)
@@ -586,9 +620,9 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : MT == 2 ? 2 : 1) void k_
         const int cache = (L + kBlock - 1) / kBlock;
         const bool none = L == 0 && (!a.d.K || n == 0);  // a pair without keys has no scores either
         const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1] + d0;
-        const float* sc = a.scores +
-                          ((size_t)((b - a.b0) * a.gs + g - a.g0) * tiles + tile) * ROWS *
-                              a.plan.ld_scores;
+        const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d0;
+        const float* sc = a.scores + score_row(a, 0, (b - a.b0) * a.gs + g - a.g0, tile * ROWS);
+        const size_t next_share = score_row(a, 1, 0, 0);
         float m[MT], l[MT], used[MT], x[MT][8];
         v4f o[MT][1][VL];
 #pragma unroll
@@ -604,19 +638,38 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : MT == 2 ? 2 : 1) void k_
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const float* from = sc + (size_t)(16 * t + sr) * a.plan.ld_scores + i * kBlock + sk;
-                float4 u, w;
-                u.x = u.y = u.z = u.w = -INFINITY;
-                w = u;
+                v4f u = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, w = u;
                 if (sk < (sp.last - i) * kBlock) {
-                    u = *reinterpret_cast<const float4*>(from);
-                    w = *reinterpret_cast<const float4*>(from + 4);
+                    u = *reinterpret_cast<const v4f*>(from);
+                    w = *reinterpret_cast<const v4f*>(from + 4);
+                    for (int y = 1; y < a.plan.shares; ++y) {
+                        from += next_share;
+                        u += *reinterpret_cast<const v4f*>(from);
+                        w += *reinterpret_cast<const v4f*>(from + 4);
+                    }
                 }
-                x[t][0] = u.x, x[t][1] = u.y, x[t][2] = u.z, x[t][3] = u.w;
-                x[t][4] = w.x, x[t][5] = w.y, x[t][6] = w.z, x[t][7] = w.w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[t][e] = u[e], x[t][4 + e] = w[e];
             }
         };
-        // ... into weights in LDS
-        auto weights = [&](int buf) {
+        // V of the x-th PK keys of the span's blocks on (past its end: of the last ones)
+        auto load_v = [&](typename N::Vals& to, int x) {
+            const int i = min(sp.first + x / (kBlock / PK), sp.last - 1);
+            const bool in = i < cache;
+            N::load_v(to, in ? vc : vd, in ? a.c.vs[2] : a.d.vs[2],
+                      (in ? i : i - cache) * kBlock + x % (kBlock / PK) * PK, in ? L : n, D - d0,
+                      lane);
+        };
+        // Two buffers of weights: a wave past a barrier writes the other one, and comes to write
+        // this one only after the next barrier, when every wave has read it.
+        constexpr int STEP = kValueKeys / kBlock;
+        typename N::Vals v0, v1;
+        __syncthreads();  // (the last span's)
+        if (!none) load_x(sp.first);
+        if (!none && busy) load_v(v0, 0);
+        int buf = 0;
+        for (int i = sp.first; !none && i < sp.last; i += STEP, buf ^= 1) {
+            // scores into weights
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 float top = x[t][0];
@@ -653,8 +706,9 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : MT == 2 ? 2 : 1) void k_
                         make_float4(x[t][4], x[t][5], x[t][6], x[t][7]);
                 }
             }
-        };
-        auto rescale = [&](int buf) {
+            if (i + STEP < sp.last) load_x(i + STEP);
+            __syncthreads();
+            if (!busy) continue;
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const float f = alpha[buf][16 * t + col];
@@ -663,54 +717,24 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : MT == 2 ? 2 : 1) void k_
                     for (int c = 0; c < VL; ++c) o[t][0][c] *= f;
                 }
             }
-        };
-        auto load_whole = [&](typename N::Vals& v, int j) {  // rows j .. of the cache
-            N::template load_v<true>(v, vc + (int64_t)j * a.c.vs[2], a.c.vs[2], PK, D - d0, lane);
-        };
-        // Two buffers of weights: a wave past a barrier writes the other one, and comes to write
-        // this one only after the next barrier, when every wave has read it.
-        int i = sp.first, buf = 0;
-        const int whole = min(sp.last, L / kBlock);
-        constexpr int STEP = kValueKeys / kBlock;
-        __syncthreads();  // (the last span's)
-        if (!none && i < sp.last) load_x(i);
-        // steps of whole cache blocks: the next rows of V and the next scores on their way
-        if (i + STEP <= whole) {
-            typename N::Vals v[2];
-            if (busy) load_whole(v[0], i * kBlock);
-            for (; i + STEP <= whole; i += STEP, buf ^= 1) {
-                weights(buf);
-                if (i + STEP < sp.last) load_x(i + STEP);
-                __syncthreads();
-                if (!busy) continue;
-                rescale(buf);
-#pragma unroll
-                for (int k = 0; k < NB; ++k) {
-                    if (k + 1 < NB || i + 2 * STEP <= whole)
-                        load_whole(v[(k + 1) & 1], i * kBlock + (k + 1) * PK);
-                    __builtin_amdgcn_sched_barrier(0);
-                    N::accumulate_lds(o, v[k & 1], pl[buf] + k * PK, LDP, lane);
-                }
-            }
-        }
-        for (; !none && i < sp.last; i += STEP, buf ^= 1) {
-            weights(buf);
-            if (i + STEP < sp.last) load_x(i + STEP);
-            __syncthreads();
-            if (!busy) continue;
-            rescale(buf);
-            for (int k = 0; k < kValueKeys && k < (sp.last - i) * kBlock; k += PK) {
-                const int x = i + k / kBlock;
-                const bool in = x < cache;
-                const int j0 = (in ? x : x - cache) * kBlock + k % kBlock;
-                const int rows = min(PK, (in ? L : n) - j0);
-                if (rows <= 0) continue;  // (fp32: the second half of a last block)
-                const T* vb = in ? vc : (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d0;
-                const int64_t s = in ? a.c.vs[2] : a.d.vs[2];
-                typename N::Vals v;
-                N::template load_v<false>(v, vb + j0 * s, s, rows, D - d0, lane);
-                if (!in) odd |= clear_not_finite<T>(v);
+            // each PK keys' V on their way while the ones before are used
+            auto use = [&](typename N::Vals& v, int k) {
+                const int y = i + k / kBlock;
+                const bool in = y < cache;
+                const int j0 = (in ? y : y - cache) * kBlock + k % kBlock;
+                if (y >= sp.last || j0 >= (in ? L : n)) return;
+                if (!in || j0 + PK > L) odd |= clear_not_finite<T>(v);
                 N::accumulate_lds(o, v, pl[buf] + k, LDP, lane);
+            };
+            const int x0 = (i - sp.first) * (kBlock / PK);
+#pragma unroll 1
+            for (int k = 0; k < NB; k += 2) {
+                load_v(v1, x0 + k + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                use(v0, k * PK);
+                load_v(v0, x0 + k + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                use(v1, (k + 1) * PK);
             }
         }
         // sums of the rows, for the waves that hold their outputs
@@ -721,42 +745,52 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : MT == 2 ? 2 : 1) void k_
         }
         __syncthreads();
         if (!busy) continue;
+        // (computed here: hoisted out of the loop over spans, these take the loop's registers)
+        const int late = opaque(lane), lq = late >> 4, lc = late & 15;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int row = tile * ROWS + 16 * t + col, tok = row % a.d.T, h = g * rep + row / a.d.T;
+            const int row = tile * ROWS + 16 * t + lc, h = head_of(a.d, row), tok = row - h * a.d.T;
             if (row >= R || tok >= n) continue;
-            const float4 z = fin[16 * t + col];
-            const bool teller = q == 0 && d0 == 0;
-            if (sp.part >= 0) {
-                const size_t to = part_row(a, sp.part, row);
-                float* dims = part_dims(a) + to * D + d0;
-                if (teller) part_stats(a)[to] = z;
+            const float4 z = fin[16 * t + lc];
+            const bool teller = lq == 0 && d0 == 0;
+            const size_t part = part_row(a, max(sp.part, 0), row);
+            const float inv = sp.part >= 0 ? 1.f : z.z == 0.f ? 0.f : 1.f / z.z;
+            float* dims = part_dims(a) + part * D + d0;
+            T* to = (T*)a.out + b * a.os[0] + (g * rep + h) * a.os[1] + tok * a.os[2] + d0;
+            if (teller && sp.part >= 0) part_stats(a)[part] = z;
+            if (teller && sp.part < 0 && a.lse)
+                a.lse[((size_t)b * a.d.H + g * rep + h) * a.d.T + tok] =
+                    z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = N::dim_of(0, 4 * q + e, D - d0);
+            for (int e = 0; e < 4; ++e) {
+                const int d = N::dim_of(0, 4 * lq + e, D - d0);
 #pragma unroll
-                    for (int c = 0; c < VL; ++c)
-                        if (d + c >= 0) dims[d + c] = o[t][0][c][e];
-                }
-            } else {
-                T* to = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2] + d0;
-                const float inv = z.z == 0.f ? 0.f : 1.f / z.z;
-                if (teller && a.lse)
-                    a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
-                        z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
+                for (int c = 0; c < VL; c += 4) {
+                    const float y[4] = {o[t][0][c][e] * inv, o[t][0][c + 1][e] * inv,
+                                        o[t][0][c + 2][e] * inv, o[t][0][c + 3][e] * inv};
+                    if (d + c >= 0) {
+                        if (sp.part >= 0)
+                            store4(dims + d + c, y, 4);
+                        else
+                            store4(to + d + c, y, 4);
+                    } else {  // (a row's last dims, fewer than a piece)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = N::dim_of(0, 4 * q + e, D - d0);
-#pragma unroll
-                    for (int c = 0; c < VL; ++c)
-                        if (d + c >= 0) Elem<T>::st(to, d + c, o[t][0][c][e] * inv);
+                        for (int r = 1; r < 4; ++r)
+                            if (d + c + r >= 0) {
+                                if (sp.part >= 0)
+                                    dims[d + c + r] = y[r];
+                                else
+                                    Elem<T>::st(to, d + c + r, y[r]);
+                            }
+                    }
                 }
             }
         }
         if (odd) {
-            __threadfence_block();
+            __threadfence_block();  // (this wave's own stores, from other lanes)
             for (int r = 0; r < ROWS; ++r)
-                add_not_finite<T>(a, sp, tile * ROWS + r, n, d0, min(D, d0 + WD), lane);
+                add_not_finite<T>(a, sp, tile * ROWS + r, L / PK * PK, L, n, d0, min(D, d0 + WD),
+                                  late);
         }
     }
 }
@@ -772,7 +806,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn
     const int D = a.c.D, chunks = (D + 255) / 256, rep = a.d.H / a.c.G, R = rep * a.d.T;
     const int d0 = (blockIdx.x % chunks) * 256, row = blockIdx.x / chunks % R;
     const int pair = blockIdx.x / chunks / R, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
-    const int tok = row % a.d.T, h = g * rep + row / a.d.T;
+    const int tok = row - head_of(a.d, row) * a.d.T, h = g * rep + head_of(a.d, row);
     if (tok >= drafts_of(a.d, b)) return;
     int before = 0, total = 0;  // blocks of a kv head of the sequences before, and of all
     for (int i = lane; i < a.bs; i += 64) {
@@ -867,7 +901,8 @@ template <typename T, int MT>
 void go_wide(const TreeArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(
         (k_tree_scores<T, MT>),
-        dim3((unsigned)(a.bs * a.gs * a.plan.row_tiles * (a.plan.ld_scores / kBlock))),
+        dim3((unsigned)(a.bs * a.gs * a.plan.row_tiles * a.plan.shares *
+                        (a.plan.ld_scores / kBlock))),
         dim3(64 * kScoreWaves), 0, st, a);
     const int wd = wide_dims(sizeof(T) == 2), groups = (a.c.D + wd - 1) / wd;
     hipLaunchKernelGGL((k_tree_values<T, MT>),
@@ -880,8 +915,7 @@ void go(const TreeArgs& a, hipStream_t st) {
     const int D = a.c.D;
     if (D > kTreeNarrow) {
         if (a.plan.rows == 16) go_wide<T, 1>(a, st);
-        else if (a.plan.rows == 32) go_wide<T, 2>(a, st);
-        else go_wide<T, 4>(a, st);
+        else go_wide<T, 2>(a, st);
     } else if (D <= 64) {
         go_dims<T, 64>(a, st);
     } else if (D <= 128) {
@@ -909,7 +943,7 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     TreePlan p{};
     const bool bf = dtype == kDtypeBF16, wide = D > kTreeNarrow;
     const int R = H / G * T;
-    const int most = wide || (bf && D <= 128) ? 64 : 32;
+    const int most = bf && D <= 128 ? 64 : 32;
     p.rows = R <= 16 ? 16 : R <= 32 ? 32 : most;
     p.row_tiles = (int)ceil_div(R, p.rows);
     p.waves = 4;
@@ -920,7 +954,7 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     const int groups = wide ? (int)ceil_div(D, wide_dims(bf)) : 1;
     p.ld_scores = wide ? (int)blocks * kBlock : 0;
     // workgroups that the card holds at once (256 CUs; the kernels' registers)
-    const int per_cu = wide ? (mt == 1 ? 3 : mt == 2 ? 2 : 1)
+    const int per_cu = wide ? (mt == 1 ? 3 : 2)
                             : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
     const int64_t slots = std::max<int64_t>(1, 256 * per_cu / (p.row_tiles * groups));
     const int64_t turn = wide ? kValueKeys / kBlock : p.waves;
@@ -930,7 +964,12 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     p.split = !small && ranges > 1 && pairs < 4 * slots && blocks > turn;
     if (small) p.waves = 8;
     const size_t room = scratch_cap / sizeof(float);
-    const size_t sc = wide ? (size_t)rows * p.ld_scores : 0;  // floats of a pair
+    // score workgroups: two a CU, where the dims give each wave two steps still
+    p.shares = 1;
+    while (wide && pairs * p.row_tiles * blocks * p.shares < 512 && p.shares < 8 &&
+           D >= 2 * p.shares * kScoreWaves * (bf ? 256 : 128))
+        p.shares *= 2;
+    const size_t sc = wide ? (size_t)rows * p.ld_scores * p.shares : 0;  // floats of a pair
     const size_t part = 2 * (size_t)rows * (D + 4);           // ... of a range
     int64_t in_pass = pairs;
     if (sc * pairs + (p.split ? part * ranges : 0) > room) {
@@ -950,7 +989,7 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     p.scores = sc * in_pass;
     p.scratch = (p.scores + (p.split ? part * ranges : 0)) * sizeof(float);
     p.workgroups = std::max({(int64_t)p.ranges * p.row_tiles * groups,
-                             in_pass * p.row_tiles * (p.ld_scores / kBlock),
+                             in_pass * p.row_tiles * p.shares * (p.ld_scores / kBlock),
                              in_pass * R * ceil_div(D, 256)});
     return p;
 }
