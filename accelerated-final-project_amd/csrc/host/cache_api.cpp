@@ -16,6 +16,8 @@ using atn_host::kSyncRegion;
 
 static_assert(ATN_TREE_MAX_TOKENS == atn::kTreeMaxTokens, "token limit");
 
+constexpr int64_t kMaxRow = (int64_t)1 << 27;  // bytes from a row of K or V to the next
+
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 // Bytes [lo, hi) that a call reads or writes.
@@ -84,6 +86,8 @@ int check_cache(const atn_kv_cache* c, atn::CacheView* v, Ranges* r) {
         st = check_tensor(c->V, c->v_stride, c->batch, c->kv_heads, c->capacity, c->head_d, es,
                           true, v->vs, &r->v);
     if (st != ATN_OK) return st;
+    // (the kernels address the 32 rows of a block by 32-bit byte offsets)
+    if (std::max(v->ks[2], v->vs[2]) * (int64_t)es > kMaxRow) return ATN_ERR_SIZE_OVERFLOW;
     for (const void* p : {(const void*)c->len, (const void*)c->seen, (const void*)c->weight,
                           (const void*)c->pos})
         if (!aligned(p, 4)) return ATN_ERR_MISALIGNED;
@@ -123,6 +127,7 @@ int check_drafts(const atn_kv_cache* c, const atn_drafts* d, bool need_q, bool n
         st = check_tensor(d->V, d->v_stride, c->batch, c->kv_heads, d->tokens, c->head_d, es, false,
                           v->vs, &r->vd);
     if (st != ATN_OK) return st;
+    if (std::max(v->ks[2], v->vs[2]) * (int64_t)es > kMaxRow) return ATN_ERR_SIZE_OVERFLOW;
     if (!aligned(d->count, 4) || !aligned(d->mask, 4)) return ATN_ERR_MISALIGNED;
     v->Q = need_q ? d->Q : nullptr;
     v->K = d->K;

@@ -141,30 +141,37 @@ struct CacheTiles {
         VPiece p[KEYS][VS];
     };
 
-    // Piece i of a row of K or Q for the lanes of group q (`row`: piece 0's place in the row)
-    static __device__ __forceinline__ KPiece piece(const T* row, int i, int q, int D) {
+    // Rows are addressed as a uniform base and each lane's 32-bit byte offset: a block's rows lie
+    // within 4 GiB.
+    static __device__ __forceinline__ const T* at(const T* base, uint32_t off) {
+        return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off);
+    }
+
+    // Piece i of a row of K or Q for the lanes of group q (`off`: of their piece 0)
+    static __device__ __forceinline__ KPiece piece(const T* base, uint32_t off, int i, int q, int D) {
         const int d = 4 * EL * i + EL * q;
         if constexpr (MODE == kElem) {
-            return ld_some<16>(row + 4 * EL * i, D - d);
+            return ld_some<16>(at(base, off) + 4 * EL * i, D - d);
         } else if (MODE == kExact || 4 * EL * (i + 1) <= DP - 64) {
-            return ld_words<16>(row + 4 * EL * i);
+            return ld_words<16>(at(base, off) + 4 * EL * i);
         } else {
             const int past = max(0, opaque(d) - (D - EL));
-            KPiece v = ld_words<16>(row + 4 * EL * i - past);
+            KPiece v = ld_words<16>(at(base, off + (4 * EL * i - past) * (int)sizeof(T)));
             clear_first(v, past);
             return v;
         }
     }
 
-    // K of the block at row j0 of `rows` rows from `base` on (the last one again in the places
-    // behind it)
-    static __device__ __forceinline__ void load_k(Keys& k, const T* base, int64_t stride, int j0,
-                                                  int rows, int D, int lane) {
+    // K of a block of `rows` rows from `base` on (the last one again in the places behind them)
+    static __device__ __forceinline__ void load_k(Keys& k, const T* base, int64_t stride, int rows,
+                                                  int D, int lane) {
+        const uint32_t row = (uint32_t)stride * (uint32_t)sizeof(T);
+        const uint32_t end = (uint32_t)(min(rows, KB) - 1) * row, mine = (lane & 15) * row;
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const T* p = base + min(j0 + 16 * s + (lane & 15), rows - 1) * stride + EL * (lane >> 4);
+            const uint32_t off = min(mine + 16 * s * row, end) + 16 * (lane >> 4);
 #pragma unroll
-            for (int i = 0; i < KS; ++i) k.p[s][i] = piece(p, i, lane >> 4, D);
+            for (int i = 0; i < KS; ++i) k.p[s][i] = piece(base, off, i, lane >> 4, D);
         }
     }
 
@@ -177,19 +184,25 @@ struct CacheTiles {
         const int d = VD * i + VL * m;
         return MODE == kClamp ? min(d, D - VL) : d;
     }
-
-    // V of the block, likewise (the rows behind enter with a weight of 0: whoever calls takes out
-    // what times 0 is not 0)
-    static __device__ __forceinline__ void load_v(Vals& v, const T* base, int64_t stride, int j0,
-                                                  int rows, int D, int lane) {
+    // (the rows behind a block's enter with a weight of 0: whoever calls takes out what times 0 is
+    // not 0)
+    static __device__ __forceinline__ VPiece v_piece(const T* base, uint32_t off, int i, int D,
+                                                     int lane) {
+        const int d = dim_of(i, lane & 15, D);
+        if constexpr (MODE == kElem) return ld_some<VB>(at(base, off) + d, D - d);
+        // (dims before the base, where a row's last piece begins: the sum does not wrap)
+        const int before = min(D - VL, 0);
+        return ld_words<VB>(at(base + before, off + (uint32_t)((d - before) * (int)sizeof(T))));
+    }
+    static __device__ __forceinline__ void load_v(Vals& v, const T* base, int64_t stride, int rows,
+                                                  int D, int lane) {
+        const uint32_t row = (uint32_t)stride * (uint32_t)sizeof(T);
+        const uint32_t end = (uint32_t)(min(rows, KB) - 1) * row, mine = key_of(lane, 0) * row;
 #pragma unroll
         for (int j = 0; j < KEYS; ++j) {
-            const T* p = base + min(j0 + key_of(lane, j), rows - 1) * stride;
+            const uint32_t off = min(mine + key_of(0, j) * row, end);
 #pragma unroll
-            for (int i = 0; i < VS; ++i) {
-                const int d = dim_of(i, lane & 15, D);
-                v.p[j][i] = MODE == kElem ? ld_some<VB>(p + d, D - d) : ld_words<VB>(p + d);
-            }
+            for (int i = 0; i < VS; ++i) v.p[j][i] = v_piece(base, off, i, D, lane);
         }
     }
 
@@ -300,17 +313,9 @@ __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp
         for (int u = 0; u < 2; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
     const int per = ((D + STEP * U - 1) / (STEP * U) + waves - 1) / waves * STEP * U;
     const int d1 = min(D, (wave + 1) * per);
-    typename N::KPiece k[U][2], f[U][MT];
-    auto products = [&] {
-#pragma unroll
-        for (int e = 0; e < U; ++e)
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) s[t][u] = N::dot(k[e][u], f[e][t], s[t][u]);
-    };
     int d = wave * per;
     for (; d + STEP * U <= d1; d += STEP * U) {
+        typename N::KPiece k[U][2], f[U][MT];
 #pragma unroll
         for (int e = 0; e < U; ++e) {
             const int at = d + STEP * e + EL * q;
@@ -320,24 +325,31 @@ __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp
             for (int t = 0; t < MT; ++t) f[e][t] = ld_words<16>(qp[t] + at);
         }
         __builtin_amdgcn_sched_barrier(0);
-        products();
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[t][u] = N::dot(k[e][u], f[e][t], s[t][u]);
     }
     if (d < d1) {  // the row's end (kClamp's pieces)
-#pragma unroll
+#pragma unroll 1
         for (int e = 0; e < U; ++e) {
             const int want = d + STEP * e + EL * q, at = min(want, D - EL);
+            typename N::KPiece x[2], y;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                k[e][u] = ld_words<16>(kp[u] + at);
-                clear_first(k[e][u], want - at);
+                x[u] = ld_words<16>(kp[u] + at);
+                clear_first(x[u], want - at);
             }
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                f[e][t] = ld_words<16>(qp[t] + at);
-                clear_first(f[e][t], want - at);
+                y = ld_words<16>(qp[t] + at);
+                clear_first(y, want - at);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[t][u] = N::dot(x[u], y, s[t][u]);
             }
         }
-        products();
     }
 }
 

@@ -70,15 +70,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
     const int bg = blockIdx.y, g = bg % a.c.G, b = bg / a.c.G, D = a.c.D;
-    const int L = rows_in_use(a.c, b), A = rows_accepted(a.c, a.d, a.p, b);
+    const int L = of_wave(rows_in_use(a.c, b)), A = of_wave(rows_accepted(a.c, a.d, a.p, b));
     const int end = L + A, blocks = (end + KB - 1) / KB, R = a.d.H / a.c.G * A;
     const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
     const int i0 = blockIdx.x * kWaves + wave, step = gridDim.x * kWaves;
     if ((int)blockIdx.x * kWaves >= blocks) return;
     for (int row0 = 0; row0 == 0 || row0 < R; row0 += kRows) {
         typename N::Keys k;
-        if (i0 < blocks)
-            N::load_k(k, kc, a.c.ks[2], i0 * KB, end, D, lane);
+        auto load_k = [&](int i) {
+            N::load_k(k, kc + (int64_t)i * KB * a.c.ks[2], a.c.ks[2], end - i * KB, D, lane);
+        };
+        if (i0 < blocks) load_k(i0);
         const int tiles = (min(kRows, R - row0) + 15) / 16;
         __syncthreads();
         for (int e = threadIdx.x; e < tiles * KS * 64; e += 64 * kWaves) {
@@ -88,8 +90,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
             if (row < R) {
                 const QueryRow x = query_row(a, b, g, A, row);
                 z = N::piece((const T*)a.d.Q + b * a.d.qs[0] + x.head * a.d.qs[1] +
-                                 x.tok * a.d.qs[2] + N::EL * (el >> 4),
-                             i, el >> 4, D);
+                                 x.tok * a.d.qs[2],
+                             16 * (el >> 4), i, el >> 4, D);
             }
             qs[e] = z;
         }
@@ -122,8 +124,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
                     }
             }
             const int nx = i + step;
-            if (nx < blocks)
-                N::load_k(k, kc, a.c.ks[2], nx * KB, end, D, lane);
+            if (nx < blocks) load_k(nx);
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const float4 w = make_float4(row16_sum(sum[u][0]), row16_sum(sum[u][1]),
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
     const int bg = blockIdx.y, g = bg % a.c.G, b = bg / a.c.G, D = a.c.D;
-    const int L = rows_in_use(a.c, b), A = rows_accepted(a.c, a.d, a.p, b);
+    const int L = of_wave(rows_in_use(a.c, b)), A = of_wave(rows_accepted(a.c, a.d, a.p, b));
     const int end = L + A, j0 = blockIdx.x * kBlock, rows = min(kBlock, end - j0);
     const int R = a.d.H / a.c.G * A;
     if (rows <= 0) return;

@@ -51,7 +51,9 @@ struct PathView {
     int n;
 };
 
-// rows in use of sequence b, and its drafts
+// Rows in use of a sequence, and its drafts; of_wave: of one that the whole wave shares (the
+// compiler keeps what follows from it in scalar registers only if told).
+__device__ __forceinline__ int of_wave(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int rows_in_use(const CacheView& c, int b) {
     return min(max(c.len[b], 0), c.rows);
 }

@@ -104,7 +104,7 @@ __device__ __forceinline__ Span span_whole(const TreeArgs& a, int r, int kb) {
     s.b = a.b0 + r / a.gs;
     s.g = a.g0 + r % a.gs;
     s.first = 0;
-    s.last = blocks_of(a, s.b, kb);
+    s.last = of_wave(blocks_of(a, s.b, kb));
     s.part = -1;
     return s;
 }
@@ -240,7 +240,8 @@ struct Narrow : CacheTiles<T, DP, MT, MODE> {
     static constexpr int LDO = DP + 4;  // row of the waves' results, floats
     static constexpr int kQBytes = N::ROWS * DP * (int)sizeof(T);
     static constexpr int kXBytes = WAVES * N::ROWS * LDO * 4;
-    static constexpr int kLds = (kQBytes > kXBytes ? kQBytes : kXBytes) + WAVES * N::ROWS * 16;
+    static constexpr int kOut = kQBytes > kXBytes ? kQBytes : kXBytes;
+    static constexpr int kLds = kOut + (WAVES + 1) * N::ROWS * 16;
     static constexpr int kQ = (MT * N::KS * 64 + 64 * WAVES - 1) / (64 * WAVES);  // pieces a thread
     static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -274,18 +275,49 @@ k_tree_narrow(TreeArgs a) {
         }
         const int b = sp.b, g = sp.g;
 
+        const int L = of_wave(rows_in_use(a.c, b)), n = of_wave(drafts_of(a.d, b));
+        const int cache = (L + KB - 1) / KB;  // its blocks; the drafts' follow
+        const int whole = L / KB;
+        const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
+        const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1];
+        const T* kd = (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
+        const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
+        // (a pair without keys has one block of none)
+        const int last = L > 0 || (a.d.K && n > 0) ? sp.last : 0;
+        auto load_k = [&](typename N::Keys& to, int i) {
+            const bool in = i < cache;
+            const int j0 = (in ? i : i - cache) * KB;
+            const int64_t s = in ? a.c.ks[2] : a.d.ks[2];
+            N::load_k(to, (in ? kc : kd) + j0 * s, s, (in ? L : n) - j0, D, lane);
+        };
+        auto load_v = [&](typename N::Vals& to, int i) {
+            const bool in = i < cache;
+            const int j0 = (in ? i : i - cache) * KB;
+            const int64_t s = in ? a.c.vs[2] : a.d.vs[2];
+            N::load_v(to, (in ? vc : vd) + j0 * s, s, (in ? L : n) - j0, D, lane);
+        };
+
         // Q in the order of the fragments: piece (t, i) of lane L is piece i of row 16 t + L % 16.
         // (Rows of no token hold the last token's: nobody reads their results.)
         auto* qs = reinterpret_cast<typename N::KPiece*>(lds);
+        typename N::Keys k;
+        typename N::Vals v;
+        int i = sp.first + wave;
         {
             typename N::KPiece z[N::kQ];
-            const T* qb = (const T*)a.d.Q + b * a.d.qs[0] + g * rep * a.d.qs[1] + N::EL * q;
+            const T* qb = (const T*)a.d.Q + b * a.d.qs[0] + g * rep * a.d.qs[1];
 #pragma unroll
             for (int x = 0; x < N::kQ; ++x) {
                 const int e = x * WAVES + wave, i = e % KS, t = min(e / KS, MT - 1);
                 const int row = min(tile * N::ROWS + 16 * t + col, R - 1), h = head_of(a.d, row);
-                z[x] = N::piece(qb + h * a.d.qs[1] + (row - h * a.d.T) * a.d.qs[2], i, q, D);
+                z[x] = N::piece(qb + h * a.d.qs[1] + (row - h * a.d.T) * a.d.qs[2], 16 * q, i, q, D);
             }
+            // (the first block's K and V right behind, before anything waits for Q)
+            if (i < last) {
+                load_k(k, i);
+                load_v(v, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             if (a.scale < 0.f) {
 #pragma unroll
                 for (int x = 0; x < N::kQ; ++x)
@@ -300,15 +332,7 @@ k_tree_narrow(TreeArgs a) {
         }
         __syncthreads();
 
-        const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
-        const int cache = (L + KB - 1) / KB;  // its blocks; the drafts' follow
-        const int whole = L / KB;
-        const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
-        const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1];
-        const T* kd = (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
-        const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
-        // (a pair without keys has one block of none)
-        const int last = L > 0 || (a.d.K && n > 0) ? sp.last : 0;
+
         v4f o[MT][VS][VL];
         float m[MT], l[MT], used[MT];
 #pragma unroll
@@ -321,20 +345,9 @@ k_tree_narrow(TreeArgs a) {
                 for (int c = 0; c < VL; ++c) o[t][i][c] = v4f{0.f, 0.f, 0.f, 0.f};
         }
         bool odd = false;
-        typename N::Keys k;
-        auto load_k = [&](int i) {
-            const bool in = i < cache;
-            N::load_k(k, in ? kc : kd, in ? a.c.ks[2] : a.d.ks[2], (in ? i : i - cache) * KB,
-                      in ? L : n, D, lane);
-        };
-        int i = sp.first + wave;
-        if (N::kAhead && i < last) load_k(i);
         for (; i < last; i += WAVES) {
-            if (!N::kAhead) load_k(i);
             const bool in = i < cache;
             const int j0 = (in ? i : i - cache) * KB;
-            typename N::Vals v;
-            N::load_v(v, in ? vc : vd, in ? a.c.vs[2] : a.d.vs[2], j0, in ? L : n, D, lane);
             __builtin_amdgcn_sched_barrier(0);
             float p[MT][SUB][4];
             {
@@ -358,7 +371,7 @@ k_tree_narrow(TreeArgs a) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) p[t][u][e] = s[t][u][e];
             }
-            if (N::kAhead && i + WAVES < last) load_k(i + WAVES);
+            if (N::kAhead && i + WAVES < last) load_k(k, i + WAVES);
             __builtin_amdgcn_sched_barrier(0);
             if (i >= whole) {
                 odd |= clear_not_finite<T>(v);
@@ -415,6 +428,11 @@ k_tree_narrow(TreeArgs a) {
                     }
             }
             N::accumulate(o, v, p, used);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + WAVES < last) {
+                if (!N::kAhead) load_k(k, i + WAVES);
+                load_v(v, i + WAVES);
+            }
         }
 
         // The waves' results added up: each scales its own to the maximum of all and leaves it in
@@ -425,19 +443,33 @@ k_tree_narrow(TreeArgs a) {
             used[t] = sizeof(T) == 2 ? row_sum(used[t]) : l[t];
         }
         float* xo = reinterpret_cast<float*>(lds);
-        float4* xs = reinterpret_cast<float4*>(lds + N::kLds - WAVES * N::ROWS * 16);
+        float4* xs = reinterpret_cast<float4*>(lds + N::kOut);
         if (q == 0) {
 #pragma unroll
             for (int t = 0; t < MT; ++t)
                 xs[wave * N::ROWS + 16 * t + col] = make_float4(m[t], l[t], used[t], odd ? 1.f : 0.f);
         }
         __syncthreads();  // (and Q is no longer read)
+        float4* fin = xs + WAVES * N::ROWS;  // of each row: maximum, sums, whether anything is odd
+        odd = false;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             float top = m[t];
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) top = fmaxf(top, xs[w * N::ROWS + 16 * t + col].x);
-            const float f = exp2_(m[t] - base_of(top));
+            const float base = base_of(top), f = exp2_(m[t] - base);
+            if (wave == t % WAVES) {
+                float4 z = make_float4(top, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    const float4 y = xs[w * N::ROWS + 16 * t + col];
+                    const float e = exp2_(y.x - base);
+                    z.y += y.y * e;
+                    z.z += y.z * e;
+                    odd |= y.w != 0.f;
+                }
+                if (q == 0) fin[16 * t + col] = z;
+            }
             float* to = xo + (wave * N::ROWS + 16 * t + col) * N::LDO + N::RUN * q;
 #pragma unroll
             for (int x = 0; x < VS; ++x)
@@ -450,24 +482,15 @@ k_tree_narrow(TreeArgs a) {
                                         o[t][x][c + 2][e] * f, o[t][x][c + 3][e] * f);
         }
         __syncthreads();
-        odd = false;
         // (opaque: or what this computes is hoisted out of the loop over spans, into registers)
+#pragma unroll 2
         for (int e = opaque(threadIdx.x); e < N::ROWS * (DP / 4); e += 64 * WAVES) {
             const int r = e / (DP / 4), d = e % (DP / 4) * 4, row = tile * N::ROWS + r;
             const int h = head_of(a.d, row), tok = row - h * a.d.T;
-            if (row >= R || tok >= n || d >= D) continue;
-            float M = -INFINITY, sum = 0.f, su = 0.f;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) M = fmaxf(M, xs[w * N::ROWS + r].x);
-            const float base = base_of(M);
+            const float4 z = fin[r];
             float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float4 z = xs[w * N::ROWS + r];
-                const float f = exp2_(z.x - base);
-                sum += z.y * f;
-                su += z.z * f;
-                odd |= z.w != 0.f;
                 const float* from = xo + (w * N::ROWS + r) * N::LDO;
                 if constexpr (MODE == kClamp) {
                     // (a piece that the row's end cut holds the row's last dims)
@@ -481,16 +504,17 @@ k_tree_narrow(TreeArgs a) {
                     x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
                 }
             }
+            if (row >= R || tok >= n || d >= D) continue;
             if (sp.part >= 0) {
                 const size_t to = part_row(a, sp.part, row);
-                if (d == 0) part_stats(a)[to] = make_float4(M, sum, su, 0.f);
+                if (d == 0) part_stats(a)[to] = z;
                 store4(part_dims(a) + to * D + d, x, D - d);
             } else {
                 // (0: nothing visible, or no score above -infinity)
-                const float inv = su == 0.f ? 0.f : 1.f / su;
+                const float inv = z.z == 0.f ? 0.f : 1.f / z.z;
                 if (d == 0 && a.lse)
                     a.lse[((size_t)b * a.d.H + g * rep + h) * a.d.T + tok] =
-                        sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
+                        z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) x[c] *= inv;
                 store4((T*)a.out + b * a.os[0] + (g * rep + h) * a.os[1] + tok * a.os[2] + d, x, D - d);
@@ -533,7 +557,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
     tile_of(blockIdx.x, a.bs * a.gs * a.plan.shares * most, tiles, &unit, &tile);
     const int share = unit % a.plan.shares, i = unit / a.plan.shares % most;
     const int pair = unit / a.plan.shares / most, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
-    const int L = rows_in_use(a.c, b), n = drafts_of(a.d, b), D = a.c.D;
+    const int L = of_wave(rows_in_use(a.c, b)), n = of_wave(drafts_of(a.d, b)), D = a.c.D;
     const int cache = (L + kBlock - 1) / kBlock;
     const int all = cache + (a.d.K ? (n + kBlock - 1) / kBlock : 0);
     if (i >= all) return;
@@ -591,7 +615,7 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
     __shared__ float alpha[2][ROWS];
     __shared__ float4 fin[ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int q = lane >> 4, col = lane & 15;
+    const int col = lane & 15;
     const int D = a.c.D, groups = (D + WD * kWaves - 1) / (WD * kWaves);
     const int tiles = a.plan.row_tiles;
     int unit, tile;
@@ -616,7 +640,8 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
             sp = span_whole(a, range, kBlock);
             at = end;
         }
-        const int b = sp.b, g = sp.g, L = rows_in_use(a.c, b), n = drafts_of(a.d, b);
+        const int b = sp.b, g = sp.g;
+        const int L = of_wave(rows_in_use(a.c, b)), n = of_wave(drafts_of(a.d, b));
         const int cache = (L + kBlock - 1) / kBlock;
         const bool none = L == 0 && (!a.d.K || n == 0);  // a pair without keys has no scores either
         const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1] + d0;
@@ -656,9 +681,11 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
         auto load_v = [&](typename N::Vals& to, int x) {
             const int i = min(sp.first + x / (kBlock / PK), sp.last - 1);
             const bool in = i < cache;
-            N::load_v(to, in ? vc : vd, in ? a.c.vs[2] : a.d.vs[2],
-                      (in ? i : i - cache) * kBlock + x % (kBlock / PK) * PK, in ? L : n, D - d0,
-                      lane);
+            // (a block's second half may have no rows: its first row again)
+            const int j1 = (in ? i : i - cache) * kBlock, half = j1 + x % (kBlock / PK) * PK;
+            const int j0 = half < (in ? L : n) ? half : j1;
+            const int64_t s = in ? a.c.vs[2] : a.d.vs[2];
+            N::load_v(to, (in ? vc : vd) + j0 * s, s, (in ? L : n) - j0, D - d0, lane);
         };
         // Two buffers of weights: a wave past a barrier writes the other one, and comes to write
         // this one only after the next barrier, when every wave has read it.
@@ -796,17 +823,20 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
 }
 
 // ---------------------------------------------------------------- parts
-// The parts of a row added up, in their order: a workgroup per (row, 256 dims), its 4 waves
-// every fourth part.  Rows of one range alone are written already.
-template <typename T>
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn) {
+// The parts of a row added up, in their order: WAVES waves a row (and 256 dims), each every
+// WAVES-th part; 4 rows a workgroup where there are many rows.  Rows of one range alone are
+// written already.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn, unsigned units) {
     __shared__ float acc[4][256];
     __shared__ float2 sums[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int D = a.c.D, chunks = (D + 255) / 256, rep = a.d.H / a.c.G, R = rep * a.d.T;
-    const int d0 = (blockIdx.x % chunks) * 256, row = blockIdx.x / chunks % R;
-    const int pair = blockIdx.x / chunks / R, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
-    const int tok = row - head_of(a.d, row) * a.d.T, h = g * rep + head_of(a.d, row);
+    const unsigned unit = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
+    if (unit >= units) return;
+    const int d0 = (unit % chunks) * 256, row = unit / chunks % R;
+    const int pair = unit / chunks / R, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
+    const int h = head_of(a.d, row), tok = row - h * a.d.T;
     if (tok >= drafts_of(a.d, b)) return;
     int before = 0, total = 0;  // blocks of a kv head of the sequences before, and of all
     for (int i = lane; i < a.bs; i += 64) {
@@ -819,9 +849,9 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn
         total += __shfl_xor(total, o);
         before += __shfl_xor(before, o);
     }
-    const int blocks = blocks_of(a, b, kb);
-    const Line line = line_from(a, total * a.gs, turn);
-    const int first = before * a.gs + (g - a.g0) * blocks;
+    const int blocks = of_wave(blocks_of(a, b, kb));
+    const Line line = line_from(a, __builtin_amdgcn_readfirstlane(total) * a.gs, turn);
+    const int first = __builtin_amdgcn_readfirstlane(before) * a.gs + (g - a.g0) * blocks;
     const int r0 = first / line.per, r1 = (first + blocks - 1) / line.per;
     if (r0 == r1) return;
     const float4* st = part_stats(a);
@@ -834,7 +864,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn
     const float base = base_of(M);
     float l = 0.f, used = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = wave; i < parts; i += 4) {
+    for (int i = WAVES == 4 ? wave : 0; i < parts; i += WAVES) {
         const size_t at = row_of(i);
         const float4 z = st[at];
         const float f = exp2_(z.x - base);
@@ -849,19 +879,26 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn
             x[c] += f == 0.f && !(fabsf(y) < INFINITY) ? y : f * y;
         }
     }
+    T* out = (T*)a.out + b * a.os[0] + (g * rep + h) * a.os[1] + tok * a.os[2] + d0;
+    if constexpr (WAVES == 4) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[wave][lane + 64 * c] = x[c];
-    if (lane == 0) sums[wave] = make_float2(l, used);
-    __syncthreads();
-    l = (sums[0].x + sums[1].x) + (sums[2].x + sums[3].x);
-    used = (sums[0].y + sums[1].y) + (sums[2].y + sums[3].y);
-    const float inv = used == 0.f ? 0.f : 1.f / used;
-    const int d = threadIdx.x;
-    if (d0 + d < D)
-        Elem<T>::st((T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2], d0 + d,
-                    ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv);
-    if (d0 + d == 0 && a.lse)
-        a.lse[((size_t)b * a.d.H + h) * a.d.T + tok] =
+        for (int c = 0; c < 4; ++c) acc[wave][lane + 64 * c] = x[c];
+        if (lane == 0) sums[wave] = make_float2(l, used);
+        __syncthreads();
+        l = (sums[0].x + sums[1].x) + (sums[2].x + sums[3].x);
+        used = (sums[0].y + sums[1].y) + (sums[2].y + sums[3].y);
+        const int d = threadIdx.x;
+        const float inv = used == 0.f ? 0.f : 1.f / used;
+        if (d0 + d < D)
+            Elem<T>::st(out, d, ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv);
+    } else {
+        const float inv = used == 0.f ? 0.f : 1.f / used;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (d0 + lane + 64 * c < D) Elem<T>::st(out, lane + 64 * c, x[c] * inv);
+    }
+    if (d0 == 0 && (WAVES == 4 ? threadIdx.x : lane) == 0 && a.lse)
+        a.lse[((size_t)b * a.d.H + g * rep + h) * a.d.T + tok] =
             l == 0.f ? -INFINITY : (M + log2f(l)) * kLn2;
 }
 
@@ -927,10 +964,16 @@ void go(const TreeArgs& a, hipStream_t st) {
     }
     if (a.plan.split) {
         const bool wide = D > kTreeNarrow;
-        const size_t rows = (size_t)a.bs * a.gs * (a.d.H / a.c.G) * a.d.T;
-        hipLaunchKernelGGL(k_tree_merge<T>, dim3((unsigned)(rows * ((D + 255) / 256))), dim3(256),
-                           0, st, a, wide || sizeof(T) == 2 ? 32 : 16,
-                           wide ? kValueKeys / kBlock : a.plan.waves);
+        const unsigned units = (unsigned)((size_t)a.bs * a.gs * (a.d.H / a.c.G) * a.d.T *
+                                          ((D + 255) / 256));
+        const int kb = wide || sizeof(T) == 2 ? 32 : 16;
+        const int turn = wide ? kValueKeys / kBlock : a.plan.waves;
+        if (units >= 1024)
+            hipLaunchKernelGGL((k_tree_merge<T, 1>), dim3((units + 3) / 4), dim3(256), 0, st, a, kb,
+                               turn, units);
+        else
+            hipLaunchKernelGGL((k_tree_merge<T, 4>), dim3(units), dim3(256), 0, st, a, kb, turn,
+                               units);
     }
 }
 
