@@ -93,7 +93,7 @@ struct TreePlan {
     int rows;        // query rows of a tile
     int row_tiles;   // tiles of the query rows of one kv head
     int waves;       // of a workgroup (head_d <= 256)
-    int split;
+    int split, turn; // ranges in whole turns of so many blocks
     int ranges;
     int seqs, kv;
     int ld_scores;   // head_d > 256: row of the scores, floats

@@ -221,6 +221,110 @@ __device__ void add_not_finite(const TreeArgs& a, const Span& s, int row, int fr
     }
 }
 
+// ---------------------------------------------------------------- steps of a block
+// Scores of what a row does not attend become -infinity, in a block that is not whole cache rows:
+// its `rows` rows from j0 on of the cache (in), or of the drafts.
+template <int MT, int SUB>
+__device__ __forceinline__ void hide(const TreeArgs& a, float (&p)[MT][SUB][4], int t, int b, int row,
+                                     bool in, int j0, int rows, int q) {
+    uint32_t see = rows >= 32 ? ~0u : (1u << rows) - 1;  // bit j: the row attends key j
+    if (!in) {
+        const int tok = row - head_of(a.d, row) * a.d.T;
+        if (a.d.mask) {
+            see &= a.d.mask[((size_t)b * a.d.T + tok) * a.d.W + (j0 >> 5)] >> (j0 & 31);
+        } else {
+            const int upto = tok - j0;  // keys 0 .. upto
+            see &= upto < 0 ? 0u : upto >= 31 ? ~0u : (2u << upto) - 1;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (!((see >> (16 * u + 4 * q + e)) & 1u)) p[t][u][e] = -INFINITY;
+}
+
+// Scores into weights.  The running maximum moves only when a score passes it by more than 8
+// (weights up to 2^8 lose nothing in fp32 or bf16), so the tile is rarely rescaled.
+template <int MT, int SUB, int VS, int VL>
+__device__ __forceinline__ void weights(float (&p)[MT][SUB][4], v4f (&o)[MT][VS][VL], float (&m)[MT],
+                                        float (&l)[MT], float (&used)[MT], float scale) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        float top = p[t][0][0];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, p[t][u][e]);
+        if (__builtin_amdgcn_ballot_w64(top * scale > m[t] + 8.f)) {
+            const float m_new = fmaxf(m[t], row_max(top) * scale);
+            const float f = exp2_(m[t] - base_of(m_new));
+            m[t] = m_new;
+            l[t] *= f;
+            used[t] *= f;
+#pragma unroll
+            for (int x = 0; x < VS; ++x)
+#pragma unroll
+                for (int c = 0; c < VL; ++c) o[t][x][c] *= f;
+        }
+        const float base = base_of(m[t]);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[t][u][e] = exp2_(fmaf(p[t][u][e], scale, -base));
+                l[t] += p[t][u][e];
+            }
+    }
+}
+
+// The results of `parts` waves a row, scaled alike, in LDS (rows of LDO floats), summed and
+// written: to the output, or the span's part.  fin: the rows' maxima and sums.
+template <typename T, int DP, int ROWS, int PARTS, int LDO, int VL, int MODE, int THREADS>
+__device__ __forceinline__ void write_rows(const TreeArgs& a, const Span& sp, int tile, int n,
+                                           const float* xo, const float4* fin) {
+    const int D = a.c.D, rep = a.d.H / a.c.G, R = rep * a.d.T;
+    // (opaque: or what this computes is hoisted out of the loop over spans, into registers)
+#pragma unroll 2
+    for (int e = opaque(threadIdx.x); e < ROWS * (DP / 4); e += THREADS) {
+        const int r = e / (DP / 4), d = e % (DP / 4) * 4, row = tile * ROWS + r;
+        const int h = head_of(a.d, row), tok = row - h * a.d.T;
+        const float4 z = fin[r];
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < PARTS; ++w) {
+            const float* from = xo + (w * ROWS + r) * LDO;
+            if constexpr (MODE == kClamp) {
+                // (a piece that the row's end cut holds the row's last dims)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int piece = (d + c) / VL * VL;
+                    x[c] += from[min(d + c + max(0, piece - (D - VL)), DP - 1)];
+                }
+            } else {
+                const float4 y = *reinterpret_cast<const float4*>(from + d);
+                x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+            }
+        }
+        if (row >= R || tok >= n || d >= D) continue;
+        if (sp.part >= 0) {
+            const size_t to = part_row(a, sp.part, row);
+            if (d == 0) part_stats(a)[to] = z;
+            store4(part_dims(a) + to * D + d, x, D - d);
+        } else {
+            // (0: nothing visible, or no score above -infinity)
+            const float inv = z.z == 0.f ? 0.f : 1.f / z.z;
+            if (d == 0 && a.lse)
+                a.lse[((size_t)sp.b * a.d.H + sp.g * rep + h) * a.d.T + tok] =
+                    z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[c] *= inv;
+            store4((T*)a.out + sp.b * a.os[0] + (sp.g * rep + h) * a.os[1] + tok * a.os[2] + d, x,
+                   D - d);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- head_d <= 256
 // Every wave walks its own blocks of keys, alone: scores, running maximum and
 // sum, and its own output tile in registers (cache_tiles.hpp); nothing passes through LDS
@@ -375,58 +479,12 @@ k_tree_narrow(TreeArgs a) {
             __builtin_amdgcn_sched_barrier(0);
             if (i >= whole) {
                 odd |= clear_not_finite<T>(v);
-                const int rows = (in ? L : n) - j0;
-                const uint32_t valid = rows >= 32 ? ~0u : (1u << rows) - 1;
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    uint32_t see = valid;  // bit j: the row attends key j of the block
-                    if (!in) {
-                        const int row = tile * N::ROWS + 16 * t + col;
-                        const int tok = row - head_of(a.d, row) * a.d.T;
-                        if (a.d.mask) {
-                            see &= a.d.mask[((size_t)b * a.d.T + tok) * a.d.W + (j0 >> 5)] >>
-                                   (j0 & 31);
-                        } else {
-                            const int upto = tok - j0;  // keys 0 .. upto
-                            see &= upto < 0 ? 0u : upto >= 31 ? ~0u : (2u << upto) - 1;
-                        }
-                    }
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!((see >> (16 * u + 4 * q + e)) & 1u)) p[t][u][e] = -INFINITY;
-                }
+                for (int t = 0; t < MT; ++t)
+                    hide<MT, SUB>(a, p, t, b, tile * N::ROWS + 16 * t + col, in, j0,
+                                  (in ? L : n) - j0, q);
             }
-            // The running maximum moves only when a score passes it by more than 8 (weights up
-            // to 2^8 lose nothing in fp32 or bf16), so the tile is rarely rescaled.
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                float top = p[t][0][0];
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, p[t][u][e]);
-                if (__builtin_amdgcn_ballot_w64(top * scale > m[t] + 8.f)) {
-                    const float m_new = fmaxf(m[t], row_max(top) * scale);
-                    const float f = exp2_(m[t] - base_of(m_new));
-                    m[t] = m_new;
-                    l[t] *= f;
-                    used[t] *= f;
-#pragma unroll
-                    for (int x = 0; x < VS; ++x)
-#pragma unroll
-                        for (int c = 0; c < VL; ++c) o[t][x][c] *= f;
-                }
-                const float base = base_of(m[t]);
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        p[t][u][e] = exp2_(fmaf(p[t][u][e], scale, -base));
-                        l[t] += p[t][u][e];
-                    }
-            }
+            weights<MT, SUB, VS, VL>(p, o, m, l, used, scale);
             N::accumulate(o, v, p, used);
             __builtin_amdgcn_sched_barrier(0);
             if (i + WAVES < last) {
@@ -482,48 +540,225 @@ k_tree_narrow(TreeArgs a) {
                                         o[t][x][c + 2][e] * f, o[t][x][c + 3][e] * f);
         }
         __syncthreads();
-        // (opaque: or what this computes is hoisted out of the loop over spans, into registers)
-#pragma unroll 2
-        for (int e = opaque(threadIdx.x); e < N::ROWS * (DP / 4); e += 64 * WAVES) {
-            const int r = e / (DP / 4), d = e % (DP / 4) * 4, row = tile * N::ROWS + r;
-            const int h = head_of(a.d, row), tok = row - h * a.d.T;
-            const float4 z = fin[r];
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                const float* from = xo + (w * N::ROWS + r) * N::LDO;
-                if constexpr (MODE == kClamp) {
-                    // (a piece that the row's end cut holds the row's last dims)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int piece = (d + c) / VL * VL;
-                        x[c] += from[min(d + c + max(0, piece - (D - VL)), DP - 1)];
-                    }
-                } else {
-                    const float4 y = *reinterpret_cast<const float4*>(from + d);
-                    x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
-                }
-            }
-            if (row >= R || tok >= n || d >= D) continue;
-            if (sp.part >= 0) {
-                const size_t to = part_row(a, sp.part, row);
-                if (d == 0) part_stats(a)[to] = z;
-                store4(part_dims(a) + to * D + d, x, D - d);
-            } else {
-                // (0: nothing visible, or no score above -infinity)
-                const float inv = z.z == 0.f ? 0.f : 1.f / z.z;
-                if (d == 0 && a.lse)
-                    a.lse[((size_t)b * a.d.H + g * rep + h) * a.d.T + tok] =
-                        z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[c] *= inv;
-                store4((T*)a.out + b * a.os[0] + (g * rep + h) * a.os[1] + tok * a.os[2] + d, x, D - d);
-            }
-        }
+        write_rows<T, DP, N::ROWS, WAVES, N::LDO, VL, MODE, 64 * WAVES>(a, sp, tile, n, xo, fin);
         if (__syncthreads_or(odd)) {
             // (behind the barrier, which waits for the workgroup's stores)
             for (int r = wave; r < N::ROWS; r += WAVES)
                 add_not_finite<T>(a, sp, tile * N::ROWS + r, whole * KB, L, n, 0, D, lane);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- many query rows
+// bf16, 65 to 128 dims, more than 32 query rows of a kv head.  K and V now serve several waves'
+// rows, and products and softmax weigh as much as the reads: 8 waves a workgroup, each with 32
+// rows in registers (two waves a SIMD, one's softmax beside the other's products), RG of them
+// over different rows and KG = 8 / RG over different blocks.  A stage of KG blocks comes
+// through LDS in the order of its fragments -- each wave loads 2 KG of the pieces that
+// k_tree_narrow's lanes load for themselves -- while the stage before is worked on.
+template <int RG, int MODE>
+struct Shared : CacheTiles<uint16_t, 128, 2, MODE> {
+    using N = CacheTiles<uint16_t, 128, 2, MODE>;
+    static constexpr int KG = 8 / RG, ROWS_WG = 32 * RG;
+    static constexpr int PIECES = N::SUB * N::KS + N::KEYS;  // of a block, 1 KiB each
+    static_assert(PIECES == 16 && N::VS == 1, "a K and a V piece of each block a wave");
+    static constexpr int LDO = 128 + 4;
+    static constexpr int kStage = KG * PIECES * 1024;
+    static constexpr int kXBytes = KG * ROWS_WG * LDO * 4;
+    static constexpr int kOut = 2 * kStage > kXBytes ? 2 * kStage : kXBytes;
+    static constexpr int kLds = kOut + (KG + 1) * ROWS_WG * 16;
+    static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+template <int RG, int MODE>
+__global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
+    using N = Shared<RG, MODE>;
+    using T = uint16_t;
+    constexpr int MT = 2, KB = N::KB, SUB = N::SUB, KS = N::KS, VL = N::VL, KG = N::KG, DP = 128;
+    __shared__ __align__(16) char lds[N::kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q = lane >> 4, col = lane & 15, rg = wave % RG, kg = wave / RG;
+    int range, tile;
+    tile_of(blockIdx.x, a.plan.ranges, a.plan.row_tiles, &range, &tile);
+    const int D = a.c.D, rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const float scale = fabsf(a.scale);
+
+    int at = 0, end = 1;
+    if (a.plan.split) {
+        const Line line = line_of(a, KB, KG, lane);
+        at = range * line.per;
+        end = min(line.total, at + line.per);
+    }
+    while (at < end) {
+        Span sp;
+        if (a.plan.split) {
+            sp = span_at(a, range, at, end, KB, lane, &at);
+        } else {
+            sp = span_whole(a, range, KB);
+            at = end;
+        }
+        const int b = sp.b, g = sp.g;
+        const int L = of_wave(rows_in_use(a.c, b)), n = of_wave(drafts_of(a.d, b));
+        const int cache = (L + KB - 1) / KB, whole = L / KB;
+        // (a pair without keys has one block of none)
+        const int last = L > 0 || (a.d.K && n > 0) ? sp.last : 0;
+        const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
+        const T* vc = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1];
+        const T* kd = (const T*)a.d.K + b * a.d.ks[0] + g * a.d.ks[1];
+        const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
+
+        // this wave's pieces of the stage at block i: of every block K piece (wave / KS, wave % KS)
+        // and V's row `wave` of each lane (past the last block, of it)
+        typename N::KPiece z[2 * KG];
+        auto load = [&](int i) {
+#pragma unroll
+            for (int x = 0; x < KG; ++x) {
+                const int y = min(i + x, last - 1);
+                const bool in = y < cache;
+                const int j0 = (in ? y : y - cache) * KB, rows = min(KB, (in ? L : n) - j0);
+                const int64_t ks = in ? a.c.ks[2] : a.d.ks[2], vs = in ? a.c.vs[2] : a.d.vs[2];
+                const uint32_t kr = (uint32_t)ks * 2, vr = (uint32_t)vs * 2;
+                z[2 * x] = N::piece((in ? kc : kd) + j0 * ks,
+                                    min(16 * (wave / KS) + col, rows - 1) * kr + 16 * q, wave % KS, q,
+                                    D);
+                z[2 * x + 1] = N::v_piece((in ? vc : vd) + j0 * vs,
+                                          min(N::key_of(lane, wave), rows - 1) * vr, 0, D, lane);
+            }
+        };
+        auto* stage = reinterpret_cast<typename N::KPiece*>(lds);
+        auto put = [&](int buf) {
+#pragma unroll
+            for (int x = 0; x < 2 * KG; ++x)
+                stage[((buf * KG + x / 2) * N::PIECES + (x & 1) * 8 + wave) * 64 + lane] = z[x];
+        };
+        if (sp.first < last) load(sp.first);
+        // Q: this wave's rows in registers (those of no token hold the last token's: nobody reads
+        // their results)
+        typename N::KPiece qf[MT][KS];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int row = min(tile * N::ROWS_WG + rg * 32 + 16 * t + col, R - 1);
+            const int h = head_of(a.d, row);
+            const T* qb = (const T*)a.d.Q + b * a.d.qs[0] + (g * rep + h) * a.d.qs[1] +
+                          (row - h * a.d.T) * a.d.qs[2];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                qf[t][i] = N::piece(qb, 16 * q, i, q, D);
+                if (a.scale < 0.f)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) qf[t][i].w[w] ^= 0x80008000u;
+            }
+        }
+        v4f o[MT][1][VL];
+        float m[MT], l[MT], used[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = used[t] = 0.f;
+#pragma unroll
+            for (int c = 0; c < VL; ++c) o[t][0][c] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        bool odd = false;
+        __syncthreads();  // (the last span's results are out of LDS)
+        if (sp.first < last) put(0);
+        __syncthreads();
+        int buf = 0;
+        for (int i0 = sp.first; i0 < last; i0 += KG, buf ^= 1) {
+            const bool more = i0 + KG < last;
+            if (more) load(i0 + KG);
+            __builtin_amdgcn_sched_barrier(0);
+            const int i = i0 + kg;
+            if (i < last) {
+                const auto* mine = stage + (buf * KG + kg) * N::PIECES * 64 + lane;
+                v4f s[MT][SUB];
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < KS; ++e)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) {
+                        const typename N::KPiece k = mine[(u * KS + e) * 64];
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) s[t][u] = N::dot(k, qf[t][e], s[t][u]);
+                    }
+                typename N::Vals v;
+#pragma unroll
+                for (int j = 0; j < N::KEYS; ++j) v.p[j][0] = mine[(8 + j) * 64];
+                float p[MT][SUB][4];
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[t][u][e] = s[t][u][e];
+                if (i >= whole) {
+                    const bool in = i < cache;
+                    const int j0 = (in ? i : i - cache) * KB, rows = (in ? L : n) - j0;
+                    odd |= clear_not_finite<T>(v);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+                        hide<MT, SUB>(a, p, t, b, tile * N::ROWS_WG + rg * 32 + 16 * t + col, in, j0,
+                                      rows, q);
+                }
+                weights<MT, SUB, 1, VL>(p, o, m, l, used, scale);
+                N::accumulate(o, v, p, used);
+            }
+            if (more) put(buf ^ 1);
+            __syncthreads();
+        }
+
+        // the KG waves of a row tile added up, as in k_tree_narrow
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            l[t] = row_sum(l[t]);
+            used[t] = row_sum(used[t]);
+        }
+        float* xo = reinterpret_cast<float*>(lds);
+        float4* xs = reinterpret_cast<float4*>(lds + N::kOut);
+        float4* fin = xs + KG * N::ROWS_WG;
+        if (q == 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                xs[kg * N::ROWS_WG + rg * 32 + 16 * t + col] =
+                    make_float4(m[t], l[t], used[t], odd ? 1.f : 0.f);
+        }
+        __syncthreads();
+        odd = false;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int r = rg * 32 + 16 * t + col;
+            float top = m[t];
+#pragma unroll
+            for (int w = 0; w < KG; ++w) top = fmaxf(top, xs[w * N::ROWS_WG + r].x);
+            const float base = base_of(top), f = exp2_(m[t] - base);
+            if (kg == 0) {
+                float4 y = make_float4(top, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < KG; ++w) {
+                    const float4 x = xs[w * N::ROWS_WG + r];
+                    const float e = exp2_(x.x - base);
+                    y.y += x.y * e;
+                    y.z += x.z * e;
+                    odd |= x.w != 0.f;
+                }
+                if (q == 0) fin[r] = y;
+            }
+            float* to = xo + (kg * N::ROWS_WG + r) * N::LDO + N::RUN * q;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < VL; c += 4)
+                    *reinterpret_cast<float4*>(to + VL * e + c) =
+                        make_float4(o[t][0][c][e] * f, o[t][0][c + 1][e] * f, o[t][0][c + 2][e] * f,
+                                    o[t][0][c + 3][e] * f);
+        }
+        __syncthreads();
+        write_rows<T, DP, N::ROWS_WG, KG, N::LDO, VL, MODE, 512>(a, sp, tile, n, xo, fin);
+        if (__syncthreads_or(odd)) {
+            for (int r = wave; r < N::ROWS_WG; r += 8)
+                add_not_finite<T>(a, sp, tile * N::ROWS_WG + r, whole * KB, L, n, 0, D, lane);
         }
     }
 }
@@ -919,7 +1154,16 @@ template <typename T, int DP, int MODE>
 void go_rows(const TreeArgs& a, hipStream_t st) {
     if (a.plan.rows == 16) return go_narrow<T, DP, 1, MODE>(a, st);
     if (a.plan.rows == 32) return go_narrow<T, DP, 2, MODE>(a, st);
-    if constexpr (DP <= 128 && sizeof(T) == 2) go_narrow<T, DP, 4, MODE>(a, st);
+    if constexpr (DP == 64 && sizeof(T) == 2) go_narrow<T, DP, 4, MODE>(a, st);
+    if constexpr (DP == 128 && sizeof(T) == 2) {
+        const dim3 grid((unsigned)(a.plan.ranges * a.plan.row_tiles));
+        if (a.plan.rows == 64)
+            hipLaunchKernelGGL((k_tree_shared<2, MODE>), grid, dim3(512), 0, st, a);
+        else if (a.plan.rows == 128)
+            hipLaunchKernelGGL((k_tree_shared<4, MODE>), grid, dim3(512), 0, st, a);
+        else
+            hipLaunchKernelGGL((k_tree_shared<8, MODE>), grid, dim3(512), 0, st, a);
+    }
 }
 
 template <typename T, int DP>
@@ -967,7 +1211,7 @@ void go(const TreeArgs& a, hipStream_t st) {
         const unsigned units = (unsigned)((size_t)a.bs * a.gs * (a.d.H / a.c.G) * a.d.T *
                                           ((D + 255) / 256));
         const int kb = wide || sizeof(T) == 2 ? 32 : 16;
-        const int turn = wide ? kValueKeys / kBlock : a.plan.waves;
+        const int turn = wide ? kValueKeys / kBlock : a.plan.turn;
         if (units >= 1024)
             hipLaunchKernelGGL((k_tree_merge<T, 1>), dim3((units + 3) / 4), dim3(256), 0, st, a, kb,
                                turn, units);
@@ -986,8 +1230,13 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     TreePlan p{};
     const bool bf = dtype == kDtypeBF16, wide = D > kTreeNarrow;
     const int R = H / G * T;
-    const int most = bf && D <= 128 ? 64 : 32;
-    p.rows = R <= 16 ? 16 : R <= 32 ? 32 : most;
+    const bool shared = bf && D > 64 && D <= 128 && R > 32;
+    p.rows = R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64;
+    if (shared) {  // the rows of a workgroup that leave the fewest places empty
+        p.rows = 256;
+        for (int r : {128, 64})
+            if (ceil_div(R, r) * r < ceil_div(R, p.rows) * p.rows) p.rows = r;
+    }
     p.row_tiles = (int)ceil_div(R, p.rows);
     p.waves = 4;
     const int kb = wide || bf ? 32 : 16, mt = p.rows / 16;
@@ -999,13 +1248,15 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     // workgroups that the card holds at once (256 CUs; the kernels' registers)
     const int per_cu = wide ? (mt == 1 ? 3 : 2)
                             : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
-    const int64_t slots = std::max<int64_t>(1, 256 * per_cu / (p.row_tiles * groups));
-    const int64_t turn = wide ? kValueKeys / kBlock : p.waves;
+    const int64_t slots =
+        std::max<int64_t>(1, 256 * (shared ? 1 : per_cu) / (p.row_tiles * groups));
+    const int64_t turn = wide ? kValueKeys / kBlock : shared ? 256 / p.rows : p.waves;
     int64_t ranges = std::min(slots, ceil_div(pairs * blocks, 2 * turn));
     // one workgroup of 8 waves a pair where that leaves a wave few blocks: no second launch
     const bool small = !wide && mt <= 2 && D <= 128 && blocks <= 32 && pairs * p.row_tiles <= 512;
     p.split = !small && ranges > 1 && pairs < 4 * slots && blocks > turn;
     if (small) p.waves = 8;
+    p.turn = small ? p.waves : (int)turn;
     const size_t room = scratch_cap / sizeof(float);
     // score workgroups: two a CU, where the dims give each wave two steps still
     p.shares = 1;
