@@ -31,71 +31,98 @@ __device__ __forceinline__ int blocks_of(const TreeArgs& a, int b, int kb) {
     return max(1, (L + kb - 1) / kb + (a.d.K ? (n + kb - 1) / kb : 0));
 }
 
-__device__ __forceinline__ int wave_scan(int x, int lane) {  // sums of the lanes up to this one
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+// Sums of the lanes up to each.
+__device__ __forceinline__ int wave_scan(int x) {
+#define ATN_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, false)
+    ATN_SCAN_STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8 within 16 lanes
+    ATN_SCAN_STEP(0x112, 0xF);
+    ATN_SCAN_STEP(0x114, 0xF);
+    ATN_SCAN_STEP(0x118, 0xF);
+    ATN_SCAN_STEP(0x142, 0xA);  // row_bcast:15 into rows 1 and 3
+    ATN_SCAN_STEP(0x143, 0xC);  // row_bcast:31 into rows 2 and 3
+#undef ATN_SCAN_STEP
     return x;
 }
 
-// The line: its length, and the blocks of a range (whole turns of `turn`).  A wave's work, as
-// are the others here; results are uniform.
+// A pair takes as many places of the line as it has blocks, and kPad before them: beginning and
+// ending a pair costs a workgroup about as much time as so many blocks (10 us against 0.4 to
+// 0.7 us a block), so ranges of many short pairs have fewer blocks.
+constexpr int kPad = 16;
+
+// The line: its length, and the places of a range (whole turns of `turn`).  A wave's work, as
+// are the others here; results are uniform.  n, upto: of sequence b0 + lane where the pass has
+// at most 64, its pairs' places and the sum of all sequences' up to it.
 struct Line {
     int total, per;
+    int n, upto;
 };
-__device__ __forceinline__ Line line_from(const TreeArgs& a, int total, int turn) {
-    const int per = (total + a.plan.ranges - 1) / a.plan.ranges;
-    return Line{total, max((per + turn - 1) / turn * turn, 2 * turn)};
-}
 __device__ __forceinline__ Line line_of(const TreeArgs& a, int kb, int turn, int lane) {
-    int sum = 0;
-    for (int i = lane; i < a.bs; i += 64) sum += blocks_of(a, a.b0 + i, kb);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-    return line_from(a, __builtin_amdgcn_readfirstlane(sum) * a.gs, turn);
+    Line x;
+    x.n = lane < a.bs ? blocks_of(a, a.b0 + lane, kb) + kPad : 0;
+    x.upto = wave_scan(x.n * a.gs);
+    x.total = __builtin_amdgcn_readlane(x.upto, 63);
+    for (int i0 = 64; i0 < a.bs; i0 += 64) {
+        const int n = i0 + lane < a.bs ? blocks_of(a, a.b0 + i0 + lane, kb) + kPad : 0;
+        x.total += __builtin_amdgcn_readlane(wave_scan(n * a.gs), 63);
+    }
+    const int per = (x.total + a.plan.ranges - 1) / a.plan.ranges;
+    x.per = max((per + turn - 1) / turn * turn, 2 * turn);
+    return x;
 }
 
-// The sequence at position `at` of the line, and its place there.
+// The sequence at place `at` of the line.
 struct Place {
-    int b, blocks, start;  // sequence, blocks of each kv head, position of the first
+    int b, n, start;  // sequence, places of each of its pairs, place of the first
 };
-__device__ __forceinline__ Place place_at(const TreeArgs& a, int at, int kb, int lane) {
-    int before = 0;
+__device__ __forceinline__ Place place_at(const TreeArgs& a, const Line& line, int at, int kb,
+                                          int lane) {
+    int n = line.n, upto = line.upto;
     for (int i0 = 0;; i0 += 64) {
-        const int n = i0 + lane < a.bs ? blocks_of(a, a.b0 + i0 + lane, kb) : 0;
-        const int upto = before + wave_scan(n * a.gs, lane);
         const uint64_t done = __builtin_amdgcn_ballot_w64(upto <= at);
         if (done != ~0ull || i0 + 64 >= a.bs) {
             const int l = min(__builtin_popcountll(done), min(63, a.bs - 1 - i0));
             Place p;
             p.b = a.b0 + i0 + l;
-            p.blocks = __builtin_amdgcn_readlane(n, l);
-            p.start = __builtin_amdgcn_readlane(upto, l) - p.blocks * a.gs;
+            p.n = __builtin_amdgcn_readlane(n, l);
+            p.start = __builtin_amdgcn_readlane(upto, l) - p.n * a.gs;
             return p;
         }
-        before = __builtin_amdgcn_readlane(upto, 63);
+        const int before = __builtin_amdgcn_readlane(upto, 63), b = i0 + 64 + lane;
+        n = b < a.bs ? blocks_of(a, a.b0 + b, kb) + kPad : 0;
+        upto = before + wave_scan(n * a.gs);
     }
 }
+// Place of sequence b's first pair.
+__device__ __forceinline__ int start_of(const TreeArgs& a, const Line& line, int b, int kb, int lane) {
+    const int i = b - a.b0;
+    if (i < 64)
+        return __builtin_amdgcn_readlane(line.upto, i) - __builtin_amdgcn_readlane(line.n, i) * a.gs;
+    int before = 0;
+    for (int i0 = 0; i0 < i; i0 += 64) {
+        const int n = i0 + lane < i ? blocks_of(a, a.b0 + i0 + lane, kb) + kPad : 0;
+        before += __builtin_amdgcn_readlane(wave_scan(n * a.gs), 63);
+    }
+    return before;
+}
 
-// One pair's blocks [first, last) of a range, and where they go: `part` < 0: the output,
-// else the range's part of that number.
+// One pair's blocks [first, last) of a range (none where the range ends before them), and where
+// they go: `part` < 0: the output, else the range's part of that number.
 struct Span {
     int b, g, first, last, part;
 };
-// The span of range r that begins at `at` (*next: the position after it).
-__device__ __forceinline__ Span span_at(const TreeArgs& a, int r, int at, int end, int kb, int lane,
-                                        int* next) {
-    const Place p = place_at(a, at, kb, lane);
+// The span of range r that begins at `at` (*next: the place after it).
+__device__ __forceinline__ Span span_at(const TreeArgs& a, const Line& line, int r, int at, int end,
+                                        int kb, int lane, int* next) {
+    const Place p = place_at(a, line, at, kb, lane);
     Span s;
-    const int off = at - p.start;
+    const int off = at - p.start, pair = off / p.n, in = off - pair * p.n;
+    const int out = min(p.n, in + end - at);
     s.b = p.b;
-    s.g = a.g0 + off / p.blocks;
-    s.first = off % p.blocks;
-    s.last = min(p.blocks, s.first + end - at);
-    s.part = s.first == 0 && s.last == p.blocks ? -1 : 2 * r + (s.first == 0 ? 1 : 0);
-    *next = at + s.last - s.first;
+    s.g = a.g0 + pair;
+    s.first = max(0, in - kPad);
+    s.last = out - kPad;
+    s.part = s.first == 0 && out == p.n ? -1 : 2 * r + (s.first == 0 ? 1 : 0);
+    *next = at + out - in;
     return s;
 }
 // The whole of pair r, where ranges are pairs.
@@ -364,15 +391,17 @@ k_tree_narrow(TreeArgs a) {
     const float scale = fabsf(a.scale);
 
     int at = 0, end = 1;
+    Line line{};
     if (a.plan.split) {
-        const Line line = line_of(a, KB, WAVES, lane);
+        line = line_of(a, KB, a.plan.turn, lane);
         at = range * line.per;
         end = min(line.total, at + line.per);
     }
     while (at < end) {
         Span sp;
         if (a.plan.split) {
-            sp = span_at(a, range, at, end, KB, lane, &at);
+            sp = span_at(a, line, range, at, end, KB, lane, &at);
+            if (sp.last <= sp.first) continue;
         } else {
             sp = span_whole(a, range, KB);
             at = end;
@@ -553,17 +582,19 @@ k_tree_narrow(TreeArgs a) {
 // bf16, 65 to 128 dims, more than 32 query rows of a kv head.  K and V now serve several waves'
 // rows, and products and softmax weigh as much as the reads: 8 waves a workgroup, each with 32
 // rows in registers (two waves a SIMD, one's softmax beside the other's products), RG of them
-// over different rows and KG = 8 / RG over different blocks.  A stage of KG blocks comes
-// through LDS in the order of its fragments -- each wave loads 2 KG of the pieces that
+// over different rows and KG = 8 / RG over different blocks.  A stage of NB blocks comes
+// through LDS in the order of its fragments -- each wave loads 2 NB of the pieces that
 // k_tree_narrow's lanes load for themselves -- while the stage before is worked on.
 template <int RG, int MODE>
 struct Shared : CacheTiles<uint16_t, 128, 2, MODE> {
     using N = CacheTiles<uint16_t, 128, 2, MODE>;
     static constexpr int KG = 8 / RG, ROWS_WG = 32 * RG;
+    static constexpr int SB = RG == 2 ? 1 : 2;  // blocks of a wave in a stage
+    static constexpr int NB = KG * SB;          // ... of the stage
     static constexpr int PIECES = N::SUB * N::KS + N::KEYS;  // of a block, 1 KiB each
     static_assert(PIECES == 16 && N::VS == 1, "a K and a V piece of each block a wave");
     static constexpr int LDO = 128 + 4;
-    static constexpr int kStage = KG * PIECES * 1024;
+    static constexpr int kStage = NB * PIECES * 1024;
     static constexpr int kXBytes = KG * ROWS_WG * LDO * 4;
     static constexpr int kOut = 2 * kStage > kXBytes ? 2 * kStage : kXBytes;
     static constexpr int kLds = kOut + (KG + 1) * ROWS_WG * 16;
@@ -574,7 +605,8 @@ template <int RG, int MODE>
 __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
     using N = Shared<RG, MODE>;
     using T = uint16_t;
-    constexpr int MT = 2, KB = N::KB, SUB = N::SUB, KS = N::KS, VL = N::VL, KG = N::KG, DP = 128;
+    constexpr int MT = 2, KB = N::KB, SUB = N::SUB, KS = N::KS, VL = N::VL, KG = N::KG, NB = N::NB;
+    constexpr int DP = 128;
     __shared__ __align__(16) char lds[N::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15, rg = wave % RG, kg = wave / RG;
@@ -584,15 +616,17 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
     const float scale = fabsf(a.scale);
 
     int at = 0, end = 1;
+    Line line{};
     if (a.plan.split) {
-        const Line line = line_of(a, KB, KG, lane);
+        line = line_of(a, KB, a.plan.turn, lane);
         at = range * line.per;
         end = min(line.total, at + line.per);
     }
     while (at < end) {
         Span sp;
         if (a.plan.split) {
-            sp = span_at(a, range, at, end, KB, lane, &at);
+            sp = span_at(a, line, range, at, end, KB, lane, &at);
+            if (sp.last <= sp.first) continue;
         } else {
             sp = span_whole(a, range, KB);
             at = end;
@@ -609,10 +643,10 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
 
         // this wave's pieces of the stage at block i: of every block K piece (wave / KS, wave % KS)
         // and V's row `wave` of each lane (past the last block, of it)
-        typename N::KPiece z[2 * KG];
+        typename N::KPiece z[2 * NB];
         auto load = [&](int i) {
 #pragma unroll
-            for (int x = 0; x < KG; ++x) {
+            for (int x = 0; x < NB; ++x) {
                 const int y = min(i + x, last - 1);
                 const bool in = y < cache;
                 const int j0 = (in ? y : y - cache) * KB, rows = min(KB, (in ? L : n) - j0);
@@ -628,8 +662,8 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
         auto* stage = reinterpret_cast<typename N::KPiece*>(lds);
         auto put = [&](int buf) {
 #pragma unroll
-            for (int x = 0; x < 2 * KG; ++x)
-                stage[((buf * KG + x / 2) * N::PIECES + (x & 1) * 8 + wave) * 64 + lane] = z[x];
+            for (int x = 0; x < 2 * NB; ++x)
+                stage[((buf * NB + x / 2) * N::PIECES + (x & 1) * 8 + wave) * 64 + lane] = z[x];
         };
         if (sp.first < last) load(sp.first);
         // Q: this wave's rows in registers (those of no token hold the last token's: nobody reads
@@ -663,13 +697,14 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
         if (sp.first < last) put(0);
         __syncthreads();
         int buf = 0;
-        for (int i0 = sp.first; i0 < last; i0 += KG, buf ^= 1) {
-            const bool more = i0 + KG < last;
-            if (more) load(i0 + KG);
+        for (int i0 = sp.first; i0 < last; i0 += NB, buf ^= 1) {
+            const bool more = i0 + NB < last;
+            if (more) load(i0 + NB);
             __builtin_amdgcn_sched_barrier(0);
-            const int i = i0 + kg;
-            if (i < last) {
-                const auto* mine = stage + (buf * KG + kg) * N::PIECES * 64 + lane;
+            for (int y = kg; y < NB; y += KG) {
+                const int i = i0 + y;
+                if (i >= last) break;
+                const auto* mine = stage + (buf * NB + y) * N::PIECES * 64 + lane;
                 v4f s[MT][SUB];
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
@@ -862,15 +897,17 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
     const int sr = threadIdx.x >> 4, sk = (threadIdx.x & 15) * 8;
 
     int at = 0, end = 1;
+    Line line{};
     if (a.plan.split) {
-        const Line line = line_of(a, kBlock, kValueKeys / kBlock, lane);
+        line = line_of(a, kBlock, a.plan.turn, lane);
         at = range * line.per;
         end = min(line.total, at + line.per);
     }
     while (at < end) {
         Span sp;
         if (a.plan.split) {
-            sp = span_at(a, range, at, end, kBlock, lane, &at);
+            sp = span_at(a, line, range, at, end, kBlock, lane, &at);
+            if (sp.last <= sp.first) continue;
         } else {
             sp = span_whole(a, range, kBlock);
             at = end;
@@ -1062,7 +1099,7 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
 // WAVES-th part; 4 rows a workgroup where there are many rows.  Rows of one range alone are
 // written already.
 template <typename T, int WAVES>
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn, unsigned units) {
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, unsigned units) {
     __shared__ float acc[4][256];
     __shared__ float2 sums[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1073,20 +1110,9 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, int turn
     const int pair = unit / chunks / R, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
     const int h = head_of(a.d, row), tok = row - h * a.d.T;
     if (tok >= drafts_of(a.d, b)) return;
-    int before = 0, total = 0;  // blocks of a kv head of the sequences before, and of all
-    for (int i = lane; i < a.bs; i += 64) {
-        const int n = blocks_of(a, a.b0 + i, kb);
-        total += n;
-        if (a.b0 + i < b) before += n;
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        total += __shfl_xor(total, o);
-        before += __shfl_xor(before, o);
-    }
     const int blocks = of_wave(blocks_of(a, b, kb));
-    const Line line = line_from(a, __builtin_amdgcn_readfirstlane(total) * a.gs, turn);
-    const int first = __builtin_amdgcn_readfirstlane(before) * a.gs + (g - a.g0) * blocks;
+    const Line line = line_of(a, kb, a.plan.turn, lane);
+    const int first = start_of(a, line, b, kb, lane) + (g - a.g0) * (blocks + kPad) + kPad;
     const int r0 = first / line.per, r1 = (first + blocks - 1) / line.per;
     if (r0 == r1) return;
     const float4* st = part_stats(a);
@@ -1211,13 +1237,11 @@ void go(const TreeArgs& a, hipStream_t st) {
         const unsigned units = (unsigned)((size_t)a.bs * a.gs * (a.d.H / a.c.G) * a.d.T *
                                           ((D + 255) / 256));
         const int kb = wide || sizeof(T) == 2 ? 32 : 16;
-        const int turn = wide ? kValueKeys / kBlock : a.plan.turn;
         if (units >= 1024)
             hipLaunchKernelGGL((k_tree_merge<T, 1>), dim3((units + 3) / 4), dim3(256), 0, st, a, kb,
-                               turn, units);
-        else
-            hipLaunchKernelGGL((k_tree_merge<T, 4>), dim3(units), dim3(256), 0, st, a, kb, turn,
                                units);
+        else
+            hipLaunchKernelGGL((k_tree_merge<T, 4>), dim3(units), dim3(256), 0, st, a, kb, units);
     }
 }
 
@@ -1250,8 +1274,8 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
                             : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
     const int64_t slots =
         std::max<int64_t>(1, 256 * (shared ? 1 : per_cu) / (p.row_tiles * groups));
-    const int64_t turn = wide ? kValueKeys / kBlock : shared ? 256 / p.rows : p.waves;
-    int64_t ranges = std::min(slots, ceil_div(pairs * blocks, 2 * turn));
+    const int64_t turn = wide ? kValueKeys / kBlock : shared ? (p.rows == 64 ? 4 : 512 / p.rows) : p.waves;
+    int64_t ranges = std::min(slots, ceil_div(pairs * (blocks + kPad), 2 * turn));
     // one workgroup of 8 waves a pair where that leaves a wave few blocks: no second launch
     const bool small = !wide && mt <= 2 && D <= 128 && blocks <= 32 && pairs * p.row_tiles <= 512;
     p.split = !small && ranges > 1 && pairs < 4 * slots && blocks > turn;
