@@ -299,9 +299,10 @@ struct CacheTiles {
 };
 
 // Scores of 32 keys against 16 MT query rows over wave `wave`'s share of the dims (of `waves`),
-// from each lane's row pointers.  All loads of a step go out before its products: left
-// to itself the compiler keeps six in flight, and the memory idles.
-template <typename T, int MT>
+// from each lane's row pointers.  AHEAD: all loads of a step go out before its products (waves of
+// several steps: left to itself the compiler keeps six in flight, and the memory idles, 100 MB
+// in 37 against 27 us); else fewer registers and more waves (of one step: 18 against 13 us).
+template <typename T, int MT, bool AHEAD>
 __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp)[2],
                                             const T* const (&qp)[MT], int D, int wave, int waves,
                                             int q) {
@@ -324,7 +325,7 @@ __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp
 #pragma unroll
             for (int t = 0; t < MT; ++t) f[e][t] = ld_words<16>(qp[t] + at);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < U; ++e)
 #pragma unroll

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
 // head_d > 256: 8 waves share the dims of a block of 32 keys and add up through LDS.
 constexpr int kBlock = 32, kScoreWaves = 8;
 
-template <typename T, int MT>
+template <typename T, int MT, bool AHEAD>
 __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
     constexpr int SUB = kBlock / 16;
     __shared__ v4f red[kScoreWaves][MT * SUB * 64];
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
                 const QueryRow x = query_row(a, b, g, A, min(row0 + 16 * t + col, R - 1));
                 qp[t] = (const T*)a.d.Q + b * a.d.qs[0] + x.head * a.d.qs[1] + x.tok * a.d.qs[2];
             }
-            wide_scores<T, MT>(s, kp, qp, D, wave, kScoreWaves, q);
+            wide_scores<T, MT, AHEAD>(s, kp, qp, D, wave, kScoreWaves, q);
         }
 #pragma unroll
         for (int t = 0; t < MT; ++t)
@@ -212,7 +212,11 @@ void go_narrow(const WeighArgs& a, dim3 grid, hipStream_t st) {
 
 template <typename T, int MT>
 void go_wide(const WeighArgs& a, dim3 grid, hipStream_t st) {
-    hipLaunchKernelGGL((k_weigh_wide<T, MT>), grid, dim3(64 * kScoreWaves), 0, st, a);
+    // (a wave of more than a step of 128 bf16 or 64 fp32 dims)
+    if (a.c.D > kScoreWaves * 256 / (int)sizeof(T))
+        hipLaunchKernelGGL((k_weigh_wide<T, MT, true>), grid, dim3(64 * kScoreWaves), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_weigh_wide<T, MT, false>), grid, dim3(64 * kScoreWaves), 0, st, a);
 }
 
 template <typename T>

@@ -8,35 +8,58 @@ namespace atn {
 
 namespace {
 
-// One row of D elements by one wave, `vec` elements (16 bytes) at a time
-// where both rows allow it.
+// A K row and a V row of D elements copied by `width` lanes, 16 bytes at a time where all of
+// them lie so (vec); four loads go out before the first store.
 template <typename T>
-__device__ __forceinline__ void copy_row(T* __restrict__ dst, const T* __restrict__ src, int D,
-                                         bool vec, int lane) {
+__device__ __forceinline__ void copy_rows(T* __restrict__ k, const T* __restrict__ k0,
+                                          T* __restrict__ v, const T* __restrict__ v0, int D,
+                                          bool vec, int lane, int width) {
     constexpr int N = 16 / sizeof(T);
     if (vec) {
-        for (int d = lane * N; d < D; d += 64 * N)
-            *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(src + d);
+        for (int d = lane * N; d < D; d += 2 * width * N) {
+            const int e = d + width * N;
+            const bool two = e < D;
+            const uint4 a = *reinterpret_cast<const uint4*>(k0 + d);
+            const uint4 b = *reinterpret_cast<const uint4*>(v0 + d);
+            uint4 x{}, y{};
+            if (two) {
+                x = *reinterpret_cast<const uint4*>(k0 + e);
+                y = *reinterpret_cast<const uint4*>(v0 + e);
+            }
+            *reinterpret_cast<uint4*>(k + d) = a;
+            *reinterpret_cast<uint4*>(v + d) = b;
+            if (two) {
+                *reinterpret_cast<uint4*>(k + e) = x;
+                *reinterpret_cast<uint4*>(v + e) = y;
+            }
+        }
     } else {
-        for (int d = lane; d < D; d += 64) dst[d] = src[d];
+        for (int d = lane; d < D; d += width) {
+            const T a = k0[d], b = v0[d];
+            k[d] = a;
+            v[d] = b;
+        }
     }
 }
 
-// One wave per accepted row and kv head.  Nothing to compute: a chain of
-// latencies (lengths, path, row).
+// `width` lanes per accepted row and kv head: a row of D elements in 16-byte pieces, a power of
+// two up to a wave.  Nothing to compute: a chain of latencies (lengths, path, row).
 template <typename T>
-__global__ __launch_bounds__(256) void k_commit(CacheView c, DraftView d, PathView p, int vec) {
-    const int lane = threadIdx.x & 63;
-    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (long)c.B * c.G * p.n) return;
-    const int i = (int)(id % p.n), g = (int)((id / p.n) % c.G), b = (int)(id / p.n / c.G);
-    const int A = rows_accepted(c, d, p, b);
-    if (i >= A) return;
+__global__ __launch_bounds__(256) void k_commit(CacheView c, DraftView d, PathView p, int vec,
+                                                int width) {
+    const int lane = threadIdx.x & (width - 1);
+    const long id = ((long)blockIdx.x * 256 + threadIdx.x) / width;
+    const bool on = id < (long)c.B * c.G * p.n;
+    const int row_id = (int)(on ? id : 0), i = row_id % p.n, g = row_id / p.n % c.G;
+    const int b = row_id / p.n / c.G;
+    // (the rows of a wave may be of several sequences)
+    const int A = rows_accepted_by(c, d, p, b, i, lane, width);
+    if (!on || i >= A) return;
     const int row = rows_in_use(c, b) + i, t = path_at(p, b, i);
-    copy_row((T*)c.K + b * c.ks[0] + g * c.ks[1] + row * c.ks[2],
-             (const T*)d.K + b * d.ks[0] + g * d.ks[1] + t * d.ks[2], c.D, vec, lane);
-    copy_row((T*)c.V + b * c.vs[0] + g * c.vs[1] + row * c.vs[2],
-             (const T*)d.V + b * d.vs[0] + g * d.vs[1] + t * d.vs[2], c.D, vec, lane);
+    copy_rows((T*)c.K + b * c.ks[0] + g * c.ks[1] + row * c.ks[2],
+              (const T*)d.K + b * d.ks[0] + g * d.ks[1] + t * d.ks[2],
+              (T*)c.V + b * c.vs[0] + g * c.vs[1] + row * c.vs[2],
+              (const T*)d.V + b * d.vs[0] + g * d.vs[1] + t * d.vs[2], c.D, vec, lane, width);
     const size_t m = ((size_t)b * c.G + g) * c.cap + row;
     if (lane == 0 && c.weight) c.weight[m] = 0.f;
     if (lane == 0 && c.pos) c.pos[m] = c.seen[b] + i;
@@ -68,16 +91,37 @@ __device__ __forceinline__ uint32_t rank_key(float w, int pos, int since) {
 // histograms of its digits (11, 11 and 10 bits), then the rows below it that
 // leave slots under `budget` free and the kept rows from `budget` on, in
 // order, as the lists of moves.
-// scratch: [B G] counts, then [B G][slots][2] (to, from).
+// scratch: [B G] counts, then (at an even place) [B G][slots][2] (to, from).
+__host__ __device__ inline int list_at(int pairs) { return (pairs + 1) & ~1; }
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
+// The sum over the waves below this one, and over all, of a value per wave (two barriers).
+__device__ __forceinline__ int below_waves(int* slot, int x, int wave, int lane, int* all) {
+    if (lane == 0) slot[wave] = x;
+    __syncthreads();
+    int sum = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) {
+        const int y = slot[i];
+        total += y;
+        sum += i < wave ? y : 0;
+    }
+    __syncthreads();
+    *all = total;
+    return sum;
+}
+
+// KPT keys a thread stay in registers: a wave's are 64 KPT consecutive rows.  Heads of more than
+// 1024 KPT rows go through them in chunks, read again for each digit (KPT = 16, 16384 rows a
+// chunk): 12000 to 16384 rows 44 -> 12 us against a loop of one load after another.
+template <int KPT>
 __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int budget, int recent,
                                                               int slots, int* scratch) {
+    constexpr int CHUNK = kSelThreads * KPT;
     __shared__ uint32_t hist[2048];
-    __shared__ uint32_t wsum[kSelWaves];
+    __shared__ int slot[kSelWaves];
     __shared__ uint32_t pick[2];
-    __shared__ int cnt[3][kSelWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = of_wave(tid >> 6);
     const int bg = blockIdx.x, b = bg / c.G;
     const int L = rows_in_use(c, b);
     if (L <= budget) {
@@ -89,29 +133,43 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int b
     // (a position is at least seen - recent; in 64 bits, so that no difference wraps)
     const long lo = (long)c.seen[b] - recent;
     const int since = lo < INT32_MIN ? INT32_MIN : (int)lo;
+    const int chunks = (L + CHUNK - 1) / CHUNK, mine = wave * 64 * KPT + lane;
+    uint32_t key[KPT];
+    auto load = [&](int chunk) {
+        float x[KPT];
+        int y[KPT];
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+            const int r = min(chunk * CHUNK + mine + 64 * k, L - 1);
+            x[k] = w[r];
+            y[k] = pos[r];
+        }
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) key[k] = rank_key(x[k], y[k], since);
+    };
+    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
     uint32_t prefix = 0, mask = 0, need = (uint32_t)budget;
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t bins = pass == 2 ? 1024 : 2048;
-        for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-        __syncthreads();
-        for (int r = tid; r < L; r += kSelThreads) {
-            const uint32_t k = rank_key(w[r], pos[r], since);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
-        }
-        __syncthreads();
-        // thread t holds bins 2047 - 2t and 2046 - 2t: sums from the top down
-        const uint32_t h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
-        uint32_t s = h0 + h1;
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            if (pass == 0 || chunks > 1) load(chunk);
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(s, o);
-            if (lane >= o) s += v;
+            for (int k = 0; k < KPT; ++k)
+                if (chunk * CHUNK + mine + 64 * k < L && (key[k] & mask) == prefix)
+                    atomicAdd(&hist[(key[k] >> shift) & (bins - 1)], 1u);
         }
-        if (lane == 63) wsum[wave] = s;
         __syncthreads();
-        uint32_t above = s - h0 - h1;
-        for (int i = 0; i < wave; ++i) above += wsum[i];
+        // thread t holds bins 2047 - 2t and 2046 - 2t (and clears them): sums from the top down
+        const uint32_t h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
+        hist[2047 - 2 * tid] = hist[2046 - 2 * tid] = 0;
+        const int s = wave_scan((int)(h0 + h1));
+        int total;
+        const uint32_t above = (uint32_t)(below_waves(slot, __builtin_amdgcn_readlane(s, 63), wave,
+                                                      lane, &total) +
+                                          s) -
+                               h0 - h1;
         if (above < need && need <= above + h0 + h1) {
             const bool first = need <= above + h0;
             pick[0] = 2047 - 2 * tid - (first ? 0 : 1);
@@ -121,77 +179,86 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int b
         prefix |= pick[0] << shift;
         mask |= (bins - 1) << shift;
         need = pick[1];  // rows of this prefix that stay
-        __syncthreads();
     }
-    // rows with the key `prefix` stay up to the need-th; each wave takes a
-    // consecutive part of the rows
-    const int per = ((L + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
-    const int r0 = wave * per, r1 = min(L, r0 + per);
-    int eq = 0;
-    for (int r = r0 + lane; r < r0 + per; r += 64)
-        eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(
-            r < r1 && rank_key(w[r], pos[r], since) == prefix));
-    if (lane == 0) cnt[0][wave] = eq;
-    __syncthreads();
-    int eq0 = 0;
-    for (int i = 0; i < wave; ++i) eq0 += cnt[0][i];
+    // rows with the key `prefix` stay up to the need-th, in their order
     const uint64_t below = (1ull << lane) - 1;
-    int to = 0, from = 0;
-    for (int round = 0; round < 2; ++round) {
-        int e = eq0;
-        for (int r = r0 + lane; r < r0 + per; r += 64) {
-            const bool on = r < r1;
-            const uint32_t k = on ? rank_key(w[r], pos[r], since) : 0u;
-            const uint64_t same = __builtin_amdgcn_ballot_w64(on && k == prefix);
-            const bool keep =
-                on && (k > prefix ||
-                       (k == prefix &&
-                        e + __builtin_popcountll(same & below) < (int)need));
+    int* list = scratch + list_at(c.B * c.G) + (size_t)bg * slots * 2;
+    int eq0 = 0, to0 = 0, from0 = 0;  // of the chunks before
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        if (chunks > 1) load(chunk);
+        const int r0 = chunk * CHUNK + mine;
+        int eq = 0;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k)
+            eq += __builtin_popcountll(
+                __builtin_amdgcn_ballot_w64(r0 + 64 * k < L && key[k] == prefix));
+        int all;
+        int e = eq0 + below_waves(slot, eq, wave, lane, &all);
+        eq0 += all;
+        uint32_t keep = 0;  // bit k: row k of this thread stays
+        int to = 0, from = 0;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+            const int r = r0 + 64 * k;
+            const bool on = r < L, tie = on && key[k] == prefix;
+            const uint64_t same = __builtin_amdgcn_ballot_w64(tie);
+            const bool stay = (on && key[k] > prefix) ||
+                              (tie && e + __builtin_popcountll(same & below) < (int)need);
             e += __builtin_popcountll(same);
-            const uint64_t free_ = __builtin_amdgcn_ballot_w64(on && !keep && r < budget);
-            const uint64_t move = __builtin_amdgcn_ballot_w64(keep && r >= budget);
-            if (round) {
-                int* list = scratch + c.B * c.G + (size_t)bg * slots * 2;
-                if (on && !keep && r < budget)
-                    list[2 * (to + __builtin_popcountll(free_ & below))] = r;
-                if (keep && r >= budget)
-                    list[2 * (from + __builtin_popcountll(move & below)) + 1] = r;
-            }
-            to += __builtin_popcountll(free_);
-            from += __builtin_popcountll(move);
+            keep |= (uint32_t)stay << k;
+            to += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && !stay && r < budget));
+            from += __builtin_popcountll(__builtin_amdgcn_ballot_w64(stay && r >= budget));
         }
-        if (round == 0) {
-            if (lane == 0) cnt[1][wave] = to, cnt[2][wave] = from;
-            __syncthreads();
-            if (tid == 0) {
-                int n = 0;
-                for (int i = 0; i < kSelWaves; ++i) n += cnt[1][i];
-                scratch[bg] = n;
-            }
-            to = from = 0;
-            for (int i = 0; i < wave; ++i) to += cnt[1][i], from += cnt[2][i];
+        int to_all, from_all;
+        to = to0 + below_waves(slot, to, wave, lane, &to_all);
+        from = from0 + below_waves(slot, from, wave, lane, &from_all);
+        to0 += to_all;
+        from0 += from_all;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+            const int r = r0 + 64 * k;
+            const bool stay = (keep >> k) & 1u, free_ = r < L && !stay && r < budget;
+            const bool move = stay && r >= budget;
+            const uint64_t f = __builtin_amdgcn_ballot_w64(free_);
+            const uint64_t v = __builtin_amdgcn_ballot_w64(move);
+            if (free_) list[2 * (to + __builtin_popcountll(f & below))] = r;
+            if (move) list[2 * (from + __builtin_popcountll(v & below)) + 1] = r;
+            to += __builtin_popcountll(f);
+            from += __builtin_popcountll(v);
         }
+    }
+    if (tid == 0) scratch[bg] = to0;
+}
+
+// `width` lanes per move, the moves of a head dealt to gridDim.x workgroups.  Sources lie at or
+// past `budget`, targets below it: no order among them.
+template <typename T>
+__global__ __launch_bounds__(256) void k_evict_move(CacheView c, int slots, const int* scratch,
+                                                    int vec, int width) {
+    const int lane = threadIdx.x & (width - 1), bg = blockIdx.y, g = bg % c.G, b = bg / c.G;
+    const int per = 256 / width;
+    const int n = min(scratch[bg], slots);
+    const int2* list =
+        reinterpret_cast<const int2*>(scratch + list_at(c.B * c.G)) + (size_t)bg * slots;
+    T* K = (T*)c.K + b * c.ks[0] + g * c.ks[1];
+    T* V = (T*)c.V + b * c.vs[0] + g * c.vs[1];
+    for (int i = blockIdx.x * per + threadIdx.x / width; i < n; i += gridDim.x * per) {
+        const int to = list[i].x, from = list[i].y;
+        const size_t m = (size_t)bg * c.cap;
+        float w = 0.f;
+        int p = 0;
+        if (lane == 0) w = c.weight[m + from], p = c.pos[m + from];
+        copy_rows(K + to * c.ks[2], K + from * c.ks[2], V + to * c.vs[2], V + from * c.vs[2], c.D, vec,
+                  lane, width);
+        if (lane == 0) c.weight[m + to] = w, c.pos[m + to] = p;
     }
 }
 
-// One wave per move, the moves of a head dealt to gridDim.x workgroups.
-// Sources lie at or past `budget`, targets below it: no order among them.
-template <typename T>
-__global__ __launch_bounds__(256) void k_evict_move(CacheView c, int slots, const int* scratch,
-                                                    int vec) {
-    const int lane = threadIdx.x & 63, bg = blockIdx.y, g = bg % c.G, b = bg / c.G;
-    const int n = min(scratch[bg], slots);
-    const int* list = scratch + c.B * c.G + (size_t)bg * slots * 2;
-    T* K = (T*)c.K + b * c.ks[0] + g * c.ks[1];
-    T* V = (T*)c.V + b * c.vs[0] + g * c.vs[1];
-    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
-        const int to = list[2 * i], from = list[2 * i + 1];
-        copy_row(K + to * c.ks[2], K + from * c.ks[2], c.D, vec, lane);
-        copy_row(V + to * c.vs[2], V + from * c.vs[2], c.D, vec, lane);
-        const size_t m = (size_t)bg * c.cap;
-        if (lane == 0) c.weight[m + to] = c.weight[m + from];
-        if (lane == 0) c.pos[m + to] = c.pos[m + from];
-    }
+// lanes of a row: its 16-byte pieces, a power of two up to a wave
+int lanes_of(int D, size_t es) {
+    int w = 1;
+    while (w < 64 && w * 16 < (int)(D * es)) w *= 2;
+    return w;
 }
 
 bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -209,11 +276,12 @@ hipError_t launch_cache_commit(int dtype, const CacheView& c, const DraftView& d
     const size_t es = dtype == kDtypeF32 ? 4 : 2;
     const int vec = rows16(c.K, c.ks, c.D, es) && rows16(c.V, c.vs, c.D, es) &&
                     rows16(d.K, d.ks, c.D, es) && rows16(d.V, d.vs, c.D, es);
-    const dim3 grid((unsigned)(((long)c.B * c.G * p.n + 3) / 4));
+    const int width = lanes_of(c.D, es);
+    const dim3 grid((unsigned)(((long)c.B * c.G * p.n * width + 255) / 256));
     if (dtype == kDtypeF32)
-        hipLaunchKernelGGL(k_commit<float>, grid, dim3(256), 0, st, c, d, p, vec);
+        hipLaunchKernelGGL(k_commit<float>, grid, dim3(256), 0, st, c, d, p, vec, width);
     else
-        hipLaunchKernelGGL(k_commit<uint16_t>, grid, dim3(256), 0, st, c, d, p, vec);
+        hipLaunchKernelGGL(k_commit<uint16_t>, grid, dim3(256), 0, st, c, d, p, vec, width);
     return hipGetLastError();
 }
 
@@ -226,7 +294,7 @@ hipError_t launch_cache_advance(const CacheView& c, int* len, const DraftView* d
 
 size_t evict_scratch(int B, int G, int cap, int budget) {
     const size_t slots = (size_t)std::max(0, std::min(budget, cap - budget));
-    return ((size_t)B * G * (1 + 2 * slots)) * sizeof(int);
+    return (list_at(B * G) + (size_t)B * G * 2 * slots) * sizeof(int);
 }
 
 hipError_t launch_cache_evict(int dtype, const CacheView& c, int budget, int recent, int* scratch,
@@ -236,16 +304,25 @@ hipError_t launch_cache_evict(int dtype, const CacheView& c, int budget, int rec
     const size_t es = dtype == kDtypeF32 ? 4 : 2;
     const int vec = rows16(c.K, c.ks, c.D, es) && rows16(c.V, c.vs, c.D, es);
     const int BG = c.B * c.G;
-    hipLaunchKernelGGL(k_evict_select, dim3(BG), dim3(kSelThreads), 0, st, c, budget, recent,
-                       slots, scratch);
+    if (c.cap <= kSelThreads)
+        hipLaunchKernelGGL(k_evict_select<1>, dim3(BG), dim3(kSelThreads), 0, st, c, budget, recent,
+                           slots, scratch);
+    else if (c.cap <= 4 * kSelThreads)
+        hipLaunchKernelGGL(k_evict_select<4>, dim3(BG), dim3(kSelThreads), 0, st, c, budget, recent,
+                           slots, scratch);
+    else
+        hipLaunchKernelGGL(k_evict_select<16>, dim3(BG), dim3(kSelThreads), 0, st, c, budget, recent,
+                           slots, scratch);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)std::max(1, std::min((slots + 3) / 4, 8192 / std::min(BG, 8192))),
+    const int width = lanes_of(c.D, es), per = 256 / width;
+    const dim3 grid((unsigned)std::max(1, std::min((slots + per - 1) / per, 4096 / std::min(BG, 4096))),
                     (unsigned)BG);
     if (dtype == kDtypeF32)
-        hipLaunchKernelGGL(k_evict_move<float>, grid, dim3(256), 0, st, c, slots, scratch, vec);
+        hipLaunchKernelGGL(k_evict_move<float>, grid, dim3(256), 0, st, c, slots, scratch, vec, width);
     else
-        hipLaunchKernelGGL(k_evict_move<uint16_t>, grid, dim3(256), 0, st, c, slots, scratch, vec);
+        hipLaunchKernelGGL(k_evict_move<uint16_t>, grid, dim3(256), 0, st, c, slots, scratch, vec,
+                           width);
     return hipGetLastError();
 }
 

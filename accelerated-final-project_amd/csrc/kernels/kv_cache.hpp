@@ -51,6 +51,19 @@ struct PathView {
     int n;
 };
 
+// Sums of the lanes up to each.
+__device__ __forceinline__ int wave_scan(int x) {
+#define ATN_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, false)
+    ATN_SCAN_STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8 within 16 lanes
+    ATN_SCAN_STEP(0x112, 0xF);
+    ATN_SCAN_STEP(0x114, 0xF);
+    ATN_SCAN_STEP(0x118, 0xF);
+    ATN_SCAN_STEP(0x142, 0xA);  // row_bcast:15 into rows 1 and 3
+    ATN_SCAN_STEP(0x143, 0xC);  // row_bcast:31 into rows 2 and 3
+#undef ATN_SCAN_STEP
+    return x;
+}
+
 // Rows in use of a sequence, and its drafts; of_wave: of one that the whole wave shares (the
 // compiler keeps what follows from it in scalar registers only if told).
 __device__ __forceinline__ int of_wave(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -81,6 +94,25 @@ __device__ __forceinline__ int rows_accepted(const CacheView& c, const DraftView
         }
     }
     return min(a, c.cap - min(max(c.len[b], 0), c.cap));
+}
+// ... where `width` lanes (a power of two, `lane` of them) each have a sequence of their own: more
+// than i exactly where draft i becomes a row.
+__device__ __forceinline__ int rows_accepted_by(const CacheView& c, const DraftView& d,
+                                                const PathView& p, int b, int i, int lane,
+                                                int width) {
+    const int n = drafts_of(d, b);
+    int a = p.accepted ? min(max(p.accepted[b], 0), p.n) : p.n;
+    a = min(a, c.cap - min(max(c.len[b], 0), c.cap));
+    if (!p.path) return min(a, n);
+    if (i >= a) return a;
+    const int shift = (int)(threadIdx.x & 63) - lane;
+    const uint64_t group = width == 64 ? ~0ull : (1ull << width) - 1;
+    for (int j0 = 0; j0 <= i; j0 += width) {
+        const int j = j0 + lane, t = j <= i ? p.path[(size_t)b * p.n + j] : 0;
+        const uint64_t bad = __builtin_amdgcn_ballot_w64(t < 0 || t >= n) >> shift & group;
+        if (bad && j0 + __builtin_ctzll(bad) <= i) return j0 + __builtin_ctzll(bad);
+    }
+    return a;
 }
 __device__ __forceinline__ int path_at(const PathView& p, int b, int i) {
     return p.path ? p.path[(size_t)b * p.n + i] : i;

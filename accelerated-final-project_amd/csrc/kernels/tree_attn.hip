@@ -31,19 +31,6 @@ __device__ __forceinline__ int blocks_of(const TreeArgs& a, int b, int kb) {
     return max(1, (L + kb - 1) / kb + (a.d.K ? (n + kb - 1) / kb : 0));
 }
 
-// Sums of the lanes up to each.
-__device__ __forceinline__ int wave_scan(int x) {
-#define ATN_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, false)
-    ATN_SCAN_STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8 within 16 lanes
-    ATN_SCAN_STEP(0x112, 0xF);
-    ATN_SCAN_STEP(0x114, 0xF);
-    ATN_SCAN_STEP(0x118, 0xF);
-    ATN_SCAN_STEP(0x142, 0xA);  // row_bcast:15 into rows 1 and 3
-    ATN_SCAN_STEP(0x143, 0xC);  // row_bcast:31 into rows 2 and 3
-#undef ATN_SCAN_STEP
-    return x;
-}
-
 // A pair takes as many places of the line as it has blocks, and kPad before them: beginning and
 // ending a pair costs a workgroup about as much time as so many blocks (10 us against 0.4 to
 // 0.7 us a block), so ranges of many short pairs have fewer blocks.
@@ -849,7 +836,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
                 (row - h * a.d.T) * a.d.qs[2];
     }
     v4f s[MT][SUB];
-    wide_scores<T, MT>(s, kp, qp, D, share * kScoreWaves + wave, a.plan.shares * kScoreWaves, q);
+    wide_scores<T, MT, true>(s, kp, qp, D, share * kScoreWaves + wave, a.plan.shares * kScoreWaves, q);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll

@@ -233,7 +233,8 @@ def check_evict(am, c, budget, recent, workspace=None):
     (1, 1, 1, [1]), (2, 1, 0, [2, 1]), (5, 4, 4, [5, 5]), (64, 32, 0, [64, 63]),
     (65, 64, 10, [65, 64]), (100, 7, 3, [100, 0]), (300, 299, 1, [300, 299]),
     (1000, 500, 100, [999, 750]), (1500, 1, 1, [1025, 1024]), (4097, 2000, 2000, [4097, 3000]),
-    (9000, 8000, 64, [9000, 8001])])
+    (9000, 8000, 64, [9000, 8001]),
+    (16385, 9000, 300, [16385, 16384]), (40000, 11111, 4000, [40000, 20000])])
 def test_evict(am, dev, dtype, cap, budget, recent, lens):
     print(f"[case] evict {dtype} {cap} {budget} {recent} {lens}", flush=True)
     c = Cache(am, dtype, len(lens), 2, cap, 24, lens, seen=[cap] * len(lens), seed=cap)
