@@ -267,6 +267,18 @@ struct CacheTiles {
         }
     }
 
+    // bf16: weights as the products' operands
+    static __device__ __forceinline__ void round(KPiece (&f)[MT], const float (&p)[MT][SUB][4],
+                                                 float (&used)[MT]) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                f[t].w[h] = pack2(p[t][h >> 1][2 * (h & 1)], p[t][h >> 1][2 * (h & 1) + 1]);
+                used[t] = add2(f[t].w[h], used[t]);
+            }
+    }
+
     // O^T += V^T P^T for all tiles.  bf16: the weights enter as bf16 (V's own precision, and what
     // lets one MFMA take both), half a step (2^-8 of their size) off at most; `used` gathers
     // them as rounded, so that the output is their exact mean of V
@@ -275,13 +287,7 @@ struct CacheTiles {
                                                       float (&used)[MT]) {
         if constexpr (kBf) {
             KPiece f[MT];
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    f[t].w[h] = pack2(p[t][h >> 1][2 * (h & 1)], p[t][h >> 1][2 * (h & 1) + 1]);
-                    used[t] = add2(f[t].w[h], used[t]);
-                }
+            round(f, p, used);
             products(o, v, f);
         } else {
 #pragma unroll

@@ -566,22 +566,28 @@ k_tree_narrow(TreeArgs a) {
 }
 
 // ---------------------------------------------------------------- many query rows
-// bf16, 65 to 128 dims, more than 32 query rows of a kv head.  K and V now serve several waves'
+// bf16, 65 to 128 dims, more than 64 query rows of a kv head.  K and V now serve several waves'
 // rows, and products and softmax weigh as much as the reads: 8 waves a workgroup, each with 32
 // rows in registers (two waves a SIMD, one's softmax beside the other's products), RG of them
 // over different rows and KG = 8 / RG over different blocks.  A stage of NB blocks comes
-// through LDS in the order of its fragments -- each wave loads 2 NB of the pieces that
-// k_tree_narrow's lanes load for themselves -- while the stage before is worked on.
+// through LDS while the stage before is worked on: K in the order of its fragments, as
+// k_tree_narrow's lanes load them for themselves; V in rows, from which gfx950's transposing read
+// takes the operands of V^T (pairing them by permutes, as k_tree_narrow does, took 40 % of the
+// time here, once for every wave).
 template <int RG, int MODE>
 struct Shared : CacheTiles<uint16_t, 128, 2, MODE> {
     using N = CacheTiles<uint16_t, 128, 2, MODE>;
     static constexpr int KG = 8 / RG, ROWS_WG = 32 * RG;
-    static constexpr int SB = RG == 2 ? 1 : 2;  // blocks of a wave in a stage
+    static constexpr int SB = 2;                // blocks of a wave in a stage
     static constexpr int NB = KG * SB;          // ... of the stage
-    static constexpr int PIECES = N::SUB * N::KS + N::KEYS;  // of a block, 1 KiB each
-    static_assert(PIECES == 16 && N::VS == 1, "a K and a V piece of each block a wave");
+    static_assert(N::SUB * N::KS == 8 && N::KEYS == 8 && N::VS == 1,
+                  "a K piece and 4 V rows of each block a wave");
+    // a row of V: 32 bytes more than its 256, so that the 8 rows of half a wave's transposing
+    // read lie in different banks
+    static constexpr int LDV = 128 + 16;
+    static constexpr int kKBytes = 8 * 1024, kBytes = kKBytes + 32 * LDV * 2;  // of a block
     static constexpr int LDO = 128 + 4;
-    static constexpr int kStage = NB * PIECES * 1024;
+    static constexpr int kStage = NB * kBytes;
     static constexpr int kXBytes = KG * ROWS_WG * LDO * 4;
     static constexpr int kOut = 2 * kStage > kXBytes ? 2 * kStage : kXBytes;
     static constexpr int kLds = kOut + (KG + 1) * ROWS_WG * 16;
@@ -594,6 +600,9 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
     using T = uint16_t;
     constexpr int MT = 2, KB = N::KB, SUB = N::SUB, KS = N::KS, VL = N::VL, KG = N::KG, NB = N::NB;
     constexpr int DP = 128;
+    struct VT {
+        typename N::KPiece p[1][VL];
+    };
     __shared__ __align__(16) char lds[N::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15, rg = wave % RG, kg = wave / RG;
@@ -629,9 +638,23 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
         const T* vd = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1];
 
         // this wave's pieces of the stage at block i: of every block K piece (wave / KS, wave % KS)
-        // and V's row `wave` of each lane (past the last block, of it)
+        // and V's rows 4 wave .. 4 wave + 3 (past the last block, of it)
         typename N::KPiece z[2 * NB];
+        const uint32_t mine_k = (16 * (wave / KS) + col) * (uint32_t)a.c.ks[2] * 2 + 16 * q;
+        const uint32_t mine_v = (4 * wave + q) * (uint32_t)a.c.vs[2] * 2;
         auto load = [&](int i) {
+            if (i + NB <= min(whole, last)) {
+                const T* kb = kc + (int64_t)i * KB * a.c.ks[2];
+                const T* vb = vc + (int64_t)i * KB * a.c.vs[2];
+#pragma unroll
+                for (int x = 0; x < NB; ++x) {
+                    z[2 * x] = N::piece(kb, mine_k, wave % KS, q, D);
+                    z[2 * x + 1] = N::v_piece(vb, mine_v, 0, D, lane);
+                    kb += KB * a.c.ks[2];
+                    vb += KB * a.c.vs[2];
+                }
+                return;
+            }
 #pragma unroll
             for (int x = 0; x < NB; ++x) {
                 const int y = min(i + x, last - 1);
@@ -643,14 +666,18 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
                                     min(16 * (wave / KS) + col, rows - 1) * kr + 16 * q, wave % KS, q,
                                     D);
                 z[2 * x + 1] = N::v_piece((in ? vc : vd) + j0 * vs,
-                                          min(N::key_of(lane, wave), rows - 1) * vr, 0, D, lane);
+                                          min(4 * wave + q, rows - 1) * vr, 0, D, lane);
             }
         };
-        auto* stage = reinterpret_cast<typename N::KPiece*>(lds);
         auto put = [&](int buf) {
 #pragma unroll
-            for (int x = 0; x < 2 * NB; ++x)
-                stage[((buf * NB + x / 2) * N::PIECES + (x & 1) * 8 + wave) * 64 + lane] = z[x];
+            for (int x = 0; x < NB; ++x) {
+                char* block = lds + (buf * NB + x) * N::kBytes;
+                reinterpret_cast<typename N::KPiece*>(block)[wave * 64 + lane] = z[2 * x];
+                *reinterpret_cast<typename N::KPiece*>(block + N::kKBytes +
+                                                       (4 * wave + q) * N::LDV * 2 + 16 * col) =
+                    z[2 * x + 1];
+            }
         };
         if (sp.first < last) load(sp.first);
         // Q: this wave's rows in registers (those of no token hold the last token's: nobody reads
@@ -688,10 +715,12 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
             const bool more = i0 + NB < last;
             if (more) load(i0 + NB);
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
             for (int y = kg; y < NB; y += KG) {
                 const int i = i0 + y;
                 if (i >= last) break;
-                const auto* mine = stage + (buf * NB + y) * N::PIECES * 64 + lane;
+                const char* block = lds + (buf * NB + y) * N::kBytes;
+                const auto* mine = reinterpret_cast<const typename N::KPiece*>(block) + lane;
                 v4f s[MT][SUB];
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
@@ -705,9 +734,6 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
 #pragma unroll
                         for (int t = 0; t < MT; ++t) s[t][u] = N::dot(k, qf[t][e], s[t][u]);
                     }
-                typename N::Vals v;
-#pragma unroll
-                for (int j = 0; j < N::KEYS; ++j) v.p[j][0] = mine[(8 + j) * 64];
                 float p[MT][SUB][4];
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
@@ -718,14 +744,33 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
                 if (i >= whole) {
                     const bool in = i < cache;
                     const int j0 = (in ? i : i - cache) * KB, rows = (in ? L : n) - j0;
-                    odd |= clear_not_finite<T>(v);
 #pragma unroll
                     for (int t = 0; t < MT; ++t)
                         hide<MT, SUB>(a, p, t, b, tile * N::ROWS_WG + rg * 32 + 16 * t + col, in, j0,
                                       rows, q);
                 }
                 weights<MT, SUB, 1, VL>(p, o, m, l, used, scale);
-                N::accumulate(o, v, p, used);
+                __builtin_amdgcn_sched_barrier(0);  // (V's registers are the scores' until here)
+                // V^T: lane (m, q) takes dim 16 c + m of keys 4 q .. 4 q + 3 and 16 on
+                VT v;
+                {
+                    const uint16_t* rows = reinterpret_cast<const uint16_t*>(block + N::kKBytes) +
+                                           (4 * q + (col >> 2)) * N::LDV + 4 * (col & 3);
+#pragma unroll
+                    for (int c = 0; c < VL; ++c) {
+                        const uint2 lo = lds_tr16(rows + 16 * c);
+                        const uint2 hi = lds_tr16(rows + 16 * N::LDV + 16 * c);
+                        v.p[0][c].w[0] = lo.x, v.p[0][c].w[1] = lo.y;
+                        v.p[0][c].w[2] = hi.x, v.p[0][c].w[3] = hi.y;
+                    }
+                }
+                if (i >= whole) odd |= clear_not_finite<T>(v);
+                typename N::KPiece f[MT];  // (rounded: see CacheTiles::accumulate)
+                N::round(f, p, used);
+#pragma unroll
+                for (int c = 0; c < VL; ++c)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) o[t][0][c] = N::dot(v.p[0][c], f[t], o[t][0][c]);
             }
             if (more) put(buf ^ 1);
             __syncthreads();
@@ -767,14 +812,10 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
                 }
                 if (q == 0) fin[r] = y;
             }
-            float* to = xo + (kg * N::ROWS_WG + r) * N::LDO + N::RUN * q;
+            float* to = xo + (kg * N::ROWS_WG + r) * N::LDO + 4 * q;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int c = 0; c < VL; c += 4)
-                    *reinterpret_cast<float4*>(to + VL * e + c) =
-                        make_float4(o[t][0][c][e] * f, o[t][0][c + 1][e] * f, o[t][0][c + 2][e] * f,
-                                    o[t][0][c + 3][e] * f);
+            for (int c = 0; c < VL; ++c)
+                *reinterpret_cast<v4f*>(to + 16 * c) = o[t][0][c] * f;
         }
         __syncthreads();
         write_rows<T, DP, N::ROWS_WG, KG, N::LDO, VL, MODE, 512>(a, sp, tile, n, xo, fin);
@@ -1170,9 +1211,7 @@ void go_rows(const TreeArgs& a, hipStream_t st) {
     if constexpr (DP == 64 && sizeof(T) == 2) go_narrow<T, DP, 4, MODE>(a, st);
     if constexpr (DP == 128 && sizeof(T) == 2) {
         const dim3 grid((unsigned)(a.plan.ranges * a.plan.row_tiles));
-        if (a.plan.rows == 64)
-            hipLaunchKernelGGL((k_tree_shared<2, MODE>), grid, dim3(512), 0, st, a);
-        else if (a.plan.rows == 128)
+        if (a.plan.rows == 128)
             hipLaunchKernelGGL((k_tree_shared<4, MODE>), grid, dim3(512), 0, st, a);
         else
             hipLaunchKernelGGL((k_tree_shared<8, MODE>), grid, dim3(512), 0, st, a);
@@ -1241,12 +1280,10 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     TreePlan p{};
     const bool bf = dtype == kDtypeBF16, wide = D > kTreeNarrow;
     const int R = H / G * T;
-    const bool shared = bf && D > 64 && D <= 128 && R > 32;
+    const bool shared = bf && D > 64 && D <= 128 && R > 64;
     p.rows = R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64;
     if (shared) {  // the rows of a workgroup that leave the fewest places empty
-        p.rows = 256;
-        for (int r : {128, 64})
-            if (ceil_div(R, r) * r < ceil_div(R, p.rows) * p.rows) p.rows = r;
+        p.rows = ceil_div(R, 128) * 128 < ceil_div(R, 256) * 256 ? 128 : 256;
     }
     p.row_tiles = (int)ceil_div(R, p.rows);
     p.waves = 4;
@@ -1261,7 +1298,7 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
                             : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
     const int64_t slots =
         std::max<int64_t>(1, 256 * (shared ? 1 : per_cu) / (p.row_tiles * groups));
-    const int64_t turn = wide ? kValueKeys / kBlock : shared ? (p.rows == 64 ? 4 : 512 / p.rows) : p.waves;
+    const int64_t turn = wide ? kValueKeys / kBlock : shared ? 512 / p.rows : p.waves;
     int64_t ranges = std::min(slots, ceil_div(pairs * (blocks + kPad), 2 * turn));
     // one workgroup of 8 waves a pair where that leaves a wave few blocks: no second launch
     const bool small = !wide && mt <= 2 && D <= 128 && blocks <= 32 && pairs * p.row_tiles <= 512;
