@@ -77,8 +77,8 @@ int check_cache(const atn_kv_cache* c, atn::CacheView* v, Ranges* r) {
     if (c->batch < 1 || c->kv_heads < 1 || c->capacity < 1 || c->head_d < 1)
         return ATN_ERR_BAD_DIMENSION;
     if (c->head_d > ATN_CACHE_MAX_HEAD_D) return ATN_ERR_BAD_ARGUMENT;
-    // (grids have a (sequence, kv head) per y)
-    if ((int64_t)c->batch * c->kv_heads > 65535) return ATN_ERR_SIZE_OVERFLOW;
+    // (grids have a (sequence, kv head) per y; row numbers and steps past them are ints)
+    if ((int64_t)c->batch * c->kv_heads > 65535 || c->capacity > 1 << 30) return ATN_ERR_SIZE_OVERFLOW;
     const size_t es = c->dtype == ATN_DTYPE_F32 ? 4 : 2;
     int st = check_tensor(c->K, c->k_stride, c->batch, c->kv_heads, c->capacity, c->head_d, es,
                           true, v->ks, &r->k);
@@ -241,7 +241,7 @@ int atn_tree_attention_ex(const atn_kv_cache* cache, const atn_drafts* drafts, v
         room = workspace_bytes - kSyncRegion;
     }
     a.plan = plan_tree(a.c, a.d, cache->dtype, room);
-    if (a.plan.workgroups > INT32_MAX) return ATN_ERR_SIZE_OVERFLOW;
+    if (a.plan.workgroups > INT32_MAX || a.plan.line > INT32_MAX) return ATN_ERR_SIZE_OVERFLOW;
     if (workspace != nullptr && a.plan.scratch > room) return ATN_ERR_WORKSPACE;
     int dev;
     st = atn_host::device(&dev);
@@ -269,6 +269,10 @@ int atn_cache_commit_ex(const atn_kv_cache* cache, const atn_drafts* drafts, con
     if (c.pos && !c.seen) return ATN_ERR_NULL_POINTER;
     if (c.K == c.V || any_meet({r.k}, {r.kd, r.vd}) || any_meet({r.v}, {r.kd, r.vd}))
         return ATN_ERR_ALIASING;
+    const int64_t mb = (int64_t)c.B * c.G * c.cap * 4;
+    if (any_meet({range(c.weight, c.weight ? mb : 0), range(c.pos, c.pos ? mb : 0)},
+                 {r.k, r.v, r.kd, r.vd}))
+        return ATN_ERR_ALIASING;
     int dev;
     st = atn_host::device(&dev);
     if (st != ATN_OK) return st;
@@ -289,6 +293,8 @@ int atn_cache_weigh_ex(const atn_kv_cache* cache, const atn_drafts* drafts, cons
     st = check_path(path, accepted, path_len, &p);
     if (st != ATN_OK) return st;
     if (!lse || !c.weight) return ATN_ERR_NULL_POINTER;
+    // (a query row per head and path entry)
+    if ((int64_t)(d.H / c.G) * path_len >= (1 << 24)) return ATN_ERR_SIZE_OVERFLOW;
     if (!aligned(lse, 4) || !aligned(weight_in, 4)) return ATN_ERR_MISALIGNED;
     const int64_t wb = (int64_t)c.B * c.G * c.cap * 4;
     const Range rw = range(c.weight, wb);

@@ -132,6 +132,7 @@ struct TreePlan {
     int shares;      // ... workgroups that share the dims of a tile of scores
     size_t scores;   // floats of the scores of a pass
     size_t scratch;  // bytes
+    int64_t line;        // places of the line of blocks, at most
     int64_t workgroups;  // of a pass, at most
 };
 

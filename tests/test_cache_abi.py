@@ -242,3 +242,35 @@ def test_host_arrays_of_int32(am):
     a = hip_rt.DeviceArray.wrap(KA, (2, 3), "i32", (3, 1))
     assert a.strides is None and a.nbytes == 24
     assert hip_rt.DeviceArray.wrap(KA, (2, 3), "i32", (4, 1)).strides == (4, 1)
+
+
+def test_sizes_past_the_kernels_numbers(am):
+    """Rows more than 128 MiB apart, more than 2^30 rows, more blocks than an int counts, and
+    scales that fp32 does not hold as normal numbers."""
+    f = calls(am)
+    ld = (1 << 26) + 1  # bf16 elements: 128 MiB and one more
+    far = dict(batch=1, kv_heads=1, capacity=4)
+    for op in ALL:
+        assert f[op](cache(am, k_stride=(0, 0, ld), **far), drafts(am)) == -4
+        assert f[op](cache(am, v_stride=(0, 0, ld), **far), drafts(am)) == -4
+        assert f[op](cache(am, batch=1, kv_heads=1, capacity=(1 << 30) + 1, head_d=1), drafts(am)) == -4
+    assert f["attend"](cache(am), drafts(am, k_stride=(0, 0, ld))) == -4
+    assert f["attend"](cache(am), drafts(am, v_stride=(0, 0, ld))) == -4
+    wide = drafts(am, heads=1 << 17, tokens=1)
+    assert f["weigh"](cache(am, batch=1, kv_heads=1, head_d=1), wide, n=128) == -4
+    small = [(1 << 40) * i for i in range(20, 32)]
+    c = cache(am, K=small[0], V=small[0], len=small[6], seen=None, weight=None, pos=None, batch=100,
+              kv_heads=1, capacity=1 << 30, head_d=1)
+    d = drafts(am, Q=small[8], K=small[9], V=small[10], heads=1, tokens=1)
+    assert f["attend"](c, d, out=small[11], lse=None) == -4
+    for scale in (1e-39, -1e-40, 1e-45):
+        assert f["attend"](cache(am), drafts(am), scale=scale) == -9
+        assert f["weigh"](cache(am), drafts(am), scale=scale) == -9
+
+
+def test_commit_refuses_tables_inside_the_tensors(am):
+    f = calls(am)["commit"]
+    assert f(cache(am, weight=KA + 64), drafts(am)) == -5
+    assert f(cache(am, pos=VA + 64), drafts(am)) == -5
+    assert f(cache(am, weight=KD), drafts(am)) == -5
+    assert f(cache(am, pos=WA + 4), drafts(am)) == -5

@@ -361,3 +361,153 @@ def test_cache_past_32_bit_offsets(am, dev):
     want, want_lse, info = C.attend64(q.host, k, v, None, None, [cap], [2])
     C.attend_close("bf16", D, out.numpy(), lse.numpy(), want, want_lse, info, [2])
     big.free()
+
+
+# ---------------------------------------------------------------- many sequences, many rows
+def many_lens(rng, B, cap):
+    """Mostly short, some empty, a few to the capacity."""
+    lens = rng.integers(0, 40, B)
+    lens[rng.random(B) < 0.2] = 0
+    lens[rng.integers(0, B, 5)] = cap
+    lens[rng.integers(0, B, 5)] = rng.integers(1, cap, 5)
+    return [int(x) for x in lens]
+
+
+@pytest.mark.parametrize("dtype,Hq,G,T,D,cap", [
+    ("bf16", 4, 2, 2, 128, 1300), ("f32", 2, 2, 1, 72, 700), ("bf16", 2, 1, 3, 520, 400),
+    ("bf16", 6, 1, 20, 100, 1100)])
+@pytest.mark.parametrize("B", [63, 64, 65, 128, 131])
+def test_many_sequences(am, dev, dtype, Hq, G, T, D, cap, B):
+    """More sequences than a wave has lanes."""
+    rng = np.random.default_rng(B)
+    counts = [int(x) for x in rng.integers(0, T + 1, B)]
+    solve(am, dtype, B, Hq, G, T, D, cap, many_lens(rng, B, cap), counts=counts, mask="tree", seed=B)
+
+
+@pytest.mark.parametrize("Hq,G,T,D,lens,mask", [
+    (65, 1, 1, 128, [700, 64], "chain"), (4, 2, 50, 128, [333, 0], "random"),
+    (4, 1, 33, 96, [100, 1500], "tree"), (2, 1, 150, 65, [31, 97], "random"),
+    (4, 1, 150, 128, [64, 2000], "tree"), (8, 2, 256, 128, [40, 257], "random"),
+    (13, 1, 100, 120, [1, 640], "random"), (3, 1, 256, 100, [3000, 77], "tree")])
+@pytest.mark.parametrize("layout", [{}, dict(order="rows", offset=3, pad=5)])
+def test_many_rows(am, dev, Hq, G, T, D, lens, mask, layout):
+    """More than 64 query rows of a kv head, of one to several tiles, and NaN where none may look."""
+    solve(am, "bf16", 2, Hq, G, T, D, max(lens) + 40, lens, counts=[T, T - T // 3], mask=mask,
+          fill=np.nan, seed=T, **layout)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("Hq,T,D", [(2, 100, 64), (2, 100, 24), (5, 40, 192), (3, 70, 256),
+                                    (2, 90, 640)])
+def test_several_row_tiles(am, dev, dtype, Hq, T, D):
+    solve(am, dtype, 2, Hq, 1, T, D, 500, [460, 131], counts=[T - 9, T], mask="random", fill=np.nan,
+          seed=T)
+
+
+@pytest.mark.parametrize("fill", [np.nan, np.inf])
+@pytest.mark.parametrize("lens", [[50, 0], [64, 3000]])
+def test_masked_draft_of_anything_many_rows(am, dev, fill, lens):
+    T, D, bad = 60, 128, 31
+    print(f"[case] masked draft, many rows {fill} {lens}", flush=True)
+    p = Problem(am, "bf16", 2, 4, 2, T, D, max(lens), lens, mask="tree", seed=9)
+    kd, vd = p.Kd.host.copy(), p.Vd.host.copy()
+    kd[:, :, bad] = np.nan if np.isnan(fill) else kd[:, :, bad]
+    vd[:, :, bad] = fill
+    p.Kd.base.upload(p.Kd._flat(kd))
+    p.Vd.base.upload(p.Vd._flat(vd))
+    p.run()
+    want, want_lse, info = p.want()
+    out, lse = p.out.numpy(), p.lse.numpy()
+    for b in range(2):
+        see = C.visible(T, T, p.words, b)[:, bad]
+        assert see.any() and not see.all()
+        one = [x[b:b + 1][:, :, ~see] for x in (out, lse, want, want_lse)]
+        inf1 = {k: x[b:b + 1][:, :, ~see] for k, x in info.items()}
+        C.attend_close("bf16", D, *one, inf1, [int((~see).sum())])
+        assert not np.isfinite(out[b][:, see]).any()
+
+
+@pytest.mark.parametrize("Hq,T", [(2, 4), (4, 40)])
+def test_nothing_to_attend_many_heads(am, dev, Hq, T):
+    """Tokens whose mask is empty beside others', over an empty cache."""
+    B, D = 2, 128
+    p = Problem(am, "bf16", B, Hq, 1, T, D, 8, [0, 0], mask="random", fill=np.nan, seed=2)
+    p.words = p.words.copy()
+    p.words[0, ::2] = 0
+    p.words[1] = 0
+    p.drafts = am.Drafts(p.Q.dev, p.Kd.dev, p.Vd.dev, mask=C.ints(p.words))
+    p.run()
+    p.check()
+    assert (p.out.numpy()[1] == 0).all() and np.isneginf(p.lse.numpy()[1]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,Hq,T", [(48, 2, 3), (128, 2, 3), (128, 4, 40), (200, 2, 20), (300, 2, 3)])
+@pytest.mark.parametrize("L", [41, 64, 3000, 3001])
+def test_infinite_values(am, dev, dtype, D, Hq, T, L):
+    """Infinities in a row of V that all tokens attend, the cache's last: infinite in its dims,
+    of their sign, NaN where two of them disagree; the other dims as if it were not there."""
+    print(f"[case] infinite values {dtype} {D} {Hq} {T} {L}", flush=True)
+    p = Problem(am, dtype, 1, Hq, 1, T, D, L + 3, [L], mask="tree", sigma=0.3, seed=6)
+    v = p.V.host.copy()
+    v[0, 0, L - 1, 5], v[0, 0, L - 1, 11] = np.inf, -np.inf
+    v[0, 0, L - 1, 23], v[0, 0, L - 2, 23] = np.inf, -np.inf
+    p.V.base.upload(p.V._flat(v))
+    p.run()
+    out, lse = p.out.numpy(), p.lse.numpy()
+    assert np.isposinf(out[..., 5]).all() and np.isneginf(out[..., 11]).all()
+    assert np.isnan(out[..., 23]).all()
+    want, want_lse, info = p.want()
+    rest = np.delete(np.arange(D), [5, 11, 23])
+    info["pv"] = info["pv"][..., rest]
+    C.attend_close(dtype, D, out[..., rest], lse, want[..., rest], want_lse, info, [T])
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f32", 72), ("bf16", 520), ("f32", 1100)])
+def test_small_workspaces(am, dev, dtype, D):
+    """A workspace that holds one pair's scratch: several passes, or fewer ranges; none at all is
+    enough where no scores are kept, and refused where they are."""
+    import hip_rt
+    one = Problem(am, dtype, 1, 2, 1, 5, D, 1500, [1499], mask="tree")
+    p = Problem(am, dtype, 3, 6, 3, 5, D, 1500, [1499, 0, 700], mask="tree")
+    n = am.tree_attention_workspace_bytes(one.cache, one.drafts)
+    assert 40960 < n < am.tree_attention_workspace_bytes(p.cache, p.drafts)
+    for size in (n, n + 4096, 2 * n, 3 * n):
+        ws = hip_rt.DeviceArray((size // 4 + 64,), "i32", fill=0x5A)
+        p.out.base.upload(p.out._flat(np.full(p.out.host.shape, 7.0, np.float32)))
+        p.run(workspace=hip_rt.DeviceArray.wrap(ws.ptr, (size // 4,), "i32", keep=ws))
+        p.check()
+        words = ws.numpy()
+        assert (words[:40960 // 4] == 0x5A5A5A5A).all() and (words[size // 4:] == 0x5A5A5A5A).all()
+    ws = hip_rt.DeviceArray((40960 // 4,), "i32")
+    if D > 256:
+        with pytest.raises(am.AtnError) as e:
+            p.run(workspace=ws)
+        assert e.value.status == am.ATN_ERR_WORKSPACE
+    else:
+        p.run(workspace=ws)
+        p.check()
+
+
+def test_one_workspace_for_two_graphs(am, dev):
+    """Two captured calls of different shapes that share a caller's workspace, replayed in turn."""
+    import hip_rt
+    s = hip_rt.Stream()
+    ps = [Problem(am, "bf16", 2, 8, 2, 3, 128, 3000, [3000, 1200], mask="tree", seed=1),
+          Problem(am, "bf16", 1, 2, 1, 4, 600, 1000, [999], mask="tree", seed=2)]
+    n = max(am.tree_attention_workspace_bytes(p.cache, p.drafts) for p in ps)
+    ws = hip_rt.DeviceArray((n // 4,), "i32", fill=0)
+    calls = [am.tree_attention_call(p.cache, p.drafts, p.out.dev, p.lse, workspace=ws) for p in ps]
+    graphs = [hip_rt.Graph(s, lambda c=c: c(s)) for c in calls]
+    for _ in range(3):
+        for p, g in zip(ps, graphs):
+            p.out.base.upload(p.out._flat(np.full(p.out.host.shape, 7.0, np.float32)))
+            g.launch()
+        s.synchronize()
+        for p in ps:
+            p.check()
+        calls[0](s)
+        s.synchronize()
+    for g in graphs:
+        g.destroy()
+    s.destroy()
