@@ -135,11 +135,12 @@ int check_drafts(const atn_kv_cache* c, const atn_drafts* d, bool need_q, bool n
     v->count = d->count;
     v->mask = d->mask;
     v->H = d->heads;
+    v->rep = d->heads / c->kv_heads;
     v->T = d->tokens;
     v->W = (d->tokens + 31) / 32;
     v->by_t = d->tokens > 1 ? (uint32_t)(((1ull << 32) + d->tokens - 1) / d->tokens) : 0;
     // (rows of a kv head times tokens below 2^32: the division by multiplication is exact)
-    if ((int64_t)(d->heads / c->kv_heads) * d->tokens >= (1 << 24)) return ATN_ERR_SIZE_OVERFLOW;
+    if ((int64_t)v->rep * d->tokens >= (1 << 24)) return ATN_ERR_SIZE_OVERFLOW;
     return ATN_OK;
 }
 
@@ -294,7 +295,7 @@ int atn_cache_weigh_ex(const atn_kv_cache* cache, const atn_drafts* drafts, cons
     if (st != ATN_OK) return st;
     if (!lse || !c.weight) return ATN_ERR_NULL_POINTER;
     // (a query row per head and path entry)
-    if ((int64_t)(d.H / c.G) * path_len >= (1 << 24)) return ATN_ERR_SIZE_OVERFLOW;
+    if ((int64_t)d.rep * path_len >= (1 << 24)) return ATN_ERR_SIZE_OVERFLOW;
     if (!aligned(lse, 4) || !aligned(weight_in, 4)) return ATN_ERR_MISALIGNED;
     const int64_t wb = (int64_t)c.B * c.G * c.cap * 4;
     const Range rw = range(c.weight, wb);

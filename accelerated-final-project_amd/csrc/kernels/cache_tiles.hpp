@@ -47,11 +47,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
 }
 
-// sum + both halves of a pair of bf16
-__device__ __forceinline__ float add2(uint32_t w, float sum) {
-    const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), one, sum, false);
+// sum + the products of two pairs of bf16
+__device__ __forceinline__ float dot2(uint32_t x, uint32_t y, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x),
+                                           __builtin_bit_cast(bf16x2, y), sum, false);
 }
+// sum + both halves of a pair of bf16
+__device__ __forceinline__ float add2(uint32_t w, float sum) { return dot2(w, 0x3f803f80u, sum); }
 
 // BYTES of a row.  Rows need only element alignment (the hardware loads 16 bytes from any).
 template <typename T, int BYTES>

@@ -32,7 +32,7 @@ struct QueryRow {
 };
 __device__ __forceinline__ QueryRow query_row(const WeighArgs& a, int b, int g, int A, int row) {
     QueryRow x;
-    x.head = g * (a.d.H / a.c.G) + row / A;
+    x.head = g * (a.d.rep) + row / A;
     x.entry = row % A;
     x.tok = path_at(a.p, b, x.entry);
     return x;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
     const int q = lane >> 4, col = lane & 15;
     const int bg = blockIdx.y, g = bg % a.c.G, b = bg / a.c.G, D = a.c.D;
     const int L = of_wave(rows_in_use(a.c, b)), A = of_wave(rows_accepted(a.c, a.d, a.p, b));
-    const int end = L + A, blocks = (end + KB - 1) / KB, R = a.d.H / a.c.G * A;
+    const int end = L + A, blocks = (end + KB - 1) / KB, R = a.d.rep * A;
     const T* kc = (const T*)a.c.K + b * a.c.ks[0] + g * a.c.ks[1];
     const int i0 = blockIdx.x * kWaves + wave, step = gridDim.x * kWaves;
     if ((int)blockIdx.x * kWaves >= blocks) return;
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
     const int bg = blockIdx.y, g = bg % a.c.G, b = bg / a.c.G, D = a.c.D;
     const int L = of_wave(rows_in_use(a.c, b)), A = of_wave(rows_accepted(a.c, a.d, a.p, b));
     const int end = L + A, j0 = blockIdx.x * kBlock, rows = min(kBlock, end - j0);
-    const int R = a.d.H / a.c.G * A;
+    const int R = a.d.rep * A;
     if (rows <= 0) return;
     const T* kp[SUB];
 #pragma unroll
@@ -225,7 +225,7 @@ void go(const WeighArgs& a, hipStream_t st) {
     const int keys = std::min(a.c.cap, a.c.rows + a.p.n);
     if (D > 256) {
         const dim3 grid((unsigned)((keys + kBlock - 1) / kBlock), (unsigned)BG);
-        const int R = a.d.H / a.c.G * a.p.n;  // at most
+        const int R = a.d.rep * a.p.n;  // at most
         if (R <= 16) return go_wide<T, 1>(a, grid, st);
         if (R <= 32) return go_wide<T, 2>(a, grid, st);
         return go_wide<T, 4>(a, grid, st);

@@ -99,25 +99,21 @@ constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 __device__ __forceinline__ int below_waves(int* slot, int x, int wave, int lane, int* all) {
     if (lane == 0) slot[wave] = x;
     __syncthreads();
-    int sum = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < kSelWaves; ++i) {
-        const int y = slot[i];
-        total += y;
-        sum += i < wave ? y : 0;
-    }
+    const int upto = wave_scan(lane < kSelWaves ? slot[lane] : 0);
     __syncthreads();
-    *all = total;
-    return sum;
+    *all = __builtin_amdgcn_readlane(upto, 63);
+    return __builtin_amdgcn_readlane(upto, wave) - x;
 }
 
-// KPT keys a thread stay in registers: a wave's are 64 KPT consecutive rows.  Heads of more than
-// 1024 KPT rows go through them in chunks, read again for each digit (KPT = 16, 16384 rows a
-// chunk): 12000 to 16384 rows 44 -> 12 us against a loop of one load after another.
+// KPT keys a thread come from memory at once and stay in LDS, each read by its own thread alone: a
+// wave's are 64 KPT consecutive rows.  Heads of more than 1024 KPT rows go through it in chunks,
+// read again for each digit (KPT = 16, 16384 rows a chunk).  One read of little
+// data: what bounds it is the code, fetched as the launch runs through it, so the loops stay loops.
 template <int KPT>
 __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int budget, int recent,
                                                               int slots, int* scratch) {
     constexpr int CHUNK = kSelThreads * KPT;
+    __shared__ uint32_t keys[CHUNK];
     __shared__ uint32_t hist[2048];
     __shared__ int slot[kSelWaves];
     __shared__ uint32_t pick[2];
@@ -134,7 +130,6 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int b
     const long lo = (long)c.seen[b] - recent;
     const int since = lo < INT32_MIN ? INT32_MIN : (int)lo;
     const int chunks = (L + CHUNK - 1) / CHUNK, mine = wave * 64 * KPT + lane;
-    uint32_t key[KPT];
     auto load = [&](int chunk) {
         float x[KPT];
         int y[KPT];
@@ -145,20 +140,24 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int b
             y[k] = pos[r];
         }
 #pragma unroll
-        for (int k = 0; k < KPT; ++k) key[k] = rank_key(x[k], y[k], since);
+        for (int k = 0; k < KPT; ++k) keys[mine + 64 * k] = rank_key(x[k], y[k], since);
     };
     for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
     __syncthreads();
     uint32_t prefix = 0, mask = 0, need = (uint32_t)budget;
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t bins = pass == 2 ? 1024 : 2048;
+#pragma unroll 1
         for (int chunk = 0; chunk < chunks; ++chunk) {
             if (pass == 0 || chunks > 1) load(chunk);
-#pragma unroll
-            for (int k = 0; k < KPT; ++k)
-                if (chunk * CHUNK + mine + 64 * k < L && (key[k] & mask) == prefix)
-                    atomicAdd(&hist[(key[k] >> shift) & (bins - 1)], 1u);
+#pragma unroll 4
+            for (int k = 0; k < KPT; ++k) {
+                const uint32_t key = keys[mine + 64 * k];
+                if (chunk * CHUNK + mine + 64 * k < L && (key & mask) == prefix)
+                    atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
+            }
         }
         __syncthreads();
         // thread t holds bins 2047 - 2t and 2046 - 2t (and clears them): sums from the top down
@@ -184,37 +183,40 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int b
     const uint64_t below = (1ull << lane) - 1;
     int* list = scratch + list_at(c.B * c.G) + (size_t)bg * slots * 2;
     int eq0 = 0, to0 = 0, from0 = 0;  // of the chunks before
+#pragma unroll 1
     for (int chunk = 0; chunk < chunks; ++chunk) {
         if (chunks > 1) load(chunk);
         const int r0 = chunk * CHUNK + mine;
         int eq = 0;
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < KPT; ++k)
-            eq += __builtin_popcountll(
-                __builtin_amdgcn_ballot_w64(r0 + 64 * k < L && key[k] == prefix));
+            eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(
+                r0 + 64 * k < L && keys[mine + 64 * k] == prefix));
         int all;
         int e = eq0 + below_waves(slot, eq, wave, lane, &all);
         eq0 += all;
-        uint32_t keep = 0;  // bit k: row k of this thread stays
-        int to = 0, from = 0;
-#pragma unroll
+        uint32_t keep = 0;   // bit k: row k of this thread stays
+        uint32_t moves = 0;  // slots left free below budget; rows kept past it, times 2^16
+#pragma unroll 2
         for (int k = 0; k < KPT; ++k) {
             const int r = r0 + 64 * k;
-            const bool on = r < L, tie = on && key[k] == prefix;
+            const uint32_t key = keys[mine + 64 * k];
+            const bool on = r < L, tie = on && key == prefix;
             const uint64_t same = __builtin_amdgcn_ballot_w64(tie);
-            const bool stay = (on && key[k] > prefix) ||
+            const bool stay = (on && key > prefix) ||
                               (tie && e + __builtin_popcountll(same & below) < (int)need);
             e += __builtin_popcountll(same);
             keep |= (uint32_t)stay << k;
-            to += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && !stay && r < budget));
-            from += __builtin_popcountll(__builtin_amdgcn_ballot_w64(stay && r >= budget));
+            moves += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && !stay && r < budget));
+            moves += __builtin_popcountll(__builtin_amdgcn_ballot_w64(stay && r >= budget)) << 16;
         }
-        int to_all, from_all;
-        to = to0 + below_waves(slot, to, wave, lane, &to_all);
-        from = from0 + below_waves(slot, from, wave, lane, &from_all);
-        to0 += to_all;
-        from0 += from_all;
-#pragma unroll
+        static_assert(CHUNK < 1 << 16, "a chunk's moves in 16 bits");
+        int moves_all;
+        const uint32_t at = (uint32_t)below_waves(slot, (int)moves, wave, lane, &moves_all);
+        int to = to0 + (int)(at & 0xffffu), from = from0 + (int)(at >> 16);
+        to0 += moves_all & 0xffff;
+        from0 += (int)((uint32_t)moves_all >> 16);
+#pragma unroll 2
         for (int k = 0; k < KPT; ++k) {
             const int r = r0 + 64 * k;
             const bool stay = (keep >> k) & 1u, free_ = r < L && !stay && r < budget;

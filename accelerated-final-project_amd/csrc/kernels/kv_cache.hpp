@@ -36,6 +36,7 @@ struct DraftView {
     const int* count;             // [B] tokens of each sequence, or null: T
     const uint32_t* mask;         // [B][T][W], or null: a chain
     int H, T, W;                  // W = ceil(T / 32)
+    int rep;                      // heads of a kv head
     uint32_t by_t;                // 2^32 / T rounded up (T > 1)
 };
 

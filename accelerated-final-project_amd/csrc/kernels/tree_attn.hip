@@ -36,7 +36,7 @@ __device__ __forceinline__ int blocks_of(const TreeArgs& a, int b, int kb) {
 // 0.7 us a block), so ranges of many short pairs have fewer blocks.
 constexpr int kPad = 16;
 
-// The line: its length, and the places of a range (whole turns of `turn`).  A wave's work, as
+// The line: its length, and the places of a range (whole turns of `turn`, a power of two).  A wave's work, as
 // are the others here; results are uniform.  n, upto: of sequence b0 + lane where the pass has
 // at most 64, its pairs' places and the sum of all sequences' up to it.
 struct Line {
@@ -48,12 +48,14 @@ __device__ __forceinline__ Line line_of(const TreeArgs& a, int kb, int turn, int
     x.n = lane < a.bs ? blocks_of(a, a.b0 + lane, kb) + kPad : 0;
     x.upto = wave_scan(x.n * a.gs);
     x.total = __builtin_amdgcn_readlane(x.upto, 63);
+#pragma unroll 1
     for (int i0 = 64; i0 < a.bs; i0 += 64) {
         const int n = i0 + lane < a.bs ? blocks_of(a, a.b0 + i0 + lane, kb) + kPad : 0;
         x.total += __builtin_amdgcn_readlane(wave_scan(n * a.gs), 63);
     }
-    const int per = (x.total + a.plan.ranges - 1) / a.plan.ranges;
-    x.per = max((per + turn - 1) / turn * turn, 2 * turn);
+    const unsigned ranges = a.plan.ranges;
+    const int per = (x.total + ranges - 1) / ranges;
+    x.per = max((per + turn - 1) & -turn, 2 * turn);
     return x;
 }
 
@@ -64,6 +66,7 @@ struct Place {
 __device__ __forceinline__ Place place_at(const TreeArgs& a, const Line& line, int at, int kb,
                                           int lane) {
     int n = line.n, upto = line.upto;
+#pragma unroll 1
     for (int i0 = 0;; i0 += 64) {
         const uint64_t done = __builtin_amdgcn_ballot_w64(upto <= at);
         if (done != ~0ull || i0 + 64 >= a.bs) {
@@ -85,6 +88,7 @@ __device__ __forceinline__ int start_of(const TreeArgs& a, const Line& line, int
     if (i < 64)
         return __builtin_amdgcn_readlane(line.upto, i) - __builtin_amdgcn_readlane(line.n, i) * a.gs;
     int before = 0;
+#pragma unroll 1
     for (int i0 = 0; i0 < i; i0 += 64) {
         const int n = i0 + lane < i ? blocks_of(a, a.b0 + i0 + lane, kb) + kPad : 0;
         before += __builtin_amdgcn_readlane(wave_scan(n * a.gs), 63);
@@ -102,7 +106,7 @@ __device__ __forceinline__ Span span_at(const TreeArgs& a, const Line& line, int
                                         int kb, int lane, int* next) {
     const Place p = place_at(a, line, at, kb, lane);
     Span s;
-    const int off = at - p.start, pair = off / p.n, in = off - pair * p.n;
+    const int off = at - p.start, pair = (unsigned)off / (unsigned)p.n, in = off - pair * p.n;
     const int out = min(p.n, in + end - at);
     s.b = p.b;
     s.g = a.g0 + pair;
@@ -115,8 +119,9 @@ __device__ __forceinline__ Span span_at(const TreeArgs& a, const Line& line, int
 // The whole of pair r, where ranges are pairs.
 __device__ __forceinline__ Span span_whole(const TreeArgs& a, int r, int kb) {
     Span s;
-    s.b = a.b0 + r / a.gs;
-    s.g = a.g0 + r % a.gs;
+    const int seq = (unsigned)r / (unsigned)a.gs;
+    s.b = a.b0 + seq;
+    s.g = a.g0 + r - seq * a.gs;
     s.first = 0;
     s.last = of_wave(blocks_of(a, s.b, kb));
     s.part = -1;
@@ -175,25 +180,28 @@ __device__ __forceinline__ void store4(uint16_t* to, const float (&x)[4], int le
 // weights of 0: places behind its rows, drafts that a row does not attend.  An infinity or NaN in
 // its V belongs only to the rows that attend it.  The product runs without it; it is added
 // where the results are written.
-// Whether any lane's V holds an infinity or NaN, which are cleared.
+// Whether any lane's V holds an infinity or NaN, which are cleared.  (What finds them is short: a
+// sum of products with 0, which is NaN then.)
 template <typename T, typename V>
 __device__ __forceinline__ bool clear_not_finite(V& v) {
-    bool any = false;
+    float sum = 0.f;
+    for (auto& row : v.p)
+        for (auto& piece : row)
+            for (auto& w : piece.w)
+                sum = sizeof(T) == 4 ? fmaf(__uint_as_float(w), 0.f, sum) : dot2(w, 0u, sum);
+    if (!__builtin_amdgcn_ballot_w64(sum != sum)) return false;
     for (auto& row : v.p)
         for (auto& piece : row)
             for (auto& w : piece.w) {
+                const bool hi = (w & 0x7f800000u) == 0x7f800000u;
                 if constexpr (sizeof(T) == 4) {
-                    const bool bad = (w & 0x7f800000u) == 0x7f800000u;
-                    any |= bad;
-                    w = bad ? 0u : w;
+                    w = hi ? 0u : w;
                 } else {
                     const bool lo = (w & 0x7f80u) == 0x7f80u;
-                    const bool hi = (w & 0x7f800000u) == 0x7f800000u;
-                    any |= lo | hi;
                     w &= (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
                 }
             }
-    return __builtin_amdgcn_ballot_w64(any) != 0;
+    return true;
 }
 
 // What the infinities and NaNs that clear_not_finite() took out (of the cache's rows from
@@ -222,7 +230,7 @@ __device__ __forceinline__ float not_finite_sum(const TreeArgs& a, int b, int g,
 template <typename T>
 __device__ void add_not_finite(const TreeArgs& a, const Span& s, int row, int from, int L, int n,
                                int d0, int d1, int lane) {
-    const int rep = a.d.H / a.c.G, h = head_of(a.d, row), tok = row - h * a.d.T;
+    const int rep = a.d.rep, h = head_of(a.d, row), tok = row - h * a.d.T;
     if (row >= rep * a.d.T || tok >= n) return;
     T* out = (T*)a.out + s.b * a.os[0] + (s.g * rep + h) * a.os[1] + tok * a.os[2];
     for (int d = d0 + lane; d < d1; d += 64) {
@@ -297,9 +305,10 @@ __device__ __forceinline__ void weights(float (&p)[MT][SUB][4], v4f (&o)[MT][VS]
 template <typename T, int DP, int ROWS, int PARTS, int LDO, int VL, int MODE, int THREADS>
 __device__ __forceinline__ void write_rows(const TreeArgs& a, const Span& sp, int tile, int n,
                                            const float* xo, const float4* fin) {
-    const int D = a.c.D, rep = a.d.H / a.c.G, R = rep * a.d.T;
-    // (opaque: or what this computes is hoisted out of the loop over spans, into registers)
-#pragma unroll 2
+    const int D = a.c.D, rep = a.d.rep, R = rep * a.d.T;
+    // (opaque: or what this computes is hoisted out of the loop over spans, into registers; not
+    // unrolled: twice the code, fetched once a launch, takes longer than the loop)
+#pragma unroll 1
     for (int e = opaque(threadIdx.x); e < ROWS * (DP / 4); e += THREADS) {
         const int r = e / (DP / 4), d = e % (DP / 4) * 4, row = tile * ROWS + r;
         const int h = head_of(a.d, row), tok = row - h * a.d.T;
@@ -324,7 +333,7 @@ __device__ __forceinline__ void write_rows(const TreeArgs& a, const Span& sp, in
         if (sp.part >= 0) {
             const size_t to = part_row(a, sp.part, row);
             if (d == 0) part_stats(a)[to] = z;
-            store4(part_dims(a) + to * D + d, x, D - d);
+            store4(part_dims(a) + to * D + d, x, MODE == kExact ? 4 : D - d);
         } else {
             // (0: nothing visible, or no score above -infinity)
             const float inv = z.z == 0.f ? 0.f : 1.f / z.z;
@@ -334,7 +343,7 @@ __device__ __forceinline__ void write_rows(const TreeArgs& a, const Span& sp, in
 #pragma unroll
             for (int c = 0; c < 4; ++c) x[c] *= inv;
             store4((T*)a.out + sp.b * a.os[0] + (sp.g * rep + h) * a.os[1] + tok * a.os[2] + d, x,
-                   D - d);
+                   MODE == kExact ? 4 : D - d);
         }
     }
 }
@@ -374,7 +383,7 @@ k_tree_narrow(TreeArgs a) {
     const int q = lane >> 4, col = lane & 15;
     int range, tile;
     tile_of(blockIdx.x, a.plan.ranges, a.plan.row_tiles, &range, &tile);
-    const int D = a.c.D, rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const int D = a.c.D, rep = a.d.rep, R = rep * a.d.T;
     const float scale = fabsf(a.scale);
 
     int at = 0, end = 1;
@@ -608,7 +617,7 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
     const int q = lane >> 4, col = lane & 15, rg = wave % RG, kg = wave / RG;
     int range, tile;
     tile_of(blockIdx.x, a.plan.ranges, a.plan.row_tiles, &range, &tile);
-    const int D = a.c.D, rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const int D = a.c.D, rep = a.d.rep, R = rep * a.d.T;
     const float scale = fabsf(a.scale);
 
     int at = 0, end = 1;
@@ -861,7 +870,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_tree_scores(TreeArgs a) {
     if (i >= all) return;
     const bool in = i < cache;
     const int j0 = (in ? i : i - cache) * kBlock, rows = min(kBlock, (in ? L : n) - j0);
-    const int rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const int rep = a.d.rep, R = rep * a.d.T;
     const T* kp[SUB];
     const T* qp[MT];
 #pragma unroll
@@ -919,7 +928,7 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
     int unit, tile;
     tile_of(blockIdx.x, a.plan.ranges * groups, tiles, &unit, &tile);
     const int range = unit / groups, d0 = (unit % groups * kWaves + wave) * WD;
-    const int rep = a.d.H / a.c.G, R = rep * a.d.T;
+    const int rep = a.d.rep, R = rep * a.d.T;
     const bool busy = d0 < D;
     // softmax: 16 threads a row, 8 keys each, one pass per 16 rows
     const int sr = threadIdx.x >> 4, sk = (threadIdx.x & 15) * 8;
@@ -1126,22 +1135,23 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
 // The parts of a row added up, in their order: WAVES waves a row (and 256 dims), each every
 // WAVES-th part; 4 rows a workgroup where there are many rows.  Rows of one range alone are
 // written already.
-template <typename T, int WAVES>
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int kb, unsigned units) {
+template <typename T, int WAVES, int KB>
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a) {
     __shared__ float acc[4][256];
     __shared__ float2 sums[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int D = a.c.D, chunks = (D + 255) / 256, rep = a.d.H / a.c.G, R = rep * a.d.T;
-    const unsigned unit = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
-    if (unit >= units) return;
-    const int d0 = (unit % chunks) * 256, row = unit / chunks % R;
-    const int pair = unit / chunks / R, g = a.g0 + pair % a.gs, b = a.b0 + pair / a.gs;
+    const int D = a.c.D, rep = a.d.rep, d0 = blockIdx.z * 256;
+    const int row = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
+    if (row >= rep * a.d.T) return;
+    const unsigned pair = blockIdx.y, seq = pair / (unsigned)a.gs;
+    const int g = a.g0 + (int)(pair - seq * a.gs), b = a.b0 + (int)seq;
     const int h = head_of(a.d, row), tok = row - h * a.d.T;
     if (tok >= drafts_of(a.d, b)) return;
-    const int blocks = of_wave(blocks_of(a, b, kb));
-    const Line line = line_of(a, kb, a.plan.turn, lane);
-    const int first = start_of(a, line, b, kb, lane) + (g - a.g0) * (blocks + kPad) + kPad;
-    const int r0 = first / line.per, r1 = (first + blocks - 1) / line.per;
+    const int blocks = of_wave(blocks_of(a, b, KB));
+    const Line line = line_of(a, KB, a.plan.turn, lane);
+    const int first = start_of(a, line, b, KB, lane) + (g - a.g0) * (blocks + kPad) + kPad;
+    const int r0 = (unsigned)first / (unsigned)line.per;
+    const int r1 = (unsigned)(first + blocks - 1) / (unsigned)line.per;
     if (r0 == r1) return;
     const float4* st = part_stats(a);
     // part i is range r0 + i's: its second where the pair begins, its first after that
@@ -1243,6 +1253,17 @@ void go_wide(const TreeArgs& a, hipStream_t st) {
                        dim3(64 * kWaves), 0, st, a);
 }
 
+template <typename T, int KB>
+void go_merge(const TreeArgs& a, hipStream_t st) {
+    const int R = a.d.rep * a.d.T, chunks = (a.c.D + 255) / 256;
+    if ((int64_t)a.bs * a.gs * R * chunks >= 1024)
+        hipLaunchKernelGGL((k_tree_merge<T, 1, KB>), dim3((R + 3) / 4, a.bs * a.gs, chunks),
+                           dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_tree_merge<T, 4, KB>), dim3(R, a.bs * a.gs, chunks), dim3(256), 0, st,
+                           a);
+}
+
 template <typename T>
 void go(const TreeArgs& a, hipStream_t st) {
     const int D = a.c.D;
@@ -1259,15 +1280,10 @@ void go(const TreeArgs& a, hipStream_t st) {
         go_dims<T, 256>(a, st);
     }
     if (a.plan.split) {
-        const bool wide = D > kTreeNarrow;
-        const unsigned units = (unsigned)((size_t)a.bs * a.gs * (a.d.H / a.c.G) * a.d.T *
-                                          ((D + 255) / 256));
-        const int kb = wide || sizeof(T) == 2 ? 32 : 16;
-        if (units >= 1024)
-            hipLaunchKernelGGL((k_tree_merge<T, 1>), dim3((units + 3) / 4), dim3(256), 0, st, a, kb,
-                               units);
-        else
-            hipLaunchKernelGGL((k_tree_merge<T, 4>), dim3(units), dim3(256), 0, st, a, kb, units);
+        if constexpr (sizeof(T) == 4) {
+            if (D <= kTreeNarrow) return go_merge<T, 16>(a, st);
+        }
+        go_merge<T, 32>(a, st);
     }
 }
 
