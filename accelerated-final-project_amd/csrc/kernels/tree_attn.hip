@@ -305,7 +305,7 @@ __device__ __forceinline__ void weights(float (&p)[MT][SUB][4], v4f (&o)[MT][VS]
 template <typename T, int DP, int ROWS, int PARTS, int LDO, int VL, int MODE, int THREADS>
 __device__ __forceinline__ void write_rows(const TreeArgs& a, const Span& sp, int tile, int n,
                                            const float* xo, const float4* fin) {
-    const int D = a.c.D, rep = a.d.rep, R = rep * a.d.T;
+    const int D = MODE == kExact ? DP : a.c.D, rep = a.d.rep, R = rep * a.d.T;
     // (opaque: or what this computes is hoisted out of the loop over spans, into registers; not
     // unrolled: twice the code, fetched once a launch, takes longer than the loop)
 #pragma unroll 1
@@ -383,19 +383,21 @@ k_tree_narrow(TreeArgs a) {
     const int q = lane >> 4, col = lane & 15;
     int range, tile;
     tile_of(blockIdx.x, a.plan.ranges, a.plan.row_tiles, &range, &tile);
-    const int D = a.c.D, rep = a.d.rep, R = rep * a.d.T;
+    const int D = MODE == kExact ? DP : a.c.D, rep = a.d.rep, R = rep * a.d.T;
     const float scale = fabsf(a.scale);
 
+    // (8 waves are for pairs that one workgroup takes whole: see tree_plan)
+    const bool split = WAVES != 8 && a.plan.split;
     int at = 0, end = 1;
     Line line{};
-    if (a.plan.split) {
+    if (split) {
         line = line_of(a, KB, a.plan.turn, lane);
         at = range * line.per;
         end = min(line.total, at + line.per);
     }
     while (at < end) {
         Span sp;
-        if (a.plan.split) {
+        if (split) {
             sp = span_at(a, line, range, at, end, KB, lane, &at);
             if (sp.last <= sp.first) continue;
         } else {
@@ -617,7 +619,7 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
     const int q = lane >> 4, col = lane & 15, rg = wave % RG, kg = wave / RG;
     int range, tile;
     tile_of(blockIdx.x, a.plan.ranges, a.plan.row_tiles, &range, &tile);
-    const int D = a.c.D, rep = a.d.rep, R = rep * a.d.T;
+    const int D = MODE == kExact ? DP : a.c.D, rep = a.d.rep, R = rep * a.d.T;
     const float scale = fabsf(a.scale);
 
     int at = 0, end = 1;
