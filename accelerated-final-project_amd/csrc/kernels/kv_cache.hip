@@ -1,6 +1,7 @@
 // The key/value cache of a decoding program: accepted drafts written into it,
 // eviction of the lightest rows, and its lengths.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.hpp"
 
@@ -105,13 +106,37 @@ __device__ __forceinline__ int below_waves(int* slot, int x, int wave, int lane,
     return __builtin_amdgcn_readlane(upto, wave) - x;
 }
 
+// Moves first, first + step, ... of n of a head, `width` lanes each.  Sources lie at or past
+// `budget`, targets below it: no order among them.
+template <typename T>
+__device__ __forceinline__ void move_rows(const CacheView& c, int bg, const int* list, int n,
+                                          int first, int step, int vec, int lane, int width) {
+    const int g = bg % c.G, b = bg / c.G;
+    T* K = (T*)c.K + b * c.ks[0] + g * c.ks[1];
+    T* V = (T*)c.V + b * c.vs[0] + g * c.vs[1];
+    const size_t m = (size_t)bg * c.cap;
+    for (int i = first; i < n; i += step) {
+        const int to = list[2 * i], from = list[2 * i + 1];
+        float w = 0.f;
+        int p = 0;
+        if (lane == 0) w = c.weight[m + from], p = c.pos[m + from];
+        copy_rows(K + to * c.ks[2], K + from * c.ks[2], V + to * c.vs[2], V + from * c.vs[2], c.D, vec,
+                  lane, width);
+        if (lane == 0) c.weight[m + to] = w, c.pos[m + to] = p;
+    }
+}
+
 // KPT keys a thread come from memory at once and stay in LDS, each read by its own thread alone: a
 // wave's are 64 KPT consecutive rows.  Heads of more than 1024 KPT rows go through it in chunks,
 // read again for each digit (KPT = 16, 16384 rows a chunk).  One read of little
 // data: what bounds it is the code, fetched as the launch runs through it, so the loops stay loops.
-template <int KPT>
+// T: the workgroup moves the rows itself, where a head has few of them (a cache that is cut
+// whenever it is a little over its bound): a second launch takes longer than they do.  void: it
+// leaves them to k_evict_move.
+template <int KPT, typename T>
 __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int budget, int recent,
-                                                              int slots, int* scratch) {
+                                                              int slots, int* scratch, int vec,
+                                                              int width) {
     constexpr int CHUNK = kSelThreads * KPT;
     __shared__ uint32_t keys[CHUNK];
     __shared__ uint32_t hist[2048];
@@ -229,31 +254,22 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(CacheView c, int b
             from += __builtin_popcountll(v);
         }
     }
-    if (tid == 0) scratch[bg] = to0;
+    if constexpr (std::is_void_v<T>) {
+        if (tid == 0) scratch[bg] = to0;
+    } else {
+        __syncthreads();  // (the lists are written)
+        move_rows<T>(c, bg, list, to0, tid / width, kSelThreads / width, vec, tid & (width - 1), width);
+    }
 }
 
-// `width` lanes per move, the moves of a head dealt to gridDim.x workgroups.  Sources lie at or
-// past `budget`, targets below it: no order among them.
+// `width` lanes per move, the moves of a head dealt to gridDim.x workgroups.
 template <typename T>
 __global__ __launch_bounds__(256) void k_evict_move(CacheView c, int slots, const int* scratch,
                                                     int vec, int width) {
-    const int lane = threadIdx.x & (width - 1), bg = blockIdx.y, g = bg % c.G, b = bg / c.G;
-    const int per = 256 / width;
-    const int n = min(scratch[bg], slots);
-    const int2* list =
-        reinterpret_cast<const int2*>(scratch + list_at(c.B * c.G)) + (size_t)bg * slots;
-    T* K = (T*)c.K + b * c.ks[0] + g * c.ks[1];
-    T* V = (T*)c.V + b * c.vs[0] + g * c.vs[1];
-    for (int i = blockIdx.x * per + threadIdx.x / width; i < n; i += gridDim.x * per) {
-        const int to = list[i].x, from = list[i].y;
-        const size_t m = (size_t)bg * c.cap;
-        float w = 0.f;
-        int p = 0;
-        if (lane == 0) w = c.weight[m + from], p = c.pos[m + from];
-        copy_rows(K + to * c.ks[2], K + from * c.ks[2], V + to * c.vs[2], V + from * c.vs[2], c.D, vec,
-                  lane, width);
-        if (lane == 0) c.weight[m + to] = w, c.pos[m + to] = p;
-    }
+    const int bg = blockIdx.y, per = 256 / width;
+    const int* list = scratch + list_at(c.B * c.G) + (size_t)bg * slots * 2;
+    move_rows<T>(c, bg, list, min(scratch[bg], slots), blockIdx.x * per + threadIdx.x / width,
+                 gridDim.x * per, vec, threadIdx.x & (width - 1), width);
 }
 
 // lanes of a row: its 16-byte pieces, a power of two up to a wave
@@ -299,25 +315,38 @@ size_t evict_scratch(int B, int G, int cap, int budget) {
     return (list_at(B * G) + (size_t)B * G * 2 * slots) * sizeof(int);
 }
 
+template <typename T>
+static void select(const CacheView& c, int budget, int recent, int slots, int* scratch, int vec,
+                   int width, hipStream_t st) {
+    const dim3 grid((unsigned)(c.B * c.G)), block(kSelThreads);
+    if (c.cap <= kSelThreads)
+        hipLaunchKernelGGL((k_evict_select<1, T>), grid, block, 0, st, c, budget, recent, slots,
+                           scratch, vec, width);
+    else if (c.cap <= 4 * kSelThreads)
+        hipLaunchKernelGGL((k_evict_select<4, T>), grid, block, 0, st, c, budget, recent, slots,
+                           scratch, vec, width);
+    else
+        hipLaunchKernelGGL((k_evict_select<16, T>), grid, block, 0, st, c, budget, recent, slots,
+                           scratch, vec, width);
+}
+
 hipError_t launch_cache_evict(int dtype, const CacheView& c, int budget, int recent, int* scratch,
                               hipStream_t st) {
     const int slots = std::min(budget, c.cap - budget);
     if (slots <= 0) return hipSuccess;  // no row can lie past the budget
     const size_t es = dtype == kDtypeF32 ? 4 : 2;
     const int vec = rows16(c.K, c.ks, c.D, es) && rows16(c.V, c.vs, c.D, es);
-    const int BG = c.B * c.G;
-    if (c.cap <= kSelThreads)
-        hipLaunchKernelGGL(k_evict_select<1>, dim3(BG), dim3(kSelThreads), 0, st, c, budget, recent,
-                           slots, scratch);
-    else if (c.cap <= 4 * kSelThreads)
-        hipLaunchKernelGGL(k_evict_select<4>, dim3(BG), dim3(kSelThreads), 0, st, c, budget, recent,
-                           slots, scratch);
+    const int BG = c.B * c.G, width = lanes_of(c.D, es), per = 256 / width;
+    // the bytes of a head's moves that one workgroup still copies in less time than a launch takes
+    const bool few = (int64_t)slots * c.D * es * 2 <= 64 * 1024;
+    if (few && dtype == kDtypeF32)
+        select<float>(c, budget, recent, slots, scratch, vec, width, st);
+    else if (few)
+        select<uint16_t>(c, budget, recent, slots, scratch, vec, width, st);
     else
-        hipLaunchKernelGGL(k_evict_select<16>, dim3(BG), dim3(kSelThreads), 0, st, c, budget, recent,
-                           slots, scratch);
+        select<void>(c, budget, recent, slots, scratch, vec, width, st);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const int width = lanes_of(c.D, es), per = 256 / width;
+    if (e != hipSuccess || few) return e;
     const dim3 grid((unsigned)std::max(1, std::min((slots + per - 1) / per, 4096 / std::min(BG, 4096))),
                     (unsigned)BG);
     if (dtype == kDtypeF32)

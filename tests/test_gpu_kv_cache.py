@@ -455,3 +455,15 @@ def test_decoding(am, dev, dtype, D, Hq, G, captured):
     for g in graphs or []:
         g.destroy()
     s.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,offset", [(1, 0), (24, 0), (128, 0), (100, 1)])
+@pytest.mark.parametrize("cap,budget,recent,lens", [
+    (70, 64, 16, [70, 69]), (2000, 1990, 100, [2000, 1991]), (5000, 4960, 64, [5000, 4961]),
+    (40000, 39990, 500, [40000, 39995])])
+def test_evict_little_over_the_bound(am, dev, dtype, D, offset, cap, budget, recent, lens):
+    """Few moves a head, of caches of every size."""
+    print(f"[case] evict few {dtype} {D} {cap} {budget} {lens}", flush=True)
+    c = Cache(am, dtype, 2, 2, cap, D, lens, seen=[cap] * 2, offset=offset, seed=cap)
+    check_evict(am, c, budget, recent)
