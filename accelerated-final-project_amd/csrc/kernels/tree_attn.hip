@@ -1320,7 +1320,10 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     int64_t ranges = std::min(slots, ceil_div(pairs * (blocks + kPad), 2 * turn));
     // one workgroup of 8 waves a pair where that leaves a wave few blocks: no second launch
     const bool small = !wide && mt <= 2 && D <= 128 && blocks <= 32 && pairs * p.row_tiles <= 512;
-    p.split = !small && ranges > 1 && pairs < 4 * slots && blocks > turn;
+    // (pairs of few turns of blocks take less time whole than the parts and their merge: bf16,
+    // head_d 1024, 75 rows, 14 blocks 35 against 46 us; fp32, head_d 512, 24 rows, 16 blocks 44
+    // against 40)
+    p.split = !small && ranges > 1 && pairs < 4 * slots && blocks > 7 * turn / 2;
     if (small) p.waves = 8;
     p.turn = small ? p.waves : (int)turn;
     const size_t room = scratch_cap / sizeof(float);

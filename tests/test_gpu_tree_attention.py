@@ -375,7 +375,7 @@ def many_lens(rng, B, cap):
 
 @pytest.mark.parametrize("dtype,Hq,G,T,D,cap", [
     ("bf16", 4, 2, 2, 128, 1300), ("f32", 2, 2, 1, 72, 700), ("bf16", 2, 1, 3, 520, 400),
-    ("bf16", 6, 1, 20, 100, 1100)])
+    ("bf16", 2, 1, 3, 264, 1100), ("bf16", 6, 1, 20, 100, 1100)])
 @pytest.mark.parametrize("B", [63, 64, 65, 128, 131])
 def test_many_sequences(am, dev, dtype, Hq, G, T, D, cap, B):
     """More sequences than a wave has lanes."""
