@@ -309,7 +309,7 @@ struct CacheTiles {
 // Scores of 32 keys against 16 MT query rows over wave `wave`'s share of the dims (of `waves`),
 // from each lane's row pointers.  AHEAD: all loads of a step go out before its products (waves of
 // several steps: left to itself the compiler keeps six in flight, and the memory idles, 100 MB
-// in 37 against 27 us); else fewer registers and more waves (of one step: 18 against 13 us).
+// in 37 against 27 us); else fewer registers and more waves (of one step: 18 against 15 us).
 template <typename T, int MT, bool AHEAD>
 __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp)[2],
                                             const T* const (&qp)[MT], int D, int wave, int waves,
