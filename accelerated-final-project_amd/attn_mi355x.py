@@ -561,7 +561,7 @@ def _strides(t, name):
         return (ctypes.c_int64 * 3)(0, 0, 0)
     if t.strides[3] != 1 and t.shape[3] != 1:
         raise ValueError(f"{name}: the elements of a row must be adjacent")
-    if not any(t.strides[:3]):
+    if not any(t.strides[:3]) and max(t.shape[:3]) > 1:
         raise ValueError(f"{name}: strides 0, 0, 0 mean a contiguous array to the library")
     return (ctypes.c_int64 * 3)(*t.strides[:3])
 

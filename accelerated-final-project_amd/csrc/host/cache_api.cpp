@@ -242,7 +242,8 @@ int atn_tree_attention_ex(const atn_kv_cache* cache, const atn_drafts* drafts, v
         room = workspace_bytes - kSyncRegion;
     }
     a.plan = plan_tree(a.c, a.d, cache->dtype, room);
-    if (a.plan.workgroups > INT32_MAX || a.plan.line > INT32_MAX) return ATN_ERR_SIZE_OVERFLOW;
+    // (a dimension of a grid has less than 2^32 threads; workgroups of at most 512)
+    if (a.plan.workgroups >= 1 << 23 || a.plan.line > INT32_MAX) return ATN_ERR_SIZE_OVERFLOW;
     if (workspace != nullptr && a.plan.scratch > room) return ATN_ERR_WORKSPACE;
     int dev;
     st = atn_host::device(&dev);

@@ -134,7 +134,7 @@ struct TreePlan {
     size_t scores;   // floats of the scores of a pass
     size_t scratch;  // bytes
     int64_t line;        // places of the line of blocks, at most
-    int64_t workgroups;  // of a pass, at most
+    int64_t workgroups;  // of a grid of one dimension, at most
 };
 
 struct TreeArgs {

@@ -1367,9 +1367,8 @@ TreePlan tree_plan(int dtype, int B, int G, int H, int T, int D, int max_len, bo
     p.scratch = (p.scores + (p.split ? part * ranges : 0)) * sizeof(float);
     // (range starts pass the line's end by one range at most)
     p.line = p.split ? in_pass * (blocks + kPad) + 2 * turn * p.ranges : 0;
-    p.workgroups = std::max({(int64_t)p.ranges * p.row_tiles * groups,
-                             in_pass * p.row_tiles * p.shares * (p.ld_scores / kBlock),
-                             in_pass * R * ceil_div(D, 256)});
+    p.workgroups = std::max((int64_t)p.ranges * p.row_tiles * groups,
+                            in_pass * p.row_tiles * p.shares * (p.ld_scores / kBlock));
     return p;
 }
 

@@ -268,6 +268,22 @@ def test_sizes_past_the_kernels_numbers(am):
         assert f["weigh"](cache(am), drafts(am), scale=scale) == -9
 
 
+def test_grids_past_the_hardware(am):
+    """More workgroups than a grid's dimension holds threads for."""
+    c = cache(am, batch=65535, kv_heads=1, capacity=1, head_d=1)
+    d = drafts(am, heads=512, tokens=32)
+    assert calls(am)["attend"](c, d, lse=None) == -4
+
+
+def test_strides_of_single_rows(am):
+    """A dimension of one element may have any stride, 0 among them."""
+    import hip_rt
+    one = hip_rt.DeviceArray.wrap(KA, (1, 1, 1, 64), "bf16", (0, 0, 0, 1))
+    am.KvCache(one, one, hip_rt.DeviceArray.wrap(LA, (1,), "i32"))
+    with pytest.raises(ValueError):
+        am.Drafts(hip_rt.DeviceArray.wrap(QA, (1, 2, 1, 64), "bf16", (0, 0, 0, 1)))
+
+
 def test_commit_refuses_tables_inside_the_tensors(am):
     f = calls(am)["commit"]
     assert f(cache(am, weight=KA + 64), drafts(am)) == -5
