@@ -306,12 +306,12 @@ struct CacheTiles {
     }
 };
 
-// Scores of 32 keys against 16 MT query rows over wave `wave`'s share of the dims (of `waves`),
+// Scores of 16 SUB keys against 16 MT query rows over wave `wave`'s share of the dims (of `waves`),
 // from each lane's row pointers.  AHEAD: all loads of a step go out before its products (waves of
 // several steps: left to itself the compiler keeps six in flight, and the memory idles, 100 MB
 // in 37 against 27 us); else fewer registers and more waves (of one step: 18 against 15 us).
-template <typename T, int MT, bool AHEAD>
-__device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp)[2],
+template <typename T, int MT, bool AHEAD, int SUB>
+__device__ __forceinline__ void wide_scores(v4f (&s)[MT][SUB], const T* const (&kp)[SUB],
                                             const T* const (&qp)[MT], int D, int wave, int waves,
                                             int q) {
     using N = CacheTiles<T, 64, MT, kExact>;
@@ -319,17 +319,17 @@ __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < SUB; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
     const int per = ((D + STEP * U - 1) / (STEP * U) + waves - 1) / waves * STEP * U;
     const int d1 = min(D, (wave + 1) * per);
     int d = wave * per;
     for (; d + STEP * U <= d1; d += STEP * U) {
-        typename N::KPiece k[U][2], f[U][MT];
+        typename N::KPiece k[U][SUB], f[U][MT];
 #pragma unroll
         for (int e = 0; e < U; ++e) {
             const int at = d + STEP * e + EL * q;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) k[e][u] = ld_words<16>(kp[u] + at);
+            for (int u = 0; u < SUB; ++u) k[e][u] = ld_words<16>(kp[u] + at);
 #pragma unroll
             for (int t = 0; t < MT; ++t) f[e][t] = ld_words<16>(qp[t] + at);
         }
@@ -339,15 +339,15 @@ __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) s[t][u] = N::dot(k[e][u], f[e][t], s[t][u]);
+                for (int u = 0; u < SUB; ++u) s[t][u] = N::dot(k[e][u], f[e][t], s[t][u]);
     }
     if (d < d1) {  // the row's end (kClamp's pieces)
 #pragma unroll 1
         for (int e = 0; e < U; ++e) {
             const int want = d + STEP * e + EL * q, at = min(want, D - EL);
-            typename N::KPiece x[2], y;
+            typename N::KPiece x[SUB], y;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < SUB; ++u) {
                 x[u] = ld_words<16>(kp[u] + at);
                 clear_first(x[u], want - at);
             }
@@ -356,7 +356,7 @@ __device__ __forceinline__ void wide_scores(v4f (&s)[MT][2], const T* const (&kp
                 y = ld_words<16>(qp[t] + at);
                 clear_first(y, want - at);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) s[t][u] = N::dot(x[u], y, s[t][u]);
+                for (int u = 0; u < SUB; ++u) s[t][u] = N::dot(x[u], y, s[t][u]);
             }
         }
     }

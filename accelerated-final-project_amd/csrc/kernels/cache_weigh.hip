@@ -137,12 +137,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_narrow(WeighArgs a) {
     }
 }
 
-// head_d > 256: 8 waves share the dims of a block of 32 keys and add up through LDS.
-constexpr int kBlock = 32, kScoreWaves = 8;
+// head_d > 256: 8 waves share the dims of a block of 16 SUB keys and add up through LDS.
+constexpr int kScoreWaves = 8;
 
-template <typename T, int MT, bool AHEAD>
+template <typename T, int MT, bool AHEAD, int SUB>
 __global__ __launch_bounds__(64 * kScoreWaves) void k_weigh_wide(WeighArgs a) {
-    constexpr int SUB = kBlock / 16;
+    constexpr int kBlock = 16 * SUB;
     __shared__ v4f red[kScoreWaves][MT * SUB * 64];
     __shared__ float part[MT][kBlock];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -212,13 +212,24 @@ void go_narrow(const WeighArgs& a, dim3 grid, hipStream_t st) {
         hipLaunchKernelGGL((k_weigh_narrow<T, DP, kElem>), grid, dim3(64 * kWaves), 0, st, a);
 }
 
-template <typename T, int MT>
+template <typename T, int MT, int SUB>
 void go_wide(const WeighArgs& a, dim3 grid, hipStream_t st) {
     // (a wave of more than a step of 128 bf16 or 64 fp32 dims)
     if (a.c.D > kScoreWaves * 256 / (int)sizeof(T))
-        hipLaunchKernelGGL((k_weigh_wide<T, MT, true>), grid, dim3(64 * kScoreWaves), 0, st, a);
+        hipLaunchKernelGGL((k_weigh_wide<T, MT, true, SUB>), grid, dim3(64 * kScoreWaves), 0, st, a);
     else
-        hipLaunchKernelGGL((k_weigh_wide<T, MT, false>), grid, dim3(64 * kScoreWaves), 0, st, a);
+        hipLaunchKernelGGL((k_weigh_wide<T, MT, false, SUB>), grid, dim3(64 * kScoreWaves), 0, st, a);
+}
+
+template <typename T, int MT>
+void go_wide(const WeighArgs& a, int keys, int BG, hipStream_t st) {
+    const int blocks = (keys + 31) / 32;
+    // (blocks of 32 keys read Q half as often, blocks of 16 reach more of the card where there are
+    // fewer than two of 32 a CU: fp32, 8192 dims, 1163 rows of 3 kv heads 47 -> 33.5 us)
+    if ((int64_t)blocks * BG < 512)
+        go_wide<T, MT, 1>(a, dim3((unsigned)((keys + 15) / 16), (unsigned)BG), st);
+    else
+        go_wide<T, MT, 2>(a, dim3((unsigned)blocks, (unsigned)BG), st);
 }
 
 template <typename T>
@@ -226,11 +237,10 @@ void go(const WeighArgs& a, hipStream_t st) {
     const int D = a.c.D, BG = a.c.B * a.c.G;
     const int keys = std::min(a.c.cap, a.c.rows + a.p.n);
     if (D > 256) {
-        const dim3 grid((unsigned)((keys + kBlock - 1) / kBlock), (unsigned)BG);
         const int R = a.d.rep * a.p.n;  // at most
-        if (R <= 16) return go_wide<T, 1>(a, grid, st);
-        if (R <= 32) return go_wide<T, 2>(a, grid, st);
-        return go_wide<T, 4>(a, grid, st);
+        if (R <= 16) return go_wide<T, 1>(a, keys, BG, st);
+        if (R <= 32) return go_wide<T, 2>(a, keys, BG, st);
+        return go_wide<T, 4>(a, keys, BG, st);
     }
     const int kb = sizeof(T) == 2 ? 32 : 16;
     const int most = (keys + kb * kWaves - 1) / (kb * kWaves);

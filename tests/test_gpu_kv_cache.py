@@ -138,7 +138,8 @@ def weigh64(Q, K, lse, path, rows, lens, scale):
     (2, 8, 1, 5, 64, [300, 31], dict(order="rows")), (2, 4, 4, 3, 100, [33, 34], dict(offset=1)),
     (1, 32, 4, 6, 96, [257], dict(order="rows", pad=8, offset=8)), (2, 2, 1, 12, 512, [129, 15], {}),
     (1, 4, 2, 2, 1000, [50], dict(pad=3)), (1, 2, 1, 3, 8192, [40], {}), (1, 16, 2, 40, 72, [90], {}),
-    (2, 71, 1, 4, 256, [48, 47], {}), (1, 3, 3, 200, 48, [20], {})])
+    (2, 71, 1, 4, 256, [48, 47], {}), (1, 3, 3, 200, 48, [20], {}),
+    (65, 16, 8, 2, 264, list(range(65)), {}), (33, 36, 9, 10, 260, list(range(40, 73)), {})])
 def test_weights(am, dev, dtype, B, Hq, G, T, D, lens, layout):
     import hip_rt
     print(f"[case] weigh {dtype} {(B, Hq, G, T, D)} {lens} {layout}", flush=True)
@@ -149,7 +150,7 @@ def test_weights(am, dev, dtype, B, Hq, G, T, D, lens, layout):
     counts = [T - (T // 3) * (b % 2) for b in range(B)]
     n = max(1, min(T, 7)) if T < 100 else T
     path = np.stack([np.resize(rng.permutation(k), n) for k in counts])
-    accepted = [n, max(1, n - 2), n][:B]
+    accepted = ([n, max(1, n - 2), n] * B)[:B]
     d = am.Drafts(q.dev, kd.dev, vd.dev, count=C.ints(counts))
     rows = C.accepted_rows(path.tolist(), accepted, counts, lens, cap, n)
     lse = (rng.standard_normal((B, Hq, T)) + np.log(max(lens) + 1)).astype(np.float32)
