@@ -131,7 +131,7 @@ def contiguous_strides(shape) -> tuple:
 class DeviceArray:
     """A device allocation with a shape and an element type ('f32' | 'bf16';
     'i32' for lengths, positions and masks).  `strides` are in elements, None for
-    a contiguous array; only wrap() and strided() make others."""
+    a contiguous array; only wrap() makes others."""
 
     strides = None
 
@@ -179,13 +179,6 @@ class DeviceArray:
         obj._keep = keep
         if strides is not None and tuple(strides) != contiguous_strides(obj.shape):
             obj.strides = tuple(int(s) for s in strides)
-        return obj
-
-    @classmethod
-    def strided(cls, base: "DeviceArray", shape, strides, offset_elems: int = 0) -> "DeviceArray":
-        """Non-owning strided view of an array (kernel arguments only: it has no
-        host copy)."""
-        obj = cls.wrap(base.ptr + offset_elems * base.itemsize, shape, base.dtype, strides, base)
         return obj
 
     @classmethod
