@@ -337,8 +337,8 @@ int atn_device_count(void);
  * status and enqueue on `stream`; calls on one cache belong on one stream (or in
  * an order of the caller's).  Results do not depend on timing: no atomics on
  * floating-point values, every sum in one order.  Elements are
- * head_d-contiguous; head_d <= 8192; rows of K and V at most 128 MiB apart; any
- * alignment to the element size. */
+ * head_d-contiguous; head_d <= 8192; capacity <= 2^30; batch * kv_heads <= 65535;
+ * rows of K and V at most 128 MiB apart; any alignment to the element size. */
 #define ATN_TREE_MAX_TOKENS 256
 #define ATN_CACHE_MAX_HEAD_D 8192
 
