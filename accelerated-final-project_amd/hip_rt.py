@@ -131,7 +131,8 @@ def contiguous_strides(shape) -> tuple:
 class DeviceArray:
     """A device allocation with a shape and an element type ('f32' | 'bf16';
     'i32' for lengths, positions and masks).  `strides` are in elements, None for
-    a contiguous array; only wrap() makes others."""
+    a contiguous array; only wrap() makes others, which name memory to the calls that take
+    strides: upload(), bits(), numpy(), fill_nan() and view() refuse them (ValueError)."""
 
     strides = None
 
@@ -152,6 +153,7 @@ class DeviceArray:
     @classmethod
     def view(cls, base: "DeviceArray", offset_elems: int, shape, dtype=None):
         """Non-owning view at an element offset (for misalignment tests)."""
+        base._contiguous("view")
         obj = cls.__new__(cls)
         obj.shape = tuple(shape)
         obj.dtype = dtype or base.dtype
@@ -196,7 +198,14 @@ class DeviceArray:
         check(hip().hipMemcpy(_vp(d.ptr), host.ctypes.data_as(_vp), d.nbytes, H2D), "H2D")
         return d
 
+    def _contiguous(self, what: str) -> None:
+        """The calls below reach `nbytes` bytes from `ptr` on: a strided array's elements lie
+        elsewhere, and what lies between them is another's."""
+        if self.strides is not None:
+            raise ValueError(f"{what}: not for a strided array")
+
     def upload(self, a: np.ndarray) -> None:
+        self._contiguous("upload")
         host = f32_to_bf16_bits(a) if (self.dtype == "bf16" and a.dtype != np.uint16) else a
         host = np.ascontiguousarray(host, dtype=_HOST_TYPE[self.dtype])
         assert host.nbytes == self.nbytes
@@ -204,7 +213,7 @@ class DeviceArray:
 
     def bits(self) -> np.ndarray:
         """Raw contents: float32 or int32 array, or uint16 bf16 bits."""
-        assert self.strides is None, "a strided view has no host copy"
+        self._contiguous("bits")
         out = np.empty(self.shape, dtype=_HOST_TYPE[self.dtype])
         check(hip().hipMemcpy(out.ctypes.data_as(_vp), _vp(self.ptr), self.nbytes, D2H), "D2H")
         return out
@@ -215,6 +224,7 @@ class DeviceArray:
         return bf16_bits_to_f32(b) if self.dtype == "bf16" else b
 
     def fill_nan(self) -> None:
+        self._contiguous("fill_nan")
         check(hip().hipMemset(_vp(self.ptr), 0xFF, self.nbytes), "hipMemset")
 
     def free(self) -> None:
