@@ -305,7 +305,7 @@ def release() -> None:
 # ---------------------------------------------------------------- array helpers
 # Arguments are hip_rt.DeviceArray objects ([B,H,L,D], 'f32' or 'bf16').
 def _ptr(t):
-    if t is not None and t.strides is not None:
+    if t is not None and getattr(t, "strides", None) is not None:
         raise ValueError("a strided array where a contiguous one is needed")
     return None if t is None else t.ptr
 
@@ -368,7 +368,7 @@ def attention_ex(Q, K, V, out=None, pe: PeDesc | None = None, workspace=None, st
     _check(out, Q.dtype, (B, H, Lq, D), "out")
     ws_ptr, ws_bytes = (None, 0)
     if workspace is not None:
-        ws_ptr, ws_bytes = workspace.ptr, workspace.nbytes
+        ws_ptr, ws_bytes = _ptr(workspace), workspace.nbytes
     st = lib().atn_attention_fwd_ex(_dtype_code(Q), _ptr(Q), _ptr(K), _ptr(V), _ptr(out), B, H,
                                     Lq, Lk, D, ctypes.byref(pe) if pe is not None else None,
                                     ws_ptr, ws_bytes, _stream_handle(stream))
@@ -406,8 +406,7 @@ def path(dtype_code: int, B, H, Lq, Lk, D, pe: PeDesc | None = None) -> int:
 
 def sync_status(workspace=None, B: int = 1, H: int = 1, stream=None) -> int:
     """atn_sync_status_ex: ATN_OK or ATN_ERR_DEVICE_TIMEOUT."""
-    return lib().atn_sync_status_ex(None if workspace is None else workspace.ptr, B, H,
-                                    _stream_handle(stream))
+    return lib().atn_sync_status_ex(_ptr(workspace), B, H, _stream_handle(stream))
 
 
 def workspace_bytes(dtype_code: int, B, H, Lq, Lk, D, pe: PeDesc | None = None) -> int:
@@ -458,8 +457,8 @@ def attention_forward_rope_fused(Q, K, V, out, cos_cache, sin_cache):
     for n, t in (("cos_cache", cos_cache), ("sin_cache", sin_cache)):
         if t.shape[-1] != D or t.size < max(Lq, Lk) * D:
             raise ValueError(f"{n} must be [>= max(len_q, len_k)][head_d]")
-    lib().attention_forward_rope_fused(Q.ptr, K.ptr, V.ptr, out.ptr, cos_cache.ptr, sin_cache.ptr,
-                                       B, H, Lq, Lk, D)
+    lib().attention_forward_rope_fused(Q.ptr, K.ptr, V.ptr, out.ptr, _ptr(cos_cache),
+                                       _ptr(sin_cache), B, H, Lq, Lk, D)
     return out
 
 
@@ -478,7 +477,7 @@ def attention_forward_separate_rope(Q, K, V, Q_rope, K_rope, out, cos_cache, sin
     _check(K_rope, "f32", K.shape, "K_rope")
     _rot_check(rotary_dim, D)
     lib().attention_forward_separate_rope(Q.ptr, K.ptr, V.ptr, Q_rope.ptr, K_rope.ptr, out.ptr,
-                                          cos_cache.ptr, sin_cache.ptr, B, H, Lq, Lk, D,
+                                          _ptr(cos_cache), _ptr(sin_cache), B, H, Lq, Lk, D,
                                           rotary_dim)
     return out
 
@@ -508,8 +507,8 @@ def attention_forward_sinusoidal_fused(Q, K, V, out):
 def attention_forward_sinusoidal_hybrid(Q, K, V, sin_table, cos_table, K_emb, out):
     B, H, Lq, Lk, D = _dropin_check("f32", Q, K, V, out)
     _check(K_emb, "f32", K.shape, "K_emb")
-    lib().attention_forward_sinusoidal_hybrid(Q.ptr, K.ptr, V.ptr, sin_table.ptr, cos_table.ptr,
-                                              K_emb.ptr, out.ptr, B, H, Lq, Lk, D)
+    lib().attention_forward_sinusoidal_hybrid(Q.ptr, K.ptr, V.ptr, _ptr(sin_table),
+                                              _ptr(cos_table), K_emb.ptr, out.ptr, B, H, Lq, Lk, D)
     return out
 
 
@@ -517,8 +516,9 @@ def attention_forward_sinusoidal_separate(Q, K, V, sin_table, cos_table, Q_emb, 
     B, H, Lq, Lk, D = _dropin_check("f32", Q, K, V, out)
     _check(Q_emb, "f32", Q.shape, "Q_emb")
     _check(K_emb, "f32", K.shape, "K_emb")
-    lib().attention_forward_sinusoidal_separate(Q.ptr, K.ptr, V.ptr, sin_table.ptr, cos_table.ptr,
-                                                Q_emb.ptr, K_emb.ptr, out.ptr, B, H, Lq, Lk, D)
+    lib().attention_forward_sinusoidal_separate(Q.ptr, K.ptr, V.ptr, _ptr(sin_table),
+                                                _ptr(cos_table), Q_emb.ptr, K_emb.ptr, out.ptr, B,
+                                                H, Lq, Lk, D)
     return out
 
 

@@ -50,3 +50,35 @@ def test_contiguous_wraps_are_whole(hip_rt):
     b = hip_rt.DeviceArray.view(a, 2, (4,))
     assert (b.ptr, b.nbytes) == (ADDR + 8, 16)
     assert hip_rt.done == [("copy", 24), ("set", 24), ("copy", 24)]
+
+
+def test_calls_without_strides_refuse_strided_tables_and_workspaces(am, monkeypatch):
+    """Encoding tables and workspaces reach the library by address alone: ValueError before any
+    call of it, as for Q, K, V and the output."""
+    import hip_rt
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: pytest.fail(f"{name} was called")
+
+    monkeypatch.setattr(am, "lib", Library)
+
+    def arr(shape, strides=None):
+        return hip_rt.DeviceArray.wrap(ADDR, shape, "f32", strides)
+
+    x, ws = arr((1, 2, 4, 8)), arr((1 << 16,), (2,))
+    whole, table = arr((4, 8)), arr((4, 8), (16, 1))
+    for call in (lambda: am.attention_ex(x, x, x, x, workspace=ws), lambda: am.sync_status(ws),
+                 lambda: am.make_pe("rope", table_a=table), lambda: am.pe_apply_ex(table, x, 4, None),
+                 lambda: am.attention_forward_rope_fused(x, x, x, x, whole, table),
+                 lambda: am.attention_forward_rope_fused(x, x, x, x, table, whole),
+                 lambda: am.attention_forward_separate_rope(x, x, x, x, x, x, whole, table, 8),
+                 lambda: am.attention_forward_separate_rope(x, x, x, x, x, x, table, whole, 8),
+                 lambda: am.rope_forward(x, x, table, whole, 8, 4),
+                 lambda: am.apply_sinusoidal_embeddings(x, whole, table, x, 4),
+                 lambda: am.attention_forward_sinusoidal_hybrid(x, x, x, whole, table, x, x),
+                 lambda: am.attention_forward_sinusoidal_hybrid(x, x, x, table, whole, x, x),
+                 lambda: am.attention_forward_sinusoidal_separate(x, x, x, whole, table, x, x, x),
+                 lambda: am.attention_forward_sinusoidal_separate(x, x, x, table, whole, x, x, x)):
+        with pytest.raises(ValueError):
+            call()
