@@ -179,7 +179,9 @@ class DeviceArray:
         obj.base = obj.ptr = ptr
         obj._owner = False
         obj._keep = keep
-        if strides is not None and tuple(strides) != contiguous_strides(obj.shape):
+        # (a dimension of one element takes no step: any stride is a contiguous array's)
+        if strides is not None and any(n > 1 and s != c for n, s, c in
+                                       zip(obj.shape, strides, contiguous_strides(obj.shape))):
             obj.strides = tuple(int(s) for s in strides)
         return obj
 

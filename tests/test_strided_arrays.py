@@ -82,3 +82,21 @@ def test_calls_without_strides_refuse_strided_tables_and_workspaces(am, monkeypa
                  lambda: am.attention_forward_sinusoidal_separate(x, x, x, table, whole, x, x, x)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_single_elements_take_no_step(am):
+    """A column of a table of lengths of one sequence, one sequence's weights, a single cached row:
+    contiguous, whatever the stride of their dimensions of one element."""
+    import hip_rt
+
+    def arr(shape, dtype, strides):
+        return hip_rt.DeviceArray.wrap(ADDR, shape, dtype, strides)
+
+    lens = arr((1,), "i32", (12,))
+    weight = arr((1, 2, 4), "f32", (999, 4, 1))
+    assert lens.strides is None and weight.strides is None
+    kv = arr((1, 2, 4, 8), "bf16", (0, 32, 8, 1))
+    assert kv.strides is None
+    am.KvCache(kv, kv, lens, seen=lens, weight=weight)
+    assert arr((1, 2, 4, 8), "bf16", (0, 64, 8, 1)).strides == (0, 64, 8, 1)
+    assert arr((2,), "i32", (12,)).strides == (12,)
