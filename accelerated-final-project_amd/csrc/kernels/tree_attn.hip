@@ -176,10 +176,15 @@ __device__ __forceinline__ void store4(uint16_t* to, const float (&x)[4], int le
 }
 
 // ---------------------------------------------------------------- infinities and NaNs
-// A block that is not whole cache rows alone -- the cache's last rows, the drafts -- meets
-// weights of 0: places behind its rows, drafts that a row does not attend.  An infinity or NaN in
-// its V belongs only to the rows that attend it.  The product runs without it; it is added
-// where the results are written.
+// An infinity or NaN in V belongs to the rows that attend its key, whatever their weights, and to
+// no others.  Weights of 0 would spread and lose them: 0 times infinity is NaN.
+//   A block that is not whole cache rows alone -- the cache's last rows, the drafts -- has such
+// weights for places behind its rows and drafts that a row does not attend: the product runs on
+// V without them (clear_not_finite).
+//   Whole blocks are attended by every row, but a weight, or a factor that rescales a tile to a
+// new maximum, may have vanished: the result is NaN then.
+// Where V was cleared or a result is NaN, the values themselves are summed again and written
+// over the results that they belong to (put_not_finite).
 // Whether any lane's V holds an infinity or NaN, which are cleared.  (What finds them is short: a
 // sum of products with 0, which is NaN then.)
 template <typename T, typename V>
@@ -204,43 +209,66 @@ __device__ __forceinline__ bool clear_not_finite(V& v) {
     return true;
 }
 
-// What the infinities and NaNs that clear_not_finite() took out (of the cache's rows from
-// `from` to L, and of n drafts) add to dim d of token tok: every weight is above 0, so whatever
-// it is, theirs is the value itself.
+// The infinities and NaNs of every step-th of the rows [from, to) of a column of V, summed.
 template <typename T>
-__device__ __forceinline__ float not_finite_sum(const TreeArgs& a, int b, int g, int from, int L,
-                                                int n, int tok, int d) {
+__device__ __forceinline__ float not_finite_rows(const T* v, int64_t stride, int from, int to,
+                                                 int step) {
     float sum = 0.f;
-    const T* v = (const T*)a.c.V + b * a.c.vs[0] + g * a.c.vs[1] + d;
-    for (int r = from; r < L; ++r) {
-        const float x = Elem<T>::ld(v + r * a.c.vs[2], 0);
-        if (!(fabsf(x) < INFINITY)) sum += x;
-    }
-    if (!a.d.K) return sum;
-    v = (const T*)a.d.V + b * a.d.vs[0] + g * a.d.vs[1] + d;
-    for (int j = 0; j < n; ++j) {
-        const float x = Elem<T>::ld(v + j * a.d.vs[2], 0);
-        if (!(fabsf(x) < INFINITY) && sees(a.d, b, tok, j)) sum += x;
+#pragma unroll 4
+    for (int r = from; r < to; r += step) {
+        const float x = Elem<T>::ld(v + r * stride, 0);
+        sum += fabsf(x) < INFINITY ? 0.f : x;
     }
     return sum;
 }
 
-// not_finite_sum() added to dims [d0, d1) of a row where its result lies (a wave's work, after
-// the wave has written it): the output, or a part.
-template <typename T>
-__device__ void add_not_finite(const TreeArgs& a, const Span& s, int row, int from, int L, int n,
-                               int d0, int d1, int lane) {
+// Those of a span's V written to dims [d0, d1) of a row's result, the output or a part (a wave's
+// work, after the results are written).  whole: of dim d, those of the whole blocks, which every
+// row attends; the cache's rows from `tail` on and the drafts come to it (all of them: the ranges
+// that a pair is cut into may add them more than once, which changes no such sum).  z: the row's
+// maximum and sums.
+template <typename T, typename F>
+__device__ __forceinline__ void put_row(const TreeArgs& a, const Span& s, int row, float4 z, int tail,
+                                        int L, int n, int d0, int d1, int lane, F whole) {
     const int rep = a.d.rep, h = head_of(a.d, row), tok = row - h * a.d.T;
     if (row >= rep * a.d.T || tok >= n) return;
+    // (a NaN score: no number in any dim; no score above -infinity: zeros, which is known here
+    // where no range cut the pair)
+    if (z.y != z.y || (s.part < 0 && z.z == 0.f)) return;
     T* out = (T*)a.out + s.b * a.os[0] + (s.g * rep + h) * a.os[1] + tok * a.os[2];
+    const T* vc = (const T*)a.c.V + s.b * a.c.vs[0] + s.g * a.c.vs[1];
+    const T* vd = (const T*)a.d.V + s.b * a.d.vs[0] + s.g * a.d.vs[1];
     for (int d = d0 + lane; d < d1; d += 64) {
-        const float x = not_finite_sum<T>(a, s.b, s.g, from, L, n, tok, d);
-        if (x == 0.f) continue;
+        float sum = whole(d) + not_finite_rows(vc + d, a.c.vs[2], tail, L, 1);
+        for (int j = 0; a.d.K && j < n; ++j) {
+            const float x = Elem<T>::ld(vd + j * a.d.vs[2], d);
+            if (!(fabsf(x) < INFINITY) && sees(a.d, s.b, tok, j)) sum += x;
+        }
+        if (fabsf(sum) < INFINITY) continue;
         if (s.part >= 0)
-            part_dims(a)[part_row(a, s.part, row) * a.c.D + d] += x;
+            part_dims(a)[part_row(a, s.part, row) * a.c.D + d] = sum;
         else
-            Elem<T>::st(out, d, Elem<T>::ld(out, d) + x);
+            Elem<T>::st(out, d, sum);
     }
+}
+
+// ... of a workgroup's tile of ROWS rows of at most 256 dims.  sums: WAVES * 256 floats of LDS.
+template <typename T, int ROWS, int WAVES, int KB>
+__device__ void put_not_finite(const TreeArgs& a, const Span& s, int tile, const float4* fin,
+                               float* sums, int L, int n, int wave, int lane) {
+    const int D = a.c.D, whole = L / KB;
+    const T* v = (const T*)a.c.V + s.b * a.c.vs[0] + s.g * a.c.vs[1];
+    for (int d = lane; d < D; d += 64)
+        sums[wave * 256 + d] = not_finite_rows(v + d, a.c.vs[2], s.first * KB + wave,
+                                               min(s.last, whole) * KB, WAVES);
+    __syncthreads();
+    auto of_blocks = [&](int d) {
+        float sum = 0.f;
+        for (int w = 0; w < WAVES; ++w) sum += sums[w * 256 + d];
+        return sum;
+    };
+    for (int r = wave; r < ROWS; r += WAVES)
+        put_row<T>(a, s, tile * ROWS + r, fin[r], whole * KB, L, n, 0, D, lane, of_blocks);
 }
 
 // ---------------------------------------------------------------- steps of a block
@@ -301,11 +329,13 @@ __device__ __forceinline__ void weights(float (&p)[MT][SUB][4], v4f (&o)[MT][VS]
 }
 
 // The results of `parts` waves a row, scaled alike, in LDS (rows of LDO floats), summed and
-// written: to the output, or the span's part.  fin: the rows' maxima and sums.
+// written: to the output, or the span's part.  fin: the rows' maxima and sums.  Returns whether
+// a result of this thread is NaN where the row's scores are not.
 template <typename T, int DP, int ROWS, int PARTS, int LDO, int VL, int MODE, int THREADS>
-__device__ __forceinline__ void write_rows(const TreeArgs& a, const Span& sp, int tile, int n,
+__device__ __forceinline__ bool write_rows(const TreeArgs& a, const Span& sp, int tile, int n,
                                            const float* xo, const float4* fin) {
     const int D = MODE == kExact ? DP : a.c.D, rep = a.d.rep, R = rep * a.d.T;
+    bool nan = false;
     // (opaque: or what this computes is hoisted out of the loop over spans, into registers; not
     // unrolled: twice the code, fetched once a launch, takes longer than the loop)
 #pragma unroll 1
@@ -330,22 +360,25 @@ __device__ __forceinline__ void write_rows(const TreeArgs& a, const Span& sp, in
             }
         }
         if (row >= R || tok >= n || d >= D) continue;
+        nan |= (z.y == z.y) &
+               (__builtin_isunordered(x[0], x[1]) | __builtin_isunordered(x[2], x[3]));
         if (sp.part >= 0) {
             const size_t to = part_row(a, sp.part, row);
             if (d == 0) part_stats(a)[to] = z;
             store4(part_dims(a) + to * D + d, x, MODE == kExact ? 4 : D - d);
         } else {
             // (0: nothing visible, or no score above -infinity)
-            const float inv = z.z == 0.f ? 0.f : 1.f / z.z;
+            const float inv = 1.f / z.z;
             if (d == 0 && a.lse)
                 a.lse[((size_t)sp.b * a.d.H + sp.g * rep + h) * a.d.T + tok] =
                     z.y == 0.f ? -INFINITY : (z.x + log2f(z.y)) * kLn2;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) x[c] *= inv;
+            for (int c = 0; c < 4; ++c) x[c] = z.z == 0.f ? 0.f : x[c] * inv;
             store4((T*)a.out + sp.b * a.os[0] + (sp.g * rep + h) * a.os[1] + tok * a.os[2] + d, x,
                    MODE == kExact ? 4 : D - d);
         }
     }
+    return nan;
 }
 
 // ---------------------------------------------------------------- head_d <= 256
@@ -376,6 +409,7 @@ struct Narrow : CacheTiles<T, DP, MT, MODE> {
     static constexpr int kLds = kOut + (WAVES + 1) * N::ROWS * 16;
     static constexpr int kQ = (MT * N::KS * 64 + 64 * WAVES - 1) / (64 * WAVES);  // pieces a thread
     static_assert(kLds <= 160 * 1024, "LDS");
+    static_assert(kXBytes >= WAVES * 256 * 4, "put_not_finite's sums");
 };
 
 template <typename T, int DP, int MT, int MODE, int WAVES>
@@ -572,12 +606,11 @@ k_tree_narrow(TreeArgs a) {
                                         o[t][x][c + 2][e] * f, o[t][x][c + 3][e] * f);
         }
         __syncthreads();
-        write_rows<T, DP, N::ROWS, WAVES, N::LDO, VL, MODE, 64 * WAVES>(a, sp, tile, n, xo, fin);
-        if (__syncthreads_or(odd)) {
-            // (behind the barrier, which waits for the workgroup's stores)
-            for (int r = wave; r < N::ROWS; r += WAVES)
-                add_not_finite<T>(a, sp, tile * N::ROWS + r, whole * KB, L, n, 0, D, lane);
-        }
+        odd |= write_rows<T, DP, N::ROWS, WAVES, N::LDO, VL, MODE, 64 * WAVES>(a, sp, tile, n, xo,
+                                                                               fin);
+        // (behind the barrier, which waits for the workgroup's stores and reads of xo)
+        if (__syncthreads_or(odd))
+            put_not_finite<T, N::ROWS, WAVES, KB>(a, sp, tile, fin, xo, L, n, wave, lane);
     }
 }
 
@@ -611,6 +644,7 @@ struct Shared : CacheTiles<uint16_t, 128, 2, MODE> {
     static constexpr int kOut = 2 * kStage > kXBytes ? 2 * kStage : kXBytes;
     static constexpr int kLds = kOut + (KG + 1) * ROWS_WG * 16;
     static_assert(kLds <= 160 * 1024, "LDS");
+    static_assert(kXBytes >= 8 * 256 * 4, "put_not_finite's sums");
 };
 
 template <int RG, int MODE>
@@ -837,11 +871,9 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
                 *reinterpret_cast<v4f*>(to + 16 * c) = o[t][0][c] * f;
         }
         __syncthreads();
-        write_rows<T, DP, N::ROWS_WG, KG, N::LDO, VL, MODE, 512>(a, sp, tile, n, xo, fin);
-        if (__syncthreads_or(odd)) {
-            for (int r = wave; r < N::ROWS_WG; r += 8)
-                add_not_finite<T>(a, sp, tile * N::ROWS_WG + r, whole * KB, L, n, 0, D, lane);
-        }
+        odd |= write_rows<T, DP, N::ROWS_WG, KG, N::LDO, VL, MODE, 512>(a, sp, tile, n, xo, fin);
+        if (__syncthreads_or(odd))
+            put_not_finite<T, N::ROWS_WG, 8, KB>(a, sp, tile, fin, xo, L, n, wave, lane);
     }
 }
 
@@ -1105,9 +1137,11 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
             const float4 z = fin[16 * t + lc];
             const bool teller = lq == 0 && d0 == 0;
             const size_t part = part_row(a, max(sp.part, 0), row);
-            const float inv = sp.part >= 0 ? 1.f : z.z == 0.f ? 0.f : 1.f / z.z;
+            const bool zero = sp.part < 0 && z.z == 0.f;
+            const float inv = sp.part >= 0 ? 1.f : 1.f / z.z;
             float* dims = part_dims(a) + part * D + d0;
             T* to = (T*)a.out + b * a.os[0] + (g * rep + h) * a.os[1] + tok * a.os[2] + d0;
+            bool nan = false;
             if (teller && sp.part >= 0) part_stats(a)[part] = z;
             if (teller && sp.part < 0 && a.lse)
                 a.lse[((size_t)b * a.d.H + g * rep + h) * a.d.T + tok] =
@@ -1117,8 +1151,10 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
                 const int d = N::dim_of(0, 4 * lq + e, D - d0);
 #pragma unroll
                 for (int c = 0; c < VL; c += 4) {
-                    const float y[4] = {o[t][0][c][e] * inv, o[t][0][c + 1][e] * inv,
-                                        o[t][0][c + 2][e] * inv, o[t][0][c + 3][e] * inv};
+                    float y[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = zero ? 0.f : o[t][0][c + r][e] * inv;
+                    nan |= __builtin_isunordered(y[0], y[1]) | __builtin_isunordered(y[2], y[3]);
                     if (d + c >= 0) {
                         if (sp.part >= 0)
                             store4(dims + d + c, y, 4);
@@ -1136,12 +1172,21 @@ __global__ __launch_bounds__(64 * kWaves, MT == 1 ? 3 : 2) void k_tree_values(Tr
                     }
                 }
             }
+            odd |= nan & (z.y == z.y);
         }
-        if (odd) {
+        if (__builtin_amdgcn_ballot_w64(odd)) {
             __threadfence_block();  // (this wave's own stores, from other lanes)
+            const int tail = L / PK * PK, d1 = min(D, d0 + WD);
+            float whole[WD / 64];  // of dims d0 + lane and on
+#pragma unroll
+            for (int x = 0; x < WD / 64; ++x) {
+                const int d = min(64 * x + late, d1 - d0 - 1);
+                whole[x] = not_finite_rows(vc + d, a.c.vs[2], sp.first * kBlock,
+                                           min(sp.last * kBlock, tail), 1);
+            }
             for (int r = 0; r < ROWS; ++r)
-                add_not_finite<T>(a, sp, tile * ROWS + r, L / PK * PK, L, n, d0, min(D, d0 + WD),
-                                  late);
+                put_row<T>(a, sp, tile * ROWS + r, fin[r], tail, L, n, d0, d1, late,
+                           [&](int d) { return whole[WD == 64 || d < d0 + 64 ? 0 : 1]; });
         }
     }
 }
@@ -1190,7 +1235,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a) {
         for (int c = 0; c < 4; ++c) {
             const int d = lane + 64 * c;
             const float y = d0 + d < D ? from[d] : 0.f;
-            // (infinity times a weight too small for fp32 stays infinity)
+            // (what is not finite stays so where the factor has vanished)
             x[c] += f == 0.f && !(fabsf(y) < INFINITY) ? y : f * y;
         }
     }
@@ -1203,14 +1248,14 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a) {
         l = (sums[0].x + sums[1].x) + (sums[2].x + sums[3].x);
         used = (sums[0].y + sums[1].y) + (sums[2].y + sums[3].y);
         const int d = threadIdx.x;
-        const float inv = used == 0.f ? 0.f : 1.f / used;
-        if (d0 + d < D)
-            Elem<T>::st(out, d, ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv);
+        const float sum = (acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d]);
+        if (d0 + d < D) Elem<T>::st(out, d, used == 0.f ? 0.f : sum * (1.f / used));
     } else {
-        const float inv = used == 0.f ? 0.f : 1.f / used;
+        const float inv = 1.f / used;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-            if (d0 + lane + 64 * c < D) Elem<T>::st(out, lane + 64 * c, x[c] * inv);
+            if (d0 + lane + 64 * c < D)
+                Elem<T>::st(out, lane + 64 * c, used == 0.f ? 0.f : x[c] * inv);
     }
     if (d0 == 0 && (WAVES == 4 ? threadIdx.x : lane) == 0 && a.lse)
         a.lse[((size_t)b * a.d.H + g * rep + h) * a.d.T + tok] =

@@ -378,7 +378,8 @@ typedef struct atn_drafts {
  * (or only scores of -infinity) gets zeros.  lse (may be NULL): [batch][heads]
  * [tokens] fp32, the natural log of the softmax's denominator (-infinity for such a
  * token).  Keys and values that a token does not attend do not reach its output,
- * whatever they hold.  out_stride: as atn_drafts.q_stride, of distinct elements;
+ * whatever they hold; an infinity or NaN in a value that it attends reaches that dim of
+ * its output whatever its weight (opposite infinities: NaN).  out_stride: as atn_drafts.q_stride, of distinct elements;
  * NULL: contiguous.  max_len: an upper bound of len that the host knows (0: the
  * capacity); the call is laid out for it, and rows from there on are not attended.
  * workspace as for atn_attention_fwd_ex (NULL: the stream's library
