@@ -5,8 +5,8 @@
 // scores as in tree_attn.hip; V is not read.  One pass over K: the query rows
 // are few (heads times path), the sum over them ends in a row of 16 lanes, and a
 // row's weight has one writer and one order of sums.  The read of K bounds it: 8 sequences of 1000
-// to 8191 rows, 8 kv heads of 128 bf16 dims 17.0 us, 4.5 TB/s; fp32, 512 dims, 2 of 2000 to 4091
-// rows, 4 kv heads 14.2 us, 3.5 TB/s.
+// to 8191 rows, 8 kv heads of 128 bf16 dims 17.2 to 18.5 us, 4.2 to 4.5 TB/s; fp32, 512 dims, 2 of
+// 2000 to 4091 rows, 4 kv heads 14.2 us, 3.5 TB/s.
 #include <algorithm>
 
 #include "cache_tiles.hpp"

@@ -33,7 +33,9 @@ __device__ __forceinline__ int blocks_of(const TreeArgs& a, int b, int kb) {
 
 // A pair takes as many places of the line as it has blocks, and kPad before them: beginning and
 // ending a pair costs a workgroup about as much time as so many blocks, so ranges of many short
-// pairs have fewer blocks (8 sequences of 1000 to 8176 rows: 46.2 us with 16, 47.4 with 8).
+// pairs have fewer blocks (8 sequences of 1000 to 8176 rows of 128 bf16 dims: 46.2 us with 16, 47.4
+// with 8).  Few pairs of few blocks, as wide heads have them, are left with ranges of padding
+// alone: 5 of 25 for 4 pairs of 33 blocks.
 constexpr int kPad = 16;
 
 // The line: its length, and the places of a range (whole turns of `turn`, a power of two).  A wave's work, as
@@ -385,12 +387,13 @@ __device__ __forceinline__ bool write_rows(const TreeArgs& a, const Span& sp, in
 // Every wave walks its own blocks of keys, alone: scores, running maximum and
 // sum, and its own output tile in registers (cache_tiles.hpp); nothing passes through LDS
 // but Q and, at the end, the waves' results.  A launch starts with a cold instruction
-// cache, about 60 ns a 64-byte line, so what runs once is kept short: one loop for whole
-// and other blocks, results added up in a loop.
+// cache, so what runs once is kept short: one loop for whole and other blocks, results added up
+// in a loop (one token over 300 rows: 9.5 us with 20.6 KB of code, 9.0 with 13.8, 7.1 with 9.2).
 //   One token, 8 heads of 128 bf16 dims over 300 rows (8 waves, whole pairs): 7.1 us, most of it
-//     the code's fetch and the chain length -> K -> V -> results; 10.5 with 20 KB of code for 9.
+//     the code's fetch and the chain length -> K -> V -> results.
 //   64 query rows, 8 kv heads, 8 sequences of 1000 to 8176 rows of 128 bf16 dims: 46 us, 3.3 TB/s
-//     of K and V where reading alone reaches 3.9 (and 8 us of merge).
+//     of K and V (and 8 us of merge).  One token of 32 heads over 131000 rows, where the lengths
+//     are alike and the products few, reads 4.9 TB/s.
 //   fp32, 21 query rows, 80 dims, 3 sequences of 777 to 1991 rows: 15 us, latency.
 template <typename T, int DP, int MT, int MODE, int WAVES>
 struct Narrow : CacheTiles<T, DP, MT, MODE> {
@@ -623,8 +626,8 @@ k_tree_narrow(TreeArgs a) {
 // k_tree_narrow's lanes load them for themselves; V in rows, from which gfx950's transposing read
 // takes the operands of V^T (pairing them by permutes, as k_tree_narrow does, took 40 % of the
 // time here, once for every wave).  256 query rows, 8 kv heads, 4 sequences of 32000 to 32704 rows
-// of 128 dims: 193 us with the merge, 645 TFLOP/s; a library product of two matrices reaches 1240.
-// Without the exponentials 15 us less, without the loads 40.  33 to 64 rows in this form (2 by 4
+// of 128 dims: 192 to 205 us with the merge, 610 to 650 TFLOP/s; a library product of two matrices
+// reaches 1240.  Without the exponentials 15 us less, without the loads 40.  33 to 64 rows in this form (2 by 4
 // waves): 50.5 us against k_tree_narrow's 46.
 template <int RG, int MODE>
 struct Shared : CacheTiles<uint16_t, 128, 2, MODE> {
@@ -883,9 +886,10 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs a) {
 // workgroup's 8 waves sharing a tile's dims, or its share of them, and adding up through LDS;
 // k_tree_values is the softmax over them and the product with V, each wave 16 VL dims of the
 // output.  Keys lie in blocks of 32: the cache's, then the drafts'.
-//   fp32, 8 query rows of 2048 dims, 2 sequences of 1000 to 2040 rows, 4 kv heads: 26.5 and 24.5 us,
-//     3.8 and 4.1 TB/s, what reading alone reaches.
-//   bf16, 10 query rows of 8192 dims, 1001 rows, 4 kv heads: 17.3 and 21.2 us, 3.8 and 3.1 TB/s.
+//   fp32, 8 query rows of 2048 dims, 2 sequences of 1000 to 2040 rows, 4 kv heads: 27 and 24.5 us,
+//     3.7 and 4.1 TB/s.
+//   bf16, 10 query rows of 8192 dims, 1001 rows, 4 kv heads: 17 and 21.2 us, 3.8 and 3.1 TB/s; V by
+//     400 workgroups of 25 ranges, 5 of which hold no keys.
 //   A workgroup of scores that walks several blocks with Q in registers: no less time (fp32, 408
 //     dims, 44 rows: 40 against 36 us).
 constexpr int kBlock = 32;
