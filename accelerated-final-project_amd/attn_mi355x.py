@@ -110,6 +110,40 @@ class _DraftsDesc(ctypes.Structure):
                 ("heads", ctypes.c_int), ("tokens", ctypes.c_int)]
 
 
+class _PagedCacheDesc(ctypes.Structure):
+    """atn_paged_cache."""
+    _fields_ = [("K", ctypes.c_void_p), ("V", ctypes.c_void_p),
+                ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+                ("table", ctypes.c_void_p), ("len", ctypes.c_void_p),
+                ("dtype", ctypes.c_int), ("batch", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("pages", ctypes.c_int), ("page_rows", ctypes.c_int),
+                ("table_pages", ctypes.c_int), ("head_d", ctypes.c_int)]
+
+
+class _RotaryDesc(ctypes.Structure):
+    """atn_rotary."""
+    _fields_ = [("pairing", ctypes.c_int), ("rotary_dim", ctypes.c_int),
+                ("freq", ctypes.c_void_p), ("amplitude", ctypes.c_float)]
+
+
+class _RotatedDesc(ctypes.Structure):
+    """atn_rotated."""
+    _fields_ = [("inp", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("in_stride", ctypes.c_int64 * 3), ("out_stride", ctypes.c_int64 * 3),
+                ("heads", ctypes.c_int)]
+
+
+class _SharedPrefixDesc(ctypes.Structure):
+    """atn_shared_prefix."""
+    _fields_ = [("first", ctypes.c_void_p), ("rows", ctypes.c_void_p), ("groups", ctypes.c_int)]
+
+
+class _RopeScaling(ctypes.Structure):
+    """atn_rope_scaling."""
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_double), ("original", ctypes.c_int),
+                ("low", ctypes.c_double), ("high", ctypes.c_double)]
+
+
 class AtnError(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -157,6 +191,13 @@ _SIGS = {
     "atn_cache_evict_ex": ([_vp, _i, _i, _vp, ctypes.c_size_t, _vp], _i),
     "atn_cache_evict_workspace_bytes": ([_vp, _i], ctypes.c_size_t),
     "atn_cache_advance_ex": ([_vp, _vp, _vp, _vp, _i, _i, _vp], _i),
+    "atn_rope_frequencies": ([_vp, _i, ctypes.c_double, _vp, _vp], _i),
+    "atn_rotary_ex": ([_i, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp], _i),
+    "atn_paged_append_ex": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp], _i),
+    "atn_paged_attention_ex": ([_vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp, ctypes.c_size_t, _vp],
+                               _i),
+    "atn_paged_attention_workspace_bytes": ([_vp, _vp, _vp, _i], ctypes.c_size_t),
+    "atn_paged_advance_ex": ([_vp, _vp, _vp], _i),
     "atn_rerun_count": ([_i], ctypes.c_long),
     "atn_retained_bytes_ex": ([], ctypes.c_size_t),
     "atn_release_ex": ([], _i),
@@ -759,6 +800,172 @@ def cache_advance_call(cache: KvCache, drafts: Drafts | None = None, path=None, 
 def cache_advance_ex(cache, drafts=None, path=None, accepted=None, limit=0, stream=None):
     """atn_cache_advance_ex: the lengths take in the committed rows, then come down to `limit`."""
     return cache_advance_call(cache, drafts, path, accepted, limit)(stream)
+
+
+# ---------------------------------------------------------------- serving from a paged cache
+ATN_PAGED_MAX_TOKENS = 65536
+_ROPE_SCALE = {None: 0, "linear": 1, "base": 2, "parts": 3}
+_PAIRING = {"interleaved": ATN_ROPE_INTERLEAVED, "half": ATN_ROPE_HALF}
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None,
+                     factor: float = 1.0, original: int = 0, low: float = 0.0, high: float = 0.0):
+    """atn_rope_frequencies: (radians a position, float32 numpy [rotary_dim / 2]; amplitude).
+    scaling: None, "linear", "base" or "parts"."""
+    import numpy as np
+    f = np.zeros(max(rotary_dim, 0) // 2, dtype=np.float32)
+    s = _RopeScaling(_ROPE_SCALE[scaling], factor, original, low, high)
+    amplitude = ctypes.c_float(0)
+    st = lib().atn_rope_frequencies(f.ctypes.data, rotary_dim, base, ctypes.addressof(s),
+                                    ctypes.addressof(amplitude))
+    if st != ATN_OK:
+        raise AtnError(st, "atn_rope_frequencies")
+    return f, amplitude.value
+
+
+class Rotary:
+    """Rotation by position (atn_rotary): freq [rotary_dim / 2] fp32 on the device, pairing
+    "interleaved" or "half", rotary_dim 0: two dims a frequency."""
+
+    def __init__(self, freq, pairing: str = "interleaved", rotary_dim: int = 0, amplitude: float = 1.0):
+        if len(freq.shape) != 1:
+            raise ValueError("freq must be [rotary_dim / 2]")
+        rotary_dim = rotary_dim or 2 * freq.shape[0]
+        _check(freq, "f32", (rotary_dim // 2,), "freq")
+        self.freq, self.rotary_dim = freq, rotary_dim
+        self.desc = _RotaryDesc(_PAIRING[pairing], rotary_dim, _ptr(freq), amplitude)
+
+
+def rotary_call(rotary: Rotary, tensors, pos=None, inverse: bool = False) -> Call:
+    """atn_rotary_ex bound to its arguments.  tensors: up to three (x, out) of [B][heads][T][D]
+    arrays, out may be x; pos [B][T]."""
+    x0 = tensors[0][0]
+    if len(x0.shape) != 4 or len(tensors) > 3:
+        raise ValueError("tensors: one to three pairs of [batch][heads][tokens][head_d] arrays")
+    B, _, T, D = x0.shape
+    descs = (_RotatedDesc * len(tensors))()
+    for i, (x, out) in enumerate(tensors):
+        _check(x, x0.dtype, (B, x.shape[1], T, D), f"x{i}", strided=True)
+        _check(out, x0.dtype, x.shape, f"out{i}", strided=True)
+        descs[i] = _RotatedDesc(x.ptr, out.ptr, _strides(x, f"x{i}"), _strides(out, f"out{i}"),
+                                x.shape[1])
+    if pos is not None:
+        _check(pos, "i32", (B, T), "pos")
+    outs = tuple(out for _, out in tensors)
+    args = (_dtype_code(x0), _ref(rotary.desc), ctypes.cast(descs, _vp), len(tensors), B, T, D,
+            _ptr(pos), int(inverse))
+    return Call("atn_rotary_ex", args, outs, (rotary, tuple(tensors), descs, pos))
+
+
+def rotary_ex(rotary, tensors, pos=None, inverse=False, stream=None):
+    """atn_rotary_ex: each x turned by its tokens' positions into its out (inverse: the gradient)."""
+    return rotary_call(rotary, tensors, pos, inverse)(stream)
+
+
+class PagedCache:
+    """A paged key/value cache (atn_paged_cache): K and V [pages][kv heads][page rows][D], `table`
+    [B][pages of a sequence], `length` [B] rows in use.  Holds the arrays it is made of."""
+
+    def __init__(self, K, V, table, length):
+        if len(K.shape) != 4:
+            raise ValueError("K must be [pages][kv heads][page rows][head_d]")
+        _check(K, K.dtype, K.shape, "K", strided=True)
+        _check(V, K.dtype, K.shape, "V", strided=True)
+        if len(table.shape) != 2:
+            raise ValueError("table must be [batch][pages of a sequence]")
+        _check(table, "i32", table.shape, "table")
+        B, slots = table.shape
+        _check(length, "i32", (B,), "length")
+        pages, G, rows, D = K.shape
+        self.K, self.V, self.table, self.length = K, V, table, length
+        self.dtype, self.batch, self.kv_heads, self.head_d = K.dtype, B, G, D
+        self.desc = _PagedCacheDesc(K.ptr, V.ptr, _strides(K, "K"), _strides(V, "V"), _ptr(table),
+                                    _ptr(length), _dtype_code(K), B, G, pages, rows, slots, D)
+
+    def check(self, drafts: Drafts) -> None:
+        if drafts.dtype != self.dtype or drafts.shape[0] != self.batch or \
+                drafts.shape[3] != self.head_d:
+            raise ValueError(f"tokens {drafts.dtype} {drafts.shape} do not fit a cache {self.dtype} of "
+                             f"{self.batch} sequences, head_d {self.head_d}")
+        if drafts.shape[1] % self.kv_heads:
+            raise ValueError("heads must be a multiple of the cache's kv heads")
+        if drafts.K is not None and drafts.K.shape[1] != self.kv_heads:
+            raise ValueError(f"K must have the cache's {self.kv_heads} kv heads")
+
+
+class SharedPrefix:
+    """Groups of sequences that begin with the same rows (atn_shared_prefix): `first` [groups + 1],
+    `rows` [groups]."""
+
+    def __init__(self, first, rows):
+        if len(rows.shape) != 1:
+            raise ValueError("rows must be [groups]")
+        _check(rows, "i32", rows.shape, "rows")
+        _check(first, "i32", (rows.shape[0] + 1,), "first")
+        self.first, self.rows = first, rows
+        self.desc = _SharedPrefixDesc(_ptr(first), _ptr(rows), rows.shape[0])
+
+
+def paged_append_call(cache: PagedCache, drafts: Drafts, rotary: Rotary | None = None, pos=None,
+                      q_out=None) -> Call:
+    """atn_paged_append_ex bound to its arguments; calling it returns q_out."""
+    cache.check(drafts)
+    B, H, T, D = drafts.shape
+    strides = None
+    if q_out is not None:
+        _check(q_out, drafts.dtype, drafts.shape, "q_out", strided=True)
+        strides = _strides(q_out, "q_out")
+    if pos is not None:
+        _check(pos, "i32", (B, T), "pos")
+    args = (_ref(cache.desc), _ref(drafts.desc), None if rotary is None else _ref(rotary.desc),
+            _ptr(pos), None if q_out is None else q_out.ptr,
+            None if strides is None else ctypes.cast(strides, _vp))
+    return Call("atn_paged_append_ex", args, q_out, (cache, drafts, rotary, pos, strides))
+
+
+def paged_append_ex(cache, drafts, rotary=None, pos=None, q_out=None, stream=None):
+    """atn_paged_append_ex: the tokens' keys and values become rows of the cache (lengths stay)."""
+    return paged_append_call(cache, drafts, rotary, pos, q_out)(stream)
+
+
+def paged_attention_workspace_bytes(cache: PagedCache, drafts: Drafts,
+                                    prefix: SharedPrefix | None = None, max_len: int = 0) -> int:
+    return lib().atn_paged_attention_workspace_bytes(
+        _ref(cache.desc), _ref(drafts.desc), None if prefix is None else _ref(prefix.desc), max_len)
+
+
+def paged_attention_call(cache: PagedCache, drafts: Drafts, out=None, lse=None,
+                         prefix: SharedPrefix | None = None, scale: float = 0.0, max_len: int = 0,
+                         workspace=None) -> Call:
+    """atn_paged_attention_ex bound to its arguments; calling it returns out [B][heads][T][D]."""
+    from hip_rt import DeviceArray
+    cache.check(drafts)
+    if out is None:
+        out = DeviceArray(drafts.shape, drafts.dtype)
+    _check(out, drafts.dtype, drafts.shape, "out", strided=True)
+    if lse is not None:
+        _check(lse, "f32", drafts.shape[:3], "lse")
+    strides = _strides(out, "out")
+    args = (_ref(cache.desc), _ref(drafts.desc), None if prefix is None else _ref(prefix.desc),
+            out.ptr, ctypes.cast(strides, _vp), _ptr(lse), scale, max_len, _ptr(workspace),
+            workspace.nbytes if workspace is not None else 0)
+    return Call("atn_paged_attention_ex", args, out, (cache, drafts, prefix, lse, strides, workspace))
+
+
+def paged_attention_ex(cache, drafts, out=None, lse=None, prefix=None, scale=0.0, max_len=0,
+                       workspace=None, stream=None):
+    """atn_paged_attention_ex; asynchronous on `stream`.  Raises AtnError."""
+    return paged_attention_call(cache, drafts, out, lse, prefix, scale, max_len, workspace)(stream)
+
+
+def paged_advance_call(cache: PagedCache, drafts: Drafts) -> Call:
+    cache.check(drafts)
+    return Call("atn_paged_advance_ex", (_ref(cache.desc), _ref(drafts.desc)), cache, (cache, drafts))
+
+
+def paged_advance_ex(cache, drafts, stream=None):
+    """atn_paged_advance_ex: the lengths take in the appended rows."""
+    return paged_advance_call(cache, drafts)(stream)
 
 
 def precompute_rope_cache(max_seq_len: int, rotary_dim: int, base: float = 10000.0):

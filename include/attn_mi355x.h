@@ -432,6 +432,125 @@ int atn_cache_advance_ex(const atn_kv_cache *cache, const atn_drafts *drafts,
                          const int32_t *path, const int32_t *accepted, int path_len, int limit,
                          void *stream);
 
+/* ==================== serving from a paged key/value cache ====================
+ * No counterpart in the reference.  The rows of a sequence lie in pages of a pool that all
+ * sequences share: row r is row r % page_rows of the page table[b][r / page_rows].  A step is
+ *     atn_paged_append_ex       the new tokens' keys (rotated by their positions) and values
+ *                               become rows, their queries are rotated (every layer's cache)
+ *     atn_paged_attention_ex    the new tokens over the rows up to their own (every layer's)
+ *     atn_paged_advance_ex      the lengths move on, once.
+ * A prompt enters the same way, in one step or in several.  The host hands out pages (and
+ * writes the tables) beforehand.  Sequences may share pages: whole ones that they begin with, say,
+ * of which attention then reads the rows once for all of them (atn_shared_prefix).  Rows that a
+ * call writes must be of one sequence alone.
+ *
+ * New tokens are atn_drafts with mask NULL and tokens <= ATN_PAGED_MAX_TOKENS: token t of sequence b,
+ * t < count[b], is row len[b] + t.
+ *
+ * Lengths, tables, counts and prefixes are device memory, read when the kernels run.  len is
+ * clamped to the rows of the table; a table entry that names no page has no rows: they are neither
+ * attended nor written.  Calls validate their arguments before any HIP call, return an ATN_* status
+ * and enqueue on `stream`.  Results do not depend on timing.  head_d <= 8192; table_pages * page_rows
+ * <= 2^30; batch * kv_heads <= 65535; batch * tokens < 2^23; rows of K and V at most 128 MiB apart;
+ * any alignment to the element size. */
+#define ATN_PAGED_MAX_TOKENS 65536
+
+/* A paged cache.  Strides in elements for page, kv head and row; all three 0: contiguous
+ * [pages][kv_heads][page_rows][head_d]. */
+typedef struct atn_paged_cache {
+    void *K, *V;
+    int64_t k_stride[3], v_stride[3];
+    const int32_t *table; /* [batch][table_pages] */
+    int32_t *len;         /* [batch] rows in use before the new tokens */
+    int dtype;            /* ATN_DTYPE_* of the cache, the tokens and the output */
+    int batch, kv_heads, pages, page_rows, table_pages, head_d;
+} atn_paged_cache;
+
+/* Rotation by position: pair i of a token at position p turns by p * freq[i] (the exact product,
+ * reduced in fp64: positions far into a context lose nothing), its cosine and sine times amplitude. */
+typedef struct atn_rotary {
+    int pairing;       /* ATN_ROPE_* */
+    int rotary_dim;    /* rotated width (even, <= head_d); 0 = head_d */
+    const float *freq; /* [rotary_dim / 2] radians per position (atn_rope_frequencies), device */
+    float amplitude;   /* 0 = 1 */
+} atn_rotary;
+
+/* Frequencies base^(-2i / rotary_dim), as they are or stretched for contexts `factor` times as long
+ * (host memory; computed in fp64, rounded once):
+ *   ATN_ROPE_SCALE_LINEAR  all divided by factor;
+ *   ATN_ROPE_SCALE_BASE    the base times factor^(rotary_dim / (rotary_dim - 2)): the fastest pair
+ *                          stays, the slowest is divided by factor;
+ *   ATN_ROPE_SCALE_PARTS   by the turns that a pair makes within `original` positions: from `high`
+ *                          on it stays, up to `low` it is divided by factor, between them a linear
+ *                          blend of the two; amplitude 1 + 0.1 ln factor.
+ * amplitude (may be NULL): the factor that goes with them (1 for the others). */
+#define ATN_ROPE_SCALE_NONE 0
+#define ATN_ROPE_SCALE_LINEAR 1
+#define ATN_ROPE_SCALE_BASE 2
+#define ATN_ROPE_SCALE_PARTS 3
+typedef struct atn_rope_scaling {
+    int kind;        /* ATN_ROPE_SCALE_* */
+    double factor;   /* >= 1 */
+    int original;    /* PARTS: positions of the unscaled context */
+    double low, high; /* PARTS: turns; 0, 0 = 1, 32 */
+} atn_rope_scaling;
+int atn_rope_frequencies(float *freq, int rotary_dim, double base, const atn_rope_scaling *scaling,
+                         float *amplitude);
+
+/* One tensor [batch][heads][tokens][head_d] and where it goes: strides as atn_drafts.q_stride; `out`
+ * of distinct elements; out == in with the same strides rotates in place. */
+typedef struct atn_rotated {
+    const void *in;
+    void *out;
+    int64_t in_stride[3], out_stride[3];
+    int heads;
+} atn_rotated;
+
+/* n (1 to 3) tensors turned by the same angles: token t of sequence b by position pos[b][t]
+ * ([batch][tokens]; NULL: t).  inverse != 0: the transposed (inverse, but for amplitude) map, so
+ * the gradient of the inputs from that of the outputs.  Dims from rotary_dim on are copied.  The
+ * tensors may be views of one buffer whose rows hold them side by side. */
+int atn_rotary_ex(int dtype, const atn_rotary *rotary, const atn_rotated *x, int n, int batch,
+                  int tokens, int head_d, const int32_t *pos, int inverse, void *stream);
+
+/* Cache rows len[b] + t = K (rotated) and V of token t < count[b]; q_out (if not NULL) = Q rotated
+ * (may be Q itself, with its strides; rows past count stay).  Positions: pos[b][t], or len[b] + t
+ * where pos is NULL.  rotary NULL: nothing is rotated.  Rows that the table does not hold are
+ * dropped. */
+int atn_paged_append_ex(const atn_paged_cache *cache, const atn_drafts *tokens,
+                        const atn_rotary *rotary, const int32_t *pos, void *q_out,
+                        const int64_t *q_out_stride, void *stream);
+
+/* Groups of consecutive sequences that begin with the same rows: sequences first[i] ... first[i + 1]
+ * - 1 have rows 0 ... rows[i] - 1 in common (in the same pages, or in copies of them), all before
+ * their new tokens: rows[i] <= len of each.  first ascends and lies in [0, batch]; sequences outside
+ * have no group; a group of one, or of no rows, reads its rows as its own.  (Other values: results
+ * are unspecified, accesses stay inside the tensors.) */
+typedef struct atn_shared_prefix {
+    const int32_t *first; /* [groups + 1], device */
+    const int32_t *rows;  /* [groups], device */
+    int groups;           /* <= batch */
+} atn_shared_prefix;
+
+/* out[b][h][t] = softmax over the rows r <= len[b] + t of (scale q . k_r) times v_r, for t < count[b];
+ * the rows behind are left as they were.  tokens: the queries (K and V are not used: they are rows of
+ * the cache by now).  prefix (NULL: none): its rows are read once a group; results differ from those
+ * without it by the order of sums alone.  scale, lse, out_stride and workspace as for
+ * atn_tree_attention_ex.  max_len: an upper bound of len[b] + count[b] that the host knows (0: the
+ * rows of a table); the call is laid out for it, and rows from there on are not attended.
+ * Rows that a token does not attend do not reach its output, whatever they hold; an infinity or NaN in
+ * a value that it attends makes that dim of its output infinite or NaN. */
+int atn_paged_attention_ex(const atn_paged_cache *cache, const atn_drafts *tokens,
+                           const atn_shared_prefix *prefix, void *out, const int64_t *out_stride,
+                           float *lse, float scale, int max_len, void *workspace,
+                           size_t workspace_bytes, void *stream);
+/* 0 on bad input.  Needs no device. */
+size_t atn_paged_attention_workspace_bytes(const atn_paged_cache *cache, const atn_drafts *tokens,
+                                           const atn_shared_prefix *prefix, int max_len);
+
+/* len[b] += min(count[b], what the table still holds). */
+int atn_paged_advance_ex(const atn_paged_cache *cache, const atn_drafts *tokens, void *stream);
+
 /* ==================== tuning, test controls and introspection ====================
  * None of these has a counterpart in the reference (whose launchers take no
  * options).  They exist for measurement and tests; a program that never
