@@ -147,7 +147,7 @@ int go_rotary(int dtype, atn::RotaryArgs* a, void* stream) {
 
 // The parts of an attention call that its size query needs too.
 int check_attention(const atn_paged_cache* cache, const atn_drafts* d, const atn_shared_prefix* prefix,
-                    int max_len, atn::PagedArgs* a, Pool* p, Tensor* q) {
+                    int max_len, atn::PagedArgs* a, Pool* p, Tensor* q, bool* whole16) {
     int st = check_paged(cache, &a->c, p);
     if (st == ATN_OK) st = check_sizes(cache, d);
     if (st != ATN_OK) return st;
@@ -167,6 +167,8 @@ int check_attention(const atn_paged_cache* cache, const atn_drafts* d, const atn
         a->first = prefix->first;
         a->shared = prefix->rows;
     }
+    *whole16 = cache->head_d * q->es % 16 == 0 && pieces16(q->p, q->s, q->es) &&
+               pieces16(p->k.p, p->k.s, q->es) && pieces16(p->v.p, p->v.s, q->es);
     a->Q = d->Q;
     for (int i = 0; i < 3; ++i) a->qs[i] = q->s[i];
     a->count = d->count;
@@ -322,9 +324,11 @@ size_t atn_paged_attention_workspace_bytes(const atn_paged_cache* cache, const a
     atn::PagedArgs a{};
     Pool p;
     Tensor q;
-    if (check_attention(cache, tokens, prefix, max_len, &a, &p, &q) != ATN_OK) return 0;
-    return kSyncRegion +
-           atn::paged_plan(cache->dtype, a.c, a.H, a.T, a.groups, atn_host::workspace_cap()).scratch;
+    bool whole16;
+    if (check_attention(cache, tokens, prefix, max_len, &a, &p, &q, &whole16) != ATN_OK) return 0;
+    return kSyncRegion + atn::paged_plan(cache->dtype, a.c, a.H, a.T, a.groups, whole16,
+                                         atn_host::workspace_cap())
+                             .scratch;
 }
 
 int atn_paged_attention_ex(const atn_paged_cache* cache, const atn_drafts* tokens,
@@ -334,7 +338,8 @@ int atn_paged_attention_ex(const atn_paged_cache* cache, const atn_drafts* token
     atn::PagedArgs a{};
     Pool p;
     Tensor q, o;
-    int st = check_attention(cache, tokens, prefix, max_len, &a, &p, &q);
+    bool whole16;
+    int st = check_attention(cache, tokens, prefix, max_len, &a, &p, &q, &whole16);
     if (st != ATN_OK) return st;
     if (!out) return ATN_ERR_NULL_POINTER;
     const int B = cache->batch;
@@ -355,7 +360,7 @@ int atn_paged_attention_ex(const atn_paged_cache* cache, const atn_drafts* token
         if (workspace_bytes < kSyncRegion) return ATN_ERR_WORKSPACE;
         room = workspace_bytes - kSyncRegion;
     }
-    a.plan = atn::paged_plan(cache->dtype, a.c, a.H, a.T, a.groups, room);
+    a.plan = atn::paged_plan(cache->dtype, a.c, a.H, a.T, a.groups, whole16, room);
     // (a dimension of a grid has less than 2^32 threads; workgroups of at most 512)
     if (a.plan.own.workgroups >= 1 << 23 || a.plan.own.line > INT32_MAX ||
         (a.groups > 0 && a.plan.pre.line > INT32_MAX))

@@ -84,6 +84,8 @@ hipError_t launch_paged_advance(const PagedView& c, const int* count, int T, hip
 // ---------------------------------------------------------------- attention
 // One of the two passes: the rows that groups of sequences share, then each sequence's own.
 struct PagedPass {
+    int many;        // 1: k_paged_many
+    int kb;          // keys of a block
     int rows;        // query rows of a tile
     int part_rows;   // rows of a tile that any item has
     int tiles;       // tiles of a segment, at most
@@ -119,9 +121,13 @@ struct PagedArgs {
     float* pre_part;
     int g0, gs;           // this launch's kv heads
 };
-PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, size_t scratch_cap);
+// whole16: the rows of K, V and Q are whole 16-byte pieces that lie so.
+PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
+                     size_t scratch_cap);
 hipError_t launch_paged_attention(int dtype, PagedArgs a, void* scratch, hipStream_t st);
 hipError_t launch_paged_f32(const PagedArgs& a, hipStream_t st);
 hipError_t launch_paged_bf16(const PagedArgs& a, hipStream_t st);
+// ... bf16, tiles of many query rows, in a pass of `grid` workgroups
+hipError_t launch_paged_many(const PagedArgs& a, int pre, dim3 grid, hipStream_t st);
 
 }  // namespace atn

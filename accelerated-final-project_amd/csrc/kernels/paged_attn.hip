@@ -7,25 +7,37 @@ namespace {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A pass of `segments` segments of at most R query rows of a kv head (and `kv` kv heads), over at
-// most `blocks` blocks an item; `all`: tiles of all segments of a kv head, at most.
-PagedPass plan_pass(int dtype, int D, int64_t R, int64_t segments, int64_t all_rows, int64_t blocks,
-                    int kv) {
+// A pass of `segments` segments of at most R query rows of a kv head (all: of all segments), over at
+// most `keys` keys an item; kv: kv heads of a launch.
+PagedPass plan_pass(int dtype, int D, int64_t R, int64_t segments, int64_t all, int64_t keys, int kv,
+                    bool whole16) {
     PagedPass p{};
     const bool bf = dtype == kDtypeBF16, wide = D > kPagedNarrow;
-    p.rows = R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64;
+    p.many = bf && whole16 && D <= 128 && R > 32;
+    int per_cu;  // workgroups that a CU holds at once (the kernels' registers and LDS)
+    if (p.many) {
+        // the tile that leaves the fewest rows empty, the larger of equals
+        p.rows = 64;
+        for (int rows : {128, 256})
+            if (ceil_div(R, rows) * rows <= ceil_div(R, p.rows) * p.rows) p.rows = rows;
+        per_cu = 256 / p.rows;
+        p.kb = p.rows == 64 ? 32 : 64;
+        p.turn = 1;
+    } else {
+        p.rows = R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64;
+        const int mt = p.rows / 16;
+        per_cu = wide ? (mt == 1 ? 2 : 1)
+                      : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
+        p.kb = wide ? kPagedWideKeys : bf ? 32 : 16;
+        p.turn = wide ? 1 : 4;
+    }
     p.part_rows = (int)std::min<int64_t>(p.rows, R);
     p.tiles = (int)ceil_div(R, p.rows);
     const int dims = D > 1024 ? 2048 : D > 512 ? 1024 : 512;
     p.groups = wide ? (int)ceil_div(D, dims) : 1;
-    const int mt = p.rows / 16;
-    // workgroups that the card holds at once (256 CUs; the kernels' registers)
-    const int per_cu = wide ? (mt == 1 ? 2 : 1)
-                            : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
-    p.turn = wide ? 1 : 4;
-    const int64_t items =
-        kv * std::min(segments * p.tiles, ceil_div(all_rows, p.rows) + segments);
+    const int64_t items = kv * std::min(segments * p.tiles, ceil_div(all, p.rows) + segments);
     const int64_t slots = std::max<int64_t>(1, 256 * per_cu / p.groups);
+    const int64_t blocks = ceil_div(keys, p.kb) + 1;
     p.ranges =
         (int)std::max<int64_t>(1, std::min(slots, ceil_div(items * (blocks + kPagedPad), 2 * p.turn)));
     p.line = items * (blocks + kPagedPad) + 2ll * p.turn * p.ranges;
@@ -41,17 +53,17 @@ size_t part_bytes(const PagedPass& p, int D) {
 
 }  // namespace
 
-PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, size_t scratch_cap) {
+PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
+                     size_t scratch_cap) {
     PagedPlan p{};
-    const int rep = H / c.G, wide = c.D > kPagedNarrow;
-    const int kb = wide ? kPagedWideKeys : dtype == kDtypeBF16 ? 32 : 16;
-    const int64_t R = (int64_t)rep * T, all = R * c.B, blocks = ceil_div(c.rows, kb) + 1;
+    const int64_t R = (int64_t)(H / c.G) * T, all = R * c.B;
+    whole16 = whole16 && c.page_rows % 16 == 0;
     // all kv heads at once, unless the scratch does not hold their parts
     for (p.kv = c.G;; p.kv = (p.kv + 1) / 2) {
-        p.own = plan_pass(dtype, c.D, R, c.B, all, blocks, p.kv);
+        p.own = plan_pass(dtype, c.D, R, c.B, all, c.rows, p.kv, whole16);
         p.scratch = 0;
         if (groups > 0) {
-            p.pre = plan_pass(dtype, c.D, all, groups, all, blocks, p.kv);
+            p.pre = plan_pass(dtype, c.D, all, groups, all, c.rows, p.kv, whole16);
             p.pre.split = 1;
             p.scratch = paged_starts_bytes(c.B) + part_bytes(p.pre, c.D);
         }

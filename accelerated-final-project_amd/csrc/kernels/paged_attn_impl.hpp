@@ -361,6 +361,12 @@ __device__ __forceinline__ uint32_t flags_of(uint32_t x) {
                ((x & 0x7f800000u) == 0x7f800000u ? hi : 0u);
     }
 }
+// What a sum of flags adds to an output.
+__device__ __forceinline__ float spread_of(float sum) {
+    const int k = (int)sum, pos = k & 63, neg = k >> 6 & 63;
+    const float add = k >= 4096 || (pos && neg) ? __builtin_nanf("") : pos ? INFINITY : -INFINITY;
+    return k ? add : 0.f;
+}
 // In a block with keys that some rows do not attend, an infinity or NaN in V times a weight of 0
 // would reach them.  V is cleared of these, and they go to the rows that attend their keys by a
 // product of their own, the flags' with weights 1: sums over at most 32 keys, exact, whose
@@ -403,13 +409,7 @@ __device__ __forceinline__ void spread_not_finite(v4f (&o)[MT][N::VS][N::VL], ty
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int k = (int)n[t][e], pos = k & 63, neg = k >> 6 & 63;
-                    const float add = k >= 4096 || (pos && neg) ? __builtin_nanf("")
-                                      : pos                     ? INFINITY
-                                                                : -INFINITY;
-                    o[t][i][c][e] += k ? add : 0.f;
-                }
+                for (int e = 0; e < 4; ++e) o[t][i][c][e] += spread_of(n[t][e]);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -589,16 +589,22 @@ __device__ __forceinline__ void write_rows(const PagedArgs& a, const Span& sp, c
 // A workgroup's spans, one after another: f(span).
 template <int PRE, typename F>
 __device__ __forceinline__ void each_span(const PagedArgs& a, int id, int kb, int lane, F f) {
-    if (!PRE && !a.plan.own.split) {
-        const Span sp = span_whole(a, id, kb);
-        if (sp.last > sp.first) f(sp);
-        return;
+    const bool split = PRE || a.plan.own.split;
+    int at = 0, end = 1;
+    Line line{};
+    if (split) {
+        line = line_of<PRE>(a, kb, lane);
+        at = id * line.per;
+        end = min(line.total, at + line.per);
     }
-    const Line line = line_of<PRE>(a, kb, lane);
-    int at = id * line.per;
-    const int end = min(line.total, at + line.per);
     while (at < end) {
-        const Span sp = span_at<PRE>(a, line, id, at, end, kb, lane, &at);
+        Span sp;
+        if (split) {
+            sp = span_at<PRE>(a, line, id, at, end, kb, lane, &at);
+        } else {
+            sp = span_whole(a, id, kb);
+            at = end;
+        }
         if (sp.last > sp.first) f(sp);
     }
 }
@@ -973,7 +979,7 @@ k_paged_wide(PagedArgs a) {
 // The parts of a row added up, in their order: the prefix's, then its own.  WAVES waves a row (and
 // 256 dims), each every WAVES-th part; 4 rows a workgroup where there are many rows.  Rows of one
 // range and no prefix are written already.
-template <typename T, int WAVES, int KB>
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     __shared__ float acc[4][256];
     __shared__ float2 sums[4];
@@ -990,8 +996,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     int own0 = 0, own = 1, pre0 = 0, pre = 0;
     const int tile = row / a.plan.own.rows, in_tile = row - tile * a.plan.own.rows;
     if (a.plan.own.split) {
-        const Line line = line_of<0>(a, KB, lane);
-        const Place p = place_of<0>(a, line, b, KB, lane);
+        const Line line = line_of<0>(a, a.plan.own.kb, lane);
+        const Place p = place_of<0>(a, line, b, a.plan.own.kb, lane);
         const int item = lg * s.tiles + tile, first = p.start + item * p.n + kPagedPad;
         const int r0 = (unsigned)first / (unsigned)line.per;
         const int r1 = (unsigned)(first + p.n - kPagedPad - 1) / (unsigned)line.per;
@@ -1004,8 +1010,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     int pre_in = 0;
     if (group >= 0) {
         const Segment g = segment<1>(a, group);
-        const Line line = line_of<1>(a, KB, lane);
-        const Place p = place_of<1>(a, line, group, KB, lane);
+        const Line line = line_of<1>(a, a.plan.pre.kb, lane);
+        const Place p = place_of<1>(a, line, group, a.plan.pre.kb, lane);
         const int prow = (b - g.first) * a.T * a.rep + row, ptile = prow / a.plan.pre.rows;
         pre_in = prow - ptile * a.plan.pre.rows;
         const int item = lg * g.tiles + ptile, first = p.start + item * p.n + kPagedPad;
@@ -1104,6 +1110,9 @@ void paged_pass(const PagedArgs& a, hipStream_t st) {
     const int64_t units = PRE || p.split ? p.ranges : (int64_t)a.c.B * a.gs * p.tiles;
     const dim3 grid((unsigned)(units * p.groups));
     const int D = a.c.D;
+    if constexpr (sizeof(T) == 2) {
+        if (p.many) return (void)launch_paged_many(a, PRE, grid, st);
+    }
     if (D > 1024) return paged_wide<T, 256, PRE>(a, grid, st);
     if (D > 512) return paged_wide<T, 128, PRE>(a, grid, st);
     if (D > kPagedNarrow) return paged_wide<T, 64, PRE>(a, grid, st);
@@ -1112,26 +1121,20 @@ void paged_pass(const PagedArgs& a, hipStream_t st) {
     if (D <= 192) return paged_dims<T, 192, PRE>(a, grid, st);
     paged_dims<T, 256, PRE>(a, grid, st);
 }
-template <typename T, int KB>
+template <typename T>
 void paged_merge(const PagedArgs& a, hipStream_t st) {
     const int R = a.rep * a.T, chunks = (a.c.D + 255) / 256;
     if ((int64_t)a.c.B * a.gs * R * chunks >= 1024)
-        hipLaunchKernelGGL((k_paged_merge<T, 1, KB>), dim3((R + 3) / 4, a.c.B * a.gs, chunks),
-                           dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_paged_merge<T, 1>), dim3((R + 3) / 4, a.c.B * a.gs, chunks), dim3(256),
+                           0, st, a);
     else
-        hipLaunchKernelGGL((k_paged_merge<T, 4, KB>), dim3(R, a.c.B * a.gs, chunks), dim3(256), 0, st,
-                           a);
+        hipLaunchKernelGGL((k_paged_merge<T, 4>), dim3(R, a.c.B * a.gs, chunks), dim3(256), 0, st, a);
 }
 template <typename T>
 void paged_go(const PagedArgs& a, hipStream_t st) {
     if (a.groups > 0) paged_pass<T, 1>(a, st);
     paged_pass<T, 0>(a, st);
-    if (a.groups > 0 || a.plan.own.split) {
-        if (a.c.D > kPagedNarrow)
-            paged_merge<T, kPagedWideKeys>(a, st);
-        else
-            paged_merge<T, CacheTiles<T, 64, 1, kExact>::KB>(a, st);
-    }
+    if (a.groups > 0 || a.plan.own.split) paged_merge<T>(a, st);
 }
 
 }  // namespace
