@@ -35,21 +35,73 @@ struct PagedMany {
     }
 };
 
+constexpr int kDepth = 4;
+
 template <int DP, int WAVES, int KEYS, int PRE>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_many(PagedArgs a) {
     using N = PagedMany<DP, WAVES, KEYS>;
     using T = uint16_t;
     using W16 = Words<T, 16>;
-    // (registers: with four waves a lane loads twice the pieces, so K's go to LDS before V's come)
-    constexpr bool kLate = N::X * DP >= 512;
     constexpr int CH = N::CH, NT = N::NT, QS = N::QS, DT = N::DT, X = N::X, SUB = N::SUB;
-    __shared__ __align__(16) char kbuf[2][N::kStage];
-    __shared__ __align__(16) char vbuf[2][N::kStage];
+    constexpr int AHEAD = N::AHEAD, ROWS_X = 64 / CH;  // rows of a wave's load
+    // (each an object of its own: the compiler lets reads of one pass loads into another)
+    __shared__ __align__(16) char k0[N::kStage], k1[N::kStage], v0[N::kStage], v1[N::kStage];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int D = a.c.D, pieces = D / 8;
     const float scale = fabsf(a.scale);
     if (PRE && blockIdx.x == 0) write_starts(a);
+    if (pieces < CH) {  // (places of pieces past the row's end stay 0)
+        for (int e = 16 * tid; e < N::kStage; e += 16 * 64 * WAVES)
+            for (char* z : {k0, k1, v0, v1}) *reinterpret_cast<uint4*>(z + e) = make_uint4(0, 0, 0, 0);
+    }
+    // This wave's rows of a stage, of one run of 16: lane L loads place L % CH of row L / CH, load x
+    // those ROWS_X rows on.  Which piece lies there: PagedMany's places.
+    const int wrow = wave * X * ROWS_X, wrun = wrow / 16;
+    uint32_t kof[X], vof[X];  // bytes from the run's first row
+    bool kin[X], vin[X];
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+        const int r = wrow + x * ROWS_X + lane / CH;
+        const int kc = N::k_place(r, lane % CH), vc = N::v_place(r, lane % CH);
+        kin[x] = kc < pieces, vin[x] = vc < pieces;
+        kof[x] = ((r & 15) * (uint32_t)a.c.ks[2] + 8 * kc) * 2;
+        vof[x] = ((r & 15) * (uint32_t)a.c.vs[2] + 8 * vc) * 2;
+    }
+    auto load = [&](const T* base, const uint32_t (&of)[X], const bool (&in)[X], char* buf) {
+#pragma unroll
+        for (int x = 0; x < X; ++x)
+            if (in[x])
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)((const char*)base + of[x]),
+                    (__attribute__((address_space(3))) void*)(buf + (wrow + x * ROWS_X) * CH * 16), 16, 0,
+                    0);
+    };
+    auto landed = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __syncthreads();
+    };
+    // operands: K's piece 2 e + half of key 32 t + col
+    auto k_at = [&](const char* buf, int t, int e) {
+        const int key = 32 * t + col;
+        return reinterpret_cast<const W16*>(buf)[key * CH + N::k_place(key, 2 * e + half)];
+    };
+    // ... V's dims 32 c + lane % 32 of the keys that words [8 u, 8 u + 8) of tile t's weights are
+    const int sub = lane & 15, dhalf = lane >> 4 & 1;
+    auto v_at = [&](const char* buf, int t, int u, int c) {
+        W16 v;
+        const int key = 32 * t + 16 * u + 4 * half + (sub >> 2);
+        const int piece = 4 * c + 2 * dhalf + ((sub & 3) >> 1);
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(buf);
+        const uint2 x = lds_tr16(p + (key * CH + N::v_place(key, piece)) * 8 + 4 * (sub & 1));
+        const uint2 y = lds_tr16(p + ((key + 8) * CH + N::v_place(key + 8, piece)) * 8 + 4 * (sub & 1));
+        v.w[0] = x.x, v.w[1] = x.y, v.w[2] = y.x, v.w[3] = y.y;
+        return v;
+    };
+    auto mfma = [](const W16& x, const W16& y, const v16f& z) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
+                                                       __builtin_bit_cast(bf16x8, y), z, 0, 0, 0);
+    };
 
     each_span<PRE>(a, blockIdx.x, KEYS, lane, [&](const Span& sp) {
         const T* kp = (const T*)a.c.K + sp.g * a.c.ks[1];
@@ -58,87 +110,50 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_many(PagedArgs a) {
         const int last = min(sp.last, tile_end<PRE>(a, sp.s, sp.tile, KEYS));
         const int mine = row0 + 32 * wave + col;  // this lane's query row
         const int upto = attended<PRE>(a, sp, mine);
+        // stages [w0, w1) are attended whole by every row
         const int w0 = (lo + KEYS - 1) / KEYS, w1 = of_wave(attended<PRE>(a, sp, row0)) / KEYS;
 
-        // pages of 16 keys: lane l those of stage `at` + l / SUB, run l % SUB
+        // pages of 16 keys: lane l those of stage `at` + l / SUB, run l % SUB; `there`: which are pages
         int at = sp.first;
         auto fetch = [&](int i) {
             return page_of(a.c, sp.s.first, (i + lane / SUB) * KEYS + 16 * (lane % SUB));
         };
-        int now = fetch(at), next = fetch(at + N::AHEAD);
-        auto go = [&](int i) {
-            if (i < at + N::AHEAD) return;
-            at += N::AHEAD;
-            now = next;
-            next = fetch(at + N::AHEAD);
+        int now = fetch(at), next = fetch(at + AHEAD);
+        uint64_t there = __builtin_amdgcn_ballot_w64(is_page(a.c, now));
+        // of a stage (asked for in their order): where this wave's run begins, and its runs' pages
+        struct Run {
+            const T *k, *v;
+            uint32_t ok;
         };
-        auto run = [&](int i, int s) {
-            const int x = (i - at) * SUB + s;
-            return __builtin_amdgcn_readlane(x < 64 ? now : next, x & 63);
-        };
-        auto there_of = [&](int i) {
-            uint64_t x = 0;
-#pragma unroll
-            for (int s = 0; s < SUB; ++s)
-                x |= is_page(a.c, run(i, s)) ? (uint64_t)0xffff << (16 * s) : 0;
-            return x;
-        };
-        // piece x of this lane: row (x WAVES + wave) 64 / CH + lane / CH of the stage, piece lane % CH
-        const int lrow = lane / CH, lc = lane % CH;
-        const bool has = lc < pieces;
-        auto load = [&](W16 (&to)[X], const T* pool, const int64_t (&st)[3], int i) {
-#pragma unroll
-            for (int x = 0; x < X; ++x) {
-                const int r0 = (x * WAVES + wave) * (64 / CH);  // (of one run of 16)
-                const int r = i * KEYS + r0, in = r - over(r, a.c.by_page) * a.c.page_rows;
-                const int page = run(i, r0 / 16);
-                const T* base = pool + (is_page(a.c, page) ? page : 0) * st[0] + in * st[2];
-                to[x] = ld_words<16>(base + lrow * (uint32_t)st[2] + 8 * min(lc, pieces - 1));
+        auto run_of = [&](int i) {
+            if (i >= at + AHEAD) {
+                at += AHEAD;
+                now = next;
+                next = fetch(at + AHEAD);
+                there = __builtin_amdgcn_ballot_w64(is_page(a.c, now));
             }
+            const int x = (i - at) * SUB, r = i * KEYS + 16 * wrun;
+            const int p = __builtin_amdgcn_readlane(now, x + wrun), page = is_page(a.c, p) ? p : 0;
+            const int in = r - over(r, a.c.by_page) * a.c.page_rows;
+            Run y;
+            y.k = kp + page * a.c.ks[0] + in * a.c.ks[2];
+            y.v = vp + page * a.c.vs[0] + in * a.c.vs[2];
+            y.ok = (uint32_t)(there >> x) & ((1u << SUB) - 1);
+            return y;
         };
-        auto put_k = [&](const W16 (&from)[X], char* buf) {
-#pragma unroll
-            for (int x = 0; x < X; ++x) {
-                const int r = (x * WAVES + wave) * (64 / CH) + lrow;
-                W16 z = from[x];
-                if (!has) z = W16{};
-                reinterpret_cast<W16*>(buf)[r * CH + N::k_place(r, lc)] = z;
-            }
-        };
-        // whether some row does not attend some key of stage i
-        auto is_part = [&](int i) { return i < w0 || i >= w1 || there_of(i) != ~0ull >> (64 - KEYS); };
         bool odd = false;  // an infinity or NaN was left out
-        auto put_v = [&](W16 (&from)[X], char* buf, int i) {
-            if (is_part(i)) {
-                // (an infinity or NaN times a weight of 0 would reach rows that do not attend its key:
-                // V enters without them, and they are written over the results of the rows that do)
-                uint32_t bad = 0;
-#pragma unroll
-                for (int x = 0; x < X; ++x)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t& z = from[x].w[w];
-                        const uint32_t hi = (z & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
-                        const uint32_t lo = (z & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
-                        z &= ~(hi | lo);
-                        bad |= hi | lo;
-                    }
-                odd |= bad != 0;
-            }
-#pragma unroll
-            for (int x = 0; x < X; ++x) {
-                const int r = (x * WAVES + wave) * (64 / CH) + lrow;
-                W16 z = from[x];
-                if (!has) z = W16{};
-                reinterpret_cast<W16*>(buf)[r * CH + N::v_place(r, lc)] = z;
-            }
-        };
 
-        W16 kr[X], vr[X];
         const bool any = sp.first < last;
+        __syncthreads();  // (the last span's stages have been read)
+        Run r0{}, r1{};   // of the stage at work, and the next one
         if (any) {
-            load(kr, kp, a.c.ks, sp.first);
-            load(vr, vp, a.c.vs, sp.first);
+            r0 = run_of(sp.first);
+            load(r0.k, kof, kin, k0);
+            load(r0.v, vof, vin, v0);
+            if (sp.first + 1 < last) {
+                r1 = run_of(sp.first + 1);
+                load(r1.k, kof, kin, k1);
+            }
         }
         // Q: this lane's row (those of no token: some token's; nobody reads their results)
         W16 qf[QS];
@@ -156,74 +171,61 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_many(PagedArgs a) {
         }
         v16f o[DT];
 #pragma unroll
-        for (int c = 0; c < DT; ++c)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[c][e] = 0.f;
+        for (int c = 0; c < DT; ++c) o[c] = v16f{};
         float m = -INFINITY, l = 0.f, used = 0.f;
-        __syncthreads();  // (the last span's stages have been read)
-        if (any) {
-            put_k(kr, kbuf[0]);
-            put_v(vr, vbuf[0], sp.first);
-            if (sp.first + 1 < last) {
-                load(kr, kp, a.c.ks, sp.first + 1);
-                put_k(kr, kbuf[1]);
-            }
-        }
-        __syncthreads();
+        landed();
 
-        auto k_at = [&](const char* buf, int t, int e) {
-            const int key = 32 * t + col;
-            return reinterpret_cast<const W16*>(buf)[key * CH + N::k_place(key, 2 * e + half)];
-        };
-        // V^T's operand: dims 32 c + lane % 32 of the keys that words [8 u, 8 u + 8) of tile t's
-        // weights are
-        const int sub = lane & 15, dhalf = lane >> 4 & 1;
-        auto v_at = [&](const char* buf, int t, int u, int c) {
-            W16 v;
-            const int key = 32 * t + 16 * u + 4 * half + (sub >> 2);
-            const int piece = 4 * c + 2 * dhalf + ((sub & 3) >> 1);
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(buf);
-            const uint2 x = lds_tr16(p + (key * CH + N::v_place(key, piece)) * 8 + 4 * (sub & 1));
-            const uint2 y =
-                lds_tr16(p + ((key + 8) * CH + N::v_place(key + 8, piece)) * 8 + 4 * (sub & 1));
-            v.w[0] = x.x, v.w[1] = x.y, v.w[2] = y.x, v.w[3] = y.y;
-            return v;
-        };
-        auto mfma = [](const W16& x, const W16& y, const v16f& z) {
-            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
-                                                           __builtin_bit_cast(bf16x8, y), z, 0, 0, 0);
-        };
         v16f s0[NT], s1[NT];
         if (any) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 s0[t] = v16f{};
 #pragma unroll
-                for (int e = 0; e < QS; ++e) s0[t] = mfma(k_at(kbuf[0], t, e), qf[e], s0[t]);
+                for (int e = 0; e < QS; ++e) s0[t] = mfma(k_at(k0, t, e), qf[e], s0[t]);
             }
         }
+        __syncthreads();  // (the first stage loads into the buffer just read)
         // One stage: its scores s into weights, beside them the next stage's scores n (of what the
         // buffer holds where there is none), then the product with V.
-        auto stage = [&](int i, v16f (&s)[NT], v16f (&n)[NT], const char* kb, char* kfree,
-                         const char* vb, char* vfree) {
-            const bool more = i + 1 < last, more2 = i + 2 < last;
-            const uint64_t there = there_of(i);
-            if (more) {
-                go(i + 1);
-                if (more2) load(kr, kp, a.c.ks, i + 2);
-                if (!kLate) load(vr, vp, a.c.vs, i + 1);
+        auto stage = [&](int i, v16f (&s)[NT], v16f (&n)[NT], const char* kb, char* kfree, char* vb,
+                         char* vfree) {
+            Run r2{};
+            if (i + 1 < last) {
+                load(r1.v, vof, vin, vfree);
+                if (i + 2 < last) {
+                    r2 = run_of(i + 2);
+                    load(r2.k, kof, kin, kfree);
+                }
             }
-            if (i < w0 || i >= w1 || there != ~0ull >> (64 - KEYS)) {
+            if (i < w0 || i >= w1 || r0.ok != (1u << SUB) - 1) {
+                // (some row does not attend some key)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const int j0 = i * KEYS + 32 * t;
-                    const uint32_t on = ((uint32_t)(there >> (32 * t)) & below(upto - j0) &
-                                         ~below(lo - j0)) >>
-                                        (4 * half);
+                    const uint32_t has = (r0.ok >> (2 * t) & 1u ? 0xffffu : 0u) |
+                                         (r0.ok >> (2 * t + 1) & 1u ? 0xffff0000u : 0u);
+                    const uint32_t on = (has & below(upto - j0) & ~below(lo - j0)) >> (4 * half);
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if (!(on >> (8 * (e >> 2) + (e & 3)) & 1u)) s[t][e] = -INFINITY;
                 }
+                // An infinity or NaN times a weight of 0 would reach rows that do not attend its key: V
+                // enters without them, and they are written over the results of the rows that do.
+                uint32_t bad = 0;
+#pragma unroll 1
+                for (int e = tid; e < KEYS * CH; e += 64 * WAVES) {
+                    W16 z = reinterpret_cast<W16*>(vb)[e];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t hi = (z.w[w] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+                        const uint32_t lw = (z.w[w] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
+                        z.w[w] &= ~(hi | lw);
+                        bad |= hi | lw;
+                    }
+                    reinterpret_cast<W16*>(vb)[e] = z;
+                }
+                odd |= bad != 0;
+                __syncthreads();
             }
             // softmax, as weights() does it
             float top = s[0][0];
@@ -243,56 +245,54 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_many(PagedArgs a) {
                 for (int c = 0; c < DT; ++c) o[c] *= f;
             }
             const float base = base_of(m);
-            W16 p[NT][2];
-            constexpr int STEPS = NT * QS, PER = 16 * NT / STEPS;  // scores beside a product
-            W16 k = k_at(kb, 0, 0);
+            // Products: the next scores', with PER weights beside each, then V's.  Their operands come
+            // from LDS DEPTH products ahead.
+            constexpr int NK = NT * QS, NV = 2 * NT * DT, PER = 16 * NT / NK, DEPTH = kDepth;
+            W16 p[NT][2], x[DEPTH];
+            auto operand = [&](int y) {
+                if (y < NK) return k_at(kb, y % NT, y / NT);
+                y -= NK;
+                return v_at(vb, y / (2 * DT), y / DT % 2, y % DT);
+            };
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int y = 0; y < DEPTH; ++y) x[y] = operand(y);
 #pragma unroll
-                for (int e = 0; e < QS; ++e) {
-                    const int step = t * QS + e;
-                    const W16 now_k = k;
-                    if (step + 1 < STEPS) k = k_at(kb, (step + 1) / QS, (step + 1) % QS);
-                    n[t] = mfma(now_k, qf[e], e == 0 ? v16f{} : n[t]);
+            for (int y = 0; y < NK; ++y) {
+                const int t = y % NT, e = y / NT;
+                n[t] = mfma(x[y % DEPTH], qf[e], e == 0 ? v16f{} : n[t]);
+                x[y % DEPTH] = operand(y + DEPTH);
 #pragma unroll
-                    for (int y = step * PER; y < (step + 1) * PER; y += 2) {
-                        const int ty = y / 16, ey = y % 16;
-                        const float x0 = exp2_(fmaf(s[ty][ey], scale, -base));
-                        const float x1 = exp2_(fmaf(s[ty][ey + 1], scale, -base));
-                        l += x0 + x1;
-                        // (rounded: see CacheTiles::accumulate)
-                        const uint32_t w = pack2(x0, x1);
-                        used = add2(w, used);
-                        p[ty][ey / 8].w[ey % 8 / 2] = w;
-                        // (what the compiler knows to be needed later alone it computes later, with
-                        // the scores kept in registers until then)
-                        asm volatile("" : "+v"(p[ty][ey / 8].w[ey % 8 / 2]), "+v"(l), "+v"(used));
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int z = y * PER; z < (y + 1) * PER; z += 2) {
+                    const int tz = z / 16, ez = z % 16;
+                    const float f0 = exp2_(fmaf(s[tz][ez], scale, -base));
+                    const float f1 = exp2_(fmaf(s[tz][ez + 1], scale, -base));
+                    l += f0 + f1;
+                    // (rounded: see CacheTiles::accumulate)
+                    uint32_t& w = p[tz][ez / 8].w[ez % 8 / 2];
+                    w = pack2(f0, f1);
+                    used = add2(w, used);
+                    // (what the compiler knows to be needed later alone it computes later, with the
+                    // scores kept in registers until then)
+                    asm volatile("" : "+v"(w), "+v"(l), "+v"(used));
                 }
-            if (kLate && more) {
-                if (more2) put_k(kr, kfree);
-                load(vr, vp, a.c.vs, i + 1);
-            }
-            W16 v = v_at(vb, 0, 0, 0);
-#pragma unroll
-            for (int y = 0; y < 2 * NT * DT; ++y) {
-                const int t = y / (2 * DT), u = y / DT % 2, c = y % DT;
-                const W16 now_v = v;
-                if (y + 1 < 2 * NT * DT)
-                    v = v_at(vb, (y + 1) / (2 * DT), (y + 1) / DT % 2, (y + 1) % DT);
-                o[c] = mfma(now_v, p[t][u], o[c]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (!kLate && more2) put_k(kr, kfree);
-            if (more) put_v(vr, vfree, i + 1);
-            __syncthreads();
+#pragma unroll
+            for (int y = 0; y < NV; ++y) {
+                const int t = y / (2 * DT), u = y / DT % 2, c = y % DT;
+                o[c] = mfma(x[(NK + y) % DEPTH], p[t][u], o[c]);
+                if (y + DEPTH < NV) x[(NK + y) % DEPTH] = operand(NK + y + DEPTH);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            r0 = r1;
+            r1 = r2;
+            landed();
         };
 #pragma unroll 1
         for (int i = sp.first; i < last; i += 2) {
-            stage(i, s0, s1, kbuf[1], kbuf[0], vbuf[0], vbuf[1]);
+            stage(i, s0, s1, k1, k0, v0, v1);
             if (i + 1 >= last) break;
-            stage(i + 1, s1, s0, kbuf[0], kbuf[1], vbuf[1], vbuf[0]);
+            stage(i + 1, s1, s0, k0, k1, v1, v0);
         }
         // (a row's keys lie in two lanes)
         auto both = [](float v) {
