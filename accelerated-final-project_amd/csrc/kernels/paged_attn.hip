@@ -7,10 +7,10 @@ namespace {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A pass of `segments` segments of at most R query rows of a kv head (all: of all segments), over at
-// most `keys` keys an item; kv: kv heads of a launch.
-PagedPass plan_pass(int dtype, int D, int64_t R, int64_t segments, int64_t all, int64_t keys, int kv,
-                    bool whole16) {
+// A pass of `segments` segments of about R query rows of a kv head, at most `most` (all: of all
+// segments), over at most `keys` keys an item; kv: kv heads of a launch.
+PagedPass plan_pass(int dtype, int D, int64_t R, int64_t most, int64_t segments, int64_t all,
+                    int64_t keys, int kv, bool whole16) {
     PagedPass p{};
     const bool bf = dtype == kDtypeBF16, wide = D > kPagedNarrow;
     p.many = bf && whole16 && D <= 128 && R > 32;
@@ -20,8 +20,8 @@ PagedPass plan_pass(int dtype, int D, int64_t R, int64_t segments, int64_t all, 
         p.rows = 64;
         for (int rows : {128, 256})
             if (ceil_div(R, rows) * rows <= ceil_div(R, p.rows) * p.rows) p.rows = rows;
-        per_cu = 256 / p.rows;
-        p.kb = p.rows == 64 ? 32 : 64;
+        per_cu = 1;
+        p.kb = p.rows == 256 ? 64 : 128;
         p.turn = 1;
     } else {
         p.rows = R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64;
@@ -31,8 +31,8 @@ PagedPass plan_pass(int dtype, int D, int64_t R, int64_t segments, int64_t all, 
         p.kb = wide ? kPagedWideKeys : bf ? 32 : 16;
         p.turn = wide ? 1 : 4;
     }
-    p.part_rows = (int)std::min<int64_t>(p.rows, R);
-    p.tiles = (int)ceil_div(R, p.rows);
+    p.part_rows = (int)std::min<int64_t>(p.rows, most);
+    p.tiles = (int)ceil_div(most, p.rows);
     const int dims = D > 1024 ? 2048 : D > 512 ? 1024 : 512;
     p.groups = wide ? (int)ceil_div(D, dims) : 1;
     const int64_t items = kv * std::min(segments * p.tiles, ceil_div(all, p.rows) + segments);
@@ -60,10 +60,12 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
     whole16 = whole16 && c.page_rows % 16 == 0;
     // all kv heads at once, unless the scratch does not hold their parts
     for (p.kv = c.G;; p.kv = (p.kv + 1) / 2) {
-        p.own = plan_pass(dtype, c.D, R, c.B, all, c.rows, p.kv, whole16);
+        p.own = plan_pass(dtype, c.D, R, R, c.B, all, c.rows, p.kv, whole16);
         p.scratch = 0;
         if (groups > 0) {
-            p.pre = plan_pass(dtype, c.D, all, groups, all, c.rows, p.kv, whole16);
+            // (groups are on the device: tiles for groups of equal size)
+            p.pre = plan_pass(dtype, c.D, ceil_div(c.B, groups) * R, all, groups, all, c.rows, p.kv,
+                              whole16);
             p.pre.split = 1;
             p.scratch = paged_starts_bytes(c.B) + part_bytes(p.pre, c.D);
         }

@@ -1124,7 +1124,7 @@ void paged_pass(const PagedArgs& a, hipStream_t st) {
 template <typename T>
 void paged_merge(const PagedArgs& a, hipStream_t st) {
     const int R = a.rep * a.T, chunks = (a.c.D + 255) / 256;
-    if ((int64_t)a.c.B * a.gs * R * chunks >= 1024)
+    if ((int64_t)a.c.B * a.gs * R * chunks >= 16384)
         hipLaunchKernelGGL((k_paged_merge<T, 1>), dim3((R + 3) / 4, a.c.B * a.gs, chunks), dim3(256),
                            0, st, a);
     else
