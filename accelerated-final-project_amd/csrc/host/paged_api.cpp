@@ -362,7 +362,7 @@ int atn_paged_attention_ex(const atn_paged_cache* cache, const atn_drafts* token
     }
     a.plan = atn::paged_plan(cache->dtype, a.c, a.H, a.T, a.groups, whole16, room);
     // (a dimension of a grid has less than 2^32 threads; workgroups of at most 512)
-    if (a.plan.own.workgroups >= 1 << 23 || a.plan.own.line > INT32_MAX ||
+    if (a.plan.own.workgroups + a.plan.first >= 1 << 23 || a.plan.own.line > INT32_MAX ||
         (a.groups > 0 && a.plan.pre.line > INT32_MAX))
         return ATN_ERR_SIZE_OVERFLOW;
     if (a.plan.scratch > room) return ATN_ERR_WORKSPACE;

@@ -82,7 +82,7 @@ hipError_t launch_rotary(int dtype, const RotaryArgs& a, hipStream_t st);
 hipError_t launch_paged_advance(const PagedView& c, const int* count, int T, hipStream_t st);
 
 // ---------------------------------------------------------------- attention
-// One of the two passes: the rows that groups of sequences share, then each sequence's own.
+// One of the two passes: the rows that groups of sequences share, and each sequence's own.
 struct PagedPass {
     int many;        // 1: k_paged_many
     int kb;          // keys of a block
@@ -93,13 +93,19 @@ struct PagedPass {
     int split;       // ... 0: an item a workgroup
     int turn;
     int groups;      // workgroups that share an item's dims (head_d > 256)
+    int64_t items;   // at most
     int64_t parts;   // results kept in the scratch, at most
     int64_t workgroups;
-    int64_t line;
+    int64_t line;    // places, at most
+    int64_t scores;  // floats (head_d > 256)
 };
 struct PagedPlan {
     PagedPass own, pre;
+    int first;       // workgroups of a launch's grid that take the prefixes
     int kv;          // kv heads of a launch
+    int wide;        // head_d > 256:
+    int shares;      // ... workgroups that share the dims of a block's scores
+    unsigned score_grid;
     size_t scratch;  // bytes
 };
 struct PagedArgs {
@@ -116,7 +122,10 @@ struct PagedArgs {
     const int* shared;    // [groups] rows
     int groups;
     PagedPlan plan;
-    int2* starts;         // scratch: [B] first row of a sequence's own, its group or -1; or null
+    // scratch
+    const int2* starts;   // [B] first row of a sequence's own, its group or -1; null: few groups
+    float* own_scores;
+    float* pre_scores;
     float* own_part;
     float* pre_part;
     int g0, gs;           // this launch's kv heads
@@ -125,9 +134,10 @@ struct PagedArgs {
 PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
                      size_t scratch_cap);
 hipError_t launch_paged_attention(int dtype, PagedArgs a, void* scratch, hipStream_t st);
-hipError_t launch_paged_f32(const PagedArgs& a, hipStream_t st);
-hipError_t launch_paged_bf16(const PagedArgs& a, hipStream_t st);
-// ... bf16, tiles of many query rows, in a pass of `grid` workgroups
-hipError_t launch_paged_many(const PagedArgs& a, int pre, dim3 grid, hipStream_t st);
+// its parts: head_d <= 256, bf16 with many query rows, head_d > 256
+hipError_t launch_paged_narrow_f32(const PagedArgs& a, hipStream_t st);
+hipError_t launch_paged_narrow_bf16(const PagedArgs& a, hipStream_t st);
+hipError_t launch_paged_many(const PagedArgs& a, int pre, hipStream_t st);
+hipError_t launch_paged_wide(int dtype, const PagedArgs& a, hipStream_t st);
 
 }  // namespace atn

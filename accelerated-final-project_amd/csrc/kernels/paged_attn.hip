@@ -1,54 +1,96 @@
-// How a call of attention over a paged cache runs, and its launches (paged_attn_impl.hpp).
+// How a call of attention over a paged cache runs, its launches, and the merge of its parts
+// (paged_attn_impl.hpp).
 #include "paged_attn_impl.hpp"
 
 namespace atn {
 
 namespace {
 
+constexpr int kInWave = 64;  // groups that a wave's lanes hold
+
+// Many groups: where each sequence's own rows begin, and its group, once for the kernels that follow.
+// first ascends, so the last group that begins at or before b is the one.
+__global__ __launch_bounds__(256) void k_paged_starts(PagedArgs a, int2* starts) {
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b >= a.c.B) return;
+    int lo = 0, hi = a.groups;  // groups [0, lo) begin at or before b, [hi, groups) behind it
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.first[mid] <= b) lo = mid + 1;
+        else hi = mid;
+    }
+    int2 x = make_int2(0, -1);
+    if (lo > 0) {
+        const Groups g = group_at(a, lo - 1);
+        if (g.rows > 0 && b >= g.first && b < g.end) x = make_int2(g.rows, lo - 1);
+    }
+    starts[b] = x;
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A pass of `segments` segments of about R query rows of a kv head, at most `most` (all: of all
-// segments), over at most `keys` keys an item; kv: kv heads of a launch.
-PagedPass plan_pass(int dtype, int D, int64_t R, int64_t most, int64_t segments, int64_t all,
-                    int64_t keys, int kv, bool whole16) {
-    PagedPass p{};
-    const bool bf = dtype == kDtypeBF16, wide = D > kPagedNarrow;
-    p.many = bf && whole16 && D <= 128 && R > 32;
-    int per_cu;  // workgroups that a CU holds at once (the kernels' registers and LDS)
-    if (p.many) {
+// Which kernel takes items of about R query rows, and its tile.
+enum Kind { kNarrow, kMany, kWide };
+struct Tile {
+    Kind kind;
+    int rows;
+};
+Tile tile_of(int dtype, int D, int64_t R, bool whole16) {
+    const bool bf = dtype == kDtypeBF16;
+    if (D > kPagedNarrow) return {kWide, R <= 16 ? 16 : 32};
+    if (bf && whole16 && D <= 128 && R > 32) {
         // the tile that leaves the fewest rows empty, the larger of equals
-        p.rows = 64;
+        int best = 64;
         for (int rows : {128, 256})
-            if (ceil_div(R, rows) * rows <= ceil_div(R, p.rows) * p.rows) p.rows = rows;
+            if (ceil_div(R, rows) * rows <= ceil_div(R, best) * best) best = rows;
+        return {kMany, best};
+    }
+    return {kNarrow, R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64};
+}
+
+// A pass of `segments` segments of at most `most` query rows of a kv head (all: of all segments), over
+// at most `keys` keys an item; kv: kv heads of a launch.
+PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, int64_t all, int64_t keys,
+                    int kv) {
+    PagedPass p{};
+    const bool bf = dtype == kDtypeBF16;
+    p.many = t.kind == kMany;
+    p.rows = t.rows;
+    p.groups = 1;
+    const int mt = p.rows / 16;
+    int per_cu;  // workgroups that a CU holds at once (the kernels' registers and LDS)
+    if (t.kind == kMany) {
         per_cu = 1;
         p.kb = p.rows == 256 ? 64 : 128;
         p.turn = 1;
+    } else if (t.kind == kWide) {
+        per_cu = mt == 1 && !bf ? 3 : 2;
+        p.kb = kPagedWideBlock;
+        p.turn = kPagedWideTurn;
+        p.groups = (int)ceil_div(D, bf ? kPagedWideDims : kPagedWideDims / 2);
     } else {
-        p.rows = R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64;
-        const int mt = p.rows / 16;
-        per_cu = wide ? (mt == 1 ? 2 : 1)
-                      : std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
-        p.kb = wide ? kPagedWideKeys : bf ? 32 : 16;
-        p.turn = wide ? 1 : 4;
+        per_cu = std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
+        p.kb = bf ? 32 : 16;
+        p.turn = 4;
     }
     p.part_rows = (int)std::min<int64_t>(p.rows, most);
     p.tiles = (int)ceil_div(most, p.rows);
-    const int dims = D > 1024 ? 2048 : D > 512 ? 1024 : 512;
-    p.groups = wide ? (int)ceil_div(D, dims) : 1;
-    const int64_t items = kv * std::min(segments * p.tiles, ceil_div(all, p.rows) + segments);
+    p.items = kv * std::min(segments * p.tiles, ceil_div(all, p.rows) + segments);
     const int64_t slots = std::max<int64_t>(1, 256 * per_cu / p.groups);
     const int64_t blocks = ceil_div(keys, p.kb) + 1;
-    p.ranges =
-        (int)std::max<int64_t>(1, std::min(slots, ceil_div(items * (blocks + kPagedPad), 2 * p.turn)));
-    p.line = items * (blocks + kPagedPad) + 2ll * p.turn * p.ranges;
-    p.split = items < 4 * slots && blocks > 7 * p.turn / 2;
-    p.parts = p.ranges + items;
+    p.ranges = (int)std::max<int64_t>(
+        1, std::min(slots, ceil_div(p.items * (blocks + kPagedPad), 2 * p.turn)));
+    p.line = p.items * (blocks + kPagedPad) + 2ll * p.turn * p.ranges;
+    p.split = p.items < 4 * slots && blocks > 7 * p.turn / 2;
+    p.parts = p.ranges + p.items;
+    p.scores = t.kind == kWide ? p.items * blocks * p.rows * kPagedWideBlock : 0;
     return p;
 }
 
-size_t paged_starts_bytes(int B) { return ((size_t)B * sizeof(int2) + 15) / 16 * 16; }
+size_t to16(size_t n) { return (n + 15) / 16 * 16; }
+size_t starts_bytes(int B, int groups) { return groups > kInWave ? to16((size_t)B * sizeof(int2)) : 0; }
 size_t part_bytes(const PagedPass& p, int D) {
-    return ((size_t)p.parts * p.part_rows * (D + 4) * sizeof(float) + 15) / 16 * 16;
+    return to16((size_t)p.parts * p.part_rows * (D + 4) * sizeof(float));
 }
 
 }  // namespace
@@ -56,44 +98,86 @@ size_t part_bytes(const PagedPass& p, int D) {
 PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
                      size_t scratch_cap) {
     PagedPlan p{};
+    const int D = c.D;
     const int64_t R = (int64_t)(H / c.G) * T, all = R * c.B;
     whole16 = whole16 && c.page_rows % 16 == 0;
-    // all kv heads at once, unless the scratch does not hold their parts
+    Tile own = tile_of(dtype, D, R, whole16), pre = own;
+    if (groups > 0) {
+        // (groups are on the device: tiles for groups of equal size)
+        pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, whole16);
+        // one launch takes both, in tiles of as many rows
+        if (pre.kind != kMany) own.rows = pre.rows = std::max(own.rows, pre.rows);
+    }
+    p.wide = own.kind == kWide;
+    // all kv heads at once, unless the scratch does not hold their parts and scores
     for (p.kv = c.G;; p.kv = (p.kv + 1) / 2) {
-        p.own = plan_pass(dtype, c.D, R, R, c.B, all, c.rows, p.kv, whole16);
-        p.scratch = 0;
+        p.own = plan_pass(dtype, D, own, R, c.B, all, c.rows, p.kv);
         if (groups > 0) {
-            // (groups are on the device: tiles for groups of equal size)
-            p.pre = plan_pass(dtype, c.D, ceil_div(c.B, groups) * R, all, groups, all, c.rows, p.kv,
-                              whole16);
+            p.pre = plan_pass(dtype, D, pre, all, groups, all, c.rows, p.kv);
             p.pre.split = 1;
-            p.scratch = paged_starts_bytes(c.B) + part_bytes(p.pre, c.D);
+            p.pre.workgroups = (int64_t)p.pre.ranges * p.pre.groups;
+            p.first = pre.kind == kMany ? 0 : (int)p.pre.workgroups;
         }
         if (!p.own.split) p.own.parts = (int64_t)c.B * p.kv * p.own.tiles;
-        if (groups > 0 || p.own.split) p.scratch += part_bytes(p.own, c.D);
         p.own.workgroups =
             (p.own.split ? p.own.ranges : (int64_t)c.B * p.kv * p.own.tiles) * p.own.groups;
+        // scores: two workgroups a CU, where the dims give each wave two steps still
+        p.shares = 1;
+        const int64_t blocks = (p.own.scores + p.pre.scores) / (p.own.rows * kPagedWideBlock);
+        while (p.wide && blocks * p.shares < 512 && p.shares < 8 &&
+               D >= 2 * p.shares * 8 * (dtype == kDtypeBF16 ? 256 : 128))
+            p.shares *= 2;
+        p.score_grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks * p.shares, 1024));
+        p.scratch = starts_bytes(c.B, groups) +
+                    (size_t)(p.own.scores + p.pre.scores) * p.shares * sizeof(float);
+        if (groups > 0) p.scratch += part_bytes(p.pre, D);
+        if (groups > 0 || p.own.split) p.scratch += part_bytes(p.own, D);
         if (p.scratch <= scratch_cap || p.kv == 1) break;
     }
-    if (p.scratch > scratch_cap && groups == 0) {  // items whole: no parts
+    if (p.scratch > scratch_cap && groups == 0 && p.own.split) {  // items whole: no parts
+        p.scratch -= part_bytes(p.own, D);
         p.own.split = 0;
         p.own.workgroups = (int64_t)c.B * p.kv * p.own.tiles * p.own.groups;
-        p.scratch = 0;
     }
     return p;
 }
 
 hipError_t launch_paged_attention(int dtype, PagedArgs a, void* scratch, hipStream_t st) {
     char* at = static_cast<char*>(scratch);
+    if (a.groups > kInWave) {
+        int2* starts = reinterpret_cast<int2*>(at);
+        hipLaunchKernelGGL(k_paged_starts, dim3((unsigned)((a.c.B + 255) / 256)), dim3(256), 0, st, a,
+                           starts);
+        a.starts = starts;
+        at += starts_bytes(a.c.B, a.groups);
+    }
+    a.own_scores = reinterpret_cast<float*>(at);
+    at += (size_t)a.plan.own.scores * a.plan.shares * sizeof(float);
+    a.pre_scores = reinterpret_cast<float*>(at);
+    at += (size_t)a.plan.pre.scores * a.plan.shares * sizeof(float);
     if (a.groups > 0) {
-        a.starts = reinterpret_cast<int2*>(at);
-        a.pre_part = reinterpret_cast<float*>(at += paged_starts_bytes(a.c.B));
+        a.pre_part = reinterpret_cast<float*>(at);
         at += part_bytes(a.plan.pre, a.c.D);
     }
     a.own_part = reinterpret_cast<float*>(at);
     for (a.g0 = 0; a.g0 < a.c.G; a.g0 += a.plan.kv) {
         a.gs = std::min(a.plan.kv, a.c.G - a.g0);
-        const hipError_t e = dtype == kDtypeF32 ? launch_paged_f32(a, st) : launch_paged_bf16(a, st);
+        PagedArgs x = a;
+        if (!x.plan.own.split)
+            x.plan.own.workgroups = (int64_t)x.c.B * x.gs * x.plan.own.tiles * x.plan.own.groups;
+        hipError_t e = hipGetLastError();
+        if (e == hipSuccess && x.plan.wide) e = launch_paged_wide(dtype, x, st);
+        if (e == hipSuccess && x.plan.pre.many) e = launch_paged_many(x, 1, st);
+        if (e == hipSuccess && x.plan.own.many) e = launch_paged_many(x, 0, st);
+        if (e == hipSuccess && !x.plan.wide && !x.plan.own.many)
+            e = dtype == kDtypeF32 ? launch_paged_narrow_f32(x, st) : launch_paged_narrow_bf16(x, st);
+        if (e == hipSuccess && (x.groups > 0 || x.plan.own.split)) {
+            if (dtype == kDtypeF32)
+                go_merge<float>(x, st);
+            else
+                go_merge<uint16_t>(x, st);
+            e = hipGetLastError();
+        }
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -25,8 +25,8 @@ namespace atn {
 
 constexpr int kPagedNarrow = 256;  // head_d up to which a wave holds a row tile's output
 constexpr int kPagedPad = 12;      // places of the line that beginning and ending an item count for
-constexpr int kPagedWideKeys = 64; // keys between barriers of k_paged_wide
-constexpr int kPagedWideWaves = 8;
+constexpr int kPagedWideBlock = 32, kPagedWideTurn = 4;  // head_d above: keys of a block, blocks between barriers
+constexpr int kPagedWideDims = 512;  // ... dims of a workgroup (bf16; fp32: half)
 
 namespace {
 
@@ -42,24 +42,55 @@ struct Segment {
 __device__ __forceinline__ int tokens_of(const PagedArgs& a, int b) {
     return a.count ? min(max(a.count[b], 0), a.T) : a.T;
 }
+// The group in lane L of a wave (of the first 64): its sequences and rows.
+struct Groups {
+    int first, end, rows;
+};
 // (a group of one reads its rows as its own; first and shared may hold anything)
+__device__ __forceinline__ Groups group_at(const PagedArgs& a, int i) {
+    Groups g;
+    g.first = min(max(a.first[i], 0), a.c.B - 1);
+    g.end = min(max(a.first[i + 1], 0), a.c.B);
+    const int L = min(rows_in_use(a.c, g.first), a.c.rows);
+    g.rows = g.end - g.first >= 2 ? min(max(a.shared[i], 0), L) : 0;
+    return g;
+}
+__device__ __forceinline__ Groups groups_of(const PagedArgs& a, int lane) {
+    Groups g{0, 0, 0};
+    if (lane < a.groups && !a.starts) g = group_at(a, lane);
+    return g;
+}
+// Where sequence b's own rows begin, and its group or -1 (a wave's work; b may differ by lane).
+__device__ __forceinline__ int2 start_of(const PagedArgs& a, const Groups& g, int b) {
+    if (a.starts) return a.starts[b];
+    int2 x = make_int2(0, -1);
+    for (int i = 0; i < a.groups; ++i) {
+        const int rows = __builtin_amdgcn_readlane(g.rows, i);
+        if (rows > 0 && b >= __builtin_amdgcn_readlane(g.first, i) &&
+            b < __builtin_amdgcn_readlane(g.end, i))
+            x = make_int2(rows, i);
+    }
+    return x;
+}
+// (a wave's work; i may differ by lane, and be past the last)
 template <int PRE>
-__device__ __forceinline__ Segment segment(const PagedArgs& a, int i) {
+__device__ __forceinline__ Segment segment(const PagedArgs& a, const Groups& gr, int i) {
     Segment s;
     if (PRE) {
-        s.first = min(max(a.first[i], 0), a.c.B - 1);
-        s.members = min(max(a.first[i + 1], 0), a.c.B) - s.first;
+        const Groups g = group_at(a, min(i, a.groups - 1));
+        s.first = g.first;
+        s.members = g.end - g.first;
         s.lo = 0;
-        const int L = min(rows_in_use(a.c, s.first), a.c.rows);
-        s.hi = s.members >= 2 ? min(max(a.shared[i], 0), L) : 0;
+        s.hi = g.rows;
         s.tiles = s.hi > 0 ? (s.members * a.T * a.rep + a.plan.pre.rows - 1) / a.plan.pre.rows : 0;
         s.len = 0;
     } else {
+        i = min(i, a.c.B - 1);
         const int n = tokens_of(a, i);
         s.first = i;
         s.members = 1;
         s.len = rows_in_use(a.c, i);
-        s.lo = a.starts ? a.starts[i].x : 0;
+        s.lo = start_of(a, gr, i).x;
         s.hi = min(s.len + n, a.c.rows);
         s.tiles = (n * a.rep + a.plan.own.rows - 1) / a.plan.own.rows;
     }
@@ -82,26 +113,26 @@ struct Line {
     int n, m, upto, items;
 };
 template <int PRE>
-__device__ __forceinline__ void line_lane(const PagedArgs& a, int i, int count, int kb, int* n, int* m) {
-    *n = *m = 0;
-    if (i >= count) return;
-    const Segment s = segment<PRE>(a, i);
-    *m = s.tiles * a.gs;
-    *n = blocks_of(s, kb) + kPagedPad;
+__device__ __forceinline__ void line_lane(const PagedArgs& a, const Groups& gr, int i, int count,
+                                          int kb, int pad, int* n, int* m) {
+    const Segment s = segment<PRE>(a, gr, i);
+    *m = i < count ? s.tiles * a.gs : 0;
+    *n = blocks_of(s, kb) + pad;
 }
 template <int PRE>
-__device__ __forceinline__ Line line_of(const PagedArgs& a, int kb, int lane) {
+__device__ __forceinline__ Line line_of(const PagedArgs& a, const Groups& gr, int kb, int lane,
+                                        int pad = kPagedPad) {
     const PagedPass& p = pass_of<PRE>(a);
     const int count = PRE ? a.groups : a.c.B;
     Line x;
-    line_lane<PRE>(a, lane, count, kb, &x.n, &x.m);
+    line_lane<PRE>(a, gr, lane, count, kb, pad, &x.n, &x.m);
     x.upto = wave_scan(x.n * x.m);
     x.items = wave_scan(x.m);
     x.total = __builtin_amdgcn_readlane(x.upto, 63);
 #pragma unroll 1
     for (int i0 = 64; i0 < count; i0 += 64) {
         int n, m;
-        line_lane<PRE>(a, i0 + lane, count, kb, &n, &m);
+        line_lane<PRE>(a, gr, i0 + lane, count, kb, pad, &n, &m);
         x.total += __builtin_amdgcn_readlane(wave_scan(n * m), 63);
     }
     const int per = (x.total + p.ranges - 1) / p.ranges;
@@ -113,8 +144,8 @@ struct Place {
     int seg, n, start, items;
 };
 template <int PRE>
-__device__ __forceinline__ Place place_at(const PagedArgs& a, const Line& line, int at, int kb,
-                                          int lane) {
+__device__ __forceinline__ Place place_at(const PagedArgs& a, const Groups& gr, const Line& line, int at,
+                                          int kb, int lane, int pad = kPagedPad) {
     const int count = PRE ? a.groups : a.c.B;
     int n = line.n, m = line.m, upto = line.upto, items = line.items;
 #pragma unroll 1
@@ -132,22 +163,22 @@ __device__ __forceinline__ Place place_at(const PagedArgs& a, const Line& line, 
         }
         const int before = __builtin_amdgcn_readlane(upto, 63);
         const int ibefore = __builtin_amdgcn_readlane(items, 63);
-        line_lane<PRE>(a, i0 + 64 + lane, count, kb, &n, &m);
+        line_lane<PRE>(a, gr, i0 + 64 + lane, count, kb, pad, &n, &m);
         upto = before + wave_scan(n * m);
         items = ibefore + wave_scan(m);
     }
 }
 // ... of segment i
 template <int PRE>
-__device__ __forceinline__ Place place_of(const PagedArgs& a, const Line& line, int i, int kb,
-                                          int lane) {
+__device__ __forceinline__ Place place_of(const PagedArgs& a, const Groups& gr, const Line& line, int i,
+                                          int kb, int lane, int pad = kPagedPad) {
     const int count = PRE ? a.groups : a.c.B;
     int n = line.n, m = line.m, upto = line.upto, items = line.items, i0 = 0;
 #pragma unroll 1
     for (; i >= i0 + 64; i0 += 64) {
         const int before = __builtin_amdgcn_readlane(upto, 63);
         const int ibefore = __builtin_amdgcn_readlane(items, 63);
-        line_lane<PRE>(a, i0 + 64 + lane, count, kb, &n, &m);
+        line_lane<PRE>(a, gr, i0 + 64 + lane, count, kb, pad, &n, &m);
         upto = before + wave_scan(n * m);
         items = ibefore + wave_scan(m);
     }
@@ -162,9 +193,11 @@ __device__ __forceinline__ Place place_of(const PagedArgs& a, const Line& line, 
 
 // A range's blocks [first, last) of one item (counted from row 0 of the cache), and where they go:
 // part < 0: the output.
+// blocks_before: of the line, before the item's.
 struct Span {
     Segment s;
     int seg, g, tile, first, last, part;
+    int blocks_before;
 };
 __device__ __forceinline__ int bounded(const PagedPass& p, int part) {
     // (groups that overlap have more items than the host counts on)
@@ -178,12 +211,12 @@ __device__ __forceinline__ int tile_end(const PagedArgs& a, const Segment& s, in
     return (min(s.hi, s.len + tok + 1) + kb - 1) / kb;
 }
 template <int PRE>
-__device__ __forceinline__ Span span_at(const PagedArgs& a, const Line& line, int r, int at, int end,
-                                        int kb, int lane, int* next) {
-    const Place p = place_at<PRE>(a, line, at, kb, lane);
+__device__ __forceinline__ Span span_at(const PagedArgs& a, const Groups& gr, const Line& line, int r,
+                                        int at, int end, int kb, int lane, int* next) {
+    const Place p = place_at<PRE>(a, gr, line, at, kb, lane);
     Span x;
     x.seg = p.seg;
-    x.s = segment<PRE>(a, p.seg);
+    x.s = segment<PRE>(a, gr, p.seg);
     x.s.lo = of_wave(x.s.lo), x.s.hi = of_wave(x.s.hi), x.s.len = of_wave(x.s.len);
     x.s.first = of_wave(x.s.first), x.s.members = of_wave(x.s.members), x.s.tiles = of_wave(x.s.tiles);
     const int off = at - p.start, item = (unsigned)off / (unsigned)p.n, in = off - item * p.n;
@@ -195,6 +228,7 @@ __device__ __forceinline__ Span span_at(const PagedArgs& a, const Line& line, in
     x.last = out - kPagedPad;
     const bool alone = !PRE && x.s.lo == 0 && x.first == 0 && out == p.n;
     x.part = alone ? -1 : bounded(pass_of<PRE>(a), r + p.items + item);
+    x.blocks_before = at - in - kPagedPad * (p.items + item);
     x.first += b0;
     x.last += b0;
     *next = at + out - in;
@@ -202,12 +236,12 @@ __device__ __forceinline__ Span span_at(const PagedArgs& a, const Line& line, in
 }
 // The whole of item `id`, where items are workgroups (own pass alone): the tiles with the most keys
 // first.
-__device__ __forceinline__ Span span_whole(const PagedArgs& a, int id, int kb) {
+__device__ __forceinline__ Span span_whole(const PagedArgs& a, const Groups& gr, int id, int kb) {
     Span x;
     const int items = a.c.B * a.gs, tile = a.plan.own.tiles - 1 - (unsigned)id / (unsigned)items;
     const int pair = id % (unsigned)items;
     x.seg = pair / (unsigned)a.gs;
-    x.s = segment<0>(a, x.seg);
+    x.s = segment<0>(a, gr, x.seg);
     x.s.lo = of_wave(x.s.lo), x.s.hi = of_wave(x.s.hi), x.s.len = of_wave(x.s.len);
     x.s.tiles = of_wave(x.s.tiles);
     x.g = a.g0 + pair - x.seg * a.gs;
@@ -271,40 +305,28 @@ __device__ __forceinline__ float* part_dims(const PagedArgs& a) {
     return (PRE ? a.pre_part : a.own_part) + 4 * part_row<PRE>(a, (int)pass_of<PRE>(a).parts, 0);
 }
 
-// Where each sequence's own rows begin, and its group: the prefix pass's first workgroup writes them
-// for what follows on the stream.
-__device__ __forceinline__ void write_starts(const PagedArgs& a) {
-    for (int b = threadIdx.x; b < a.c.B; b += blockDim.x) {
-        int2 x = make_int2(0, -1);
-        for (int i = 0; i < a.groups; ++i) {
-            const Segment s = segment<1>(a, i);
-            if (s.hi > 0 && b >= s.first && b < s.first + s.members) x = make_int2(s.hi, i);
-        }
-        a.starts[b] = x;
-    }
-}
-
 // ---------------------------------------------------------------- steps of a block
 // bit j: j < n
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
 
-// Scores of what a row does not attend become -infinity: of the 32 (16) keys from j0 on, those
-// past the row's, before the item's, and of no page (`there`).  Returns the keys that stay, as
-// this lane holds them: bit 4 u + e.
+// The keys that a row attends of the 32 (16) from j0 on, as a lane of group q holds them (bit 4 u +
+// e): not those past the row's, before the item's, and of no page (`there`).
 template <int SUB>
-__device__ __forceinline__ uint32_t hide(float (&p)[SUB][4], int j0, int lo, int upto, uint32_t there,
-                                         int q) {
+__device__ __forceinline__ uint32_t seen(int j0, int lo, int upto, uint32_t there, int q) {
     const uint32_t see = there & below(upto - j0) & ~below(lo - j0);
     uint32_t mine = 0;
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-        const uint32_t four = see >> (16 * u + 4 * q) & 15u;
-        mine |= four << (4 * u);
+    for (int u = 0; u < SUB; ++u) mine |= (see >> (16 * u + 4 * q) & 15u) << (4 * u);
+    return mine;
+}
+// Scores of the others become -infinity.
+template <int SUB>
+__device__ __forceinline__ void hide(float (&p)[SUB][4], uint32_t mine) {
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (!((four >> e) & 1u)) p[u][e] = -INFINITY;
-    }
-    return mine;
+            if (!((mine >> (4 * u + e)) & 1u)) p[u][e] = -INFINITY;
 }
 
 // Scores into weights.  The running maximum moves only when a score passes it by more than 8
@@ -587,23 +609,28 @@ __device__ __forceinline__ void write_rows(const PagedArgs& a, const Span& sp, c
 }
 
 // A workgroup's spans, one after another: f(span).
-template <int PRE, typename F>
+template <int PRE, bool SCORES = false, typename F>
 __device__ __forceinline__ void each_span(const PagedArgs& a, int id, int kb, int lane, F f) {
     const bool split = PRE || a.plan.own.split;
     int at = 0, end = 1;
     Line line{};
+    const Groups gr = groups_of(a, lane);
     if (split) {
-        line = line_of<PRE>(a, kb, lane);
+        line = line_of<PRE>(a, gr, kb, lane);
         at = id * line.per;
         end = min(line.total, at + line.per);
     }
     while (at < end) {
         Span sp;
         if (split) {
-            sp = span_at<PRE>(a, line, id, at, end, kb, lane, &at);
+            sp = span_at<PRE>(a, gr, line, id, at, end, kb, lane, &at);
         } else {
-            sp = span_whole(a, id, kb);
+            sp = span_whole(a, gr, id, kb);
             at = end;
+            if (SCORES) {
+                const Place p = place_of<0>(a, gr, line_of<0>(a, gr, kb, lane, 0), sp.seg, kb, lane, 0);
+                sp.blocks_before = p.start + ((sp.g - a.g0) * sp.s.tiles + sp.tile) * p.n;
+            }
         }
         if (sp.last > sp.first) f(sp);
     }
@@ -619,7 +646,7 @@ struct PagedNarrow : CacheTiles<T, DP, MT, MODE> {
     static constexpr int WAVES = 4;
     // registers: the output tile, K and V of a block, the scores and weights, addresses; with the
     // next block's K loaded ahead except where only that would not leave two waves a SIMD
-    static constexpr int kRegs = DP / 4 * (MT + 1) + 20 * MT + 56;
+    static constexpr int kRegs = DP / 4 * (MT + 1) + 20 * MT + 44;
     static constexpr int kWith = kRegs + DP / 4;
     static constexpr bool kAhead = kWith <= 250 || kRegs > 220;
     static constexpr int kMinWaves = kWith <= 124 ? 4 : kWith <= 164 ? 3 : kRegs <= 220 ? 2 : 1;
@@ -633,18 +660,15 @@ struct PagedNarrow : CacheTiles<T, DP, MT, MODE> {
 };
 
 template <typename T, int DP, int MT, int MODE, bool RUNS, int PRE>
-__global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE>::kMinWaves)) void k_paged_narrow(
-    PagedArgs a) {
+__device__ __forceinline__ void paged_narrow(const PagedArgs& a, int id, char* lds) {
     using N = PagedNarrow<T, DP, MT, MODE>;
     constexpr int KB = N::KB, SUB = N::SUB, KS = N::KS, VS = N::VS, VL = N::VL, WAVES = N::WAVES;
-    __shared__ __align__(16) char lds[N::kLds];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
     const int D = MODE == kExact ? DP : a.c.D;
     const float scale = fabsf(a.scale);
-    if (PRE && blockIdx.x == 0) write_starts(a);
 
-    each_span<PRE>(a, blockIdx.x, KB, lane, [&](const Span& sp) {
+    each_span<PRE>(a, id, KB, lane, [&](const Span& sp) {
         const T* kp = (const T*)a.c.K + sp.g * a.c.ks[1];
         const T* vp = (const T*)a.c.V + sp.g * a.c.vs[1];
         const int row0 = sp.tile * N::ROWS, lo = sp.s.lo;
@@ -731,9 +755,10 @@ __global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE>::kMinWaves)) voi
             uint32_t see[MT];
             if (part) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
-                    see[t] = hide<SUB>(p[t], i * KB, lo, attended<PRE>(a, sp, row0 + 16 * t + col),
-                                       there, q);
+                for (int t = 0; t < MT; ++t) {
+                    see[t] = seen<SUB>(i * KB, lo, attended<PRE>(a, sp, row0 + 16 * t + col), there, q);
+                    hide<SUB>(p[t], see[t]);
+                }
             }
 #pragma unroll
             for (int t = 0; t < MT; ++t)
@@ -798,181 +823,17 @@ __global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE>::kMinWaves)) voi
     });
 }
 
-// ---------------------------------------------------------------- head_d > 256
-// No output tile fits a wave's registers: the 8 waves of a workgroup share the dims.  For each 64
-// keys every wave adds its share of the dims to the scores, the shares meet in LDS, and every wave
-// has all weights for its 16 VL VS dims of the output.  Heads of more dims than the workgroup's
-// waves hold take several workgroups, each with all scores (K comes again from the L2 that they
-// share: their numbers are 8 apart).
-template <typename T, int DP, int MT>
-struct PagedWide : CacheTiles<T, DP, MT, kClamp> {
-    using N = CacheTiles<T, DP, MT, kClamp>;
-    static constexpr int DIMS = DP * kPagedWideWaves;  // of a workgroup
-};
-
-template <typename T, int DP, int MT, int PRE>
-__global__ __launch_bounds__(64 * kPagedWideWaves, 2) void
-k_paged_wide(PagedArgs a) {
-    using N = PagedWide<T, DP, MT>;
-    constexpr int WK = kPagedWideKeys, U = WK / 16, SUB = N::SUB, KB = N::KB, VS = N::VS, VL = N::VL;
-    constexpr int W = kPagedWideWaves;
-    __shared__ v4f red[W][MT * U * 64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int q = lane >> 4, col = lane & 15, D = a.c.D;
-    const float scale = a.scale;
-    const PagedPass& pass = pass_of<PRE>(a);
-    const int groups = pass.groups;
-    // (the workgroups of a range are 8 apart, on one XCD)
-    const int units = (int)(gridDim.x / (unsigned)groups), full = units / 8 * 8 * groups;
-    const int id = blockIdx.x;
-    const int y = id < full ? id / 8 : id - full;
-    const int unit = id < full ? y / groups * 8 + id % 8 : units / 8 * 8 + y / groups;
-    const int d0 = (y % groups * W + wave) * DP;
-    const bool busy = d0 < D;
-    if (PRE && blockIdx.x == 0) write_starts(a);
-
-    each_span<PRE>(a, unit, WK, lane, [&](const Span& sp) {
-        const T* kp = (const T*)a.c.K + sp.g * a.c.ks[1];
-        const T* vp = (const T*)a.c.V + sp.g * a.c.vs[1] + d0;
-        const int row0 = sp.tile * N::ROWS, lo = sp.s.lo;
-        const int last = min(sp.last, tile_end<PRE>(a, sp.s, sp.tile, WK));
-        const int w0 = (lo + WK - 1) / WK, w1 = of_wave(attended<PRE>(a, sp, row0)) / WK;
-        const T* qp[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) qp[t] = (const T*)a.Q + q_at<PRE>(a, sp, row0 + 16 * t + col);
-        v4f o[MT][VS][VL];
-        float m[MT], l[MT], used[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            m[t] = -INFINITY;
-            l[t] = used[t] = 0.f;
-#pragma unroll
-            for (int x = 0; x < VS; ++x)
-#pragma unroll
-                for (int c = 0; c < VL; ++c) o[t][x][c] = v4f{0.f, 0.f, 0.f, 0.f};
-        }
-        int page[U], next[U];  // of keys 16 u + col
-        auto fetch = [&](int (&to)[U], int i) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) to[u] = page_of(a.c, sp.s.first, i * WK + 16 * u + col);
-        };
-        auto at = [&](const int64_t (&st)[3], int r, int p) {
-            return (is_page(a.c, p) ? p : 0) * st[0] +
-                   (r - over(r, a.c.by_page) * a.c.page_rows) * st[2];
-        };
-        fetch(page, sp.first);
-#pragma unroll 1
-        for (int i = sp.first; i < last; ++i) {
-            const T* kr[U];
-            uint64_t there = 0;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                kr[u] = kp + at(a.c.ks, i * WK + 16 * u + col, page[u]);
-                there |= (__builtin_amdgcn_ballot_w64(is_page(a.c, page[u])) & 0xffffu) << (16 * u);
-            }
-            fetch(next, i + 1);
-            // the first KB keys' V on their way beside K
-            typename N::Vals v;
-            auto load_v = [&](int k) {
-#pragma unroll
-                for (int j = 0; j < N::KEYS; ++j) {
-                    const int key = N::key_of(lane, j), r = i * WK + k * KB + key;
-                    const int p = __shfl(page[k * SUB + (j >> 2)], key & 15);
-                    const T* row = vp + at(a.c.vs, r, p);
-#pragma unroll
-                    for (int x = 0; x < VS; ++x) v.p[j][x] = N::v_piece(row, 0, x, D - d0, lane);
-                }
-            };
-            if (busy) load_v(0);
-            v4f s[MT][U];
-            wide_scores<T, MT, false>(s, kr, qp, D, wave, W, q);
-            __syncthreads();  // (the scores before have been read)
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int u = 0; u < U; ++u) red[wave][(t * U + u) * 64 + lane] = s[t][u];
-            __syncthreads();
-            const bool part = i < w0 || i >= w1 || there != ~0ull;
-#pragma unroll
-            for (int k = 0; k < WK / KB; ++k) {
-                float p[MT][SUB][4];
-                uint32_t see[MT];
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u) {
-                        v4f z = red[0][(t * U + k * SUB + u) * 64 + lane];
-#pragma unroll
-                        for (int w = 1; w < W; ++w) z += red[w][(t * U + k * SUB + u) * 64 + lane];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) p[t][u][e] = z[e] * scale;
-                    }
-                    if (part)
-                        see[t] = hide<SUB>(p[t], i * WK + k * KB, lo,
-                                           attended<PRE>(a, sp, row0 + 16 * t + col),
-                                           (uint32_t)(there >> (k * KB)), q);
-                    weights<SUB, VS, VL>(p[t], o[t], m[t], l[t], used[t], 1.f);
-                }
-                if (busy && part && not_finite<T>(v)) spread_not_finite<T, N, MT>(o, v, see);
-                if (busy) {
-                    N::accumulate(o, v, p, used);
-                    if (k + 1 < WK / KB) load_v(k + 1);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) page[u] = next[u];
-        }
-        if (!busy) return;
-        // (computed here: hoisted out of the loop over spans, these take the loop's registers)
-        const int late = opaque(lane), lq = late >> 4, lc = late & 15;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            l[t] = row_sum(l[t]);
-            used[t] = sizeof(T) == 2 ? row_sum(used[t]) : l[t];
-            const int r = 16 * t + lc;
-            const Row to = row_of<PRE>(a, sp, row0 + r);
-            if (to.b < 0) continue;
-            const float4 z = make_float4(m[t], l[t], used[t], 0.f);
-            const bool parted = PRE || sp.part >= 0, zero = !parted && z.z == 0.f;
-            const size_t pr = part_row<PRE>(a, max(sp.part, 0), r);
-            const float inv = parted ? 1.f : 1.f / z.z;
-            if (lq == 0 && d0 == 0) {
-                if (parted)
-                    part_stats<PRE>(a)[pr] = z;
-                else if (a.lse)
-                    a.lse[((size_t)to.b * a.H + to.h) * a.T + to.tok] = lse_of(z);
-            }
-            float* dims = part_dims<PRE>(a) + pr * D + d0;
-            T* out = (T*)a.out + to.b * a.os[0] + to.h * a.os[1] + to.tok * a.os[2] + d0;
-#pragma unroll
-            for (int x = 0; x < VS; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = N::dim_of(x, 4 * lq + e, D - d0);
-#pragma unroll
-                    for (int c = 0; c < VL; c += 4) {
-                        float y[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) y[r] = zero ? 0.f : o[t][x][c + r][e] * inv;
-                        if (d + c >= 0) {
-                            if (parted)
-                                store4(dims + d + c, y, 4);
-                            else
-                                store4(out + d + c, y, 4);
-                        } else {  // (a row's last dims, fewer than a piece)
-#pragma unroll
-                            for (int r = 1; r < 4; ++r)
-                                if (d + c + r >= 0) {
-                                    if (parted)
-                                        dims[d + c + r] = y[r];
-                                    else
-                                        Elem<T>::st(out, d + c + r, y[r]);
-                                }
-                        }
-                    }
-                }
-        }
-    });
+// The first workgroups take the prefixes' ranges (where those are tiles of as many rows), the others
+// the sequences' own.
+template <typename T, int DP, int MT, int MODE, bool RUNS>
+__global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE>::kMinWaves)) void k_paged_narrow(
+    PagedArgs a) {
+    __shared__ __align__(16) char lds[PagedNarrow<T, DP, MT, MODE>::kLds];
+    const int id = (int)blockIdx.x - a.plan.first;
+    if (id < 0)
+        paged_narrow<T, DP, MT, MODE, RUNS, 1>(a, blockIdx.x, lds);
+    else
+        paged_narrow<T, DP, MT, MODE, RUNS, 0>(a, id, lds);
 }
 
 // ---------------------------------------------------------------- parts
@@ -990,14 +851,15 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     const unsigned pair = blockIdx.y, seq = pair / (unsigned)a.gs;
     const int b = (int)seq, lg = (int)(pair - seq * a.gs);
     const int tok = over(row, a.by_rep), h = (a.g0 + lg) * a.rep + row - tok * a.rep;
-    const Segment s = segment<0>(a, b);
+    const Groups gr = groups_of(a, lane);
+    const Segment s = segment<0>(a, gr, b);
     if (tok >= tokens_of(a, b)) return;
     // the parts: own0 .. own0 + own - 1 of the own pass, pre0 .. pre0 + pre - 1 of the other
     int own0 = 0, own = 1, pre0 = 0, pre = 0;
     const int tile = row / a.plan.own.rows, in_tile = row - tile * a.plan.own.rows;
     if (a.plan.own.split) {
-        const Line line = line_of<0>(a, a.plan.own.kb, lane);
-        const Place p = place_of<0>(a, line, b, a.plan.own.kb, lane);
+        const Line line = line_of<0>(a, gr, a.plan.own.kb, lane);
+        const Place p = place_of<0>(a, gr, line, b, a.plan.own.kb, lane);
         const int item = lg * s.tiles + tile, first = p.start + item * p.n + kPagedPad;
         const int r0 = (unsigned)first / (unsigned)line.per;
         const int r1 = (unsigned)(first + p.n - kPagedPad - 1) / (unsigned)line.per;
@@ -1006,12 +868,12 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     } else {
         own0 = (b * a.gs + lg) * a.plan.own.tiles + tile;
     }
-    const int group = a.starts ? a.starts[b].y : -1;
+    const int group = of_wave(start_of(a, gr, b).y);
     int pre_in = 0;
     if (group >= 0) {
-        const Segment g = segment<1>(a, group);
-        const Line line = line_of<1>(a, a.plan.pre.kb, lane);
-        const Place p = place_of<1>(a, line, group, a.plan.pre.kb, lane);
+        const Segment g = segment<1>(a, gr, group);
+        const Line line = line_of<1>(a, gr, a.plan.pre.kb, lane);
+        const Place p = place_of<1>(a, gr, line, group, a.plan.pre.kb, lane);
         const int prow = (b - g.first) * a.T * a.rep + row, ptile = prow / a.plan.pre.rows;
         pre_in = prow - ptile * a.plan.pre.rows;
         const int item = lg * g.tiles + ptile, first = p.start + item * p.n + kPagedPad;
@@ -1075,66 +937,44 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
 }
 
 // ---------------------------------------------------------------- launches
-template <typename T, int DP, int MT, int MODE, int PRE>
-void paged_pages(const PagedArgs& a, dim3 grid, hipStream_t st) {
+template <typename T, int DP, int MT, int MODE>
+void go_pages(const PagedArgs& a, dim3 grid, hipStream_t st) {
     if (a.c.page_rows % 16 == 0)
-        hipLaunchKernelGGL((k_paged_narrow<T, DP, MT, MODE, true, PRE>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_paged_narrow<T, DP, MT, MODE, true>), grid, dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((k_paged_narrow<T, DP, MT, MODE, false, PRE>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_paged_narrow<T, DP, MT, MODE, false>), grid, dim3(256), 0, st, a);
 }
-template <typename T, int DP, int MODE, int PRE>
-void paged_rows(const PagedArgs& a, dim3 grid, hipStream_t st) {
-    if (pass_of<PRE>(a).rows == 16) return paged_pages<T, DP, 1, MODE, PRE>(a, grid, st);
-    if (pass_of<PRE>(a).rows == 32) return paged_pages<T, DP, 2, MODE, PRE>(a, grid, st);
-    if constexpr (DP == 64 && sizeof(T) == 2) paged_pages<T, DP, 4, MODE, PRE>(a, grid, st);
+template <typename T, int DP, int MODE>
+void go_rows(const PagedArgs& a, dim3 grid, hipStream_t st) {
+    if (a.plan.own.rows == 16) return go_pages<T, DP, 1, MODE>(a, grid, st);
+    if (a.plan.own.rows == 32) return go_pages<T, DP, 2, MODE>(a, grid, st);
+    if constexpr (DP == 64 && sizeof(T) == 2) go_pages<T, DP, 4, MODE>(a, grid, st);
 }
-template <typename T, int DP, int PRE>
-void paged_dims(const PagedArgs& a, dim3 grid, hipStream_t st) {
-    if (a.c.D == DP) return paged_rows<T, DP, kExact, PRE>(a, grid, st);
+template <typename T, int DP>
+void go_dims(const PagedArgs& a, dim3 grid, hipStream_t st) {
+    if (a.c.D == DP) return go_rows<T, DP, kExact>(a, grid, st);
     if constexpr (DP == 64) {
-        if (a.c.D < 16 / (int)sizeof(T)) return paged_rows<T, DP, kElem, PRE>(a, grid, st);
+        if (a.c.D < 16 / (int)sizeof(T)) return go_rows<T, DP, kElem>(a, grid, st);
     }
-    paged_rows<T, DP, kClamp, PRE>(a, grid, st);
-}
-template <typename T, int DP, int PRE>
-void paged_wide(const PagedArgs& a, dim3 grid, hipStream_t st) {
-    const dim3 block(64 * kPagedWideWaves);
-    if (pass_of<PRE>(a).rows == 16)
-        hipLaunchKernelGGL((k_paged_wide<T, DP, 1, PRE>), grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL((k_paged_wide<T, DP, 2, PRE>), grid, block, 0, st, a);
-}
-template <typename T, int PRE>
-void paged_pass(const PagedArgs& a, hipStream_t st) {
-    const PagedPass& p = pass_of<PRE>(a);
-    const int64_t units = PRE || p.split ? p.ranges : (int64_t)a.c.B * a.gs * p.tiles;
-    const dim3 grid((unsigned)(units * p.groups));
-    const int D = a.c.D;
-    if constexpr (sizeof(T) == 2) {
-        if (p.many) return (void)launch_paged_many(a, PRE, grid, st);
-    }
-    if (D > 1024) return paged_wide<T, 256, PRE>(a, grid, st);
-    if (D > 512) return paged_wide<T, 128, PRE>(a, grid, st);
-    if (D > kPagedNarrow) return paged_wide<T, 64, PRE>(a, grid, st);
-    if (D <= 64) return paged_dims<T, 64, PRE>(a, grid, st);
-    if (D <= 128) return paged_dims<T, 128, PRE>(a, grid, st);
-    if (D <= 192) return paged_dims<T, 192, PRE>(a, grid, st);
-    paged_dims<T, 256, PRE>(a, grid, st);
+    go_rows<T, DP, kClamp>(a, grid, st);
 }
 template <typename T>
-void paged_merge(const PagedArgs& a, hipStream_t st) {
+void go_narrow(const PagedArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)(a.plan.first + a.plan.own.workgroups));
+    const int D = a.c.D;
+    if (D <= 64) return go_dims<T, 64>(a, grid, st);
+    if (D <= 128) return go_dims<T, 128>(a, grid, st);
+    if (D <= 192) return go_dims<T, 192>(a, grid, st);
+    go_dims<T, 256>(a, grid, st);
+}
+template <typename T>
+void go_merge(const PagedArgs& a, hipStream_t st) {
     const int R = a.rep * a.T, chunks = (a.c.D + 255) / 256;
     if ((int64_t)a.c.B * a.gs * R * chunks >= 16384)
         hipLaunchKernelGGL((k_paged_merge<T, 1>), dim3((R + 3) / 4, a.c.B * a.gs, chunks), dim3(256),
                            0, st, a);
     else
         hipLaunchKernelGGL((k_paged_merge<T, 4>), dim3(R, a.c.B * a.gs, chunks), dim3(256), 0, st, a);
-}
-template <typename T>
-void paged_go(const PagedArgs& a, hipStream_t st) {
-    if (a.groups > 0) paged_pass<T, 1>(a, st);
-    paged_pass<T, 0>(a, st);
-    if (a.groups > 0 || a.plan.own.split) paged_merge<T>(a, st);
 }
 
 }  // namespace

@@ -61,7 +61,6 @@ __global__ __launch_bounds__(512, 2) void k_paged_many(PagedArgs a) {
     const int col = lane & 31, half = lane >> 5, rg = wave % RG, kg = wave / RG;
     const int D = a.c.D, pieces = D / 8;
     const float scale = fabsf(a.scale);
-    if (PRE && blockIdx.x == 0) write_starts(a);
     if (pieces < CH) {  // (places of pieces past the row's end stay 0)
         for (int e = 16 * tid; e < N::kStage; e += 16 * 512)
             for (char* z : {k0, k1, v0, v1}) *reinterpret_cast<uint4*>(z + e) = make_uint4(0, 0, 0, 0);
@@ -464,7 +463,8 @@ void go_many(const PagedArgs& a, dim3 grid, hipStream_t st) {
 
 }  // namespace
 
-hipError_t launch_paged_many(const PagedArgs& a, int pre, dim3 grid, hipStream_t st) {
+hipError_t launch_paged_many(const PagedArgs& a, int pre, hipStream_t st) {
+    const dim3 grid((unsigned)(pre ? a.plan.pre.workgroups : a.plan.own.workgroups));
     if (a.c.D <= 64) {
         if (pre) go_many<64, 1>(a, grid, st);
         else go_many<64, 0>(a, grid, st);

@@ -1,0 +1,369 @@
+// Attention over a paged cache, head_d > 256 (paged_attn_impl.hpp has what its kernels share).  No
+// output tile fits a wave's registers, so two kernels with the scores between them: k_paged_scores
+// writes x (a row's are few floats beside K and V's rows of head_d), each workgroup's 8 waves
+// sharing a tile's dims, or its share of them, and adding up through LDS; k_paged_values is the
+// softmax over them and the product with V, each wave 16 VL dims of the output.  Keys lie in blocks
+// of 32.  Both take the prefixes' items and the sequences' own in one launch.
+#include "paged_attn_impl.hpp"
+
+namespace atn {
+
+namespace {
+
+constexpr int kBlock = 32;
+constexpr int kScoreWaves = 8;
+constexpr int kWaves = 4;        // of a value workgroup
+constexpr int kValueKeys = 128;  // keys between barriers of k_paged_values
+
+// Scores of a block: [share][place in the line without padding][rows][32], to be added over the shares.
+template <int PRE>
+__device__ __forceinline__ float* scores_of(const PagedArgs& a, int share, int place) {
+    const int64_t block = pass_of<PRE>(a).rows * kBlock;
+    return (PRE ? a.pre_scores : a.own_scores) + share * pass_of<PRE>(a).scores + place * block;
+}
+
+template <typename T, int MT, int PRE>
+__device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& gr, const Line& line,
+                                             int unit, v4f (*red)[MT * 2 * 64]) {
+    constexpr int SUB = kBlock / 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q = lane >> 4, col = lane & 15;
+    const int shares = a.plan.shares, place = (unsigned)unit / (unsigned)shares;
+    const int share = unit - place * shares;
+    const Place p = place_at<PRE>(a, gr, line, place, kBlock, lane, 0);
+    Span sp;
+    sp.s = segment<PRE>(a, gr, p.seg);
+    sp.s.lo = of_wave(sp.s.lo), sp.s.hi = of_wave(sp.s.hi), sp.s.len = of_wave(sp.s.len);
+    sp.s.first = of_wave(sp.s.first), sp.s.members = of_wave(sp.s.members);
+    const int off = place - p.start, item = (unsigned)off / (unsigned)p.n;
+    const int tiles = of_wave(sp.s.tiles), g = (unsigned)item / (unsigned)max(1, tiles);
+    sp.g = a.g0 + min(g, a.gs - 1);
+    sp.tile = item - g * tiles;
+    const int i = sp.s.lo / kBlock + off - item * p.n;
+    if (i >= tile_end<PRE>(a, sp.s, sp.tile, kBlock)) return;
+    const int row0 = sp.tile * 16 * MT;
+    const T* kp[SUB];
+    const T* qp[MT];
+    uint32_t there = 0;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+        const int r = i * kBlock + 16 * u + col, page = page_of(a.c, sp.s.first, r);
+        const bool is = is_page(a.c, page);
+        kp[u] = (const T*)a.c.K + (is ? page : 0) * a.c.ks[0] + sp.g * a.c.ks[1] +
+                (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.ks[2];
+        there |= ((uint32_t)__builtin_amdgcn_ballot_w64(is) & 0xffffu) << (16 * u);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) qp[t] = (const T*)a.Q + q_at<PRE>(a, sp, row0 + 16 * t + col);
+    v4f s[MT][SUB];
+    wide_scores<T, MT, true>(s, kp, qp, a.c.D, share * kScoreWaves + wave, shares * kScoreWaves, q);
+    __syncthreads();  // (the block before has been read)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) red[wave][(t * SUB + u) * 64 + lane] = s[t][u];
+    __syncthreads();
+    // one thread per row and 4 keys
+    if (threadIdx.x >= MT * SUB * 64) return;
+    const int u = wave % SUB, t = wave / SUB;
+    v4f x = red[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < kScoreWaves; ++w) x += red[w][threadIdx.x];
+    const uint32_t see = seen<SUB>(i * kBlock, sp.s.lo, attended<PRE>(a, sp, row0 + 16 * t + col), there,
+                                   q) >> (4 * u);
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = see >> e & 1u ? x[e] * a.scale : -INFINITY;
+    float* to = scores_of<PRE>(a, share, place) + (16 * t + col) * kBlock + 16 * u + 4 * q;
+    *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+}
+
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * kScoreWaves) void k_paged_scores(PagedArgs a) {
+    __shared__ v4f red[kScoreWaves][MT * 2 * 64];
+    const int lane = threadIdx.x & 63;
+    const Groups gr = groups_of(a, lane);
+    Line pre{};
+    if (a.groups > 0) pre = line_of<1>(a, gr, kBlock, lane, 0);
+    const Line own = line_of<0>(a, gr, kBlock, lane, 0);
+    const int first = pre.total * a.plan.shares, all = first + own.total * a.plan.shares;
+#pragma unroll 1
+    for (int u = blockIdx.x; u < all; u += gridDim.x) {
+        if (u < first)
+            block_scores<T, MT, 1>(a, gr, pre, u, red);
+        else
+            block_scores<T, MT, 0>(a, gr, own, u - first, red);
+    }
+}
+
+template <typename T>
+constexpr int wide_dims() {  // of a value workgroup
+    return (sizeof(T) == 2 ? 128 : 64) * kWaves;
+}
+
+template <typename T, int MT>
+struct Values : CacheTiles<T, (sizeof(T) == 2 ? 128 : 64), MT, kClamp> {
+    static constexpr int LDP = kValueKeys + 16 / (int)sizeof(T);
+    T pl[2][16 * MT * LDP];
+    float alpha[2][16 * MT];
+    float4 fin[16 * MT];
+};
+
+template <typename T, int MT, int PRE>
+__device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<T, MT>& x_) {
+    constexpr bool kBf = sizeof(T) == 2;
+    // (a wave's dims: one V step of 128 in bf16, 64 in fp32; where the row ends before, its last
+    // ones; those before d0 are the wave's before)
+    using N = Values<T, MT>;
+    constexpr int VL = N::VL, WD = N::VD, ROWS = N::ROWS, PK = N::KB, NB = kValueKeys / PK;
+    constexpr int LDP = N::LDP, STEP = kValueKeys / kBlock;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q = lane >> 4, col = lane & 15, D = a.c.D;
+    const int groups = pass_of<PRE>(a).groups, unit = (unsigned)id / (unsigned)groups;
+    const int d0 = ((id - unit * groups) * kWaves + wave) * WD;
+    const bool busy = d0 < D;
+    // softmax: 16 threads a row, 8 keys each, one pass per 16 rows
+    const int sr = threadIdx.x >> 4, sk = (threadIdx.x & 15) * 8;
+
+    each_span<PRE, true>(a, unit, kBlock, lane, [&](const Span& sp) {
+        const T* vp = (const T*)a.c.V + sp.g * a.c.vs[1] + d0;
+        const int row0 = sp.tile * ROWS, lo = sp.s.lo, b0 = sp.s.lo / kBlock;
+        const int last = min(sp.last, tile_end<PRE>(a, sp.s, sp.tile, kBlock));
+        const int whole0 = (lo + PK - 1) / PK, whole1 = of_wave(attended<PRE>(a, sp, row0)) / PK;
+        const float* sc = scores_of<PRE>(a, 0, sp.blocks_before);
+        float m[MT], l[MT], used[MT], x[MT][8];
+        v4f o[MT][1][VL];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = used[t] = 0.f;
+#pragma unroll
+            for (int c = 0; c < VL; ++c) o[t][0][c] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        // scores of the step at block i
+        auto load_x = [&](int i) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float* from = sc + (int64_t)(i - b0 + sk / kBlock) * (ROWS * kBlock) +
+                                    (16 * t + sr) * kBlock + sk % kBlock;
+                v4f u = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, w = u;
+                if (sk < (last - i) * kBlock) {
+                    u = *reinterpret_cast<const v4f*>(from);
+                    w = *reinterpret_cast<const v4f*>(from + 4);
+                    for (int y = 1; y < a.plan.shares; ++y) {
+                        from += pass_of<PRE>(a).scores;
+                        u += *reinterpret_cast<const v4f*>(from);
+                        w += *reinterpret_cast<const v4f*>(from + 4);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[t][e] = u[e], x[t][4 + e] = w[e];
+            }
+        };
+        // pages of a step's keys lane and 64 + lane
+        struct Pair {
+            int lo, hi;
+        };
+        auto pages_of = [&](int i) {
+            Pair p;
+            p.lo = page_of(a.c, sp.s.first, i * kBlock + lane);
+            p.hi = page_of(a.c, sp.s.first, i * kBlock + 64 + lane);
+            return p;
+        };
+        // V of keys [k, k + PK) of the step at block i
+        auto load_v = [&](typename N::Vals& to, const Pair& pg, int i, int k) {
+#pragma unroll
+            for (int j = 0; j < N::KEYS; ++j) {
+                const int key = k + N::key_of(lane, j), r = i * kBlock + key;
+                const int p = __shfl(k < 64 ? pg.lo : pg.hi, key & 63);
+                const T* row = vp + (is_page(a.c, p) ? p : 0) * a.c.vs[0] +
+                               (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.vs[2];
+                to.p[j][0] = N::v_piece(row, 0, 0, D - d0, lane);
+            }
+        };
+        // Two buffers of weights: a wave past a barrier writes the other one, and comes to write
+        // this one only after the next barrier, when every wave has read it.
+        typename N::Vals v0, v1;
+        __syncthreads();  // (the last span's)
+        Pair now{}, next{};
+        const bool any = sp.first < last;
+        if (any) {
+            load_x(sp.first);
+            now = pages_of(sp.first);
+            next = pages_of(sp.first + STEP);
+            if (busy) load_v(v0, now, sp.first, 0);
+        }
+        int buf = 0;
+#pragma unroll 1
+        for (int i = sp.first; i < last; i += STEP, buf ^= 1) {
+            // scores into weights
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                float top = x[t][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) top = fmaxf(top, x[t][e]);
+                top = fmaxf(top, dpp<kDppQuadXor1>(top));
+                top = fmaxf(top, dpp<kDppQuadXor2>(top));
+                top = fmaxf(top, dpp<kDppRowHalfMirror>(top));
+                top = fmaxf(top, dpp<kDppRowMirror>(top));
+                const float m_new = fmaxf(m[t], top), base = base_of(m_new);
+                const float f = exp2_(m[t] - base);
+                m[t] = m_new;
+                l[t] *= f;
+                used[t] *= f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[t][e] = exp2_(x[t][e] - base);
+                    l[t] += x[t][e];
+                }
+                if ((threadIdx.x & 15) == 0) x_.alpha[buf][16 * t + sr] = f;
+                T* to = x_.pl[buf] + (16 * t + sr) * LDP + sk;
+                if constexpr (kBf) {  // (rounded: see CacheTiles::accumulate)
+                    uint32_t w[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        w[h] = pack2(x[t][2 * h], x[t][2 * h + 1]);
+                        used[t] = add2(w[h], used[t]);
+                    }
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    *reinterpret_cast<float4*>(to) =
+                        make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
+                    *reinterpret_cast<float4*>(to + 4) =
+                        make_float4(x[t][4], x[t][5], x[t][6], x[t][7]);
+                }
+            }
+            if (i + STEP < last) load_x(i + STEP);
+            __syncthreads();
+            if (busy) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const float f = x_.alpha[buf][16 * t + col];
+                    if (__builtin_amdgcn_ballot_w64(f != 1.f)) {
+#pragma unroll
+                        for (int c = 0; c < VL; ++c) o[t][0][c] *= f;
+                    }
+                }
+                // each PK keys' V on their way while the ones before are used
+                auto use = [&](typename N::Vals& v, int k) {
+                    const int j0 = i * kBlock + k, b = j0 / PK;
+                    if (j0 >= last * kBlock) return;
+                    const uint32_t there =
+                        (uint32_t)(__builtin_amdgcn_ballot_w64(is_page(a.c, k < 64 ? now.lo : now.hi)) >>
+                                   (k & 63)) & below(PK);
+                    if ((b < whole0 || b >= whole1 || there != below(PK)) && not_finite<T>(v)) {
+                        uint32_t see[MT];
+#pragma unroll
+                        for (int t = 0; t < MT; ++t)
+                            see[t] = seen<N::SUB>(j0, lo, attended<PRE>(a, sp, row0 + 16 * t + col),
+                                                  there, q);
+                        spread_not_finite<T, N, MT>(o, v, see);
+                    }
+                    N::accumulate_lds(o, v, x_.pl[buf] + k, LDP, lane);
+                };
+#pragma unroll 1
+                for (int k = 0; k < NB; k += 2) {
+                    load_v(v1, now, i, (k + 1) * PK);
+                    __builtin_amdgcn_sched_barrier(0);
+                    use(v0, k * PK);
+                    const bool end = k + 2 >= NB;  // (the next step's first)
+                    load_v(v0, end ? next : now, end ? i + STEP : i, end ? 0 : (k + 2) * PK);
+                    __builtin_amdgcn_sched_barrier(0);
+                    use(v1, (k + 1) * PK);
+                }
+            }
+            now = next;
+            next = pages_of(i + 2 * STEP);
+        }
+        // sums of the rows, for the waves that hold their outputs
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float y = row16_sum(l[t]), z = kBf ? row16_sum(used[t]) : y;
+            if ((threadIdx.x & 15) == 0) x_.fin[16 * t + sr] = make_float4(m[t], y, z, 0.f);
+        }
+        __syncthreads();
+        if (!busy) return;
+        // (computed here: hoisted out of the loop over spans, these take the loop's registers)
+        const int late = opaque(lane), lq = late >> 4, lc = late & 15;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int r = 16 * t + lc;
+            const Row to = row_of<PRE>(a, sp, row0 + r);
+            if (to.b < 0) continue;
+            const float4 z = x_.fin[r];
+            const bool parted = PRE || sp.part >= 0, zero = !parted && z.z == 0.f;
+            const size_t pr = part_row<PRE>(a, max(sp.part, 0), r);
+            const float inv = parted ? 1.f : 1.f / z.z;
+            if (lq == 0 && d0 == 0) {
+                if (parted)
+                    part_stats<PRE>(a)[pr] = z;
+                else if (a.lse)
+                    a.lse[((size_t)to.b * a.H + to.h) * a.T + to.tok] = lse_of(z);
+            }
+            float* dims = part_dims<PRE>(a) + pr * D + d0;
+            T* out = (T*)a.out + to.b * a.os[0] + to.h * a.os[1] + to.tok * a.os[2] + d0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = N::dim_of(0, 4 * lq + e, D - d0);
+#pragma unroll
+                for (int c = 0; c < VL; c += 4) {
+                    float y[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = zero ? 0.f : o[t][0][c + r][e] * inv;
+                    if (d + c >= 0) {
+                        if (parted)
+                            store4(dims + d + c, y, 4);
+                        else
+                            store4(out + d + c, y, 4);
+                    } else {  // (a row's last dims, fewer than a piece)
+#pragma unroll
+                        for (int r = 1; r < 4; ++r)
+                            if (d + c + r >= 0) {
+                                if (parted)
+                                    dims[d + c + r] = y[r];
+                                else
+                                    Elem<T>::st(out, d + c + r, y[r]);
+                            }
+                    }
+                }
+            }
+        }
+    });
+}
+
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * kWaves, MT == 1 && sizeof(T) == 4 ? 3 : 2) void k_paged_values(PagedArgs a) {
+    __shared__ __align__(16) char lds[sizeof(Values<T, MT>)];
+    auto& x = *reinterpret_cast<Values<T, MT>*>(lds);
+    const int id = (int)blockIdx.x - a.plan.first;
+    if (id < 0)
+        paged_values<T, MT, 1>(a, blockIdx.x, x);
+    else
+        paged_values<T, MT, 0>(a, id, x);
+}
+
+template <typename T, int MT>
+void go(const PagedArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_paged_scores<T, MT>), dim3(a.plan.score_grid), dim3(64 * kScoreWaves), 0, st, a);
+    hipLaunchKernelGGL((k_paged_values<T, MT>), dim3((unsigned)(a.plan.first + a.plan.own.workgroups)),
+                       dim3(64 * kWaves), 0, st, a);
+}
+
+}  // namespace
+
+static_assert(wide_dims<float>() == kPagedWideDims / 2 && wide_dims<uint16_t>() == kPagedWideDims,
+              "dims of a value workgroup");
+static_assert(kBlock == kPagedWideBlock && kValueKeys == kBlock * kPagedWideTurn, "blocks");
+
+hipError_t launch_paged_wide(int dtype, const PagedArgs& a, hipStream_t st) {
+    if (dtype == kDtypeF32) {
+        if (a.plan.own.rows == 16) go<float, 1>(a, st);
+        else go<float, 2>(a, st);
+    } else {
+        if (a.plan.own.rows == 16) go<uint16_t, 1>(a, st);
+        else go<uint16_t, 2>(a, st);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace atn

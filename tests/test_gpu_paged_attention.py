@@ -317,9 +317,16 @@ def test_workspaces(am, dev, D):
         p.check()
         assert np.array_equal(tail.bits(), guard)
     assert ran >= 1
-    none = hip_rt.DeviceArray.wrap(ws.ptr, (20480,), "bf16", keep=ws)
+    # none at all without a prefix, but for the scores of one kv head where head_d > 256
     p.prefix = None
-    run(am, p, workspace=none)
+    if D > 256:
+        one = 3 * (1024 // 32 + 1) * 16 * 32 * 4  # sequences, blocks of a table's rows, rows, keys
+        with pytest.raises(am.AtnError):
+            run(am, p, workspace=hip_rt.DeviceArray.wrap(ws.ptr, (20480,), "bf16", keep=ws))
+        small = 40960 + one * 2
+    else:
+        small = 40960
+    run(am, p, workspace=hip_rt.DeviceArray.wrap(ws.ptr, (small // 2,), "bf16", keep=ws))
     p.check()
 
 
