@@ -175,6 +175,7 @@ int check_attention(const atn_paged_cache* cache, const atn_drafts* d, const atn
     a->H = d->heads;
     a->T = d->tokens;
     a->rep = d->heads / cache->kv_heads;
+    a->es = (int)q->es;
     a->by_rep = atn::divider(a->rep);
     a->by_t = atn::divider(a->T);
     return ATN_OK;

@@ -115,7 +115,7 @@ struct PagedArgs {
     void* out;
     float* lse;
     const int* count;
-    int H, T, rep;
+    int H, T, rep, es;    // es: bytes of an element
     Divider by_rep, by_t;
     float scale;          // times log2(e)
     const int* first;     // [groups + 1], or null

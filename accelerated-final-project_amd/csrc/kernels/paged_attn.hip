@@ -51,7 +51,7 @@ Tile tile_of(int dtype, int D, int64_t R, bool whole16) {
 // A pass of `segments` segments of at most `most` query rows of a kv head (all: of all segments), over
 // at most `keys` keys an item; kv: kv heads of a launch.
 PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, int64_t all, int64_t keys,
-                    int kv) {
+                    int kv, bool may_be_whole) {
     PagedPass p{};
     const bool bf = dtype == kDtypeBF16;
     p.many = t.kind == kMany;
@@ -81,8 +81,11 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
     p.ranges = (int)std::max<int64_t>(
         1, std::min(slots, ceil_div(p.items * (blocks + kPagedPad), 2 * p.turn)));
     p.line = p.items * (blocks + kPagedPad) + 2ll * p.turn * p.ranges;
-    p.split = p.items < 4 * slots && blocks > 7 * p.turn / 2;
+    p.split = !may_be_whole || (p.items < 4 * slots && blocks > 7 * p.turn / 2);
     p.parts = p.ranges + p.items;
+    // whole items in several runs of dims a workgroup, where there are workgroups enough
+    if (t.kind == kWide && !p.split)
+        p.groups = (int)std::min<int64_t>(p.groups, std::max<int64_t>(1, 4 * 256 * per_cu / p.items));
     p.scores = t.kind == kWide ? p.items * blocks * p.rows * kPagedWideBlock : 0;
     return p;
 }
@@ -106,15 +109,14 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
         // (groups are on the device: tiles for groups of equal size)
         pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, whole16);
         // one launch takes both, in tiles of as many rows
-        if (pre.kind != kMany) own.rows = pre.rows = std::max(own.rows, pre.rows);
+        if (pre.kind == kNarrow) own.rows = pre.rows = std::max(own.rows, pre.rows);
     }
     p.wide = own.kind == kWide;
     // all kv heads at once, unless the scratch does not hold their parts and scores
     for (p.kv = c.G;; p.kv = (p.kv + 1) / 2) {
-        p.own = plan_pass(dtype, D, own, R, c.B, all, c.rows, p.kv);
+        p.own = plan_pass(dtype, D, own, R, c.B, all, c.rows, p.kv, true);
         if (groups > 0) {
-            p.pre = plan_pass(dtype, D, pre, all, groups, all, c.rows, p.kv);
-            p.pre.split = 1;
+            p.pre = plan_pass(dtype, D, pre, all, groups, all, c.rows, p.kv, false);
             p.pre.workgroups = (int64_t)p.pre.ranges * p.pre.groups;
             p.first = pre.kind == kMany ? 0 : (int)p.pre.workgroups;
         }
@@ -123,7 +125,8 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
             (p.own.split ? p.own.ranges : (int64_t)c.B * p.kv * p.own.tiles) * p.own.groups;
         // scores: two workgroups a CU, where the dims give each wave two steps still
         p.shares = 1;
-        const int64_t blocks = (p.own.scores + p.pre.scores) / (p.own.rows * kPagedWideBlock);
+        int64_t blocks = p.own.scores / (p.own.rows * kPagedWideBlock);
+        if (groups > 0) blocks += p.pre.scores / (p.pre.rows * kPagedWideBlock);
         while (p.wide && blocks * p.shares < 512 && p.shares < 8 &&
                D >= 2 * p.shares * 8 * (dtype == kDtypeBF16 ? 256 : 128))
             p.shares *= 2;

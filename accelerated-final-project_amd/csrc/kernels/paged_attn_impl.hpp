@@ -46,13 +46,17 @@ __device__ __forceinline__ int tokens_of(const PagedArgs& a, int b) {
 struct Groups {
     int first, end, rows;
 };
-// (a group of one reads its rows as its own; first and shared may hold anything)
+// (first and shared may hold anything.)  Rows that are read once save the other members' reads, 2
+// es head_d bytes a row and kv head; but every query row's result then passes through the scratch
+// in two parts, 16 head_d bytes.  Groups with less to save read their rows as their own (5 sequences
+// of 281 tokens of 16 heads of 8192 dims, 19 rows shared: MERGE_FIGURES).
 __device__ __forceinline__ Groups group_at(const PagedArgs& a, int i) {
     Groups g;
     g.first = min(max(a.first[i], 0), a.c.B - 1);
     g.end = min(max(a.first[i + 1], 0), a.c.B);
-    const int L = min(rows_in_use(a.c, g.first), a.c.rows);
-    g.rows = g.end - g.first >= 2 ? min(max(a.shared[i], 0), L) : 0;
+    const int L = min(rows_in_use(a.c, g.first), a.c.rows), m = g.end - g.first;
+    g.rows = min(max(a.shared[i], 0), L);
+    if (m < 2 || (int64_t)g.rows * (m - 1) * a.es <= (int64_t)m * a.rep * a.T * 8) g.rows = 0;
     return g;
 }
 __device__ __forceinline__ Groups groups_of(const PagedArgs& a, int lane) {
@@ -845,7 +849,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     __shared__ float acc[4][256];
     __shared__ float2 sums[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int D = a.c.D, d0 = blockIdx.z * 256;
+    const int D = a.c.D;
     const int row = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
     if (row >= a.rep * a.T) return;
     const unsigned pair = blockIdx.y, seq = pair / (unsigned)a.gs;
@@ -893,6 +897,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     for (int i = lane; i < parts; i += 64) M = fmaxf(M, stats_of(i).x);
     M = wave_max(M);
     const float base = base_of(M);
+#pragma unroll 1
+  for (int d0 = 256 * blockIdx.z; d0 < D; d0 += 256 * gridDim.z) {
     float l = 0.f, used = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = WAVES == 4 ? wave : 0; i < parts; i += WAVES) {
@@ -924,6 +930,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
         const int d = threadIdx.x;
         const float sum = (acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d]);
         if (d0 + d < D) Elem<T>::st(out, d, used == 0.f ? 0.f : sum * (1.f / used));
+        __syncthreads();  // (for the next dims)
     } else {
         const float inv = 1.f / used;
 #pragma unroll
@@ -934,6 +941,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
     if (d0 == 0 && (WAVES == 4 ? threadIdx.x : lane) == 0 && a.lse)
         a.lse[((size_t)b * a.H + h) * a.T + tok] =
             l == 0.f ? -INFINITY : (M + log2f(l)) * kLn2;
+  }
 }
 
 // ---------------------------------------------------------------- launches
@@ -970,11 +978,14 @@ void go_narrow(const PagedArgs& a, hipStream_t st) {
 template <typename T>
 void go_merge(const PagedArgs& a, hipStream_t st) {
     const int R = a.rep * a.T, chunks = (a.c.D + 255) / 256;
-    if ((int64_t)a.c.B * a.gs * R * chunks >= 16384)
-        hipLaunchKernelGGL((k_paged_merge<T, 1>), dim3((R + 3) / 4, a.c.B * a.gs, chunks), dim3(256),
-                           0, st, a);
+    const int64_t rows = (int64_t)a.c.B * a.gs * R;
+    // (a workgroup finds its row's parts once: several runs of dims each, where there are rows enough)
+    const unsigned z = (unsigned)std::min<int64_t>(chunks, std::max<int64_t>(1, 4096 / rows));
+    if (rows * chunks >= 16384)
+        hipLaunchKernelGGL((k_paged_merge<T, 1>), dim3((R + 3) / 4, a.c.B * a.gs, z), dim3(256), 0, st,
+                           a);
     else
-        hipLaunchKernelGGL((k_paged_merge<T, 4>), dim3(R, a.c.B * a.gs, chunks), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_paged_merge<T, 4>), dim3(R, a.c.B * a.gs, z), dim3(256), 0, st, a);
 }
 
 }  // namespace

@@ -24,7 +24,7 @@ __device__ __forceinline__ float* scores_of(const PagedArgs& a, int share, int p
 
 template <typename T, int MT, int PRE>
 __device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& gr, const Line& line,
-                                             int unit, v4f (*red)[MT * 2 * 64]) {
+                                             int unit, v4f* red) {
     constexpr int SUB = kBlock / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
@@ -47,7 +47,8 @@ __device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& g
     uint32_t there = 0;
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-        const int r = i * kBlock + 16 * u + col, page = page_of(a.c, sp.s.first, r);
+        const int r = min(i * kBlock + 16 * u + col, max(i * kBlock, sp.s.hi - 1));
+        const int page = page_of(a.c, sp.s.first, r);
         const bool is = is_page(a.c, page);
         kp[u] = (const T*)a.c.K + (is ? page : 0) * a.c.ks[0] + sp.g * a.c.ks[1] +
                 (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.ks[2];
@@ -61,14 +62,14 @@ __device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& g
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) red[wave][(t * SUB + u) * 64 + lane] = s[t][u];
+        for (int u = 0; u < SUB; ++u) red[(wave * MT * SUB + t * SUB + u) * 64 + lane] = s[t][u];
     __syncthreads();
     // one thread per row and 4 keys
     if (threadIdx.x >= MT * SUB * 64) return;
     const int u = wave % SUB, t = wave / SUB;
-    v4f x = red[0][threadIdx.x];
+    v4f x = red[threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < kScoreWaves; ++w) x += red[w][threadIdx.x];
+    for (int w = 1; w < kScoreWaves; ++w) x += red[w * MT * SUB * 64 + threadIdx.x];
     const uint32_t see = seen<SUB>(i * kBlock, sp.s.lo, attended<PRE>(a, sp, row0 + 16 * t + col), there,
                                    q) >> (4 * u);
     float y[4];
@@ -78,9 +79,9 @@ __device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& g
     *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
 }
 
-template <typename T, int MT>
+template <typename T, int OWN, int PRE>
 __global__ __launch_bounds__(64 * kScoreWaves) void k_paged_scores(PagedArgs a) {
-    __shared__ v4f red[kScoreWaves][MT * 2 * 64];
+    __shared__ v4f red[kScoreWaves * (OWN > PRE ? OWN : PRE) * 2 * 64];
     const int lane = threadIdx.x & 63;
     const Groups gr = groups_of(a, lane);
     Line pre{};
@@ -90,9 +91,9 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_paged_scores(PagedArgs a) 
 #pragma unroll 1
     for (int u = blockIdx.x; u < all; u += gridDim.x) {
         if (u < first)
-            block_scores<T, MT, 1>(a, gr, pre, u, red);
+            block_scores<T, PRE, 1>(a, gr, pre, u, red);
         else
-            block_scores<T, MT, 0>(a, gr, own, u - first, red);
+            block_scores<T, OWN, 0>(a, gr, own, u - first, red);
     }
 }
 
@@ -120,15 +121,22 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15, D = a.c.D;
     const int groups = pass_of<PRE>(a).groups, unit = (unsigned)id / (unsigned)groups;
-    const int d0 = ((id - unit * groups) * kWaves + wave) * WD;
-    const bool busy = d0 < D;
+    const int chunk0 = id - unit * groups;
     // softmax: 16 threads a row, 8 keys each, one pass per 16 rows
     const int sr = threadIdx.x >> 4, sk = (threadIdx.x & 15) * 8;
 
     each_span<PRE, true>(a, unit, kBlock, lane, [&](const Span& sp) {
+      // (short items: a workgroup takes several runs of dims, one after another)
+#pragma unroll 1
+      for (int chunk = chunk0; chunk * kWaves * WD < D; chunk += groups) {
+        const int d0 = (chunk * kWaves + wave) * WD;
+        const bool busy = d0 < D;
         const T* vp = (const T*)a.c.V + sp.g * a.c.vs[1] + d0;
         const int row0 = sp.tile * ROWS, lo = sp.s.lo, b0 = sp.s.lo / kBlock;
         const int last = min(sp.last, tile_end<PRE>(a, sp.s, sp.tile, kBlock));
+        // rows of keys that any row attends
+        const int end = max(lo + 1, min(last * kBlock, PRE ? sp.s.hi : of_wave(attended<PRE>(
+                                                           a, sp, row0 + ROWS - 1))));
         const int whole0 = (lo + PK - 1) / PK, whole1 = of_wave(attended<PRE>(a, sp, row0)) / PK;
         const float* sc = scores_of<PRE>(a, 0, sp.blocks_before);
         float m[MT], l[MT], used[MT], x[MT][8];
@@ -174,8 +182,9 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
         auto load_v = [&](typename N::Vals& to, const Pair& pg, int i, int k) {
 #pragma unroll
             for (int j = 0; j < N::KEYS; ++j) {
-                const int key = k + N::key_of(lane, j), r = i * kBlock + key;
-                const int p = __shfl(k < 64 ? pg.lo : pg.hi, key & 63);
+                // (past the last row: that one again)
+                const int key = min(k + N::key_of(lane, j), end - 1 - i * kBlock), r = i * kBlock + key;
+                const int p = __shfl(key < 64 ? pg.lo : pg.hi, key & 63);
                 const T* row = vp + (is_page(a.c, p) ? p : 0) * a.c.vs[0] +
                                (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.vs[2];
                 to.p[j][0] = N::v_piece(row, 0, 0, D - d0, lane);
@@ -247,7 +256,6 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
                 // each PK keys' V on their way while the ones before are used
                 auto use = [&](typename N::Vals& v, int k) {
                     const int j0 = i * kBlock + k, b = j0 / PK;
-                    if (j0 >= last * kBlock) return;
                     const uint32_t there =
                         (uint32_t)(__builtin_amdgcn_ballot_w64(is_page(a.c, k < 64 ? now.lo : now.hi)) >>
                                    (k & 63)) & below(PK);
@@ -261,15 +269,18 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
                     }
                     N::accumulate_lds(o, v, x_.pl[buf] + k, LDP, lane);
                 };
+                const int nb = min(NB, (end - i * kBlock + PK - 1) / PK);
 #pragma unroll 1
-                for (int k = 0; k < NB; k += 2) {
-                    load_v(v1, now, i, (k + 1) * PK);
+                for (int k = 0; k < nb; k += 2) {
+                    if (k + 1 < nb) load_v(v1, now, i, (k + 1) * PK);
                     __builtin_amdgcn_sched_barrier(0);
                     use(v0, k * PK);
-                    const bool end = k + 2 >= NB;  // (the next step's first)
-                    load_v(v0, end ? next : now, end ? i + STEP : i, end ? 0 : (k + 2) * PK);
+                    if (k + 2 < nb)
+                        load_v(v0, now, i, (k + 2) * PK);
+                    else if (i + STEP < last)  // the next step's first
+                        load_v(v0, next, i + STEP, 0);
                     __builtin_amdgcn_sched_barrier(0);
-                    use(v1, (k + 1) * PK);
+                    if (k + 1 < nb) use(v1, (k + 1) * PK);
                 }
             }
             now = next;
@@ -282,7 +293,7 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
             if ((threadIdx.x & 15) == 0) x_.fin[16 * t + sr] = make_float4(m[t], y, z, 0.f);
         }
         __syncthreads();
-        if (!busy) return;
+        if (!busy) continue;
         // (computed here: hoisted out of the loop over spans, these take the loop's registers)
         const int late = opaque(lane), lq = late >> 4, lc = late & 15;
 #pragma unroll
@@ -328,25 +339,36 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
                 }
             }
         }
+      }
     });
 }
 
-template <typename T, int MT>
-__global__ __launch_bounds__(64 * kWaves, MT == 1 && sizeof(T) == 4 ? 3 : 2) void k_paged_values(PagedArgs a) {
-    __shared__ __align__(16) char lds[sizeof(Values<T, MT>)];
-    auto& x = *reinterpret_cast<Values<T, MT>*>(lds);
+template <typename T, int OWN, int PRE>
+__global__ __launch_bounds__(64 * kWaves, OWN + PRE == 2 && sizeof(T) == 4 ? 3 : 2) void k_paged_values(
+    PagedArgs a) {
+    constexpr size_t kOwn = sizeof(Values<T, OWN>), kPre = sizeof(Values<T, PRE>);
+    __shared__ __align__(16) char lds[kOwn > kPre ? kOwn : kPre];
     const int id = (int)blockIdx.x - a.plan.first;
     if (id < 0)
-        paged_values<T, MT, 1>(a, blockIdx.x, x);
+        paged_values<T, PRE, 1>(a, blockIdx.x, *reinterpret_cast<Values<T, PRE>*>(lds));
     else
-        paged_values<T, MT, 0>(a, id, x);
+        paged_values<T, OWN, 0>(a, id, *reinterpret_cast<Values<T, OWN>*>(lds));
 }
 
-template <typename T, int MT>
+template <typename T, int OWN, int PRE>
 void go(const PagedArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_paged_scores<T, MT>), dim3(a.plan.score_grid), dim3(64 * kScoreWaves), 0, st, a);
-    hipLaunchKernelGGL((k_paged_values<T, MT>), dim3((unsigned)(a.plan.first + a.plan.own.workgroups)),
-                       dim3(64 * kWaves), 0, st, a);
+    hipLaunchKernelGGL((k_paged_scores<T, OWN, PRE>), dim3(a.plan.score_grid), dim3(64 * kScoreWaves), 0,
+                       st, a);
+    hipLaunchKernelGGL((k_paged_values<T, OWN, PRE>),
+                       dim3((unsigned)(a.plan.first + a.plan.own.workgroups)), dim3(64 * kWaves), 0, st,
+                       a);
+}
+template <typename T>
+void go_rows_wide(const PagedArgs& a, hipStream_t st) {
+    const bool pre = a.groups > 0 && a.plan.pre.rows > 16;
+    if (a.plan.own.rows > 16) go<T, 2, 2>(a, st);
+    else if (pre) go<T, 1, 2>(a, st);
+    else go<T, 1, 1>(a, st);
 }
 
 }  // namespace
@@ -356,13 +378,8 @@ static_assert(wide_dims<float>() == kPagedWideDims / 2 && wide_dims<uint16_t>() 
 static_assert(kBlock == kPagedWideBlock && kValueKeys == kBlock * kPagedWideTurn, "blocks");
 
 hipError_t launch_paged_wide(int dtype, const PagedArgs& a, hipStream_t st) {
-    if (dtype == kDtypeF32) {
-        if (a.plan.own.rows == 16) go<float, 1>(a, st);
-        else go<float, 2>(a, st);
-    } else {
-        if (a.plan.own.rows == 16) go<uint16_t, 1>(a, st);
-        else go<uint16_t, 2>(a, st);
-    }
+    if (dtype == kDtypeF32) go_rows_wide<float>(a, st);
+    else go_rows_wide<uint16_t>(a, st);
     return hipGetLastError();
 }
 
