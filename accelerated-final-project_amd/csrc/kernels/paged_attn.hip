@@ -29,16 +29,20 @@ __global__ __launch_bounds__(256) void k_paged_starts(PagedArgs a, int2* starts)
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Which kernel takes items of about R query rows, and its tile.
+// Which kernel takes items of about R query rows, and its tile.  runs: rows are whole 16-byte pieces, and
+// pages whole runs of 16 rows.
 enum Kind { kNarrow, kMany, kWide };
 struct Tile {
     Kind kind;
     int rows;
 };
-Tile tile_of(int dtype, int D, int64_t R, bool whole16) {
+Tile tile_of(int dtype, int D, int64_t R, bool runs) {
     const bool bf = dtype == kDtypeBF16;
-    if (D > kPagedNarrow) return {kWide, R <= 16 ? 16 : 32};
-    if (bf && whole16 && D <= 128 && R > 32) {
+    // (64 rows where they leave no more than a fourth more rows empty than 32 do)
+    if (D > kPagedNarrow)
+        return {kWide, R <= 16 ? 16 : R > 32 && 4 * (ceil_div(R, 64) * 64) <= 5 * (ceil_div(R, 32) * 32)
+                                       ? 64 : 32};
+    if (bf && runs && D <= 128 && R > 32) {
         // the tile that leaves the fewest rows empty, the larger of equals
         int best = 64;
         for (int rows : {128, 256})
@@ -58,16 +62,18 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
     p.rows = t.rows;
     p.groups = 1;
     const int mt = p.rows / 16;
-    int per_cu;  // workgroups that a CU holds at once (the kernels' registers and LDS)
+    int subs = 1;  // workgroups that share an item's rows (head_d > 256)
+    int per_cu;    // workgroups that a CU holds at once (the kernels' registers and LDS)
     if (t.kind == kMany) {
         per_cu = 1;
         p.kb = p.rows == 256 ? 64 : 128;
         p.turn = 1;
     } else if (t.kind == kWide) {
-        per_cu = mt == 1 && !bf ? 3 : 2;
+        per_cu = mt == 1 && !bf ? 3 : 2;  // (of the values)
         p.kb = kPagedWideBlock;
         p.turn = kPagedWideTurn;
-        p.groups = (int)ceil_div(D, bf ? kPagedWideDims : kPagedWideDims / 2);
+        subs = std::max(1, p.rows / kPagedWideRows);
+        p.groups = (int)ceil_div(D, bf ? kPagedWideDims : kPagedWideDims / 2) * subs;
     } else {
         per_cu = std::max(1, (mt == 1 ? 4 : mt == 2 ? 3 : 2) - (D > 64) - (D > 128));
         p.kb = bf ? 32 : 16;
@@ -85,7 +91,8 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
     p.parts = p.ranges + p.items;
     // whole items in several runs of dims a workgroup, where there are workgroups enough
     if (t.kind == kWide && !p.split)
-        p.groups = (int)std::min<int64_t>(p.groups, std::max<int64_t>(1, 4 * 256 * per_cu / p.items));
+        p.groups = subs * (int)std::min<int64_t>(p.groups / subs, std::max<int64_t>(
+                              1, 4 * 256 * per_cu / (p.items * subs)));
     p.scores = t.kind == kWide ? p.items * blocks * p.rows * kPagedWideBlock : 0;
     return p;
 }
@@ -103,15 +110,18 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
     PagedPlan p{};
     const int D = c.D;
     const int64_t R = (int64_t)(H / c.G) * T, all = R * c.B;
-    whole16 = whole16 && c.page_rows % 16 == 0;
-    Tile own = tile_of(dtype, D, R, whole16), pre = own;
+    const bool runs = whole16 && c.page_rows % 16 == 0;
+    Tile own = tile_of(dtype, D, R, runs), pre = own;
     if (groups > 0) {
         // (groups are on the device: tiles for groups of equal size)
-        pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, whole16);
+        pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, runs);
         // one launch takes both, in tiles of as many rows
-        if (pre.kind == kNarrow) own.rows = pre.rows = std::max(own.rows, pre.rows);
+        // (head_d > 256: or own 16, prefixes 32)
+        if (pre.kind == kWide && own.rows == 16) pre.rows = std::min(pre.rows, 32);
+        else if (pre.kind != kMany) own.rows = pre.rows = std::max(own.rows, pre.rows);
     }
     p.wide = own.kind == kWide;
+    p.whole16 = whole16;
     // all kv heads at once, unless the scratch does not hold their parts and scores
     for (p.kv = c.G;; p.kv = (p.kv + 1) / 2) {
         p.own = plan_pass(dtype, D, own, R, c.B, all, c.rows, p.kv, true);

@@ -26,6 +26,7 @@ namespace atn {
 constexpr int kPagedNarrow = 256;  // head_d up to which a wave holds a row tile's output
 constexpr int kPagedPad = 12;      // places of the line that beginning and ending an item count for
 constexpr int kPagedWideBlock = 32, kPagedWideTurn = 4;  // head_d above: keys of a block, blocks between barriers
+constexpr int kPagedWideRows = 32;   // ... query rows of a workgroup of values, at most
 constexpr int kPagedWideDims = 512;  // ... dims of a workgroup (bf16; fp32: half)
 
 namespace {

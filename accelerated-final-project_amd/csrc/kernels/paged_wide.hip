@@ -22,9 +22,85 @@ __device__ __forceinline__ float* scores_of(const PagedArgs& a, int share, int p
     return (PRE ? a.pre_scores : a.own_scores) + share * pass_of<PRE>(a).scores + place * block;
 }
 
+// K's 32 rows and a tile's query rows, 128 bytes of each at a time, in a wave's own part of LDS: rows
+// are loaded 8 lanes each (a load straight into the products' operands takes 16 bytes of every row
+// from a cache that delivers 64 a cycle), pieces at places that change with the row, so that the 16
+// rows of an operand lie in different banks.
+constexpr int kRowBytes = 128;
+template <int MT>
+struct Stage {
+    static constexpr int ROWS = kBlock + 16 * MT, LOADS = ROWS / 8;
+    static constexpr int kBytes = ROWS * kRowBytes;  // (also what the partial scores need)
+    static_assert(kBytes >= MT * (kBlock / 16) * 64 * 16, "partial scores");
+    static __device__ __forceinline__ int place(int row, int piece) { return piece ^ (row >> 1 & 7); }
+};
+
+// The scores of a wave's share of the dims (every `waves`-th 128 bytes from `wave` on), from LDS.
 template <typename T, int MT, int PRE>
+__device__ __forceinline__ void staged_scores(v4f (&s)[MT][2], const PagedArgs& a, const Span& sp, int j0,
+                                              int row0, int wave, int waves, char* lds, int lane) {
+    using S = Stage<MT>;
+    using N = CacheTiles<T, 64, MT, kExact>;
+    const int q = lane >> 4, col = lane & 15, bytes = a.c.D * (int)sizeof(T);
+    // load x: rows 8 x + lane / 8 (keys, then queries), the piece that lies at place lane % 8 there
+    const char* from[S::LOADS];
+#pragma unroll
+    for (int x = 0; x < S::LOADS; ++x) {
+        const int row = 8 * x + lane / 8;
+        if (x < kBlock / 8) {  // (past the last row: that one again)
+            const int r = min(j0 + row, max(j0, sp.s.hi - 1)), page = page_of(a.c, sp.s.first, r);
+            from[x] = (const char*)((const T*)a.c.K + (is_page(a.c, page) ? page : 0) * a.c.ks[0] +
+                                    sp.g * a.c.ks[1] +
+                                    (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.ks[2]);
+        } else {
+            from[x] = (const char*)((const T*)a.Q + q_at<PRE>(a, sp, row0 + row - kBlock));
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto at = [&](int row, int piece) {
+        return __builtin_bit_cast(typename N::KPiece, *reinterpret_cast<const uint4*>(
+                                                          lds + row * kRowBytes + 16 * S::place(row, piece)));
+    };
+#pragma unroll 1
+    for (int step = wave; step * kRowBytes < bytes; step += waves) {
+        const int left = bytes - step * kRowBytes;
+        if (left < kRowBytes) {  // (pieces past the row's end are 0)
+            for (int e = 16 * lane; e < S::kBytes; e += 16 * 64)
+                *reinterpret_cast<uint4*>(lds + e) = make_uint4(0, 0, 0, 0);
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): LDS has been read and written
+        const int mine = opaque(lane);
+#pragma unroll
+        for (int x = 0; x < S::LOADS; ++x) {
+            const int of = 16 * S::place(8 * x + mine / 8, mine % 8);
+            if (of < left)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)(from[x] + step * kRowBytes + of),
+                    (__attribute__((address_space(3))) void*)(lds + 8 * x * kRowBytes), 16, 0, 0);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            typename N::KPiece k[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) k[u] = at(16 * u + col, 4 * e + q);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const typename N::KPiece f = at(kBlock + 16 * t + col, 4 * e + q);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[t][u] = N::dot(k[u], f, s[t][u]);
+            }
+        }
+    }
+}
+
+template <typename T, int MT, int PRE, bool STAGED>
 __device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& gr, const Line& line,
-                                             int unit, v4f* red) {
+                                             int unit, char* lds) {
     constexpr int SUB = kBlock / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
@@ -42,34 +118,46 @@ __device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& g
     const int i = sp.s.lo / kBlock + off - item * p.n;
     if (i >= tile_end<PRE>(a, sp.s, sp.tile, kBlock)) return;
     const int row0 = sp.tile * 16 * MT;
-    const T* kp[SUB];
-    const T* qp[MT];
     uint32_t there = 0;
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-        const int r = min(i * kBlock + 16 * u + col, max(i * kBlock, sp.s.hi - 1));
-        const int page = page_of(a.c, sp.s.first, r);
-        const bool is = is_page(a.c, page);
-        kp[u] = (const T*)a.c.K + (is ? page : 0) * a.c.ks[0] + sp.g * a.c.ks[1] +
-                (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.ks[2];
+        const bool is = is_page(a.c, page_of(a.c, sp.s.first, i * kBlock + 16 * u + col));
         there |= ((uint32_t)__builtin_amdgcn_ballot_w64(is) & 0xffffu) << (16 * u);
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) qp[t] = (const T*)a.Q + q_at<PRE>(a, sp, row0 + 16 * t + col);
     v4f s[MT][SUB];
-    wide_scores<T, MT, true>(s, kp, qp, a.c.D, share * kScoreWaves + wave, shares * kScoreWaves, q);
+    const int w = share * kScoreWaves + wave, waves = shares * kScoreWaves;
     __syncthreads();  // (the block before has been read)
+    char* mine = lds + wave * Stage<MT>::kBytes;
+    if constexpr (STAGED) {
+        staged_scores<T, MT, PRE>(s, a, sp, i * kBlock, row0, w, waves, mine, lane);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // (this wave's part of LDS has been read)
+    } else {
+        const T* kp[SUB];
+        const T* qp[MT];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const int r = min(i * kBlock + 16 * u + col, max(i * kBlock, sp.s.hi - 1));
+            const int page = page_of(a.c, sp.s.first, r);
+            kp[u] = (const T*)a.c.K + (is_page(a.c, page) ? page : 0) * a.c.ks[0] + sp.g * a.c.ks[1] +
+                    (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.ks[2];
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) qp[t] = (const T*)a.Q + q_at<PRE>(a, sp, row0 + 16 * t + col);
+        wide_scores<T, MT, true>(s, kp, qp, a.c.D, w, waves, q);
+    }
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) red[(wave * MT * SUB + t * SUB + u) * 64 + lane] = s[t][u];
+        for (int u = 0; u < SUB; ++u)
+            reinterpret_cast<v4f*>(mine)[(t * SUB + u) * 64 + lane] = s[t][u];
     __syncthreads();
     // one thread per row and 4 keys
     if (threadIdx.x >= MT * SUB * 64) return;
     const int u = wave % SUB, t = wave / SUB;
-    v4f x = red[threadIdx.x];
+    v4f x = reinterpret_cast<const v4f*>(lds)[threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < kScoreWaves; ++w) x += red[w * MT * SUB * 64 + threadIdx.x];
+    for (int w = 1; w < kScoreWaves; ++w)
+        x += reinterpret_cast<const v4f*>(lds + w * Stage<MT>::kBytes)[threadIdx.x];
     const uint32_t see = seen<SUB>(i * kBlock, sp.s.lo, attended<PRE>(a, sp, row0 + 16 * t + col), there,
                                    q) >> (4 * u);
     float y[4];
@@ -79,9 +167,10 @@ __device__ __forceinline__ void block_scores(const PagedArgs& a, const Groups& g
     *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
 }
 
-template <typename T, int OWN, int PRE>
+// STAGED: rows are whole 16-byte pieces that lie so.
+template <typename T, int OWN, int PRE, bool STAGED>
 __global__ __launch_bounds__(64 * kScoreWaves) void k_paged_scores(PagedArgs a) {
-    __shared__ v4f red[kScoreWaves * (OWN > PRE ? OWN : PRE) * 2 * 64];
+    __shared__ __align__(16) char lds[kScoreWaves * Stage<(OWN > PRE ? OWN : PRE)>::kBytes];
     const int lane = threadIdx.x & 63;
     const Groups gr = groups_of(a, lane);
     Line pre{};
@@ -91,9 +180,9 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_paged_scores(PagedArgs a) 
 #pragma unroll 1
     for (int u = blockIdx.x; u < all; u += gridDim.x) {
         if (u < first)
-            block_scores<T, PRE, 1>(a, gr, pre, u, red);
+            block_scores<T, PRE, 1, STAGED>(a, gr, pre, u, lds);
         else
-            block_scores<T, OWN, 0>(a, gr, own, u - first, red);
+            block_scores<T, OWN, 0, STAGED>(a, gr, own, u - first, lds);
     }
 }
 
@@ -120,8 +209,10 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
     constexpr int LDP = N::LDP, STEP = kValueKeys / kBlock;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15, D = a.c.D;
-    const int groups = pass_of<PRE>(a).groups, unit = (unsigned)id / (unsigned)groups;
-    const int chunk0 = id - unit * groups;
+    // (workgroups of an item: runs of dims, times tiles of ROWS of the item's rows)
+    const int all = pass_of<PRE>(a).groups, subs = pass_of<PRE>(a).rows / ROWS, groups = all / subs;
+    const int unit = (unsigned)id / (unsigned)all, mine = id - unit * all;
+    const int sub = subs > 1 ? mine % subs : 0, chunk0 = mine / subs;
     // softmax: 16 threads a row, 8 keys each, one pass per 16 rows
     const int sr = threadIdx.x >> 4, sk = (threadIdx.x & 15) * 8;
 
@@ -132,7 +223,7 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
         const int d0 = (chunk * kWaves + wave) * WD;
         const bool busy = d0 < D;
         const T* vp = (const T*)a.c.V + sp.g * a.c.vs[1] + d0;
-        const int row0 = sp.tile * ROWS, lo = sp.s.lo, b0 = sp.s.lo / kBlock;
+        const int row0 = sp.tile * pass_of<PRE>(a).rows + sub * ROWS, lo = sp.s.lo, b0 = lo / kBlock;
         const int last = min(sp.last, tile_end<PRE>(a, sp.s, sp.tile, kBlock));
         // rows of keys that any row attends
         const int end = max(lo + 1, min(last * kBlock, PRE ? sp.s.hi : of_wave(attended<PRE>(
@@ -152,8 +243,8 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
         auto load_x = [&](int i) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float* from = sc + (int64_t)(i - b0 + sk / kBlock) * (ROWS * kBlock) +
-                                    (16 * t + sr) * kBlock + sk % kBlock;
+                const float* from = sc + (int64_t)(i - b0 + sk / kBlock) * (pass_of<PRE>(a).rows * kBlock) +
+                                    (sub * ROWS + 16 * t + sr) * kBlock + sk % kBlock;
                 v4f u = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, w = u;
                 if (sk < (last - i) * kBlock) {
                     u = *reinterpret_cast<const v4f*>(from);
@@ -188,6 +279,8 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
                 const T* row = vp + (is_page(a.c, p) ? p : 0) * a.c.vs[0] +
                                (r - over(r, a.c.by_page) * a.c.page_rows) * a.c.vs[2];
                 to.p[j][0] = N::v_piece(row, 0, 0, D - d0, lane);
+                // (all rows' addresses at once would take the registers of the output)
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
         // Two buffers of weights: a wave past a barrier writes the other one, and comes to write
@@ -303,7 +396,7 @@ __device__ __forceinline__ void paged_values(const PagedArgs& a, int id, Values<
             if (to.b < 0) continue;
             const float4 z = x_.fin[r];
             const bool parted = PRE || sp.part >= 0, zero = !parted && z.z == 0.f;
-            const size_t pr = part_row<PRE>(a, max(sp.part, 0), r);
+            const size_t pr = part_row<PRE>(a, max(sp.part, 0), sub * ROWS + r);
             const float inv = parted ? 1.f : 1.f / z.z;
             if (lq == 0 && d0 == 0) {
                 if (parted)
@@ -355,19 +448,24 @@ __global__ __launch_bounds__(64 * kWaves, OWN + PRE == 2 && sizeof(T) == 4 ? 3 :
         paged_values<T, OWN, 0>(a, id, *reinterpret_cast<Values<T, OWN>*>(lds));
 }
 
+// OWN, PRE: 16 rows of tiles of the scores; the values' are of 32 rows at most
 template <typename T, int OWN, int PRE>
 void go(const PagedArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_paged_scores<T, OWN, PRE>), dim3(a.plan.score_grid), dim3(64 * kScoreWaves), 0,
-                       st, a);
-    hipLaunchKernelGGL((k_paged_values<T, OWN, PRE>),
+    const dim3 grid(a.plan.score_grid), block(64 * kScoreWaves);
+    if (a.plan.whole16)
+        hipLaunchKernelGGL((k_paged_scores<T, OWN, PRE, true>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((k_paged_scores<T, OWN, PRE, false>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((k_paged_values<T, (OWN > 2 ? 2 : OWN), (PRE > 2 ? 2 : PRE)>),
                        dim3((unsigned)(a.plan.first + a.plan.own.workgroups)), dim3(64 * kWaves), 0, st,
                        a);
 }
 template <typename T>
 void go_rows_wide(const PagedArgs& a, hipStream_t st) {
-    const bool pre = a.groups > 0 && a.plan.pre.rows > 16;
-    if (a.plan.own.rows > 16) go<T, 2, 2>(a, st);
-    else if (pre) go<T, 1, 2>(a, st);
+    const int pre = a.groups > 0 ? a.plan.pre.rows : 16;
+    if (a.plan.own.rows == 64) go<T, 4, 4>(a, st);
+    else if (a.plan.own.rows == 32) go<T, 2, 2>(a, st);
+    else if (pre == 32) go<T, 1, 2>(a, st);
     else go<T, 1, 1>(a, st);
 }
 
