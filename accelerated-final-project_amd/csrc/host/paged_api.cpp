@@ -127,18 +127,14 @@ atn::RowJob job(const Tensor& in, const Tensor& out, int rotate, int paged) {
     j.out = const_cast<void*>(out.p);
     for (int i = 0; i < 3; ++i) j.is[i] = in.s[i], j.os[i] = out.s[i];
     j.heads = in.n[1];
+    j.by_heads = atn::divider(j.heads);
     j.rotate = rotate;
     j.paged = paged;
     return j;
 }
 int go_rotary(int dtype, atn::RotaryArgs* a, void* stream) {
-    const size_t es = size_of(dtype);
-    const int w = 16 / (int)es;
-    a->vec = a->D % w == 0 && a->r.rot % (a->r.half ? 2 * w : w) == 0;
-    for (int j = 0; j < a->jobs; ++j)
-        a->vec = a->vec && pieces16(a->job[j].in, a->job[j].is, es) &&
-                 pieces16(a->job[j].out, a->job[j].os, es);
     a->by_t = atn::divider(a->T);
+    a->by_pairs = atn::divider(std::max(1, a->r.rot / 2));
     int dev;
     const int st = atn_host::device(&dev);
     if (st != ATN_OK) return st;

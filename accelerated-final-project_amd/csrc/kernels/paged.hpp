@@ -65,6 +65,7 @@ struct RowJob {
     void* out;
     int64_t is[3], os[3];
     int heads, rotate, paged;
+    Divider by_heads;
 };
 struct RotaryArgs {
     PagedView c;        // jobs that are paged: len, table
@@ -75,8 +76,7 @@ struct RotaryArgs {
     const int* count;   // [B], or null: T
     int B, T, D;
     int with_cache;
-    int vec;            // 16-byte pieces
-    Divider by_t;
+    Divider by_t, by_pairs;  // by_pairs: rot / 2
 };
 hipError_t launch_rotary(int dtype, const RotaryArgs& a, hipStream_t st);
 hipError_t launch_paged_advance(const PagedView& c, const int* count, int T, hipStream_t st);
