@@ -115,6 +115,17 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
     if (groups > 0) {
         // (groups are on the device: tiles for groups of equal size)
         pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, runs);
+        // Prefixes of many query rows beside sequences of few: a launch of k_paged_many, which begins
+        // with 24 us more than nothing and reads at 4.5 TB/s, or tiles of 32 (64) rows in the launch of
+        // the sequences' own, each of which reads the prefix again, at 6 TB/s (from L2 for the most):
+        // 8192 rows
+        // shared by 32 sequences of 64 to 1024 rows of their own, 32 over 8 heads of 128 dims, 57 against
+        // 70 us; 4 times 16384 shared by 16 each 85 against 66 in the prefixes' launch alone.
+        const int narrow = D > 64 ? 32 : 64;
+        const double bytes = (double)c.rows * groups * c.G * D * 4;
+        if (pre.kind == kMany && own.kind == kNarrow &&
+            ceil_div(ceil_div(c.B, groups) * R, narrow) * bytes / 6e6 < 24 + bytes / 4.5e6)
+            pre = {kNarrow, narrow};
         // one launch takes both, in tiles of as many rows
         // (head_d > 256: or own 16, prefixes 32)
         if (pre.kind == kWide && own.rows == 16) pre.rows = std::min(pre.rows, 32);
