@@ -30,26 +30,43 @@ __global__ __launch_bounds__(256) void k_paged_starts(PagedArgs a, int2* starts)
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Which kernel takes items of about R query rows, and its tile.  runs: rows are whole 16-byte pieces, and
-// pages whole runs of 16 rows.
+// pages whole runs of 16 rows.  pairs: of segments and kv heads;
+// keys: of an item, at most.
 enum Kind { kNarrow, kMany, kWide };
 struct Tile {
     Kind kind;
     int rows;
+    int whole;  // kMany: items whole
 };
-Tile tile_of(int dtype, int D, int64_t R, bool runs) {
+Tile tile_of(int dtype, int D, int64_t R, int64_t pairs, int64_t keys, bool runs) {
     const bool bf = dtype == kDtypeBF16;
     // (64 rows where they leave no more than a fourth more rows empty than 32 do)
     if (D > kPagedNarrow)
         return {kWide, R <= 16 ? 16 : R > 32 && 4 * (ceil_div(R, 64) * 64) <= 5 * (ceil_div(R, 32) * 32)
-                                       ? 64 : 32};
-    if (bf && runs && D <= 128 && R > 32) {
-        // the tile that leaves the fewest rows empty, the larger of equals
-        int best = 64;
-        for (int rows : {128, 256})
-            if (ceil_div(R, rows) * rows <= ceil_div(R, best) * best) best = rows;
-        return {kMany, best};
+                                       ? 64 : 32, 0};
+    if (bf && runs && D <= 128 && R > 32 && keys >= 512) {
+        // The least estimated time of three tiles, with whole items a workgroup (one a CU) or with
+        // items in ranges, whose parts go through memory and a merge: 0.97 PFLOP/s in tiles of 256 rows,
+        // tiles of 128 and 64 take 1.33 and 1.45 times as long (they read K and V from LDS for fewer
+        // rows), a merge 12 us and its parts twice at 4.5 TB/s.  512 tokens over 8000 rows, 2 sequences of
+        // 32 over 8 heads: 180 us in ranges of 256 rows, 204 in whole items of 128; 256 over 1000, 4
+        // sequences: 77 and 46.
+        Tile best{kMany, 0, 0};
+        double least = 0;
+        for (int rows : {256, 128, 64}) {
+            const int64_t items = pairs * ceil_div(R, rows), rounds = ceil_div(items, 256) * 256;
+            const double work = (double)items * rows * keys * D * 4 / 0.97e9 *
+                                (rows == 256 ? 1. : rows == 128 ? 1.33 : 1.45);
+            const double whole = work * rounds / items;
+            const double split = work + 12 + (double)pairs * R * D * 16 / 4.5e6;
+            if (least == 0 || std::min(whole, split) < least) {
+                least = std::min(whole, split);
+                best = {kMany, rows, whole <= split};
+            }
+        }
+        return best;
     }
-    return {kNarrow, R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64};
+    return {kNarrow, R <= 16 ? 16 : R <= 32 || !bf || D > 64 ? 32 : 64, 0};
 }
 
 // A pass of `segments` segments of at most `most` query rows of a kv head (all: of all segments), over
@@ -66,7 +83,7 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
     int per_cu;    // workgroups that a CU holds at once (the kernels' registers and LDS)
     if (t.kind == kMany) {
         per_cu = 1;
-        p.kb = p.rows == 256 ? 64 : 128;
+        p.kb = p.rows == 64 ? 128 : 64;
         p.turn = 1;
     } else if (t.kind == kWide) {
         per_cu = mt == 1 && !bf ? 3 : 2;  // (of the values)
@@ -88,6 +105,7 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
         1, std::min(slots, ceil_div(p.items * (blocks + kPagedPad), 2 * p.turn)));
     p.line = p.items * (blocks + kPagedPad) + 2ll * p.turn * p.ranges;
     p.split = !may_be_whole || (p.items < 4 * slots && blocks > 7 * p.turn / 2);
+    if (p.many && may_be_whole) p.split = !t.whole;
     p.parts = p.ranges + p.items;
     // whole items in several runs of dims a workgroup, where there are workgroups enough
     if (t.kind == kWide && !p.split)
@@ -111,10 +129,10 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
     const int D = c.D;
     const int64_t R = (int64_t)(H / c.G) * T, all = R * c.B;
     const bool runs = whole16 && c.page_rows % 16 == 0;
-    Tile own = tile_of(dtype, D, R, runs), pre = own;
+    Tile own = tile_of(dtype, D, R, (int64_t)c.B * c.G, c.rows, runs), pre = own;
     if (groups > 0) {
         // (groups are on the device: tiles for groups of equal size)
-        pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, runs);
+        pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, (int64_t)groups * c.G, c.rows, runs);
         // Prefixes of many query rows beside sequences of few: a launch of k_paged_many, which begins
         // with 24 us more than nothing and reads at 4.5 TB/s, or tiles of 32 (64) rows in the launch of
         // the sequences' own, each of which reads the prefix again, at 6 TB/s (from L2 for the most):
@@ -125,7 +143,7 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
         const double bytes = (double)c.rows * groups * c.G * D * 4;
         if (pre.kind == kMany && own.kind == kNarrow &&
             ceil_div(ceil_div(c.B, groups) * R, narrow) * bytes / 6e6 < 24 + bytes / 4.5e6)
-            pre = {kNarrow, narrow};
+            pre = {kNarrow, narrow, 0};
         // one launch takes both, in tiles of as many rows
         // (head_d > 256: or own 16, prefixes 32)
         if (pre.kind == kWide && own.rows == 16) pre.rows = std::min(pre.rows, 32);

@@ -27,9 +27,10 @@ struct PagedMany {
     static constexpr int X = ALL * CH / 512;             // pieces of K (and of V) a lane a stage
     static constexpr int SUB = ALL / 16, AHEAD = 64 / SUB;
     static_assert(X * 512 == ALL * CH, "whole pieces a lane");
-    // the results of a key group but the first: slabs of 64 rows, one a buffer
-    static_assert(KG == 1 || (KG - 1) * ROWS / 64 <= 3, "slabs");
-    static_assert(KG == 1 || kStage >= 64 * DP * 4, "a slab in a buffer");
+    // the results of a key group but the first: slabs of 64 rows, one a buffer where they fit it
+    static constexpr bool kInBuffers = KG > 1 && kStage >= 64 * DP * 4;
+    static_assert(!kInBuffers || (KG - 1) * ROWS / 64 <= 3, "slabs");
+    static constexpr int kSlabs = KG > 1 && !kInBuffers ? (KG - 1) * ROWS * DP / 4 : 1;
     // Pieces lie at a place of their row that changes with it, so that the rows which one LDS
     // cycle reads lie in different banks: 16 keys at one piece (K), 4 keys at four (V).
     static __device__ __forceinline__ int k_place(int key, int c) {
@@ -57,6 +58,7 @@ __global__ __launch_bounds__(512, 2) void k_paged_many(PagedArgs a) {
     constexpr int ALL = N::ALL, KG = N::KG, AHEAD = N::AHEAD, ROWS_X = 64 / CH;  // rows of a wave's load
     // (each an object of its own: the compiler lets reads of one pass loads into another)
     __shared__ __align__(16) char k0[N::kStage], k1[N::kStage], v0[N::kStage], v1[N::kStage];
+    __shared__ float4 slabs[N::kSlabs];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5, rg = wave % RG, kg = wave / RG;
     const int D = a.c.D, pieces = D / 8;
@@ -343,8 +345,9 @@ __global__ __launch_bounds__(512, 2) void k_paged_many(PagedArgs a) {
             const int here = opaque(lane), hcol = here & 31, hhalf = here >> 5, turn = hcol & (P - 1);
             float4* stats = reinterpret_cast<float4*>(k0);
             auto slab = [&](int g) {
-                const int x = (g - 1) * (N::ROWS / 64) + rg / 2;
-                return reinterpret_cast<float4*>(x == 0 ? v0 : x == 1 ? v1 : k1) + (32 * (rg & 1) + hcol) * P;
+                const int x = (g - 1) * (N::ROWS / 64) + rg / 2, row = 32 * (rg & 1) + hcol;
+                if (!N::kInBuffers) return slabs + (64 * x + row) * P;
+                return reinterpret_cast<float4*>(x == 0 ? v0 : x == 1 ? v1 : k1) + row * P;
             };
             if (kg > 0) {
                 if (hhalf == 0) stats[(kg - 1) * N::ROWS + 32 * rg + hcol] = make_float4(m, l, used, 0.f);
@@ -456,7 +459,7 @@ void go_many(const PagedArgs& a, dim3 grid, hipStream_t st) {
     if (rows == 64)
         hipLaunchKernelGGL((k_paged_many<DP, 2, 32, PRE>), grid, block, 0, st, a);
     else if (rows == 128)
-        hipLaunchKernelGGL((k_paged_many<DP, 4, 64, PRE>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((k_paged_many<DP, 4, 32, PRE>), grid, block, 0, st, a);
     else
         hipLaunchKernelGGL((k_paged_many<DP, 8, 64, PRE>), grid, block, 0, st, a);
 }
