@@ -31,14 +31,14 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Which kernel takes items of about R query rows, and its tile.  runs: rows are whole 16-byte pieces, and
 // pages whole runs of 16 rows.  pairs: of segments and kv heads;
-// keys: of an item, at most.
+// keys: of an item, at most; may_be_whole: a workgroup may take a whole item.
 enum Kind { kNarrow, kMany, kWide };
 struct Tile {
     Kind kind;
     int rows;
     int whole;  // kMany: items whole
 };
-Tile tile_of(int dtype, int D, int64_t R, int64_t pairs, int64_t keys, bool runs) {
+Tile tile_of(int dtype, int D, int64_t R, int64_t pairs, int64_t keys, bool runs, bool may_be_whole) {
     const bool bf = dtype == kDtypeBF16;
     // (64 rows where they leave no more than a fourth more rows empty than 32 do)
     if (D > kPagedNarrow)
@@ -59,9 +59,10 @@ Tile tile_of(int dtype, int D, int64_t R, int64_t pairs, int64_t keys, bool runs
                                 (rows == 256 ? 1. : rows == 128 ? 1.33 : 1.45);
             const double whole = work * rounds / items;
             const double split = work + 12 + (double)pairs * R * D * 16 / 4.5e6;
-            if (least == 0 || std::min(whole, split) < least) {
-                least = std::min(whole, split);
-                best = {kMany, rows, whole <= split};
+            const double time = may_be_whole ? std::min(whole, split) : split;
+            if (least == 0 || time < least) {
+                least = time;
+                best = {kMany, rows, may_be_whole && whole <= split};
             }
         }
         return best;
@@ -129,16 +130,16 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
     const int D = c.D;
     const int64_t R = (int64_t)(H / c.G) * T, all = R * c.B;
     const bool runs = whole16 && c.page_rows % 16 == 0;
-    Tile own = tile_of(dtype, D, R, (int64_t)c.B * c.G, c.rows, runs), pre = own;
+    Tile own = tile_of(dtype, D, R, (int64_t)c.B * c.G, c.rows, runs, true), pre = own;
     if (groups > 0) {
         // (groups are on the device: tiles for groups of equal size)
-        pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, (int64_t)groups * c.G, c.rows, runs);
+        pre = tile_of(dtype, D, ceil_div(c.B, groups) * R, (int64_t)groups * c.G, c.rows, runs,
+                      false);
         // Prefixes of many query rows beside sequences of few: a launch of k_paged_many, which begins
         // with 24 us more than nothing and reads at 4.5 TB/s, or tiles of 32 (64) rows in the launch of
         // the sequences' own, each of which reads the prefix again, at 6 TB/s (from L2 for the most):
-        // 8192 rows
-        // shared by 32 sequences of 64 to 1024 rows of their own, 32 over 8 heads of 128 dims, 57 against
-        // 70 us; 4 times 16384 shared by 16 each 85 against 66 in the prefixes' launch alone.
+        // 8192 rows shared by 32 sequences of 64 to 1024 rows of their own, 32 over 8 heads of 128 dims,
+        // 57 against 70 us; 4 times 16384 shared by 16 each 85 against 66 in the prefixes' launch alone.
         const int narrow = D > 64 ? 32 : 64;
         const double bytes = (double)c.rows * groups * c.G * D * 4;
         if (pre.kind == kMany && own.kind == kNarrow &&
