@@ -124,7 +124,8 @@ struct PagedArgs {
     int groups;
     PagedPlan plan;
     // scratch
-    const int2* starts;   // [B] first row of a sequence's own, its group or -1; null: few groups
+    const int2* starts;   // [B] first row of a sequence's own, its group or -1; [B]: whether groups
+                          // ascend; null: few groups
     float* own_scores;
     float* pre_scores;
     float* own_part;

@@ -8,11 +8,18 @@ namespace {
 
 constexpr int kInWave = 64;  // groups that a wave's lanes hold
 
-// Many groups: where each sequence's own rows begin, and its group, once for the kernels that follow.
-// first ascends, so the last group that begins at or before b is the one.
+// Many groups: where each sequence's own rows begin, and its group, once for the kernels that follow;
+// behind them, whether first ascends: then the last group that begins at or before b is the one.
 __global__ __launch_bounds__(256) void k_paged_starts(PagedArgs a, int2* starts) {
     const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b >= a.c.B) return;
+    int down = 0;
+    for (int i = threadIdx.x; i < a.groups; i += 256) down |= a.first[i + 1] < a.first[i];
+    down = __syncthreads_or(down);
+    if (b > a.c.B) return;
+    if (b == a.c.B || down) {
+        starts[b] = b == a.c.B ? make_int2(!down, 0) : make_int2(0, -1);
+        return;
+    }
     int lo = 0, hi = a.groups;  // groups [0, lo) begin at or before b, [hi, groups) behind it
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
@@ -117,7 +124,7 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
 }
 
 size_t to16(size_t n) { return (n + 15) / 16 * 16; }
-size_t starts_bytes(int B, int groups) { return groups > kInWave ? to16((size_t)B * sizeof(int2)) : 0; }
+size_t starts_bytes(int B, int groups) { return groups > kInWave ? to16(((size_t)B + 1) * sizeof(int2)) : 0; }
 size_t part_bytes(const PagedPass& p, int D) {
     return to16((size_t)p.parts * p.part_rows * (D + 4) * sizeof(float));
 }
@@ -189,7 +196,7 @@ hipError_t launch_paged_attention(int dtype, PagedArgs a, void* scratch, hipStre
     char* at = static_cast<char*>(scratch);
     if (a.groups > kInWave) {
         int2* starts = reinterpret_cast<int2*>(at);
-        hipLaunchKernelGGL(k_paged_starts, dim3((unsigned)((a.c.B + 255) / 256)), dim3(256), 0, st, a,
+        hipLaunchKernelGGL(k_paged_starts, dim3((unsigned)(a.c.B / 256 + 1)), dim3(256), 0, st, a,
                            starts);
         a.starts = starts;
         at += starts_bytes(a.c.B, a.groups);

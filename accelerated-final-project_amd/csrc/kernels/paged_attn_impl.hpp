@@ -47,10 +47,11 @@ __device__ __forceinline__ int tokens_of(const PagedArgs& a, int b) {
 struct Groups {
     int first, end, rows;
 };
-// (first and shared may hold anything.)  Rows that are read once save the other members' reads, 2
-// es head_d bytes a row and kv head; but every query row's result then passes through the scratch
-// in two parts, 16 head_d bytes.  Groups with less to save read their rows as their own (5 sequences
-// of 281 tokens of 16 heads of 8192 dims, 19 rows shared: 1200 against 2450 us).
+// (first and shared may hold anything: groups of a list that does not ascend, which might overlap and
+// have more items than the host counted on, share nothing.)  Rows that are read once save the other
+// members' reads, 2 es head_d bytes a row and kv head; but every query row's result then passes
+// through the scratch in two parts, 16 head_d bytes.  Groups with less to save read their rows as
+// their own (5 sequences of 281 tokens of 16 heads of 8192 dims, 19 rows shared: 1200 against 2450 us).
 __device__ __forceinline__ Groups group_at(const PagedArgs& a, int i) {
     Groups g;
     g.first = min(max(a.first[i], 0), a.c.B - 1);
@@ -58,11 +59,17 @@ __device__ __forceinline__ Groups group_at(const PagedArgs& a, int i) {
     const int L = min(rows_in_use(a.c, g.first), a.c.rows), m = g.end - g.first;
     g.rows = min(max(a.shared[i], 0), L);
     if (m < 2 || (int64_t)g.rows * (m - 1) * a.es <= (int64_t)m * a.rep * a.T * 8) g.rows = 0;
+    if (a.starts && !a.starts[a.c.B].x) g.rows = 0;  // (does not ascend)
     return g;
 }
 __device__ __forceinline__ Groups groups_of(const PagedArgs& a, int lane) {
     Groups g{0, 0, 0};
-    if (lane < a.groups && !a.starts) g = group_at(a, lane);
+    bool down = false;
+    if (lane < a.groups && !a.starts) {
+        g = group_at(a, lane);
+        down = a.first[lane + 1] < a.first[lane];
+    }
+    if (__builtin_amdgcn_ballot_w64(down)) g.rows = 0;
     return g;
 }
 // Where sequence b's own rows begin, and its group or -1 (a wave's work; b may differ by lane).
@@ -82,7 +89,12 @@ template <int PRE>
 __device__ __forceinline__ Segment segment(const PagedArgs& a, const Groups& gr, int i) {
     Segment s;
     if (PRE) {
-        const Groups g = group_at(a, min(i, a.groups - 1));
+        const int j = min(i, a.groups - 1);
+        Groups g;
+        if (a.starts)
+            g = group_at(a, j);
+        else
+            g.first = __shfl(gr.first, j), g.end = __shfl(gr.end, j), g.rows = __shfl(gr.rows, j);
         s.first = g.first;
         s.members = g.end - g.first;
         s.lo = 0;

@@ -524,8 +524,9 @@ int atn_paged_append_ex(const atn_paged_cache *cache, const atn_drafts *tokens,
 /* Groups of consecutive sequences that begin with the same rows: sequences first[i] ... first[i + 1]
  * - 1 have rows 0 ... rows[i] - 1 in common (in the same pages, or in copies of them), all before
  * their new tokens: rows[i] <= len of each.  first ascends and lies in [0, batch]; sequences outside
- * have no group; a group of one, or of no rows, reads its rows as its own.  (Other values: results
- * are unspecified, accesses stay inside the tensors.) */
+ * have no group; a group of one, or of few rows beside its query rows, reads them as its sequences'
+ * own, and so do all where first does not ascend.  (Other values: results are unspecified, accesses
+ * stay inside the tensors.) */
 typedef struct atn_shared_prefix {
     const int32_t *first; /* [groups + 1], device */
     const int32_t *rows;  /* [groups], device */

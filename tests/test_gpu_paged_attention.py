@@ -419,3 +419,15 @@ def test_half_a_pool_past_4_gib(am, dev):
     k, v = (x.transpose(1, 0, 2, 3).reshape(1, G, 3 * page, D) for x in h16)
     want, wl, info = C.attend64(q.host, k, v, None, None, [151], [1])
     C.attend_close("bf16", D, out.numpy(), lse.numpy(), want, wl, info, [1])
+
+
+@pytest.mark.parametrize("D", [64, 128, 300])
+def test_groups_that_overlap(am, dev, D):
+    """A list that does not ascend shares nothing: every sequence's rows are read as its own."""
+    for B, first in ((6, [0, 6, 0, 6]), (6, [0, 4, 2, 6]), (6, [3, 6, 0, 6, 0, 6]),
+                     (70, [0, 70] * 33 + [0]), (70, list(range(68)) + [0, 70])):
+        p = P.Paged(am, "bf16", B, 4, 2, 1, D, 16, [90 + b % 7 for b in range(B)], first=[0, B], rows=[80])
+        groups = len(first) - 1
+        p.prefix = am.SharedPrefix(C.ints(first), C.ints([80] * groups))
+        run(am, p)
+        p.check()
