@@ -63,10 +63,13 @@ __global__ __launch_bounds__(512, 2) void k_paged_many(PagedArgs a) {
     const int col = lane & 31, half = lane >> 5, rg = wave % RG, kg = wave / RG;
     const int D = a.c.D, pieces = D / 8;
     const float scale = fabsf(a.scale);
-    if (pieces < CH) {  // (places of pieces past the row's end stay 0)
+    // Places of pieces past the row's end are 0 (and stay so, but where a span leaves its results there).
+    auto clear = [&]() {
         for (int e = 16 * tid; e < N::kStage; e += 16 * 512)
             for (char* z : {k0, k1, v0, v1}) *reinterpret_cast<uint4*>(z + e) = make_uint4(0, 0, 0, 0);
-    }
+        __syncthreads();
+    };
+    if (KG == 1 && pieces < CH) clear();
     // This wave's rows of a stage, of one run of 16: lane L loads place L % CH of row L / CH, load x
     // those ROWS_X rows on.  Which piece lies there: PagedMany's places.
     const int wrow = wave * X * ROWS_X, wrun = wrow / 16;
@@ -159,6 +162,7 @@ __global__ __launch_bounds__(512, 2) void k_paged_many(PagedArgs a) {
 
         const bool any = sp.first < last;
         __syncthreads();  // (the last span's stages have been read)
+        if (KG > 1 && pieces < CH) clear();
         Run r0{}, r1{};   // of the stage at work, and the next one
         if (any) {
             r0 = run_of(sp.first);

@@ -321,3 +321,23 @@ def test_many_groups_of_many_rows(am, dev, B, groups, D):
         p = P.Paged(am, "bf16", B, 2, 1, T, D, 16, lens, first=first, rows=rows)
         run(am, p)
         p.check()
+
+
+@pytest.mark.parametrize("D", [40, 80, 64, 128])
+@pytest.mark.parametrize("T", [40, 120])
+def test_several_items_a_workgroup(am, dev, D, T):
+    """Ranges that hold an item's end and the next one's beginning, rows of few pieces."""
+    rng = np.random.default_rng(D + T)
+    lens = [int(x) for x in rng.integers(0, 200, 75)]
+    p = P.Paged(am, "bf16", 75, 4, 4, T, D, 16, lens, slots=512)
+    run(am, p)
+    p.check()
+
+
+def test_overlapping_groups(am, dev):
+    for first in ([0, 6, 0, 6], [0, 4, 2, 6]):
+        p = P.Paged(am, "bf16", 6, 4, 2, 40, 128, 16, [600 + b for b in range(6)], first=[0, 6],
+                    rows=[590], slots=64)
+        p.prefix = am.SharedPrefix(C.ints(first), C.ints([590] * (len(first) - 1)))
+        run(am, p)
+        p.check()
