@@ -913,31 +913,53 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int each) {
                        ? part_stats<1>(a)[part_row<1>(a, bounded(a.plan.pre, pre.x + i), pre_in)]
                        : part_stats<0>(a)[part_row<0>(a, bounded(a.plan.own, own.x + i - pre.y), in_tile)];
         };
-        float M = -INFINITY;
-        for (int i = lane; i < parts; i += 64) M = fmaxf(M, stats_of(i).x);
-        M = wave_max(M);
-        const float base = base_of(M);
-        T* out = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2];
-#pragma unroll 1
-        for (int d0 = 256 * blockIdx.z; d0 < D; d0 += 256 * gridDim.z) {
-            float l = 0.f, used = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-            for (int i = WAVES == 4 ? wave : 0; i < parts; i += WAVES) {
-                const float4 z = stats_of(i);
-                const float f = exp2_(z.x - base);
-                l += f * z.y;
-                used += f * z.z;
+        // (4 parts' dims are asked for at once, the first ones beside the statistics)
+        constexpr int AT_ONCE = 4;
+        const int i_first = WAVES == 4 ? wave : 0;
+        float y[AT_ONCE][4];
+        auto load = [&](int i0, int d0) {
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int i = min(i0 + WAVES * u, parts - 1);
                 const float* from =
                     d0 + (i < pre.y ? part_dims<1>(a) +
                                           part_row<1>(a, bounded(a.plan.pre, pre.x + i), pre_in) * D
                                     : part_dims<0>(a) + part_row<0>(a, bounded(a.plan.own, own.x + i - pre.y),
                                                                     in_tile) * D);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int d = lane + 64 * c;
-                    const float y = d0 + d < D ? from[d] : 0.f;
+                for (int c = 0; c < 4; ++c) y[u][c] = d0 + lane + 64 * c < D ? from[lane + 64 * c] : 0.f;
+            }
+        };
+        const float4 mine = stats_of(min(lane, parts - 1));
+        load(i_first, 256 * blockIdx.z);
+        float M = mine.x;
+        for (int i = lane + 64; i < parts; i += 64) M = fmaxf(M, stats_of(i).x);
+        M = wave_max(M);
+        const float base = base_of(M);
+        T* out = (T*)a.out + b * a.os[0] + h * a.os[1] + tok * a.os[2];
+#pragma unroll 1
+        for (int d0 = 256 * blockIdx.z; d0 < D; d0 += 256 * gridDim.z) {
+            float l = 0.f, used = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int i0 = i_first; i0 < parts; i0 += WAVES * AT_ONCE) {
+                if (i0 > i_first || d0 > (int)(256 * blockIdx.z)) load(i0, d0);
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    const int i = i0 + WAVES * u;
+                    if (i >= parts) break;
+                    float4 z;
+                    if (i < 64) {
+                        z.x = __shfl(mine.x, i), z.y = __shfl(mine.y, i), z.z = __shfl(mine.z, i);
+                    } else {
+                        z = stats_of(i);
+                    }
+                    const float f = exp2_(z.x - base);
+                    l += f * z.y;
+                    used += f * z.z;
                     // (what is not finite stays so where the factor has vanished)
-                    x[c] += f == 0.f && !(fabsf(y) < INFINITY) ? y : f * y;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        x[c] += f == 0.f && !(fabsf(y[u][c]) < INFINITY) ? y[u][c] : f * y[u][c];
                 }
             }
             if constexpr (WAVES == 4) {
