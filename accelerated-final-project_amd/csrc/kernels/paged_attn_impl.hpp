@@ -25,7 +25,8 @@ namespace atn {
 
 constexpr int kPagedNarrow = 256;  // head_d up to which a wave holds a row tile's output
 constexpr int kPagedPad = 12;      // places of the line that beginning and ending an item count for
-constexpr int kPagedWideBlock = 32, kPagedWideTurn = 4;  // head_d above: keys of a block, blocks between barriers
+constexpr int kPagedWideBlock = 32;  // head_d above: keys of a block
+constexpr int kPagedWideTurn = 4;    // ... blocks between barriers
 constexpr int kPagedWideRows = 32;   // ... query rows of a workgroup of values, at most
 constexpr int kPagedWideDims = 512;  // ... dims of a workgroup (bf16; fp32: half)
 
@@ -656,7 +657,10 @@ __device__ __forceinline__ void each_span(const PagedArgs& a, int id, int kb, in
 // ---------------------------------------------------------------- head_d <= 256
 // Every wave walks its own blocks of keys, alone: scores, running maximum and sum, and its own
 // output tile in registers (cache_tiles.hpp); nothing passes through LDS but Q and, at the
-// end, the waves' results.
+// end, the waves' results.  The read of K and V bounds it: one token of 32 over 8 heads, 128 bf16 dims,
+// 8 sequences of 1000 to 32000 rows, 100 us, 5.4 TB/s; 32 sequences of 64 to 1024 rows under 8192
+// shared ones, 45 us, 4.5 TB/s with the shared rows' four reads, three of which L2 answers.  Of short
+// contexts latency: 300 rows 8.4 us, of which code, lengths, pages, K and V are a chain.
 template <typename T, int DP, int MT, int MODE>
 struct PagedNarrow : CacheTiles<T, DP, MT, MODE> {
     using N = CacheTiles<T, DP, MT, MODE>;
@@ -856,8 +860,9 @@ __global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE>::kMinWaves)) voi
 // ---------------------------------------------------------------- parts
 // The parts of a row added up, in their order: the prefix's, then its own.  A workgroup takes `each`
 // rows a wave (or, WAVES = 4, `each` rows, whose parts its waves share) of one pair, whose place in
-// the lines it finds once.  A launch and a chain of loads (first, len, counts, statistics, dims): 6
-// to 8 us beside 5 for the launch; 33 us where 32768 rows of two parts come back from memory.  Rows of
+// the lines it finds once.  A launch and a chain of loads (groups, lengths, statistics, dims): 8 us for
+// 256 rows, 11 to 17 for 1024 to 2048 of 10 to 17 parts, 29 where 32768 rows of two parts come back
+// from memory.  With each part's dims asked for behind its statistics it took 1 to 6 us more.  Rows of
 // one range and no prefix are written already.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int each) {
