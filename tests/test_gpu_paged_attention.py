@@ -431,3 +431,47 @@ def test_groups_that_overlap(am, dev, D):
         p.prefix = am.SharedPrefix(C.ints(first), C.ints([80] * groups))
         run(am, p)
         p.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 90), (512, 2)])
+def test_without_lse(am, dev, dtype, D, T):
+    """The same output; in place of the queries is refused, as the library's other calls do it."""
+    for first in (None, [0, 3]):
+        p = P.Paged(am, dtype, 3, 4, 2, T, D, 16, [900, 700, 810], first=first,
+                    rows=None if first is None else [650])
+        run(am, p)
+        p.check()
+        out = p.out.base.bits()
+        p.out.base.upload(p.out._flat(np.full(p.out.host.shape, 7.0, np.float32)))
+        am.paged_attention_ex(p.cache, p.drafts, p.out.dev, None, prefix=p.prefix)
+        assert np.array_equal(p.out.base.bits(), out)
+    with pytest.raises(am.AtnError) as e:
+        am.paged_attention_ex(p.cache, p.drafts, p.Q.dev, None)
+    assert e.value.status == -5
+
+
+@pytest.mark.parametrize("D", [64, 512])
+def test_prefix_that_passes_a_member(am, dev, D):
+    """Rows behind a member's own: unspecified results for it, the others' as they should be."""
+    p = P.Paged(am, "f32", 4, 2, 1, 1, D, 16, [300, 310, 20, 305], first=[0, 2, 4], rows=[280, 16])
+    p.prefix = am.SharedPrefix(C.ints([0, 2, 4]), C.ints([280, 1 << 30]))
+    run(am, p)
+    want, lse, info = p.want()
+    got = p.out.numpy()
+    tol, _ = C.attend_tol("f32", D, want, info)
+    assert (np.abs(got[:2] - want[:2]) <= tol[:2]).all() and np.isfinite(p.lse.numpy()[:2]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 384])
+def test_the_same_page_many_times(am, dev, D):
+    """A table may name a page in several places; max_len may be less than the prefix."""
+    p = P.Paged(am, "bf16", 3, 4, 2, 1, D, 16, [200, 190, 210], first=[0, 3], rows=[160])
+    table = p.table.copy()
+    table[:, 1:10] = table[0, 0]
+    p.tab.upload(table)
+    p.table = table
+    run(am, p)
+    p.check()
+    run(am, p, max_len=100)
+    p.check(p.want(lens=[99, 99, 99]))
