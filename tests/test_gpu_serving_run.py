@@ -96,3 +96,90 @@ def test_run(am, dev, dtype, D, page):
         assert lens.numpy().tolist() == at
     assert at == [73, 51, 94]
     s.destroy()
+
+
+@pytest.mark.parametrize("dtype,D,T", [("bf16", 128, 1), ("bf16", 64, 40), ("f32", 80, 3), ("f32", 512, 2)])
+def test_captured_steps(am, dev, dtype, D, T):
+    """Append, attention and advance in one graph, replayed with other tokens, counts and tables between
+    the replays, beside the same program run eagerly on another stream: the same bits."""
+    import hip_rt
+    B, H, G, page, slots, pages = 3, 4, 2, 16, 64, 150
+    freq, _ = am.rope_frequencies(D)
+    rng = np.random.default_rng(8)
+    order = rng.permutation(pages)
+    start, shared = [540, 530, 560], 512
+    rows = rng.standard_normal((2, pages, G, page, D))
+
+    class Program:
+        def __init__(self):
+            self.K, self.V = (C.Tensor(x, dtype) for x in rows)
+            self.table = np.full((B, slots), -1, np.int32)
+            self.table[:, :32] = order[:32]
+            self.table[:, 32:62] = order[32:122].reshape(B, 30)
+            self.tab, self.lens = C.ints(self.table), C.ints(start)
+            cache = am.PagedCache(self.K.dev, self.V.dev, self.tab, self.lens)
+            self.Q, self.Kd, self.Vd = (C.Tensor(np.zeros((B, n, T, D)), dtype, order="rows")
+                                        for n in (H, G, G))
+            self.count = C.ints([T] * B)
+            self.out = C.Tensor(np.full((B, H, T, D), 7.0), dtype, order="rows")
+            self.lse = C.floats(np.full((B, H, T), 7.0))
+            drafts = am.Drafts(self.Q.dev, self.Kd.dev, self.Vd.dev, count=self.count)
+            rotary = am.Rotary(C.floats(freq), "half", D)
+            prefix = am.SharedPrefix(C.ints([0, B]), C.ints([shared]))
+            self.calls = [am.paged_append_call(cache, drafts, rotary, q_out=self.Q.dev),
+                          am.paged_attention_call(cache, drafts, self.out.dev, self.lse, prefix=prefix),
+                          am.paged_advance_call(cache, drafts)]
+            self.stream = hip_rt.Stream()
+
+        def step(self):
+            for call in self.calls:
+                call(self.stream)
+
+        def put(self, q, k, v, counts):
+            for x, y in ((self.Q, q), (self.Kd, k), (self.Vd, v)):
+                x.base.upload(x._flat(y.astype(np.float32)))
+            self.count.upload(np.array(counts))
+
+    a, b = Program(), Program()
+    b.step()  # (the stream's workspace has to be there before the capture)
+    b.stream.synchronize()
+    for x, y in zip((b.K, b.V), rows):
+        x.base.upload(x._flat(y.astype(np.float32)))
+    b.lens.upload(np.array(start))
+    graph = hip_rt.Graph(b.stream, b.step)
+    at = list(start)
+    for i in range(5):
+        q, k, v = (rng.standard_normal((B, n, T, D)) for n in (H, G, G))
+        counts = [T, (T + i) % (T + 1), max(0, T - i)]
+        if i == 3:  # a page of each moves elsewhere
+            for p in (a, b):
+                for x in (p.K, p.V):
+                    y = x.numpy()
+                    y[order[122:125]] = y[p.table[:, 33]]
+                    x.base.upload(x._flat(y))
+                p.table[:, 33] = order[122:125]
+                p.tab.upload(p.table)
+        for p in (a, b):
+            p.put(q, k, v, counts)
+        a.step()
+        graph.launch()
+        for p in (a, b):
+            p.stream.synchronize()
+        at = [x + n for x, n in zip(at, counts)]
+        assert a.lens.numpy().tolist() == b.lens.numpy().tolist() == at
+        for x, y in ((a.K, b.K), (a.V, b.V), (a.out, b.out), (a.Q, b.Q)):
+            assert np.array_equal(x.base.bits(), y.base.bits())
+        assert np.array_equal(a.lse.bits(), b.lse.bits())
+        # ... and they are what they should be
+        old = [n - m for n, m in zip(at, counts)]
+        Kc, Vc, Kn, Vn = (np.zeros((B, G, n, D)) for n in (max(old), max(old), T, T))
+        for pool, c, n in ((b.K.numpy(), Kc, Kn), (b.V.numpy(), Vc, Vn)):
+            for s in range(B):
+                r = P.rows_at(pool, b.table, s, at[s], page)
+                c[s, :, :old[s]], n[s, :, :counts[s]] = r[:, :old[s]], r[:, old[s]:]
+        want, wl, info = C.attend64(b.Q.numpy(), Kc, Vc, Kn, Vn, old, counts)
+        got, got_lse = b.out.numpy(), b.lse.numpy()
+        C.attend_close(dtype, D, got, got_lse, want, wl, info, counts)
+    graph.destroy()
+    for p in (a, b):
+        p.stream.destroy()
