@@ -91,6 +91,7 @@ struct PagedPass {
     int tiles;       // tiles of a segment, at most
     int ranges;      // the line of blocks in so many ranges, or
     int split;       // ... 0: an item a workgroup
+    int few;         // whole items of 8 waves each
     int turn;
     int groups;      // workgroups that share an item's dims (head_d > 256)
     int64_t items;   // at most

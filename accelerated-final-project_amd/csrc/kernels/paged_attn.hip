@@ -80,7 +80,7 @@ Tile tile_of(int dtype, int D, int64_t R, int64_t pairs, int64_t keys, bool runs
 // A pass of `segments` segments of at most `most` query rows of a kv head (all: of all segments), over
 // at most `keys` keys an item; kv: kv heads of a launch.
 PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, int64_t all, int64_t keys,
-                    int kv, bool may_be_whole) {
+                    int kv, bool may_be_whole, bool alone) {
     PagedPass p{};
     const bool bf = dtype == kDtypeBF16;
     p.many = t.kind == kMany;
@@ -114,6 +114,19 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
     p.line = p.items * (blocks + kPagedPad) + 2ll * p.turn * p.ranges;
     p.split = !may_be_whole || (p.items < 4 * slots && blocks > 7 * p.turn / 2);
     if (p.many && may_be_whole) p.split = !t.whole;
+    // Few items of short contexts: each whole, by a workgroup of 8 waves, where that is estimated to take
+    // less than ranges and their merge (8 us), at most 1024 of them, 256 where 4 waves each would take
+    // them whole too.  A CU reads 50 (fp32 38) GB/s of rows of whole tiles of dims, all of them
+    // 5.2 TB/s; 1 MiB an item at most, since the host knows no lengths but the bound and one long
+    // sequence alone takes its time.  One token of 32 over 8 heads of 128 bf16 dims: 600 rows 14.5 in
+    // ranges, 10.9 whole; 1500 rows 14.9 and 18.7; 32 sequences of 500 to 1000 rows 31.6 and 22.3, 100
+    // of 16 heads 75.6 and 72.3; 64 of 300 rows 17 by 4 waves and 21 by 8.
+    if (t.kind == kNarrow && alone && p.rows == 16) {
+        const double dim = 2. * keys * (bf ? 2 : 4), item = dim * ceil_div(D, 64) * 64;
+        p.few = p.items <= (p.split ? 1024 : 256) && item <= 1 << 20 &&
+                item / (bf ? 50e3 : 38e3) <= 8 + dim * D * p.items / 5.2e6;
+    }
+    if (p.few) p.split = 0;
     p.parts = p.ranges + p.items;
     // whole items in several runs of dims a workgroup, where there are workgroups enough
     if (t.kind == kWide && !p.split)
@@ -161,9 +174,9 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
     p.whole16 = whole16;
     // all kv heads at once, unless the scratch does not hold their parts and scores
     for (p.kv = c.G;; p.kv = (p.kv + 1) / 2) {
-        p.own = plan_pass(dtype, D, own, R, c.B, all, c.rows, p.kv, true);
+        p.own = plan_pass(dtype, D, own, R, c.B, all, c.rows, p.kv, true, groups == 0);
         if (groups > 0) {
-            p.pre = plan_pass(dtype, D, pre, all, groups, all, c.rows, p.kv, false);
+            p.pre = plan_pass(dtype, D, pre, all, groups, all, c.rows, p.kv, false, false);
             p.pre.workgroups = (int64_t)p.pre.ranges * p.pre.groups;
             p.first = pre.kind == kMany ? 0 : (int)p.pre.workgroups;
         }

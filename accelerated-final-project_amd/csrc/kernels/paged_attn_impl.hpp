@@ -660,11 +660,12 @@ __device__ __forceinline__ void each_span(const PagedArgs& a, int id, int kb, in
 // end, the waves' results.  The read of K and V bounds it: one token of 32 over 8 heads, 128 bf16 dims,
 // 8 sequences of 1000 to 32000 rows, 100 us, 5.4 TB/s; 32 sequences of 64 to 1024 rows under 8192
 // shared ones, 45 us, 4.5 TB/s with the shared rows' four reads, three of which L2 answers.  Of short
-// contexts latency: 300 rows 8.4 us, of which code, lengths, pages, K and V are a chain.
-template <typename T, int DP, int MT, int MODE>
+// contexts latency: code, lengths, pages, K and V are a chain; few items have 8 waves each (300 rows
+// 8.4 us, 9.0 with 4).
+template <typename T, int DP, int MT, int MODE, int WAVES_>
 struct PagedNarrow : CacheTiles<T, DP, MT, MODE> {
     using N = CacheTiles<T, DP, MT, MODE>;
-    static constexpr int WAVES = 4;
+    static constexpr int WAVES = WAVES_;
     // registers: the output tile, K and V of a block, the scores and weights, addresses; with the
     // next block's K loaded ahead except where only that would not leave two waves a SIMD
     static constexpr int kRegs = DP / 4 * (MT + 1) + 20 * MT + 44;
@@ -680,9 +681,9 @@ struct PagedNarrow : CacheTiles<T, DP, MT, MODE> {
     static_assert(kLds <= 160 * 1024, "LDS");
 };
 
-template <typename T, int DP, int MT, int MODE, bool RUNS, int PRE>
+template <typename T, int DP, int MT, int MODE, bool RUNS, int WAVES_, int PRE>
 __device__ __forceinline__ void paged_narrow(const PagedArgs& a, int id, char* lds) {
-    using N = PagedNarrow<T, DP, MT, MODE>;
+    using N = PagedNarrow<T, DP, MT, MODE, WAVES_>;
     constexpr int KB = N::KB, SUB = N::SUB, KS = N::KS, VS = N::VS, VL = N::VL, WAVES = N::WAVES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, col = lane & 15;
@@ -847,14 +848,20 @@ __device__ __forceinline__ void paged_narrow(const PagedArgs& a, int id, char* l
 // The first workgroups take the prefixes' ranges (where those are tiles of as many rows), the others
 // the sequences' own.
 template <typename T, int DP, int MT, int MODE, bool RUNS>
-__global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE>::kMinWaves)) void k_paged_narrow(
+__global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE, 4>::kMinWaves)) void k_paged_narrow(
     PagedArgs a) {
-    __shared__ __align__(16) char lds[PagedNarrow<T, DP, MT, MODE>::kLds];
+    __shared__ __align__(16) char lds[PagedNarrow<T, DP, MT, MODE, 4>::kLds];
     const int id = (int)blockIdx.x - a.plan.first;
     if (id < 0)
-        paged_narrow<T, DP, MT, MODE, RUNS, 1>(a, blockIdx.x, lds);
+        paged_narrow<T, DP, MT, MODE, RUNS, 4, 1>(a, blockIdx.x, lds);
     else
-        paged_narrow<T, DP, MT, MODE, RUNS, 0>(a, id, lds);
+        paged_narrow<T, DP, MT, MODE, RUNS, 4, 0>(a, id, lds);
+}
+// Few whole items: 8 waves each (paged_plan).
+template <typename T, int DP, int MODE, bool RUNS>
+__global__ __launch_bounds__(512, 2) void k_paged_few(PagedArgs a) {
+    __shared__ __align__(16) char lds[PagedNarrow<T, DP, 1, MODE, 8>::kLds];
+    paged_narrow<T, DP, 1, MODE, RUNS, 8, 0>(a, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------- parts
@@ -1001,7 +1008,15 @@ void go_pages(const PagedArgs& a, dim3 grid, hipStream_t st) {
         hipLaunchKernelGGL((k_paged_narrow<T, DP, MT, MODE, false>), grid, dim3(256), 0, st, a);
 }
 template <typename T, int DP, int MODE>
+void go_few(const PagedArgs& a, dim3 grid, hipStream_t st) {
+    if (a.c.page_rows % 16 == 0)
+        hipLaunchKernelGGL((k_paged_few<T, DP, MODE, true>), grid, dim3(512), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_paged_few<T, DP, MODE, false>), grid, dim3(512), 0, st, a);
+}
+template <typename T, int DP, int MODE>
 void go_rows(const PagedArgs& a, dim3 grid, hipStream_t st) {
+    if (a.plan.own.few) return go_few<T, DP, MODE>(a, grid, st);
     if (a.plan.own.rows == 16) return go_pages<T, DP, 1, MODE>(a, grid, st);
     if (a.plan.own.rows == 32) return go_pages<T, DP, 2, MODE>(a, grid, st);
     if constexpr (DP == 64 && sizeof(T) == 2) go_pages<T, DP, 4, MODE>(a, grid, st);
