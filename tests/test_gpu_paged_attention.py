@@ -475,3 +475,17 @@ def test_the_same_page_many_times(am, dev, D):
     p.check()
     run(am, p, max_len=100)
     p.check(p.want(lens=[99, 99, 99]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [2, 16, 64, 72, 128, 160, 192, 256])
+@pytest.mark.parametrize("page", [16, 24])
+def test_few_and_many_items(am, dev, dtype, D, page):
+    """Items whole by 8 waves or by 4, or in ranges, by how many there are and how long they may be."""
+    rng = np.random.default_rng(D)
+    for B, rows in ((2, 160), (2, 9000), (150, 160), (150, 9000), (600, 300)):
+        lens = [int(x) for x in rng.integers(0, 150, B)]
+        p = P.Paged(am, dtype, B, 4, 2, 1, D, page, lens, [int(x > 0) for x in rng.integers(0, 9, B)],
+                    slots=-(-rows // page))
+        run(am, p)
+        p.check()
