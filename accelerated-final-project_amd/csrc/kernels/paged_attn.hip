@@ -121,7 +121,9 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
     // sequence alone takes its time.  One token of 32 over 8 heads of 128 bf16 dims: 600 rows 14.5 in
     // ranges, 10.9 whole; 1500 rows 14.9 and 18.7; 32 sequences of 500 to 1000 rows 31.6 and 22.3, 100
     // of 16 heads 75.6 and 72.3; 64 of 300 rows 17 by 4 waves and 21 by 8.
-    if (t.kind == kNarrow && alone && p.rows == 16) {
+    // Tiles of 32 rows up to 128 dims (8 waves' results of more pass LDS): 32 sequences of 6 tokens over
+    // 500 to 1000 rows 38.3 and 25.3.
+    if (t.kind == kNarrow && alone && (p.rows == 16 || (p.rows == 32 && D <= 128))) {
         const double dim = 2. * keys * (bf ? 2 : 4), item = dim * ceil_div(D, 64) * 64;
         p.few = p.items <= (p.split ? 1024 : 256) && item <= 1 << 20 &&
                 item / (bf ? 50e3 : 38e3) <= 8 + dim * D * p.items / 5.2e6;

@@ -858,10 +858,10 @@ __global__ __launch_bounds__(256, (PagedNarrow<T, DP, MT, MODE, 4>::kMinWaves)) 
         paged_narrow<T, DP, MT, MODE, RUNS, 4, 0>(a, id, lds);
 }
 // Few whole items: 8 waves each (paged_plan).
-template <typename T, int DP, int MODE, bool RUNS>
+template <typename T, int DP, int MT, int MODE, bool RUNS>
 __global__ __launch_bounds__(512, 2) void k_paged_few(PagedArgs a) {
-    __shared__ __align__(16) char lds[PagedNarrow<T, DP, 1, MODE, 8>::kLds];
-    paged_narrow<T, DP, 1, MODE, RUNS, 8, 0>(a, blockIdx.x, lds);
+    __shared__ __align__(16) char lds[PagedNarrow<T, DP, MT, MODE, 8>::kLds];
+    paged_narrow<T, DP, MT, MODE, RUNS, 8, 0>(a, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------- parts
@@ -1007,16 +1007,19 @@ void go_pages(const PagedArgs& a, dim3 grid, hipStream_t st) {
     else
         hipLaunchKernelGGL((k_paged_narrow<T, DP, MT, MODE, false>), grid, dim3(256), 0, st, a);
 }
-template <typename T, int DP, int MODE>
+template <typename T, int DP, int MT, int MODE>
 void go_few(const PagedArgs& a, dim3 grid, hipStream_t st) {
     if (a.c.page_rows % 16 == 0)
-        hipLaunchKernelGGL((k_paged_few<T, DP, MODE, true>), grid, dim3(512), 0, st, a);
+        hipLaunchKernelGGL((k_paged_few<T, DP, MT, MODE, true>), grid, dim3(512), 0, st, a);
     else
-        hipLaunchKernelGGL((k_paged_few<T, DP, MODE, false>), grid, dim3(512), 0, st, a);
+        hipLaunchKernelGGL((k_paged_few<T, DP, MT, MODE, false>), grid, dim3(512), 0, st, a);
 }
 template <typename T, int DP, int MODE>
 void go_rows(const PagedArgs& a, dim3 grid, hipStream_t st) {
-    if (a.plan.own.few) return go_few<T, DP, MODE>(a, grid, st);
+    if (a.plan.own.few && a.plan.own.rows == 16) return go_few<T, DP, 1, MODE>(a, grid, st);
+    if constexpr (DP <= 128) {  // (paged_plan: their results in LDS)
+        if (a.plan.own.few) return go_few<T, DP, 2, MODE>(a, grid, st);
+    }
     if (a.plan.own.rows == 16) return go_pages<T, DP, 1, MODE>(a, grid, st);
     if (a.plan.own.rows == 32) return go_pages<T, DP, 2, MODE>(a, grid, st);
     if constexpr (DP == 64 && sizeof(T) == 2) go_pages<T, DP, 4, MODE>(a, grid, st);

@@ -489,3 +489,16 @@ def test_few_and_many_items(am, dev, dtype, D, page):
                     slots=-(-rows // page))
         run(am, p)
         p.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [2, 7, 40, 64, 72, 128, 160, 192, 250, 256])
+@pytest.mark.parametrize("page", [16, 24])
+def test_few_and_many_items_of_several_rows(am, dev, dtype, D, page):
+    rng = np.random.default_rng(D)
+    for B, T, rows in ((2, 15, 200), (2, 9, 9000), (20, 10, 600), (2, 45, 200), (140, 11, 170)):
+        lens = [int(x) for x in rng.integers(0, 150, B)]
+        p = P.Paged(am, dtype, B, 4, 2, T, D, page, lens, [int(x) for x in rng.integers(0, T + 1, B)],
+                    slots=-(-rows // page))
+        run(am, p)
+        p.check()
