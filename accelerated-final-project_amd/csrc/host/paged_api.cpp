@@ -32,19 +32,55 @@ int tensor(const void* p, const int64_t* given, int n0, int n1, int n2, int D, s
 bool same(const Tensor& a, const Tensor& b) {
     return a.p == b.p && a.n[1] == b.n[1] && a.s[0] == b.s[0] && a.s[1] == b.s[1] && a.s[2] == b.s[2];
 }
-// No element in common: apart, or columns of the same rows (all heads of a token in one row of a
-// buffer, the other tensor's beside them).
+// No element in common.  Elements of a and b in one place are whole numbers n_i in [lo_i, hi_i] of steps
+// u_i, and of single elements (between -(D - 1) and D - 1), that add up to b's distance from a: sought
+// from the largest step down, among the n_i that leave a rest which the smaller steps reach.  Strides
+// that nest leave two or three of them a step; where there are more the tensors count as meeting.
+struct Steps {
+    int n = 0;
+    int64_t u[6], lo[6], hi[6];
+    int64_t reach_lo[7], reach_hi[7];  // of the steps from i on
+    bool hit(int64_t distance, int i, int* tries) const {
+        if (distance < reach_lo[i] || distance > reach_hi[i]) return false;
+        if (i == n || --*tries < 0) return true;
+        // n_i u_i in [distance - reach_hi[i + 1], distance - reach_lo[i + 1]]
+        const int64_t from = distance - reach_hi[i + 1], to = distance - reach_lo[i + 1], d = u[i];
+        const int64_t first = std::max(lo[i], from / d + (from % d > 0));
+        const int64_t last = std::min(hi[i], to / d - (to % d < 0));
+        if (last - first > 8) return true;
+        for (int64_t k = first; k <= last; ++k)
+            if (hit(distance - k * d, i + 1, tries)) return true;
+        return false;
+    }
+};
 bool apart(const Tensor& a, const Tensor& b) {
     if (!meet(a.r, b.r)) return true;
-    const int64_t row = a.s[2] ? a.s[2] : b.s[2];
-    if (row <= 0 || a.s[2] != b.s[2] || a.n[2] != b.n[2] || a.n[0] != b.n[0] || a.s[0] != b.s[0])
-        return false;
-    if (a.s[0] % row != 0 || (a.n[0] > 1 && a.s[0] < row * a.n[2])) return false;
-    const int64_t bytes = (const char*)b.p - (const char*)a.p;
-    if (bytes % (int64_t)a.es) return false;
-    const int64_t d = (bytes / (int64_t)a.es % row + row) % row;
-    const int64_t wa = a.s[1] * (a.n[1] - 1) + a.D, wb = b.s[1] * (b.n[1] - 1) + b.D;
-    return d >= wa && d + wb <= row;
+    const int64_t bytes = (const char*)b.p - (const char*)a.p, es = (int64_t)a.es;
+    if (bytes % es) return false;
+    Steps x;
+    auto add = [&](int64_t u, int64_t lo, int64_t hi) {
+        if (u == 0 || lo == hi) return;
+        int i = x.n++;
+        for (; i > 0 && x.u[i - 1] < u; --i)
+            x.u[i] = x.u[i - 1], x.lo[i] = x.lo[i - 1], x.hi[i] = x.hi[i - 1];
+        x.u[i] = u, x.lo[i] = lo, x.hi[i] = hi;
+    };
+    for (int i = 0; i < 3; ++i) {
+        if (a.s[i] == b.s[i]) {
+            add(a.s[i], 1 - b.n[i], a.n[i] - 1);
+        } else {  // (0 where a dimension has one index)
+            add(a.s[i], 0, a.n[i] - 1);
+            add(b.s[i], 1 - b.n[i], 0);
+        }
+    }
+    x.reach_lo[x.n] = 1 - b.D;
+    x.reach_hi[x.n] = a.D - 1;
+    for (int i = x.n - 1; i >= 0; --i) {
+        x.reach_lo[i] = x.reach_lo[i + 1] + x.lo[i] * x.u[i];
+        x.reach_hi[i] = x.reach_hi[i + 1] + x.hi[i] * x.u[i];
+    }
+    int tries = 256;
+    return !x.hit(bytes / es, 0, &tries);
 }
 
 struct Pool {

@@ -509,7 +509,8 @@ typedef struct atn_rotated {
 /* n (1 to 3) tensors turned by the same angles: token t of sequence b by position pos[b][t]
  * ([batch][tokens]; NULL: t).  inverse != 0: the transposed (inverse, but for amplitude) map, so
  * the gradient of the inputs from that of the outputs.  Dims from rotary_dim on are copied.  The
- * tensors may be views of one buffer whose rows hold them side by side. */
+ * tensors may be views of one buffer (rows that hold them side by side, say): no output may have an
+ * element in common with another tensor, but for its own `in`. */
 int atn_rotary_ex(int dtype, const atn_rotary *rotary, const atn_rotated *x, int n, int batch,
                   int tokens, int head_d, const int32_t *pos, int inverse, void *stream);
 

@@ -140,3 +140,31 @@ def test_many_tokens(am, dev, B, T):
     am.paged_advance_ex(a.cache, a.drafts)
     cap = a.table.shape[1] * 16
     assert a.len.numpy().tolist() == [min(cap, l + n + T) for l, n in zip(lens, a.counts)]
+
+
+@pytest.mark.parametrize("order", ["rows", "heads"])
+@pytest.mark.parametrize("B,T", [(3, 1), (33, 1), (2, 4)])
+def test_columns_of_one_buffer(am, dev, order, B, T):
+    """Queries, keys and values as columns of a projection's rows (or heads of one buffer), the queries
+    turned where they are; a token each, as in a step of decoding, and several."""
+    import types
+
+    import hip_rt
+    Hq, G, D = 6, 2, 32
+    a = Append(am, "bf16", B, Hq, G, T, D, 16, [(11 * b) % 40 for b in range(B)], rot=D)
+    n = Hq + 2 * G
+    x = np.concatenate([a.Q.host, a.Kd.host, a.Vd.host], axis=1)  # [B][n][T][D]
+    lie = (0, 2, 1, 3) if order == "rows" else (0, 1, 2, 3)
+    base = hip_rt.DeviceArray.from_numpy(np.ascontiguousarray(x.transpose(lie)), "bf16")
+    s = (n * T * D, D, n * D, 1) if order == "rows" else (n * T * D, T * D, D, 1)
+    step = s[1]
+
+    def view(first, heads):
+        return hip_rt.DeviceArray.wrap(base.ptr + 2 * first * step, (B, heads, T, D), "bf16", strides=s,
+                                       keep=base)
+
+    q = view(0, Hq)
+    am.paged_append_ex(a.cache, am.Drafts(q, view(Hq, G), view(Hq + G, G)), a.rotary, q_out=q)
+    got = base.numpy().transpose(lie)
+    a.check(q_out=types.SimpleNamespace(numpy=lambda: got[:, :Hq]))
+    assert np.array_equal(got[:, Hq:], x[:, Hq:])

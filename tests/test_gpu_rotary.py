@@ -171,3 +171,25 @@ def test_streams_and_captured(am, dev):
         hip_rt.synchronize()
     g.destroy()
     s.destroy()
+
+
+@pytest.mark.parametrize("B,T", [(1, 1), (5, 1), (40, 1), (3, 2)])
+@pytest.mark.parametrize("order", ["rows", "heads"])
+def test_views_of_one_buffer_a_token_each(am, dev, order, B, T):
+    """Queries and keys where a projection (or a buffer of heads) holds them, few tokens."""
+    import hip_rt
+    rng = np.random.default_rng(6)
+    H, G, D = 4, 2, 48
+    n = H + 2 * G
+    x = C.rounded(rng.standard_normal((B, T, n, D) if order == "rows" else (B, n, T, D)), "bf16")
+    lie = (0, 2, 1, 3) if order == "rows" else (0, 1, 2, 3)
+    base = hip_rt.DeviceArray.from_numpy(x, "bf16")
+    s = (n * T * D, D, n * D, 1) if order == "rows" else (n * T * D, T * D, D, 1)
+    q, k = (hip_rt.DeviceArray.wrap(base.ptr + 2 * first * s[1], (B, heads, T, D), "bf16", strides=s,
+                                    keep=base) for first, heads in ((0, H), (H, G)))
+    freq, _ = am.rope_frequencies(D)
+    pos = rng.integers(0, 999, (B, T)).astype(np.int32)
+    am.rotary_ex(am.Rotary(C.floats(freq), "half"), [(q, q), (k, k)], pos=C.ints(pos))
+    got, x = base.numpy().transpose(lie), x.transpose(lie)
+    close("bf16", got[:, :H + G], x[:, :H + G], pos, freq, True, D)
+    assert np.array_equal(got[:, H + G:], x[:, H + G:])

@@ -292,3 +292,62 @@ def test_division_by_multiplication():
         x = np.unique(np.concatenate([q * d, q * d + d - 1, [0, (1 << 31) - 1]]))
         for v in x[x < 1 << 31].tolist():
             assert (v * m >> 32) >> (l - 1) == v // d
+
+
+@pytest.mark.parametrize("B,T", [(1, 1), (2, 1), (32, 1), (2, 2), (3, 5)])
+def test_columns_of_one_buffer(am, B, T):
+    """Queries, keys and values as columns of a projection's rows, one token a sequence or several."""
+    ok = no_device(am)
+    if ok == 0:
+        pytest.skip("addresses that nothing may dereference")
+    row = (4 + 2 + 2) * 64
+    s = (T * row, 64, row)
+    c = cache(am, batch=B)
+
+    def of(k):  # K's first column
+        return drafts(am, tokens=T, Q=QA, K=QA + 2 * k, V=QA + 2 * 6 * 64, q_stride=s, k_stride=s, v_stride=s)
+
+    assert append(am, c, of(4 * 64), rotary(am), q_out=QA, st=s) == ok
+    assert append(am, c, of(4 * 64 - 1), rotary(am), q_out=QA, st=s) == -5
+    x = [dict(inp=QA, out=QA, in_stride=s, out_stride=s),
+         dict(inp=QA + 512, out=QA + 512, in_stride=s, out_stride=s, heads=2)]
+    assert rotate(am, x, rotary(am), B=B, T=T) == ok
+    x[1].update(inp=QA + 510, out=QA + 510)
+    assert rotate(am, x, rotary(am), B=B, T=T) == -5
+    # (the last row's columns behind the buffer's rows: the next sequence's queries)
+    x[1].update(inp=QA + 2 * (row - 64), out=QA + 2 * (row - 64))
+    assert rotate(am, x, rotary(am), B=B, T=T) == (-5 if B * T > 1 else ok)
+
+
+def test_layouts_of_one_buffer(am):
+    """Two tensors in one buffer, in any order of its dimensions: refused where they have an element in
+    common, by the sets of their elements."""
+    ok = no_device(am)
+    if ok == 0:
+        pytest.skip("addresses that nothing may dereference")
+    rng = np.random.default_rng(11)
+    r = rotary(am, rotary_dim=2)
+    seen = {-5: 0, ok: 0}
+    for _ in range(3000):
+        B, T, D = (int(x) for x in rng.choice([1, 2, 3, 4], 3))
+        D += D % 2
+        heads = [int(x) for x in rng.integers(1, 4, 2)]
+        sizes = dict(b=B + int(rng.integers(0, 2)), h=sum(heads) + int(rng.integers(0, 2)), t=T)
+        at, s = D + int(rng.integers(0, 3)), {}
+        for d in rng.permutation(list("bht")):
+            s[d] = at
+            at *= sizes[d]
+        st = (s["b"], s["h"], s["t"])
+        first = [0, heads[0] * s["h"]]
+        if rng.random() < 0.5:
+            first[1] = int(rng.integers(0, at))
+        first = first if rng.random() < 0.5 else first[::-1]
+        e = [set((f + s["b"] * np.arange(B)[:, None, None, None] + s["h"] * np.arange(h)[:, None, None] +
+                  s["t"] * np.arange(T)[:, None] + np.arange(D)).ravel().tolist())
+             for f, h in zip(first, heads)]
+        x = [dict(inp=QA + 2 * f, out=QA + 2 * f, in_stride=st, out_stride=st, heads=h)
+             for f, h in zip(first, heads)]
+        want = -5 if e[0] & e[1] else ok
+        assert rotate(am, x, r, B=B, T=T, D=D) == want, (B, T, D, heads, st, first)
+        seen[want] += 1
+    assert min(seen.values()) > 500
