@@ -315,7 +315,7 @@ int atn_paged_append_ex(const atn_paged_cache* cache, const atn_drafts* d, const
     if (st != ATN_OK) return st;
     const Range lists[5] = {table_range(cache), ints(cache->len, B), ints(d->count, B),
                             ints(pos, (int64_t)B * T), ints(rotary ? rotary->freq : nullptr, a.r.rot / 2)};
-    if (cache->K == cache->V) return ATN_ERR_ALIASING;
+    if (!apart(p.k, p.v)) return ATN_ERR_ALIASING;
     for (const Range& w : {p.k.r, p.v.r, qo.r})
         for (const Range& o : lists)
             if (meet(w, o)) return ATN_ERR_ALIASING;

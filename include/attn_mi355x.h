@@ -517,7 +517,7 @@ int atn_rotary_ex(int dtype, const atn_rotary *rotary, const atn_rotated *x, int
 /* Cache rows len[b] + t = K (rotated) and V of token t < count[b]; q_out (if not NULL) = Q rotated
  * (may be Q itself, with its strides; rows past count stay).  Positions: pos[b][t], or len[b] + t
  * where pos is NULL.  rotary NULL: nothing is rotated.  Rows that the table does not hold are
- * dropped. */
+ * dropped.  The pools K and V may interleave, but have no element in common. */
 int atn_paged_append_ex(const atn_paged_cache *cache, const atn_drafts *tokens,
                         const atn_rotary *rotary, const int32_t *pos, void *q_out,
                         const int64_t *q_out_stride, void *stream);

@@ -351,3 +351,20 @@ def test_layouts_of_one_buffer(am):
         assert rotate(am, x, r, B=B, T=T, D=D) == want, (B, T, D, heads, st, first)
         seen[want] += 1
     assert min(seen.values()) > 500
+
+
+@pytest.mark.parametrize("c,code", [
+    (dict(V=KA + 64), -5), (dict(V=KA + 2), -5), (dict(V=KA - 2 * 9 * 2048 - 2), -5),
+    (dict(V=KA + 2 * 10 * 2048 - 2), -5), (dict(V=KA + 2 * 10 * 2048), 0),
+    # V behind K in every page, in every page's every row, and one element too near
+    (dict(V=KA + 4096, k_stride=(4096, 1024, 64), v_stride=(4096, 1024, 64)), 0),
+    (dict(V=KA + 4094, k_stride=(4096, 1024, 64), v_stride=(4096, 1024, 64)), -5),
+    (dict(V=KA + 4096, k_stride=(4096, 1024, 64), v_stride=(4096, 64, 128)), 0),
+    (dict(V=KA + 128, k_stride=(4096, 2048, 128), v_stride=(4096, 2048, 128)), 0),
+    (dict(V=KA + 126, k_stride=(4096, 2048, 128), v_stride=(4096, 2048, 128)), -5),
+    (dict(V=KA + 128, k_stride=(4096, 2048, 128), v_stride=(4096, 2048, 130)), -5)])
+def test_append_to_overlapping_pools(am, c, code):
+    ok = no_device(am)
+    if ok == 0:
+        pytest.skip("addresses that nothing may dereference")
+    assert append(am, cache(am, **c), drafts(am), rotary(am)) == (code or ok)
