@@ -186,17 +186,21 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
         p.own.workgroups =
             (p.own.split ? p.own.ranges : (int64_t)c.B * p.kv * p.own.tiles) * p.own.groups;
         // scores: two workgroups a CU, where the dims give each wave two steps still
-        p.shares = 1;
         int64_t blocks = p.own.scores / (p.own.rows * kPagedWideBlock);
         if (groups > 0) blocks += p.pre.scores / (p.pre.rows * kPagedWideBlock);
+        p.shares = 1;
         while (p.wide && blocks * p.shares < 512 && p.shares < 8 &&
                D >= 2 * p.shares * 8 * (dtype == kDtypeBF16 ? 256 : 128))
             p.shares *= 2;
+        size_t rest = starts_bytes(c.B, groups);
+        if (groups > 0) rest += part_bytes(p.pre, D);
+        if (groups > 0 || p.own.split) rest += part_bytes(p.own, D);
+        for (;; p.shares /= 2) {
+            p.scratch = rest + (size_t)(p.own.scores + p.pre.scores) * p.shares * sizeof(float);
+            // (each share's scores are apart: fewer shares before the call is refused)
+            if (p.scratch <= scratch_cap || p.kv > 1 || p.shares == 1) break;
+        }
         p.score_grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks * p.shares, 1024));
-        p.scratch = starts_bytes(c.B, groups) +
-                    (size_t)(p.own.scores + p.pre.scores) * p.shares * sizeof(float);
-        if (groups > 0) p.scratch += part_bytes(p.pre, D);
-        if (groups > 0 || p.own.split) p.scratch += part_bytes(p.own, D);
         if (p.scratch <= scratch_cap || p.kv == 1) break;
     }
     if (p.scratch > scratch_cap && groups == 0 && p.own.split) {  // items whole: no parts

@@ -368,3 +368,37 @@ def test_append_to_overlapping_pools(am, c, code):
     if ok == 0:
         pytest.skip("addresses that nothing may dereference")
     assert append(am, cache(am, **c), drafts(am), rotary(am)) == (code or ok)
+
+
+def need(am, c, d, p=None, n=0):
+    return am.lib().atn_paged_attention_workspace_bytes(ref(c), ref(d), ref(p), n)
+
+
+WS = 0x7E0000000000
+
+
+def test_workspace_of_a_larger_bound(am):
+    """A workspace asked for with one bound of the lengths serves every smaller one, where dims are
+    shared by several workgroups (each share has scores of its own) too."""
+    if no_device(am) == 0:
+        pytest.skip("addresses that nothing may dereference")
+    import random
+    rng = random.Random(5)
+    cases = [dict(D=8192, dt=0, B=1, G=1, rep=1, T=1, page=16, slots=1100, bounds=[16400, 4000]),
+             dict(D=2048, dt=0, B=1, G=1, rep=1, T=1, page=16, slots=1300, bounds=[20000, 16000])]
+    for _ in range(600):
+        D, page, slots = rng.choice([80, 128, 512, 2048, 8192]), rng.choice([16, 20]), \
+            int(2 ** rng.uniform(2, 10))
+        cases.append(dict(D=D, dt=rng.choice([0, 1]), B=int(2 ** rng.uniform(0, 5)), G=rng.choice([1, 2, 8]),
+                          rep=rng.choice([1, 4, 8]), T=int(2 ** rng.uniform(0, 9)), page=page, slots=slots,
+                          bounds=sorted((rng.randint(1, page * slots) for _ in range(4)), reverse=True)))
+    for x in cases:
+        c = cache(am, dtype=x["dt"], batch=x["B"], kv_heads=x["G"], pages=1 << 14, page_rows=x["page"],
+                  table_pages=x["slots"], head_d=x["D"])
+        d = drafts(am, heads=x["G"] * x["rep"], tokens=x["T"])
+        for p in (None, prefix(am, groups=(x["B"] + 1) // 2)):
+            for i, most in enumerate(x["bounds"]):
+                n = need(am, c, d, p, most)
+                assert n > 0
+                for less in x["bounds"][i:]:
+                    assert attend(am, c, d, p, max_len=less, ws=WS, wsb=n) == -6, (x, most, less)
