@@ -213,6 +213,31 @@ int check_attention(const atn_paged_cache* cache, const atn_drafts* d, const atn
     return ATN_OK;
 }
 
+// Whether the launches hold the plan.  (A dimension of a grid has less than 2^32 threads, workgroups of at
+// most 512.)
+bool lays_out(const atn::PagedPlan& p, int groups) {
+    return p.own.workgroups + p.first < 1 << 23 && p.own.line <= INT32_MAX &&
+           (groups == 0 || p.pre.line <= INT32_MAX);
+}
+// How a call runs in `room` bytes of scratch.  A prefix that does not fit is left out, its rows read as
+// the sequences' own, where no workspace that the library asks for would hold its parts, or where no group
+// can have anything to save, whatever its rows; else a larger workspace is worth asking for.
+void plan_call(int dtype, bool whole16, size_t room, atn::PagedArgs* a) {
+    auto plan = [&](size_t bytes) {
+        return atn::paged_plan(dtype, a->c, a->H, a->T, a->groups, whole16, bytes);
+    };
+    a->plan = plan(room);
+    if (a->groups == 0) return;
+    const size_t cap = atn_host::workspace_cap();
+    if (lays_out(a->plan, a->groups) &&
+        (a->plan.scratch <= room ||
+         (atn::saves_reads(a->c.rows, a->c.B, a->es, a->rep, a->T) && plan(cap).scratch <= cap)))
+        return;
+    a->groups = 0;
+    a->first = a->shared = nullptr;
+    a->plan = plan(room);
+}
+
 }  // namespace
 
 extern "C" {
@@ -359,9 +384,12 @@ size_t atn_paged_attention_workspace_bytes(const atn_paged_cache* cache, const a
     Tensor q;
     bool whole16;
     if (check_attention(cache, tokens, prefix, max_len, &a, &p, &q, &whole16) != ATN_OK) return 0;
-    return kSyncRegion + atn::paged_plan(cache->dtype, a.c, a.H, a.T, a.groups, whole16,
-                                         atn_host::workspace_cap())
-                             .scratch;
+    const size_t cap = atn_host::workspace_cap();
+    plan_call(cache->dtype, whole16, cap, &a);
+    // (a prefix that this bound of the lengths leaves out may fit with a smaller one)
+    const bool out = prefix && a.groups == 0 && a.c.B > 1 &&
+                     atn::saves_reads(a.c.rows, a.c.B, a.es, a.rep, a.T);
+    return kSyncRegion + (out ? std::max(cap, a.plan.scratch) : a.plan.scratch);
 }
 
 int atn_paged_attention_ex(const atn_paged_cache* cache, const atn_drafts* tokens,
@@ -393,11 +421,8 @@ int atn_paged_attention_ex(const atn_paged_cache* cache, const atn_drafts* token
         if (workspace_bytes < kSyncRegion) return ATN_ERR_WORKSPACE;
         room = workspace_bytes - kSyncRegion;
     }
-    a.plan = atn::paged_plan(cache->dtype, a.c, a.H, a.T, a.groups, whole16, room);
-    // (a dimension of a grid has less than 2^32 threads; workgroups of at most 512)
-    if (a.plan.own.workgroups + a.plan.first >= 1 << 23 || a.plan.own.line > INT32_MAX ||
-        (a.groups > 0 && a.plan.pre.line > INT32_MAX))
-        return ATN_ERR_SIZE_OVERFLOW;
+    plan_call(cache->dtype, whole16, room, &a);
+    if (!lays_out(a.plan, a.groups)) return ATN_ERR_SIZE_OVERFLOW;
     if (a.plan.scratch > room) return ATN_ERR_WORKSPACE;
     int dev;
     st = atn_host::device(&dev);

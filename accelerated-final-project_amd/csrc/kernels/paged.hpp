@@ -133,6 +133,13 @@ struct PagedArgs {
     float* pre_part;
     int g0, gs;           // this launch's kv heads
 };
+// Whether reading `rows` shared rows once for m sequences saves anything.  It saves the other members' reads,
+// 2 es head_d bytes a row and kv head; but every query row's result then passes through the scratch in two
+// parts, 16 head_d bytes (5 sequences of 281 tokens of 16 heads of 8192 dims, 19 rows shared: 1200 us read
+// as their own, 2450 read once).
+__host__ __device__ __forceinline__ bool saves_reads(int64_t rows, int m, int es, int rep, int T) {
+    return m >= 2 && rows * (m - 1) * es > (int64_t)m * rep * T * 8;
+}
 // whole16: the rows of K, V and Q are whole 16-byte pieces that lie so.
 PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
                      size_t scratch_cap);

@@ -203,6 +203,18 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
         p.score_grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks * p.shares, 1024));
         if (p.scratch <= scratch_cap || p.kv == 1) break;
     }
+    // A prefix needs parts, of a tile of rows each, and another bound of the lengths may have larger tiles:
+    // a workspace that was asked for with it holds a half or a fourth of the ranges.
+    for (int i = 0; i < 2 && groups > 0 && p.scratch > scratch_cap; ++i)
+        for (PagedPass* x : {&p.pre, &p.own}) {
+            if (x == &p.own && !x->split) continue;
+            p.scratch -= part_bytes(*x, D);
+            x->ranges = (x->ranges + 1) / 2;
+            x->parts = x->ranges + x->items;
+            x->workgroups = (int64_t)x->ranges * x->groups;
+            p.scratch += part_bytes(*x, D);
+            if (x == &p.pre && p.first > 0) p.first = (int)x->workgroups;
+        }
     if (p.scratch > scratch_cap && groups == 0 && p.own.split) {  // items whole: no parts
         p.scratch -= part_bytes(p.own, D);
         p.own.split = 0;

@@ -49,17 +49,14 @@ struct Groups {
     int first, end, rows;
 };
 // (first and shared may hold anything: groups of a list that does not ascend, which might overlap and
-// have more items than the host counted on, share nothing.)  Rows that are read once save the other
-// members' reads, 2 es head_d bytes a row and kv head; but every query row's result then passes
-// through the scratch in two parts, 16 head_d bytes.  Groups with less to save read their rows as
-// their own (5 sequences of 281 tokens of 16 heads of 8192 dims, 19 rows shared: 1200 against 2450 us).
+// have more items than the host counted on, share nothing; nor do those with too little to save.)
 __device__ __forceinline__ Groups group_at(const PagedArgs& a, int i) {
     Groups g;
     g.first = min(max(a.first[i], 0), a.c.B - 1);
     g.end = min(max(a.first[i + 1], 0), a.c.B);
     const int L = min(rows_in_use(a.c, g.first), a.c.rows), m = g.end - g.first;
     g.rows = min(max(a.shared[i], 0), L);
-    if (m < 2 || (int64_t)g.rows * (m - 1) * a.es <= (int64_t)m * a.rep * a.T * 8) g.rows = 0;
+    if (!saves_reads(g.rows, m, a.es, a.rep, a.T)) g.rows = 0;
     if (a.starts && !a.starts[a.c.B].x) g.rows = 0;  // (does not ascend)
     return g;
 }

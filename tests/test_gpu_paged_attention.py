@@ -502,3 +502,62 @@ def test_few_and_many_items_of_several_rows(am, dev, dtype, D, page):
                     slots=-(-rows // page))
         run(am, p)
         p.check()
+
+
+@pytest.mark.parametrize("dtype,D,T,page", [("bf16", 128, 40, 16), ("bf16", 128, 6, 20), ("f32", 80, 12, 16),
+                                            ("bf16", 512, 4, 16), ("f32", 2048, 4, 20)])
+def test_prefixes_that_no_workspace_holds(am, dev, tuner, dtype, D, T, page):
+    """A prefix whose parts the library's workspace does not hold: its rows are the sequences' own. The
+    size that a query gives runs, and so does a larger one, which holds the parts."""
+    import hip_rt
+    p = P.Paged(am, dtype, 4, 16, 2, T, D, page, [1200, 1100, 1300, 1000], [T, T, 1, T], first=[0, 4],
+                rows=[990])
+    whole = am.paged_attention_workspace_bytes(p.cache, p.drafts, p.prefix)
+    ws = hip_rt.DeviceArray((whole // 2,), "bf16", fill=0)
+    tuner.set(workspace_cap_mib=1)
+    need = am.paged_attention_workspace_bytes(p.cache, p.drafts, p.prefix)
+    assert need <= (1 << 20) + 40960 < whole
+    run(am, p)
+    p.check()
+    for n in (need, whole):
+        p.out.base.upload(p.out._flat(np.full(p.out.host.shape, 7.0, np.float32)))
+        run(am, p, workspace=hip_rt.DeviceArray.wrap(ws.ptr, (n // 2,), "bf16", keep=ws))
+        p.check()
+
+
+@pytest.mark.parametrize("dtype,D,T", [("bf16", 64, 48), ("f32", 80, 31), ("bf16", 512, 31)])
+def test_prefixes_of_too_few_rows_need_no_room(am, dev, dtype, D, T):
+    """Rows that no group reads once, whatever its list says: a workspace for the call without it."""
+    import hip_rt
+    p = P.Paged(am, dtype, 3, 8, 2, T, D, 16, [150, 140, 160], first=[0, 3], rows=[130])
+    most = 256
+    need = am.paged_attention_workspace_bytes(p.cache, p.drafts, None, most)
+    ws = hip_rt.DeviceArray((need // 2,), "bf16", fill=0)
+    run(am, p, workspace=ws, max_len=most)
+    p.check()
+
+
+@pytest.mark.parametrize("dtype,D", [("f32", 2048), ("bf16", 8192), ("f32", 8192)])
+@pytest.mark.parametrize("rows", [None, [700]])
+def test_fewer_shares_and_ranges(am, dev, dtype, D, rows):
+    """Workspaces from what the library asks for down to the least: fewer shares of the dims, fewer ranges."""
+    import hip_rt
+    p = P.Paged(am, dtype, 2, 2, 1, 1, D, 16, [800, 730], first=None if rows is None else [0, 2],
+                rows=rows)
+    need = am.paged_attention_workspace_bytes(p.cache, p.drafts, p.prefix)
+    ws = hip_rt.DeviceArray((need + 4096,), "bf16", fill=0)
+    tail = hip_rt.DeviceArray.view(ws, need // 2, (2048,))
+    tail.upload(np.full(2048, 3, np.uint16))
+    ran = 0
+    for i in range(16):
+        size = 40960 + (need - 40960) * (16 - i) // 16 // 16 * 16
+        small = hip_rt.DeviceArray.wrap(ws.ptr, (size // 2,), "bf16", keep=ws)
+        p.out.base.upload(p.out._flat(np.full(p.out.host.shape, 7.0, np.float32)))
+        try:
+            run(am, p, workspace=small)
+        except am.AtnError as e:
+            assert e.status == -8
+            break
+        ran += 1
+        p.check()
+    assert ran >= 4 and (tail.bits() == 3).all()

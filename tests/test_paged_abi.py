@@ -402,3 +402,53 @@ def test_workspace_of_a_larger_bound(am):
                 assert n > 0
                 for less in x["bounds"][i:]:
                     assert attend(am, c, d, p, max_len=less, ws=WS, wsb=n) == -6, (x, most, less)
+
+
+def test_prefixes_that_no_workspace_holds(am):
+    """A prefix saves reads and promises another order of sums, no more: where its parts do not fit the
+    library's workspace, or no group could save what they cost, the call runs as without it."""
+    ok = no_device(am)
+    if ok == 0:
+        pytest.skip("addresses that nothing may dereference")
+    for dtype, B, H, G, T, D, page, slots, groups in [
+            (1, 8, 32, 1, 4096, 128, 16, 512, 1), (1, 8, 32, 1, 4096, 128, 16, 4096, 2),
+            (1, 16, 64, 8, 8192, 128, 16, 1024, 4), (1, 58, 8, 1, 431, 512, 16, 32, 3),
+            (0, 8, 32, 1, 4096, 80, 20, 400, 3), (1, 40, 16, 1, 2048, 256, 16, 300, 20),
+            (0, 100, 8, 1, 256, 2048, 20, 8, 70)]:
+        c = cache(am, dtype=dtype, batch=B, kv_heads=G, pages=1 << 14, page_rows=page, table_pages=slots,
+                  head_d=D)
+        d, p = drafts(am, heads=H, tokens=T), prefix(am, groups=groups)
+        assert attend(am, c, d) == ok
+        assert attend(am, c, d, p) == ok
+        n = need(am, c, d, p)
+        assert need(am, c, d) <= n <= (1 << 30) + 40960
+        assert attend(am, c, d, p, ws=WS, wsb=n) == ok
+        # no group of so short rows beside so many queries is read once: no room for one is needed
+        least = need(am, c, d)
+        assert attend(am, c, d, p, max_len=64, ws=WS, wsb=least) == ok
+        # (a larger one than the library's holds them)
+        assert attend(am, c, d, p, ws=WS, wsb=1 << 40) == ok
+
+
+def test_prefixes_where_they_run_without(am):
+    """No call with a prefix is refused that runs without it, for want of room in the library's workspace or in
+    one that was asked for."""
+    if no_device(am) == 0:
+        pytest.skip("addresses that nothing may dereference")
+    import random
+    rng = random.Random(8)
+    for _ in range(1500):
+        D, page = rng.choice([64, 80, 128, 192, 512, 2048]), rng.choice([16, 20])
+        B, rep, T = int(2 ** rng.uniform(1, 6)), rng.choice([1, 4, 8, 32]), int(2 ** rng.uniform(0, 13))
+        c = cache(am, dtype=rng.choice([0, 1]), batch=B, kv_heads=rng.choice([1, 2, 8]), pages=1 << 14,
+                  page_rows=page, table_pages=int(2 ** rng.uniform(1, 12)), head_d=D)
+        d, p = drafts(am, heads=c.kv_heads * rep, tokens=T), prefix(am, groups=rng.randint(1, B))
+        plain = attend(am, c, d)
+        if plain != -6:
+            continue
+        assert attend(am, c, d, p) == -6
+        n = need(am, c, d, p)
+        assert attend(am, c, d, p, ws=WS, wsb=n) == -6
+        # ... with any smaller bound of the lengths
+        for _ in range(3):
+            assert attend(am, c, d, p, max_len=rng.randint(1, page * c.table_pages), ws=WS, wsb=n) == -6
