@@ -103,7 +103,7 @@ struct PagedPass {
 struct PagedPlan {
     PagedPass own, pre;
     int first;       // workgroups of a launch's grid that take the prefixes
-    int kv;          // kv heads of a launch
+    int seqs, kv;    // sequences (all, where there are groups) and kv heads of a launch
     int whole16;     // rows are whole 16-byte pieces that lie so
     int wide;        // head_d > 256:
     int shares;      // ... workgroups that share the dims of a block's scores

@@ -144,12 +144,12 @@ size_t part_bytes(const PagedPass& p, int D) {
     return to16((size_t)p.parts * p.part_rows * (D + 4) * sizeof(float));
 }
 
-}  // namespace
-
-PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
-                     size_t scratch_cap) {
+// ... of the sequences of c in one pass
+PagedPlan plan_sequences(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
+                         size_t scratch_cap) {
     PagedPlan p{};
     const int D = c.D;
+    p.seqs = c.B;
     const int64_t R = (int64_t)(H / c.G) * T, all = R * c.B;
     const bool runs = whole16 && c.page_rows % 16 == 0;
     Tile own = tile_of(dtype, D, R, (int64_t)c.B * c.G, c.rows, runs, true), pre = own;
@@ -223,6 +223,20 @@ PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bo
     return p;
 }
 
+}  // namespace
+
+PagedPlan paged_plan(int dtype, const PagedView& c, int H, int T, int groups, bool whole16,
+                     size_t scratch_cap) {
+    PagedView x = c;
+    PagedPlan p = plan_sequences(dtype, x, H, T, groups, whole16, scratch_cap);
+    // (head_d > 256: the scores of a part of the sequences at a time)
+    while (p.scratch > scratch_cap && groups == 0 && x.B > 1) {
+        x.B = (x.B + 1) / 2;
+        p = plan_sequences(dtype, x, H, T, groups, whole16, scratch_cap);
+    }
+    return p;
+}
+
 hipError_t launch_paged_attention(int dtype, PagedArgs a, void* scratch, hipStream_t st) {
     char* at = static_cast<char*>(scratch);
     if (a.groups > kInWave) {
@@ -241,25 +255,35 @@ hipError_t launch_paged_attention(int dtype, PagedArgs a, void* scratch, hipStre
         at += part_bytes(a.plan.pre, a.c.D);
     }
     a.own_part = reinterpret_cast<float*>(at);
-    for (a.g0 = 0; a.g0 < a.c.G; a.g0 += a.plan.kv) {
-        a.gs = std::min(a.plan.kv, a.c.G - a.g0);
-        PagedArgs x = a;
-        if (!x.plan.own.split)
-            x.plan.own.workgroups = (int64_t)x.c.B * x.gs * x.plan.own.tiles * x.plan.own.groups;
-        hipError_t e = hipGetLastError();
-        if (e == hipSuccess && x.plan.wide) e = launch_paged_wide(dtype, x, st);
-        if (e == hipSuccess && x.plan.pre.many) e = launch_paged_many(x, 1, st);
-        if (e == hipSuccess && x.plan.own.many) e = launch_paged_many(x, 0, st);
-        if (e == hipSuccess && !x.plan.wide && !x.plan.own.many)
-            e = dtype == kDtypeF32 ? launch_paged_narrow_f32(x, st) : launch_paged_narrow_bf16(x, st);
-        if (e == hipSuccess && (x.groups > 0 || x.plan.own.split)) {
-            if (dtype == kDtypeF32)
-                go_merge<float>(x, st);
-            else
-                go_merge<uint16_t>(x, st);
-            e = hipGetLastError();
+    const PagedArgs all = a;
+    for (int b0 = 0; b0 < all.c.B; b0 += a.plan.seqs) {
+        a.c.B = std::min(a.plan.seqs, all.c.B - b0);
+        a.c.table = all.c.table + (int64_t)b0 * a.c.slots;
+        a.c.len = all.c.len + b0;
+        a.count = all.count ? all.count + b0 : nullptr;
+        a.Q = (const char*)all.Q + b0 * a.qs[0] * a.es;
+        a.out = (char*)all.out + b0 * a.os[0] * a.es;
+        a.lse = all.lse ? all.lse + (int64_t)b0 * a.H * a.T : nullptr;
+        for (a.g0 = 0; a.g0 < a.c.G; a.g0 += a.plan.kv) {
+            a.gs = std::min(a.plan.kv, a.c.G - a.g0);
+            PagedArgs x = a;
+            if (!x.plan.own.split)
+                x.plan.own.workgroups = (int64_t)x.c.B * x.gs * x.plan.own.tiles * x.plan.own.groups;
+            hipError_t e = hipGetLastError();
+            if (e == hipSuccess && x.plan.wide) e = launch_paged_wide(dtype, x, st);
+            if (e == hipSuccess && x.plan.pre.many) e = launch_paged_many(x, 1, st);
+            if (e == hipSuccess && x.plan.own.many) e = launch_paged_many(x, 0, st);
+            if (e == hipSuccess && !x.plan.wide && !x.plan.own.many)
+                e = dtype == kDtypeF32 ? launch_paged_narrow_f32(x, st) : launch_paged_narrow_bf16(x, st);
+            if (e == hipSuccess && (x.groups > 0 || x.plan.own.split)) {
+                if (dtype == kDtypeF32)
+                    go_merge<float>(x, st);
+                else
+                    go_merge<uint16_t>(x, st);
+                e = hipGetLastError();
+            }
+            if (e != hipSuccess) return e;
         }
-        if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }

@@ -538,8 +538,9 @@ typedef struct atn_shared_prefix {
  * the rows behind are left as they were.  tokens: the queries (K and V are not used: they are rows of
  * the cache by now).  prefix (NULL: none): its rows are read once a group; results differ from those
  * without it by the order of sums alone.  scale, lse, out_stride and workspace as for
- * atn_tree_attention_ex (head_d > 256: one kv head's scores have to fit, 4 bytes for each query row
- * and row up to max_len, in tiles of 16 to 64 and 32; with a prefix one kv head's parts too, but for
+ * atn_tree_attention_ex (head_d > 256: one kv head's scores of one sequence have to fit, 4 bytes for
+ * each query row and row up to max_len, in tiles of 16 to 64 and 32; with a prefix those of all sequences
+ * and one kv head's parts too, but for
  * prefixes that the library's own workspace could not hold, or that are too short beside their query
  * rows to be read once: those are read as the sequences' own rows).  max_len: an upper bound of
  * len[b] + count[b] that the host knows (0: the rows of a table); the call is laid out for it, and rows

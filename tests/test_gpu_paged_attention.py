@@ -561,3 +561,43 @@ def test_fewer_shares_and_ranges(am, dev, dtype, D, rows):
         ran += 1
         p.check()
     assert ran >= 4 and (tail.bits() == 3).all()
+
+
+@pytest.mark.parametrize("dtype,D,T,page,order", [("bf16", 512, 30, 16, "heads"), ("bf16", 320, 21, 20, "rows"),
+                                                  ("f32", 1025, 13, 16, "rows"), ("f32", 512, 40, 16, "heads")])
+def test_sequences_in_turn(am, dev, tuner, dtype, D, T, page, order):
+    """head_d > 256 where the scores of all sequences pass the workspace: some sequences a launch, the
+    last ones fewer; on a stream and from a graph too, with a prefix that is left out."""
+    import hip_rt
+    B = 7
+    rng = np.random.default_rng(D)
+    lens = [int(x) for x in rng.integers(40, 1100, B)]
+    counts = [T, 0, T - 3, 1, T, 7, T]
+    p = P.Paged(am, dtype, B, 8, 2, T, D, page, lens, counts, first=[0, 3, 7], rows=[30, 20], order=order,
+                offset=3, pad=5, slots=70)
+    tuner.set(workspace_cap_mib=1)
+    want = p.want()
+    for prefix in (p.prefix, None):
+        p.prefix = prefix
+        p.out.base.upload(p.out._flat(np.full(p.out.host.shape, 7.0, np.float32)))
+        run(am, p)
+        p.check(want)
+    need = am.paged_attention_workspace_bytes(p.cache, p.drafts)
+    assert need <= (1 << 20) + 40960
+    ws = hip_rt.DeviceArray((need // 2 + 2048,), "bf16", fill=0)
+    tail = hip_rt.DeviceArray.view(ws, need // 2, (2048,))
+    tail.upload(np.full(2048, 3, np.uint16))
+    ws = hip_rt.DeviceArray.wrap(ws.ptr, (need // 2,), "bf16", keep=ws)
+    call = am.paged_attention_call(p.cache, p.drafts, p.out.dev, p.lse, workspace=ws)
+    s = hip_rt.Stream()
+    g = hip_rt.Graph(s, lambda: call(s))
+    for _ in range(3):
+        p.out.base.upload(p.out._flat(np.full(p.out.host.shape, 7.0, np.float32)))
+        g.launch()
+        s.synchronize()
+        p.check(want)
+        run(am, p)  # eager work between the replays
+        hip_rt.synchronize()
+    assert (tail.bits() == 3).all()
+    g.destroy()
+    s.destroy()

@@ -452,3 +452,23 @@ def test_prefixes_where_they_run_without(am):
         # ... with any smaller bound of the lengths
         for _ in range(3):
             assert attend(am, c, d, p, max_len=rng.randint(1, page * c.table_pages), ws=WS, wsb=n) == -6
+
+
+@pytest.mark.parametrize("dtype,B,H,G,T,D,rows", [
+    (1, 4, 32, 8, 2048, 512, 8192), (1, 64, 16, 1, 512, 1024, 8192), (0, 16, 8, 8, 4096, 2048, 8192),
+    (0, 1000, 4, 1, 300, 512, 4096), (1, 7, 32, 8, 2048, 512, 24576)])
+def test_prompts_of_wide_heads(am, dtype, B, H, G, T, D, rows):
+    """head_d > 256, scores of all sequences past the library's workspace: sequences in turn."""
+    ok = no_device(am)
+    if ok == 0:
+        pytest.skip("addresses that nothing may dereference")
+    c = cache(am, dtype=dtype, batch=B, kv_heads=G, pages=1 << 16, page_rows=16,
+              table_pages=rows // 16, head_d=D)
+    d = drafts(am, heads=H, tokens=T)
+    assert 40960 < need(am, c, d) <= (1 << 30) + 40960
+    assert attend(am, c, d) == ok
+    assert attend(am, c, d, prefix(am, groups=2)) == ok
+    # one sequence's scores of one kv head have to fit
+    one = 4 * (H // G) * T * rows
+    assert attend(am, c, d, ws=WS, wsb=one + (one >> 4)) == ok
+    assert attend(am, c, d, ws=WS, wsb=one // 2) == -8
