@@ -243,19 +243,24 @@ __global__ __launch_bounds__(512, 2) void k_paged_many(PagedArgs a) {
                         if (!(on >> (8 * (e >> 2) + (e & 3)) & 1u)) s[t][e] = -INFINITY;
                 }
                 // An infinity or NaN times a weight of 0 would reach rows that do not attend its key: V
-                // enters without them, and they are written over the results of the rows that do.
+                // enters without them, and they are written over the results of the rows that do (of
+                // keys that nobody attends, or of no page, there are none).
+                const int end = of_wave(attended<PRE>(a, sp, row0 + N::ROWS - 1));
                 uint32_t bad = 0;
 #pragma unroll 1
-                for (int e = tid; e < ALL * CH; e += 512) {
+                for (int e = opaque(tid); e < ALL * CH; e += 512) {
                     W16 z = reinterpret_cast<W16*>(vb)[e];
+                    const int key = e / CH, j = i * ALL + key;
+                    uint32_t any = 0;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const uint32_t hi = (z.w[w] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
                         const uint32_t lw = (z.w[w] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
                         z.w[w] &= ~(hi | lw);
-                        bad |= hi | lw;
+                        any |= hi | lw;
                     }
                     reinterpret_cast<W16*>(vb)[e] = z;
+                    if (j >= lo && j < end && (r0.ok >> (key / 16) & 1u)) bad |= any;
                 }
                 odd |= bad != 0;
                 __syncthreads();
@@ -432,30 +437,44 @@ __global__ __launch_bounds__(512, 2) void k_paged_many(PagedArgs a) {
                     store4(out + d, y, 4);
             }
         if (__syncthreads_or(odd) && kg == 0) {
+            // V's rows once more, dims 2 L and 2 L + 1 in lane L: for each of the two the rows (a bit each) that
+            // attend an infinity or NaN there (two parts of 512 tokens over 3000 rows, one infinity: 90 us,
+            // 57 without).
+            const bool live = to.b >= 0 && l == l;  // (NaN scores: NaN in every dim)
+            const int mine_upto = attended<PRE>(a, sp, row0 + r);
+            const int d = 2 * late, end = min(of_wave(attended<PRE>(a, sp, row0 + 32 * rg + 31)), last * ALL);
+            uint32_t pos[2] = {0, 0}, neg[2] = {0, 0}, nan[2] = {0, 0};
+#pragma unroll 1
+            for (int j0 = max(lo, sp.first * ALL) & -16; j0 < end; j0 += 16) {
+                const int page = of_wave(page_of(a.c, sp.s.first, j0));
+                if (!is_page(a.c, page)) continue;
+                const int in = j0 - over(j0, a.c.by_page) * a.c.page_rows;
+                const T* v = vp + page * a.c.vs[0] + in * a.c.vs[2] + min(d, D - 2);
+                uint32_t y[16];
+#pragma unroll
+                for (int u = 0; u < 16; ++u) __builtin_memcpy(&y[u], v + u * a.c.vs[2], 4);
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    const bool lw = (y[u] & 0x7f80u) == 0x7f80u, hi = (y[u] & 0x7f800000u) == 0x7f800000u;
+                    if (!__builtin_amdgcn_ballot_w64(lw || hi) || j0 + u < lo) continue;
+                    const uint32_t rows = (uint32_t)__builtin_amdgcn_ballot_w64(live && mine_upto > j0 + u);
+                    if (lw) (y[u] & 0x7fu ? nan : y[u] & 0x8000u ? neg : pos)[0] |= rows;
+                    if (hi) (y[u] & 0x7f0000u ? nan : y[u] >> 31 ? neg : pos)[1] |= rows;
+                }
+            }
             __threadfence_block();  // (this wave's own stores, from other lanes)
 #pragma unroll 1
             for (int x = 0; x < 32; ++x) {
-                const int row = row0 + 32 * rg + x;
-                const Row w = row_of<PRE>(a, sp, row);
-                const float lx = __shfl(l, x);
-                if (w.b < 0 || lx != lx) continue;  // (NaN scores: NaN in every dim)
-                const int end = min(attended<PRE>(a, sp, row), last * ALL);
-#pragma unroll 1
-                for (int d = late; d < D; d += 64) {
-                    float sum = 0.f;
-#pragma unroll 1
-                    for (int j = max(lo, sp.first * ALL); j < end; ++j) {
-                        const int page = page_of(a.c, sp.s.first, j);
-                        if (!is_page(a.c, page)) continue;
-                        const int in = j - over(j, a.c.by_page) * a.c.page_rows;
-                        const float y = Elem<T>::ld(vp + page * a.c.vs[0] + in * a.c.vs[2], d);
-                        sum += fabsf(y) < INFINITY ? 0.f : y;
-                    }
-                    if (fabsf(sum) < INFINITY) continue;
+                const Row w = row_of<PRE>(a, sp, row0 + 32 * rg + x);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (d >= D || !((pos[h] | neg[h] | nan[h]) >> x & 1u)) continue;
+                    const float y = (nan[h] | (pos[h] & neg[h])) >> x & 1u ? __builtin_nanf("")
+                                    : pos[h] >> x & 1u ? INFINITY : -INFINITY;
                     if (parted)
-                        part_dims<PRE>(a)[part_row<PRE>(a, max(sp.part, 0), 32 * rg + x) * D + d] = sum;
+                        part_dims<PRE>(a)[part_row<PRE>(a, max(sp.part, 0), 32 * rg + x) * D + d + h] = y;
                     else
-                        Elem<T>::st((T*)a.out + w.b * a.os[0] + w.h * a.os[1] + w.tok * a.os[2], d, sum);
+                        Elem<T>::st((T*)a.out + w.b * a.os[0] + w.h * a.os[1] + w.tok * a.os[2], d + h, y);
                 }
             }
         }

@@ -341,3 +341,58 @@ def test_overlapping_groups(am, dev):
         p.prefix = am.SharedPrefix(C.ints(first), C.ints([590] * (len(first) - 1)))
         run(am, p)
         p.check()
+
+
+@pytest.mark.parametrize("D,T,Hq,G,rows", [(128, 300, 8, 2, None), (64, 40, 4, 2, None), (80, 20, 4, 1, [896]),
+                                           (128, 20, 4, 2, [1504])])
+def test_many_values_that_are_not_finite(am, dev, D, T, Hq, G, rows):
+    """Infinities and NaN all over: in the dims of what a token attends, and nowhere else."""
+    lens = [1700, 1623, 1580]
+    first = None if rows is None else [0, 3]
+    p = P.Paged(am, "bf16", 3, Hq, G, T, D, 32, lens, [T, T - 6, 1], first=first, rows=rows, slots=70)
+    run(am, p)
+    p.check()
+    before, lse = p.out.numpy(), p.lse.numpy()
+    rng = np.random.default_rng(D + T)
+    V = p.V.host.copy()
+    hit = np.zeros(before.shape, bool)
+    for b in range(3):
+        for _ in range(60):
+            r = int(rng.integers(lens[b] - (30 if rng.random() < 0.5 else 900), lens[b] + p.counts[b]))
+            g, d = int(rng.integers(0, G)), int(rng.integers(0, D))
+            page = p.table[b, r // 32]
+            V[page, g, r % 32, d] = rng.choice([np.inf, -np.inf, np.nan])
+            for m in range(3):  # (a shared page is every member's)
+                if p.table[m, r // 32] == page:
+                    hit[m, g * Hq // G:(g + 1) * Hq // G, max(0, r - lens[m]):p.counts[m], d] = True
+    p.V.base.upload(p.V._flat(V))
+    run(am, p)
+    got = p.out.numpy()
+    assert np.array_equal(np.isfinite(got), ~hit)
+    assert np.array_equal(got[~hit], before[~hit]) and np.array_equal(p.lse.numpy(), lse)
+
+
+@pytest.mark.parametrize("T,lens,slots", [(512, [3000, 2990], 240), (40, [3000, 1], 240), (200, [60, 900], 2000)])
+def test_tails_of_any_content_cost_nothing(am, dev, T, lens, slots):
+    """What lies behind a sequence's rows costs no more where it holds NaN or infinities.  (Rows' values
+    looked at one key after another for each row would take 20 to 100 times the call.)"""
+    import time
+
+    import hip_rt
+
+    def least(fill):
+        p = P.Paged(am, "bf16", 2, 8, 2, T, 128, 16, lens, fill=fill, slots=slots)
+        call = am.paged_attention_call(p.cache, p.drafts, p.out.dev, p.lse)
+        times = []
+        for _ in range(7):
+            hip_rt.synchronize()
+            t0 = time.perf_counter()
+            for _ in range(3):
+                call()
+            hip_rt.synchronize()
+            times.append(time.perf_counter() - t0)
+        return min(times)
+
+    plain = least(0.0)
+    for fill in (np.nan, -np.inf):
+        assert least(fill) < 4 * plain
