@@ -839,9 +839,9 @@ class Rotary:
 def rotary_call(rotary: Rotary, tensors, pos=None, inverse: bool = False) -> Call:
     """atn_rotary_ex bound to its arguments.  tensors: up to three (x, out) of [B][heads][T][D]
     arrays, out may be x; pos [B][T]."""
-    x0 = tensors[0][0]
-    if len(x0.shape) != 4 or len(tensors) > 3:
+    if not 1 <= len(tensors) <= 3 or len(tensors[0][0].shape) != 4:
         raise ValueError("tensors: one to three pairs of [batch][heads][tokens][head_d] arrays")
+    x0 = tensors[0][0]
     B, _, T, D = x0.shape
     descs = (_RotatedDesc * len(tensors))()
     for i, (x, out) in enumerate(tensors):

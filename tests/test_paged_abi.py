@@ -472,3 +472,8 @@ def test_prompts_of_wide_heads(am, dtype, B, H, G, T, D, rows):
     one = 4 * (H // G) * T * rows
     assert attend(am, c, d, ws=WS, wsb=one + (one >> 4)) == ok
     assert attend(am, c, d, ws=WS, wsb=one // 2) == -8
+
+
+def test_rotary_call_of_no_tensors(am):
+    with pytest.raises(ValueError):
+        am.rotary_call(am.Rotary(arr((32,), "f32", FA)), [])
