@@ -135,8 +135,8 @@ struct PagedArgs {
 };
 // Whether reading `rows` shared rows once for m sequences saves anything.  It saves the other members' reads,
 // 2 es head_d bytes a row and kv head; but every query row's result then passes through the scratch in two
-// parts, 16 head_d bytes (5 sequences of 281 tokens of 16 heads of 8192 dims, 19 rows shared: 1200 us read
-// as their own, 2450 read once).
+// parts, 16 head_d bytes (5 sequences of 281 tokens of 16 heads over 4 of 8192 dims, 19 rows shared: 1209 us
+// read as their own, 2335 read once).
 __host__ __device__ __forceinline__ bool saves_reads(int64_t rows, int m, int es, int rep, int T) {
     return m >= 2 && rows * (m - 1) * es > (int64_t)m * rep * T * 8;
 }

@@ -56,8 +56,8 @@ Tile tile_of(int dtype, int D, int64_t R, int64_t pairs, int64_t keys, bool runs
         // items in ranges, whose parts go through memory and a merge: 0.97 PFLOP/s in tiles of 256 rows,
         // tiles of 128 and 64 take 1.33 and 1.45 times as long (they read K and V from LDS for fewer
         // rows), a merge 12 us and its parts twice at 4.5 TB/s.  512 tokens over 8000 rows, 2 sequences of
-        // 32 over 8 heads: 180 us in ranges of 256 rows, 204 in whole items of 128; 256 over 1000, 4
-        // sequences: 77 and 46.
+        // 32 over 8 heads: 179 us in ranges of 256 rows, 210 in whole items of 128; 256 over 1000, 4
+        // sequences: 76 and 49.
         Tile best{kMany, 0, 0};
         double least = 0;
         for (int rows : {256, 128, 64}) {
@@ -118,11 +118,11 @@ PagedPass plan_pass(int dtype, int D, Tile t, int64_t most, int64_t segments, in
     // less than ranges and their merge (8 us), at most 1024 of them, 256 where 4 waves each would take
     // them whole too.  A CU reads 50 (fp32 38) GB/s of rows of whole tiles of dims, all of them
     // 5.2 TB/s; 1 MiB an item at most, since the host knows no lengths but the bound and one long
-    // sequence alone takes its time.  One token of 32 over 8 heads of 128 bf16 dims: 600 rows 14.5 in
-    // ranges, 10.9 whole; 1500 rows 14.9 and 18.7; 32 sequences of 500 to 1000 rows 31.6 and 22.3, 100
-    // of 16 heads 75.6 and 72.3; 64 of 300 rows 17 by 4 waves and 21 by 8.
+    // sequence alone takes its time.  One token of 32 over 8 heads of 128 bf16 dims: 600 rows 15.1 in
+    // ranges, 10.8 whole; 1500 rows 14.7 and 18.6; 32 sequences of 500 to 1000 rows 31.8 and 22.4, 100
+    // of 16 heads over 8 75.6 and 72.8; 64 of 300 rows 17 by 4 waves and 21 by 8.
     // Tiles of 32 rows up to 128 dims (8 waves' results of more pass LDS): 32 sequences of 6 tokens over
-    // 500 to 1000 rows 38.3 and 25.3.
+    // 500 to 1000 rows 39.0 and 25.9.
     if (t.kind == kNarrow && alone && (p.rows == 16 || (p.rows == 32 && D <= 128))) {
         const double dim = 2. * keys * (bf ? 2 : 4), item = dim * ceil_div(D, 64) * 64;
         p.few = p.items <= (p.split ? 1024 : 256) && item <= 1 << 20 &&
@@ -161,7 +161,7 @@ PagedPlan plan_sequences(int dtype, const PagedView& c, int H, int T, int groups
         // with 24 us more than nothing and reads at 4.5 TB/s, or tiles of 32 (64) rows in the launch of
         // the sequences' own, each of which reads the prefix again, at 6 TB/s (from L2 for the most):
         // 8192 rows shared by 32 sequences of 64 to 1024 rows of their own, 32 over 8 heads of 128 dims,
-        // 57 against 70 us; 4 times 16384 shared by 16 each 85 against 66 in the prefixes' launch alone.
+        // 56 against 63 us; 4 times 16384 shared by 16 each 123 against 108.
         const int narrow = D > 64 ? 32 : 64;
         const double bytes = (double)c.rows * groups * c.G * D * 4;
         if (pre.kind == kMany && own.kind == kNarrow &&

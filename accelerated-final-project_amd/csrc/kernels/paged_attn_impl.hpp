@@ -215,7 +215,8 @@ struct Span {
     int blocks_before;
 };
 __device__ __forceinline__ int bounded(const PagedPass& p, int part) {
-    // (groups that overlap have more items than the host counts on)
+    // (the host counts with the most items that lengths and groups can make; the bound is for those that
+    // change between the kernels of a call)
     return (int)min((int64_t)part, p.parts - 1);
 }
 // The last block that any row of the item's tile attends, and one more.

@@ -7,8 +7,8 @@
 // Nothing but the bytes bounds it, once each angle is computed once for all heads: a workgroup
 // takes a few tokens, puts their cosines and sines into LDS and goes through the tokens' rows of
 // all tensors 16 bytes a lane.  4 sequences of 4096 tokens, 40 heads of 128 bf16 dims: 67 us, 5.0
-// TB/s; whole prompts of 16384 tokens into the cache (48 heads) 76 us, 4.6 TB/s; a few tokens 8 us, of
-// which the call is 4.
+// TB/s; prompts of 14338 tokens (8 of 2048 or 1366) into the cache, 48 heads, 75 us, 4.7 TB/s; a few
+// tokens 7 us, of which the call is 4.
 // Angles: p freq in fp64 (24 + 31 bits: exact to 2^-53), reduced to half turns there, so that
 // positions far into a context lose nothing; the rest is fp32, rounded to the type once.
 #include <algorithm>
