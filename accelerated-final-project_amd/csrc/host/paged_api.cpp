@@ -385,11 +385,18 @@ size_t atn_paged_attention_workspace_bytes(const atn_paged_cache* cache, const a
     bool whole16;
     if (check_attention(cache, tokens, prefix, max_len, &a, &p, &q, &whole16) != ATN_OK) return 0;
     const size_t cap = atn_host::workspace_cap();
-    plan_call(cache->dtype, whole16, cap, &a);
-    // (a prefix that this bound of the lengths leaves out may fit with a smaller one)
-    const bool out = prefix && a.groups == 0 && a.c.B > 1 &&
-                     atn::saves_reads(a.c.rows, a.c.B, a.es, a.rep, a.T);
-    return kSyncRegion + (out ? std::max(cap, a.plan.scratch) : a.plan.scratch);
+    // Parts follow the tiles, which may be larger with a smaller bound of the lengths; and a prefix that this
+    // bound leaves out may fit with a smaller one.  What is asked for serves them too.
+    size_t most = 0;
+    for (int rows = a.c.rows; rows >= 1; rows /= 2) {
+        atn::PagedArgs x = a;
+        x.c.rows = rows;
+        plan_call(cache->dtype, whole16, cap, &x);
+        most = std::max(most, x.plan.scratch);
+        if (a.groups == 0) break;
+        if (x.groups == 0 && atn::saves_reads(rows, x.c.B, x.es, x.rep, x.T)) most = std::max(most, cap);
+    }
+    return kSyncRegion + most;
 }
 
 int atn_paged_attention_ex(const atn_paged_cache* cache, const atn_drafts* tokens,

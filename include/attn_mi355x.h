@@ -539,12 +539,12 @@ typedef struct atn_shared_prefix {
  * the cache by now).  prefix (NULL: none): its rows are read once a group; results differ from those
  * without it by the order of sums alone.  scale, lse, out_stride and workspace as for
  * atn_tree_attention_ex (head_d > 256: one kv head's scores of one sequence have to fit, 4 bytes for
- * each query row and row up to max_len, in tiles of 16 to 64 and 32; with a prefix those of all sequences
- * and one kv head's parts too, but for
- * prefixes that the library's own workspace could not hold, or that are too short beside their query
- * rows to be read once: those are read as the sequences' own rows).  max_len: an upper bound of
- * len[b] + count[b] that the host knows (0: the rows of a table); the call is laid out for it, and rows
- * from there on are not attended.  A workspace of the size for one max_len serves smaller ones.
+ * each query row and row up to max_len, in tiles of 16 to 64 and 32; with a prefix those of all
+ * sequences and one kv head's parts too, but for prefixes that the library's own workspace could not
+ * hold, or that are too short beside their query rows to be read once: those are read as the sequences'
+ * own rows).  max_len: an upper bound of len[b] + count[b] that the host knows (0: the rows of a table);
+ * the call is laid out for it, and rows from there on are not attended.  A workspace of the size for one
+ * max_len serves smaller ones.
  * Rows that a token does not attend do not reach its output, whatever they hold; an infinity or NaN in
  * a value that it attends makes that dim of its output infinite or NaN. */
 int atn_paged_attention_ex(const atn_paged_cache *cache, const atn_drafts *tokens,

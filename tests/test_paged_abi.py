@@ -477,3 +477,18 @@ def test_prompts_of_wide_heads(am, dtype, B, H, G, T, D, rows):
 def test_rotary_call_of_no_tensors(am):
     with pytest.raises(ValueError):
         am.rotary_call(am.Rotary(arr((32,), "f32", FA)), [])
+
+
+@pytest.mark.parametrize("D,B,rep,T,slots,groups,bounds", [
+    (8, 244, 1, 76, 71, 67, [1136, 511, 300, 20]), (8, 504, 8, 11, 202, 186, [3232, 2759, 511, 500]),
+    (64, 476, 1, 69, 164, 100, [2624, 2500, 511, 100])])
+def test_workspace_of_a_larger_bound_and_smaller_tiles(am, D, B, rep, T, slots, groups, bounds):
+    """Prefixes whose tiles, and so the parts, grow where the bound of the lengths shrinks."""
+    if no_device(am) == 0:
+        pytest.skip("addresses that nothing may dereference")
+    c = cache(am, batch=B, kv_heads=1, pages=1 << 14, table_pages=slots, head_d=D)
+    d, p = drafts(am, heads=rep, tokens=T), prefix(am, groups=groups)
+    for i, most in enumerate(bounds):
+        n = need(am, c, d, p, most)
+        for less in bounds[i:]:
+            assert attend(am, c, d, p, max_len=less, ws=WS, wsb=n) == -6
